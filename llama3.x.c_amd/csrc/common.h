@@ -24,7 +24,9 @@ struct Device {
   int ordinal = 0;
   hipStream_t stream = nullptr;
   int *error_flags = nullptr; // device: [0] non-finite activation seen by a quantizer, [1] non-finite attention score,
-                              // [2] an embedding row id outside the table
+                              // [2] an embedding row id outside the table, [3] a request batch outside its buffers,
+                              // [4] two requests of a store in one slot, [5] an adapter id outside its table,
+                              // [6] undecidable logits or [7] a draft outside the vocabulary in a verification
   int *host_flags = nullptr;  // pinned host copy of the 16 flag words, read back with the synchronization
   int cu_count = 0;
   bool capturing = false;
@@ -137,7 +139,7 @@ class Call {
   void *resolve_registered(const void *p, size_t *room = nullptr);
   const char *name_;
   uintptr_t current_mapping_ = 0; // a registered file mapping found current during this call
-  Copy copies_[16];
+  Copy copies_[32];
   int ncopies_ = 0;
   size_t arena_used_ = 0;
   bool staged_ = false, failed_ = false;
@@ -260,6 +262,59 @@ size_t attention_partial_floats(int rows, int n_heads, int head_dim, int last_po
 bool launch_attention(const AttentionJob &job, float *partial, hipStream_t stream);
 // The batched kernel takes the job; its partials, when it splits a tile's positions, stay within job.partial_room.
 bool attention_uses_flash(const AttentionJob &job);
+
+// ---- many requests on one model (requests.hip, lora.hip, verify.hip) ------------------------------------------------
+// RequestBatch with device addresses, and the strides of the caches it indexes: position t of KV head g at
+// + t * pos_stride + g * head_base of a slot, slots slot_floats apart; the prefix likewise.
+struct RequestsDev {
+  const int *start, *length, *slot;
+  int count, rows, prefix, seq_len, slots;
+  size_t pos_stride, head_base, slot_floats, prefix_pos_stride, prefix_head_base;
+};
+struct RopeRequestsJob {
+  float *q_out;
+  const float *q, *k, *v, *table;
+  size_t q_stride, kv_stride;
+  RequestsDev batch;
+  int n_heads, n_kv_heads, head_dim;
+  float *key, *value;
+};
+bool launch_rope_requests(const RopeRequestsJob &job, hipStream_t stream);
+struct AttentionRequestsJob {
+  float *out;
+  const float *q, *prefix_key, *prefix_value, *key, *value;
+  RequestsDev batch;
+  int n_heads, n_kv_heads, head_dim;
+};
+bool launch_attention_requests(const AttentionRequestsJob &job, hipStream_t stream);
+
+struct LoraSegmentDev {
+  float *c;
+  const float *base, *base3;
+  const void *a, *b, *a3, *b3; // float, or bf16 bits
+  const float *scale;
+  int ldc, n, rank;
+  bool swiglu;
+};
+struct LoraJob {
+  const float *x;
+  const int *adapter;
+  int ldx, m, k, adapters, nseg;
+  bool bf16;
+  LoraSegmentDev seg[3];
+};
+bool launch_lora(const LoraJob &job, hipStream_t stream);
+
+struct VerifyJob {
+  int *accepted, *next;
+  const float *logits, *draft; // draft null: drafts not drawn
+  size_t ld, draft_ld;
+  const int *tokens, *start;
+  const float *uniform; // null: greedy
+  int count, rows, vocab;
+  float temperature;
+};
+bool launch_verify(const VerifyJob &job, hipStream_t stream);
 
 struct GemmSegmentDev {
   float *c;

@@ -168,13 +168,20 @@ bool ensure_device() {
 // A device error flag set since the last check becomes the failure of this call (the flags then cleared).
 bool report_flags(const int *flags) {
   Device &dev = the_device;
-  if (flags[0] || flags[1] || flags[2]) {
-    int zero[16] = {0};
-    (void)hipMemcpy(dev.error_flags, zero, sizeof(zero), hipMemcpyHostToDevice);
-    return raise(flags[0]   ? "nonfinite activation during INT8 quantization"
-                 : flags[1] ? "nonfinite value in softmax"
-                            : "embedding row id outside the table");
-  }
+  static const char *const kMessages[] = {"nonfinite activation during INT8 quantization",
+                                          "nonfinite value in softmax",
+                                          "embedding row id outside the table",
+                                          "a request's rows, positions or slot lie outside the batch's buffers",
+                                          "two requests of one call store into the same slot",
+                                          "adapter id outside the table",
+                                          "logits of a verified row leave no token (a NaN, an infinity or all masked)",
+                                          "drafted token outside the vocabulary"};
+  for (size_t i = 0; i < sizeof(kMessages) / sizeof(kMessages[0]); i++)
+    if (flags[i]) {
+      int zero[16] = {0};
+      (void)hipMemcpy(dev.error_flags, zero, sizeof(zero), hipMemcpyHostToDevice);
+      return raise("%s", kMessages[i]);
+    }
   return true;
 }
 

@@ -31,6 +31,8 @@ GEMM_STORE, GEMM_ADD, GEMM_SWIGLU, GEMM_PARTIAL = 0, 1, 2, 3
 Q8_GEMM_PORTABLE, Q8_GEMM_AVX512, Q8_GEMM_AMX, Q8_GEMM_HIP_MFMA = 0, 1, 2, 3
 # include/llama_hip.h
 LLHIP_FAIL_EXIT, LLHIP_FAIL_RECORD = 0, 1
+# include/llama_hip_requests.h
+LLHIP_MAX_REQUESTS, LLHIP_MAX_LORA_RANK = 1024, 256
 LOGITS_NONE, LOGITS_LAST, LOGITS_ALL = 0, 1, 2
 
 
@@ -111,7 +113,29 @@ class AttentionWork(ctypes.Structure):  # kernels.h:127-132
                 ("external", I32), ("capacity", SZ)]
 
 
+
+
+class RequestBatch(ctypes.Structure):  # include/llama_hip_requests.h
+    _fields_ = [("start", P), ("length", P), ("slot", P)] + \
+               [(f, I32) for f in ("count", "rows", "prefix", "prefix_seq_len", "seq_len", "slots")]
+
+
+class LoraSegment(ctypes.Structure):
+    _fields_ = [("c", P), ("ldc", I32), ("base", P), ("base3", P), ("a", P), ("b", P), ("a3", P), ("b3", P),
+                ("scale", P), ("n", I32), ("rank", I32), ("kind", I32)]
+
+
+class LoraBf16Segment(ctypes.Structure):  # a, b, a3, b3: BF16 bits
+    _fields_ = LoraSegment._fields_
+
+
 _SIGNATURES = {
+    # many requests on one model (llama_hip_requests.h)
+    "llhip_rope_kv_store_requests": (None, [P, P, SZ, P, P, SZ, P, ctypes.POINTER(RequestBatch), I32, I32, I32, P, P]),
+    "llhip_attention_requests": (None, [P, P, P, P, P, P, ctypes.POINTER(RequestBatch), I32, I32, I32]),
+    "llhip_lora_f32": (None, [P, I32, I32, I32, P, I32, ctypes.POINTER(LoraSegment), I32]),
+    "llhip_lora_bf16": (None, [P, I32, I32, I32, P, I32, ctypes.POINTER(LoraBf16Segment), I32]),
+    "llhip_verify_drafts": (None, [P, P, P, SZ, P, SZ, P, P, P, I32, I32, I32, ctypes.c_float]),
     # the forward around the matmuls (llama_hip_forward.h)
     "k_rmsnorm": (None, [P, P, P, I32, ctypes.c_float]),
     "k_rmsnorm_rows": (None, [P, P, P, I32, I32, ctypes.c_float]),

@@ -1,0 +1,714 @@
+"""Many requests on one model, on the GPU: each operator against its plain float64 form (tests/requests_util.py, the bounds
+derived there), its index checks, host buffers and captured calls; and a small model served by all of them together."""
+import numpy as np
+import pytest
+
+import llama_hip as lh
+from tests import hip_util as hu
+from tests import requests_util as ru
+
+pytestmark = pytest.mark.gpu
+F = np.float32
+
+
+@pytest.fixture
+def L():
+    lib = lh.load()
+    assert lib.llhip_init() == 0, lh.last_error()
+    lh.record_failures()
+    layout = lib.kernels_kv_layout_name().decode()
+    yield lib
+    lib.kernels_kv_layout_select(layout.encode())
+    lib.llhip_synchronize()
+    lib.llhip_clear_error()
+    lib.llhip_set_fail_mode(lh.LLHIP_FAIL_EXIT)
+
+
+def quiet(L):
+    L.llhip_synchronize()
+    assert not lh.last_error(), lh.last_error()
+
+
+def fails(L, words):
+    L.llhip_synchronize()
+    message = lh.last_error()
+    L.llhip_clear_error()
+    assert words in message, message
+
+
+def within(got, want, bound, what=""):
+    off = np.abs(got.astype(np.float64) - want)
+    assert np.isfinite(got).all(), what
+    worst = np.unravel_index(np.argmax(off - bound), off.shape)
+    assert (off <= bound).all(), (what, worst, got[worst], want[worst], off[worst], bound[worst])
+
+
+def shifted(a, floats=1):
+    """A device copy of `a` whose address is 4 * floats bytes off the allocation's 16-byte alignment."""
+    t = hu.torch()
+    flat = hu.empty(a.size + floats, t.float32)
+    view = flat[floats:].reshape(a.shape)
+    view.copy_(t.from_numpy(a))
+    t.cuda.synchronize()
+    return view
+
+
+# ---- RoPE and cache rows ------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("layout", ["head", "rows"])
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (3, 1, 128), (5, 5, 6), (8, 2, 80), (2, 1, 256)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_rope_rows_equal_the_single_calls_bit_for_bit(L, layout, heads, kv, hd, packed):
+    """Against k_rope_apply and k_kv_store of each row alone: ragged requests (none, one and many rows), permuted slots,
+    rows before the first and behind the last request, in place on packed QKV rows or into another buffer."""
+    L.kernels_kv_layout_select(layout.encode())
+    rng = np.random.default_rng(hd + heads)
+    b = ru.Batch(hu.dev, [3, 0, 1, 40, 2], [0, 99, 7, 11, 30], slot=[4, 77, 0, 5, 2], slots=7, prefix=9, seq_len=53, first=2,
+                 spare=3)
+    dq, dkv = heads * hd, kv * hd
+    cfg = lh.Config(head_dim=hd, rope_theta=500000.0)
+    table = np.zeros((9 + 53, 2 * hd), F)
+    for p in range(len(table)):
+        L.k_rope_table(ru.byref(cfg), p, lh.ptr(table[p]))
+    caches = [rng.standard_normal((7,) + ru.cache_shape(layout, 53, kv, hd), dtype=F) for _ in range(2)]
+    wide = rng.standard_normal((b.rows, dq + 2 * dkv + 4), dtype=F)
+    q, k, v = wide[:, :dq], wide[:, dq:dq + dkv], wide[:, dq + dkv:dq + 2 * dkv]
+    kd, vd, td = hu.dev(caches[0]), hu.dev(caches[1]), hu.dev(table)
+    if packed:
+        rows = hu.dev(wide)
+        qd, kr, vr = rows, rows[:, dq:], rows[:, dq + dkv:]
+        out, stride, kv_stride = rows, wide.shape[1], wide.shape[1]
+    else:
+        qd, kr, vr = (hu.dev(np.ascontiguousarray(x)) for x in (q, k, v))
+        out, stride, kv_stride = hu.dev(np.full((b.rows, dq), 7.0, F)), dq, dkv
+    L.llhip_rope_kv_store_requests(lh.ptr(out), lh.ptr(qd), stride, lh.ptr(kr), lh.ptr(vr), kv_stride, lh.ptr(td),
+                                   b.struct, heads, kv, hd, lh.ptr(kd), lh.ptr(vd))
+    quiet(L)
+    got = hu.host(out)[:, :dq]
+    want = q.copy() if packed else np.full((b.rows, dq), 7.0, F)
+    for _, rows_, length, slot in b.requests():
+        for j, i in enumerate(range(rows_.start, rows_.stop)):
+            qi, ki, vi = q[i].copy(), k[i].copy(), v[i].copy()
+            L.k_rope_apply(lh.ptr(qi), lh.ptr(ki), lh.ptr(table[9 + length + j]), heads, kv, hd)
+            want[i] = qi
+            for c, x in ((caches[0], ki), (caches[1], vi)):
+                ru.by_head(c[slot], layout)[:, length + j] = x.reshape(kv, hd)
+    assert np.array_equal(hu.bits(got), hu.bits(want))
+    assert np.array_equal(hu.bits(hu.host(kd)), hu.bits(caches[0]))
+    assert np.array_equal(hu.bits(hu.host(vd)), hu.bits(caches[1]))
+    if packed:
+        assert np.array_equal(hu.host(rows)[:, dq:], wide[:, dq:])
+
+
+def test_rope_rows_refuse_what_lies_outside(L):
+    """A request outside the buffers stores nothing and fails at the wait, the others are done; two requests in one slot
+    fail."""
+    heads, kv, hd, seq = 2, 1, 8, 10
+    L.kernels_kv_layout_select(b"head")
+    table = hu.dev(np.ones((seq, 2 * hd), F))
+    q, k = hu.dev(np.ones((4, heads * hd), F)), hu.dev(np.ones((4, kv * hd), F))
+
+    def call(**over):
+        args = {"rows_of": [2, 2], "length": [0, 3], "slot": [0, 1], "slots": 2, "seq_len": seq}
+        args.update(over)
+        b = ru.Batch(hu.dev, **args)
+        out = hu.dev(np.zeros((4, heads * hd), F))
+        caches = [hu.dev(np.zeros((2, kv, seq, hd), F)) for _ in range(2)]
+        L.llhip_rope_kv_store_requests(lh.ptr(out), lh.ptr(q), heads * hd, lh.ptr(k), lh.ptr(k), kv * hd, lh.ptr(table),
+                                       b.struct, heads, kv, hd, lh.ptr(caches[0]), lh.ptr(caches[1]))
+        return out, caches
+
+    call()
+    quiet(L)
+    for over in ({"length": [0, 9]}, {"length": [0, -1]}, {"slot": [0, 2]}, {"slot": [0, -1]},
+                 {"length": [0, 2 ** 31 - 1]}):
+        out, caches = call(**over)
+        fails(L, "outside the batch's buffers")
+        got, cache = hu.host(out), hu.host(caches[1])  # (1, 1) turned by (1, 1) is (0, 2): the values are counted
+        assert (got[2:] == 0).all() and (got[:2] != 0).any()
+        assert np.count_nonzero(cache[0]) == 2 * hd and not cache[1].any()
+    call(slot=[1, 1])
+    fails(L, "into the same slot")
+    # a request without rows may hold any length and slot
+    call(rows_of=[4, 0], length=[0, -7], slot=[0, 99])
+    quiet(L)
+
+
+# ---- attention --------------------------------------------------------------------------------------------------------
+
+
+def attention_case(L, seed, heads, kv, hd, layout, b, offset=0, scale=1.0, nan_spare=True):
+    """Random operands of a batch, the call's output and the float64 one; the spare rows' q is NaN and their out kept."""
+    L.kernels_kv_layout_select(layout.encode())
+    rng = np.random.default_rng(seed)
+    q = scale * rng.standard_normal((b.rows, heads * hd), dtype=F)
+    pk, pv = (rng.standard_normal(ru.cache_shape(layout, max(b.prefix_seq_len, 1), kv, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((b.slots,) + ru.cache_shape(layout, b.seq_len, kv, hd), dtype=F) for _ in range(2))
+    live = np.zeros(b.rows, bool)
+    for _, rows, length, slot in b.requests():
+        live[rows] = True
+    if nan_spare:  # what no row may see: idle rows, cache places behind every request's last row
+        q[~live] = np.nan
+        end = np.zeros(b.slots, int)
+        for _, rows, length, slot in b.requests():
+            end[slot] = max(end[slot], length + rows.stop - rows.start)
+        for c in (k, v):
+            for s in range(b.slots):
+                ru.by_head(c[s], layout)[:, end[s]:] = np.nan
+        for c in (pk, pv):
+            ru.by_head(c, layout)[:, b.prefix:] = np.nan
+    put = (lambda a: shifted(a, offset)) if offset else hu.dev
+    out = put(np.full((b.rows, heads * hd), 5.0, F))
+    args = [put(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in args], b.struct, heads, kv, hd)
+    quiet(L)
+    got = hu.host(out)
+    clean = [np.nan_to_num(a) for a in (q, pk, pv, k, v)]
+    want, bound = ru.attention(b, clean[0], clean[1], clean[2], clean[3], clean[4], heads, kv, hd, layout)
+    want[~live] = 5.0
+    within(got, want, bound)
+    return got
+
+
+SHAPES = [(4, 2, 64), (8, 2, 128), (32, 8, 64), (3, 3, 128), (6, 1, 64), (16, 1, 128), (4, 2, 80), (2, 1, 256), (3, 1, 7),
+          (5, 1, 96), (12, 4, 48)]
+
+
+@pytest.mark.parametrize("layout", ["head", "rows"])
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+def test_attention_decode(L, layout, heads, kv, hd):
+    """One row a request (and requests without rows) at ragged lengths from the first own position on, permuted slots."""
+    b = ru.Batch(hu.dev, [1, 1, 0, 1, 1, 1], [0, 63, 5, 64, 200, 1], slot=[3, 1, 0, 6, 2, 4], slots=7, prefix=131,
+                 prefix_seq_len=140, seq_len=202, first=1, spare=2)
+    attention_case(L, hd, heads, kv, hd, layout, b)
+
+
+@pytest.mark.parametrize("prefix", [0, 1, 31, 32, 33, 64, 255, 700])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 2, 64), (4, 4, 96)])
+def test_attention_prefix_lengths(L, prefix, heads, kv, hd):
+    b = ru.Batch(hu.dev, [1, 3, 1], [0, 0, 32], prefix=prefix, prefix_seq_len=prefix + 3, seq_len=40)
+    attention_case(L, prefix, heads, kv, hd, "head", b)
+
+
+@pytest.mark.parametrize("rows_of,length", [([2, 7, 1, 5], [10, 0, 64, 31]), ([1], [0]), ([33], [0]), ([130, 1, 65], [0, 90, 3]),
+                                            ([16, 17, 32, 31], [1, 2, 3, 4]), ([1] * 70, list(range(70)))])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 4, 64), (10, 2, 64), (6, 2, 80)])
+def test_attention_drafts_and_prompts(L, rows_of, length, heads, kv, hd):
+    """Several rows a request, causal among themselves, over tile edges; more vectors than a tile holds."""
+    b = ru.Batch(hu.dev, rows_of, length, prefix=77, prefix_seq_len=80, seq_len=160, spare=1)
+    attention_case(L, len(rows_of), heads, kv, hd, "head", b)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 2, 64)])
+def test_attention_shared_slots_and_long_own(L, heads, kv, hd):
+    """Requests that read one slot, and lengths far apart: one of 3000 own positions beside short ones."""
+    b = ru.Batch(hu.dev, [1, 1, 2, 1], [2999, 3, 40, 0], slot=[1, 0, 1, 2], prefix=2000, prefix_seq_len=2000, seq_len=3001)
+    attention_case(L, 5, heads, kv, hd, "head", b)
+
+
+@pytest.mark.parametrize("offset", [1, 2])
+def test_attention_unaligned(L, offset):
+    b = ru.Batch(hu.dev, [1, 4], [20, 0], prefix=50, prefix_seq_len=51, seq_len=30)
+    attention_case(L, 9, 4, 2, 64, "head", b, offset=offset)
+
+
+def test_attention_sharp_scores(L):
+    """Scores of some hundred units: one position takes nearly the whole weight, in the prefix or behind it."""
+    b = ru.Batch(hu.dev, [1, 2, 1], [100, 40, 0], prefix=300, prefix_seq_len=300, seq_len=128)
+    attention_case(L, 10, 8, 2, 128, "head", b, scale=30.0)
+
+
+def test_attention_spread_values(L):
+    """Keys and values of very different sizes from position to position and dimension to dimension."""
+    L.kernels_kv_layout_select(b"head")
+    heads, kv, hd = 8, 2, 128
+    b = ru.Batch(hu.dev, [1, 3], [90, 0], prefix=200, prefix_seq_len=200, seq_len=100)
+    rng = np.random.default_rng(11)
+    spread = lambda shape: (rng.standard_normal(shape) * 10.0 ** rng.uniform(-6, 4, shape)).astype(F)  # noqa: E731
+    q = (1e-3 * rng.standard_normal((b.rows, heads * hd))).astype(F)
+    pk, k = (1e-2 * spread((kv, 200, hd))).astype(F), (1e-2 * spread((2, kv, 100, hd))).astype(F)
+    pv, v = spread((kv, 200, hd)), spread((2, kv, 100, hd))
+    out = hu.dev(np.zeros_like(q))
+    args = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in args], b.struct, heads, kv, hd)
+    quiet(L)
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
+    within(hu.host(out), want, bound)
+
+
+def test_attention_refuses_what_lies_outside(L):
+    """The rows of a request outside the buffers are left, the others are done, and the wait reports it; a non-finite
+    score is reported as k_attention reports it."""
+    heads, kv, hd, seq = 4, 2, 64, 40
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(3)
+    q = rng.standard_normal((4, heads * hd), dtype=F)
+    pk, pv = (rng.standard_normal((kv, 50, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((2, kv, seq, hd), dtype=F) for _ in range(2))
+
+    def call(q=q, start=None, **over):
+        args = {"rows_of": [2, 2], "length": [0, 3], "slot": [0, 1], "slots": 2, "seq_len": seq, "prefix": 50}
+        args.update(over)
+        b = ru.Batch(hu.dev, **args)
+        if start is not None:
+            b.rows = b.struct.rows = 4
+            b.keep += (hu.dev(np.asarray(start, np.int32)),)
+            b.struct.start = lh.ptr(b.keep[-1])
+        out = hu.dev(np.zeros_like(q))
+        dev = [hu.dev(a) for a in (q, pk, pv, k, v)]
+        L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in dev], b.struct, heads, kv, hd)
+        return out
+
+    want = hu.host(call())
+    quiet(L)
+    for over in ({"length": [0, seq - 1]}, {"length": [0, -1]}, {"slot": [0, 2]}, {"slot": [0, -5]}, {"start": [0, 2, 5]},
+                 {"start": [0, 2, 1]}, {"start": [0, 2, 2 ** 31 - 1]}):
+        out = call(**over)
+        fails(L, "outside the batch's buffers")
+        got = hu.host(out)
+        assert np.array_equal(got[:2], want[:2]) and (got[2:] == 0).all(), over
+    out = call(start=[-1, 2, 4])
+    fails(L, "outside the batch's buffers")
+    assert np.array_equal(hu.host(out)[2:], want[2:]) and (hu.host(out)[:2] == 0).all()
+    worse = q.copy()
+    worse[3, 5] = np.inf
+    call(q=worse)
+    fails(L, "nonfinite value in softmax")
+
+
+def test_attention_from_host_memory(L):
+    """Plain host buffers and arrays: copied in and out, rows without a request kept."""
+    heads, kv, hd = 4, 2, 64
+    L.kernels_kv_layout_select(b"rows")
+    rng = np.random.default_rng(4)
+    b = ru.Batch(lambda a: a, [1, 2], [4, 0], prefix=20, prefix_seq_len=24, seq_len=8, spare=1)
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    pk, pv = (rng.standard_normal((24, kv, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((2, 8, kv, hd), dtype=F) for _ in range(2))
+    out = np.full_like(q, 3.0)
+    L.llhip_attention_requests(*[lh.ptr(a) for a in (out, q, pk, pv, k, v)], b.struct, heads, kv, hd)
+    assert not lh.last_error(), lh.last_error()
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "rows")
+    within(out[:3], want[:3], bound[:3])
+    assert (out[3] == 3.0).all()
+
+
+def test_attention_repeats_itself_and_does_not_depend_on_neighbours_order(L):
+    """Bit for bit the same on every call."""
+    b = ru.Batch(hu.dev, [1] * 9 + [5, 40], [17 * i for i in range(9)] + [500, 0], prefix=1000, prefix_seq_len=1000,
+                 seq_len=600)
+    first = attention_case(L, 12, 8, 2, 128, "head", b)
+    for _ in range(3):
+        assert np.array_equal(hu.bits(first), hu.bits(attention_case(L, 12, 8, 2, 128, "head", b)))
+
+
+# ---- adapters ---------------------------------------------------------------------------------------------------------
+
+
+def bf16(a):
+    """`a` rounded to BF16: its bits, and the values they stand for."""
+    bits = hu.bits(a)
+    up = ((bits.astype(np.uint64) + 0x7FFF + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+    return up, (up.astype(np.uint32) << 16).view(F).reshape(a.shape)
+
+
+class Adapters:
+    """One segment's operands on the device, and what the call should give."""
+
+    def __init__(self, rng, m, k, n, rank, adapters, is_bf16, swiglu, ldc=None, in_place=False, offset=0, scaled=True):
+        self.n, self.rank, self.ldc, self.swiglu, self.is_bf16 = n, rank, ldc or n, swiglu, is_bf16
+        self.m = m
+        put = (lambda a: shifted(a, offset)) if offset else hu.dev
+        self.base = [rng.standard_normal((m, self.ldc), dtype=F) for _ in range(1 + swiglu)]
+        self.scale = rng.uniform(0.5, 2.0, adapters).astype(F) if scaled else None
+        self.pairs, dev = [], []
+        for _ in range(1 + swiglu):
+            a = (rng.standard_normal((adapters, rank, k)) / np.sqrt(k)).astype(F)
+            b = (rng.standard_normal((adapters, n, rank)) / np.sqrt(rank)).astype(F)
+            if is_bf16:
+                (abits, a), (bbits, b) = bf16(a), bf16(b)
+                if offset:
+                    t = hu.torch()
+                    pads = []
+                    for x in (abits, bbits):
+                        flat = hu.dev(np.concatenate((np.zeros(offset, np.uint16), x.reshape(-1))).view(np.int16))
+                        pads.append(flat[offset:])
+                    dev.append(pads)
+                else:
+                    dev.append([hu.dev(abits.view(np.int16)), hu.dev(bbits.view(np.int16))])
+            else:
+                dev.append([put(a), put(b)])
+            self.pairs.append((a, b))
+        self.c = hu.dev(self.base[0]) if in_place else put(np.full((m, self.ldc), 9.0, F))
+        base_dev = [self.c if in_place else put(self.base[0])] + [put(x) for x in self.base[1:]]
+        self.in_place = in_place
+        scale_dev = None if self.scale is None else hu.dev(self.scale)
+        self.keep = (dev, base_dev, scale_dev)
+        third = {"base3": base_dev[1], "a3": dev[1][0], "b3": dev[1][1]} if swiglu else {}
+        self.struct = ru.lora_segment(is_bf16, self.c, self.ldc, base_dev[0], dev[0][0], dev[0][1], scale_dev, n, rank,
+                                      **third)
+
+    def check(self, x, ids):
+        scale = np.ones(len(self.pairs[0][0])) if self.scale is None else self.scale.astype(np.float64)
+        n = self.n
+        want, bound = ru.adapters(x, ids, self.base[0][:, :n], *self.pairs[0], scale)
+        if self.swiglu:
+            want, bound = ru.swiglu(want, bound, *ru.adapters(x, ids, self.base[1][:, :n], *self.pairs[1], scale))
+        got = hu.host(self.c)
+        within(got[:, :n], want, bound + 2 * ru.U * np.abs(want), (self.m, n, self.rank))
+        pad = self.base[0][:, n:] if self.in_place else np.full((self.m, self.ldc - n), 9.0, F)
+        assert np.array_equal(got[:, n:], pad)
+        return got
+
+
+def run_lora(L, x, ldx, k, ids, adapters, segs, is_bf16):
+    xd, idd = x if hasattr(x, "data_ptr") else hu.dev(x), hu.dev(np.asarray(ids, np.int32))
+    fn = L.llhip_lora_bf16 if is_bf16 else L.llhip_lora_f32
+    fn(lh.ptr(xd), ldx, len(ids), k, lh.ptr(idd), adapters, ru.array([s.struct for s in segs]), len(segs))
+    return xd, idd
+
+
+def ids_of(rng, m, adapters, form):
+    if form == "each":
+        return rng.integers(-1, adapters, m)
+    if form == "runs":
+        return np.repeat(rng.integers(-1, adapters, m // 7 + 1), 7)[:m]
+    return np.full(m, {"one": adapters - 1, "none": -1}[form])
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("form", ["each", "runs", "one", "none"])
+@pytest.mark.parametrize("m", [1, 2, 5, 16, 17, 33, 64, 65, 130])
+def test_lora_rows(L, is_bf16, form, m):
+    """Rows from one to more than a tile, their adapters mixed, in runs, all one, and none at all; three segments."""
+    rng = np.random.default_rng(m)
+    k, adapters = 320, 6
+    x = rng.standard_normal((m, k), dtype=F)
+    ids = ids_of(rng, m, adapters, form)
+    segs = [Adapters(rng, m, k, n, rank, adapters, is_bf16, False) for n, rank in ((192, 16), (64, 8), (40, 32))]
+    keep = run_lora(L, x, k, k, ids, adapters, segs, is_bf16)
+    quiet(L)
+    for s in segs:
+        s.check(x, ids)
+    del keep
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("k,n,rank", [(8, 1, 1), (257, 33, 3), (1000, 130, 12), (64, 16, 4), (96, 50, 256), (2048, 257, 64),
+                                      (4096, 48, 100), (40, 4000, 24)])
+@pytest.mark.parametrize("m", [3, 90])
+def test_lora_sizes(L, is_bf16, k, n, rank, m):
+    """Odd sizes, ranks to the largest, strided rows and outputs, no scale array."""
+    rng = np.random.default_rng(k + n)
+    ldx, adapters = k + 5, 3
+    wide = rng.standard_normal((m, ldx), dtype=F)
+    ids = ids_of(rng, m, adapters, "each")
+    s = Adapters(rng, m, k, n, rank, adapters, is_bf16, False, ldc=n + 3, scaled=False)
+    keep = run_lora(L, wide, ldx, k, ids, adapters, [s], is_bf16)
+    quiet(L)
+    s.check(wide[:, :k], ids)
+    del keep
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("m", [1, 20, 200])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_lora_swiglu(L, is_bf16, m, in_place):
+    rng = np.random.default_rng(m + 1)
+    k, n, rank, adapters = 256, 352, 16, 4
+    x = rng.standard_normal((m, k), dtype=F)
+    ids = ids_of(rng, m, adapters, "runs")
+    segs = [Adapters(rng, m, k, n, rank, adapters, is_bf16, True, in_place=in_place),
+            Adapters(rng, m, k, 64, 8, adapters, is_bf16, False, in_place=in_place)]
+    keep = run_lora(L, x, k, k, ids, adapters, segs, is_bf16)
+    quiet(L)
+    for s in segs:
+        s.check(x, ids)
+    del keep
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("m", [4, 100])
+def test_lora_unaligned(L, is_bf16, m):
+    rng = np.random.default_rng(77)
+    k, adapters = 128, 3
+    x = rng.standard_normal((m, k), dtype=F)
+    ids = ids_of(rng, m, adapters, "each")
+    s = Adapters(rng, m, k, 96, 16, adapters, is_bf16, False, offset=1)
+    keep = run_lora(L, shifted(x), k, k, ids, adapters, [s], is_bf16)
+    quiet(L)
+    s.check(x, ids)
+    del keep
+
+
+@pytest.mark.parametrize("m", [6, 90])
+def test_lora_refuses_unknown_adapters(L, m):
+    """An id outside the table is never followed: its row is left, the others are done, the wait reports it."""
+    rng = np.random.default_rng(5)
+    k, adapters = 64, 2
+    x = rng.standard_normal((m, k), dtype=F)
+    for wrong in (2, -2, 2 ** 31 - 1, -2 ** 31):
+        ids = np.array([0, 1, -1] * (m // 3))
+        ids[3] = wrong
+        s = Adapters(rng, m, k, 48, 8, adapters, True, False)
+        keep = run_lora(L, x, k, k, ids, adapters, [s], True)
+        fails(L, "adapter id outside the table")
+        got = hu.host(s.c)
+        assert (got[3] == 9.0).all()
+        ids[3] = -1
+        want, bound = ru.adapters(x, ids, s.base[0], *s.pairs[0], s.scale)
+        rest = np.arange(m) != 3
+        within(got[rest], want[rest], bound[rest])
+        del keep
+
+
+def test_lora_rows_do_not_mix(L):
+    """A row of infinities (or another adapter's) does not reach its neighbours."""
+    rng = np.random.default_rng(6)
+    for m in (9, 80):
+        k, adapters = 96, 2
+        x = rng.standard_normal((m, k), dtype=F)
+        ids = np.zeros(m, int)
+        s = Adapters(rng, m, k, 32, 16, adapters, True, False)
+        bad = x.copy()
+        bad[4] = np.inf
+        keep = run_lora(L, bad, k, k, ids, adapters, [s], True)
+        quiet(L)
+        got = hu.host(s.c)
+        want, bound = ru.adapters(x, ids, s.base[0], *s.pairs[0], s.scale)
+        rest = np.arange(m) != 4
+        within(got[rest], want[rest], bound[rest])
+        del keep
+
+
+def test_lora_from_host_memory(L):
+    rng = np.random.default_rng(8)
+    m, k, n, rank, adapters = 3, 40, 24, 4, 2
+    x, base = rng.standard_normal((m, k), dtype=F), rng.standard_normal((m, n), dtype=F)
+    a, b = rng.standard_normal((adapters, rank, k), dtype=F), rng.standard_normal((adapters, n, rank), dtype=F)
+    base3, a3, b3 = base[::-1].copy(), a[::-1].copy(), b[::-1].copy()
+    scale, ids = np.array([1.5, 0.5], F), np.array([1, -1, 0], np.int32)
+    outs, segs = [np.zeros((m, n), F) for _ in range(3)], []
+    for c in outs:
+        segs.append(ru.lora_segment(False, c, n, base, a, b, scale, n, rank, base3, a3, b3))
+    L.llhip_lora_f32(lh.ptr(x), k, m, k, lh.ptr(ids), adapters, ru.array(segs), 3)
+    assert not lh.last_error(), lh.last_error()
+    want, bound = ru.swiglu(*ru.adapters(x, ids, base, a, b, scale), *ru.adapters(x, ids, base3, a3, b3, scale))
+    for c in outs:
+        within(c, want, bound + 2 * ru.U * np.abs(want))
+
+
+# ---- verification -----------------------------------------------------------------------------------------------------
+
+
+def verify_inputs(rng, rows_of, vocab, temperature, model, masked=0.0, first=0, ld=None, spread=2.0):
+    start = np.concatenate(([first], first + np.cumsum(rows_of))).astype(np.int32)
+    rows = int(start[-1])
+    logits = (spread * rng.standard_normal((rows, ld or vocab))).astype(F)
+    if masked:
+        logits[rng.random(logits.shape) < masked] = -np.inf
+        logits[:, vocab // 2] = 0.5
+    draft = (logits + 0.5 * rng.standard_normal(logits.shape)).astype(F)
+    tokens = np.zeros(rows, np.int32)
+    for i in range(rows - 1):
+        p = ru.softmax(draft[i, :vocab].astype(np.float64) / max(temperature, 0.2))
+        tokens[i + 1] = rng.choice(vocab, p=p) if temperature else int(logits[i, :vocab].argmax())
+        if temperature == 0.0 and rng.random() < 0.3:
+            tokens[i + 1] = rng.integers(vocab)
+    return start, logits, draft if model else None, tokens, rng.random((rows, 2)).astype(F)
+
+
+def run_verify(L, start, logits, draft, tokens, uniform, vocab, temperature, keep_value=-9):
+    count = len(start) - 1
+    accepted, following = (hu.dev(np.full(count, keep_value, np.int32)) for _ in range(2))
+    dev = [None if a is None else hu.dev(a) for a in (logits, draft, tokens, uniform, start)]
+    L.llhip_verify_drafts(lh.ptr(accepted), lh.ptr(following), lh.ptr(dev[0]), logits.shape[1], lh.ptr(dev[1]),
+                          0 if draft is None else draft.shape[1], lh.ptr(dev[2]), lh.ptr(dev[3]), lh.ptr(dev[4]), count,
+                          len(logits), vocab, temperature)
+    L.llhip_synchronize()
+    return list(zip(hu.host(accepted).tolist(), hu.host(following).tolist()))
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.3, 1.0, 1.7])
+@pytest.mark.parametrize("model", [False, True])
+@pytest.mark.parametrize("vocab,ld", [(1, None), (2, 3), (31, None), (1000, 1001), (5003, None), (32000, 32768)])
+def test_verify(L, temperature, model, vocab, ld):
+    """Requests of no row, one row (a plain draw) and drafts up to eight; rows before the first request."""
+    rng = np.random.default_rng(vocab)
+    inputs = verify_inputs(rng, [3, 1, 0, 9, 2, 1, 5], vocab, temperature, model, first=2, ld=ld)
+    got = run_verify(L, *inputs, vocab, temperature)
+    assert not lh.last_error(), lh.last_error()
+    start, logits, draft, tokens, uniform = inputs
+    want = ru.verify(start, logits[:, :vocab], None if draft is None else draft[:, :vocab], tokens, uniform, temperature)
+    assert got == [(-9, -9) if w is None else w for w in want]
+
+
+def test_verify_full_vocabulary(L):
+    """128256 tokens, many borders: three hundred draws and the drafts before them."""
+    rng = np.random.default_rng(1)
+    for model in (True, False):
+        inputs = verify_inputs(rng, [1] * 60 + [2, 4, 3, 5, 2], 128256, 0.9, model, spread=3.0)
+        got = run_verify(L, *inputs, 128256, 0.9)
+        assert not lh.last_error(), lh.last_error()
+        assert got == ru.verify(*inputs, 0.9)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_verify_masked_and_extreme_rows(L, temperature):
+    """Tokens masked out by -infinity or the type's lowest value, single tokens left, logits of 1e30, equal logits (the
+    lowest token wins a tie), a draft that its own model or the target gives no weight, uniforms of 0 and just below 1."""
+    rng = np.random.default_rng(2)
+    vocab = 700
+    start, logits, draft, tokens, uniform = verify_inputs(rng, [2] * 12, vocab, temperature, True, masked=0.6)
+    low = np.finfo(F).min
+    logits[0] = -np.inf
+    logits[0, 699] = -3.0
+    tokens[1] = 699
+    logits[2] = low
+    logits[2, 5] = low / 2
+    logits[4] = 1e30 * np.sign(rng.standard_normal(vocab))
+    logits[6] = 0.25
+    logits[6, :9] = 0.2
+    tokens[7] = 9
+    logits[8, tokens[9]] = -np.inf
+    draft[10, tokens[11]] = -np.inf
+    logits[10, tokens[11]] = 1.0
+    uniform[12:14] = 0.0
+    uniform[14:18] = np.float32(1.0) - np.float32(2.0 ** -24)
+    draft[18] = logits[18]
+    draft[20] = -np.inf
+    draft[20, tokens[21]] = 0.0
+    got = run_verify(L, start, logits, draft, tokens, uniform, vocab, temperature)
+    assert not lh.last_error(), lh.last_error()
+    assert got == ru.verify(start, logits, draft, tokens, uniform, temperature)
+    one_hot = run_verify(L, start, logits, None, tokens, uniform, vocab, temperature)
+    assert one_hot == ru.verify(start, logits, None, tokens, uniform, temperature)
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_verify_refuses_rows_that_decide_nothing(L, temperature):
+    """NaN, +infinity or nothing left in a row that decides: -1 and a failure at the wait; behind the row that stopped
+    the request they do not matter. A draft or rows outside: likewise."""
+    rng = np.random.default_rng(3)
+    vocab = 300
+
+    def inputs():
+        start, logits, draft, tokens, uniform = verify_inputs(rng, [2, 2, 1], vocab, temperature, True)
+        tokens[1] = int(logits[0].argmax())
+        uniform[0, 0] = 0.0  # accepted
+        return start, logits, draft, tokens, uniform
+
+    for value in (np.nan, np.inf):
+        for row in (0, 1):
+            start, logits, draft, tokens, uniform = inputs()
+            logits[row, 17] = value
+            got = run_verify(L, start, logits, draft, tokens, uniform, vocab, temperature)
+            fails(L, "leave no token")
+            logits[row] = 0.0
+            want = ru.verify(start, logits, draft, tokens, uniform, temperature)
+            assert got == [(-1, -1)] + want[1:]
+    start, logits, draft, tokens, uniform = inputs()
+    logits[0] = -np.inf
+    assert run_verify(L, start, logits, draft, tokens, uniform, vocab, temperature)[0] == (-1, -1)
+    fails(L, "leave no token")
+    start, logits, draft, tokens, uniform = inputs()
+    logits[0] = -np.inf
+    logits[0, 3], tokens[1] = 0.0, 4  # refused for certain: row 1 is not reached
+    logits[1] = np.nan
+    draft[0] = 0.0
+    got = run_verify(L, start, logits, draft, tokens, uniform, vocab, temperature)
+    assert got[0] == (0, 3) and not lh.last_error()
+    for wrong in (-1, vocab, 2 ** 31 - 1):
+        start, logits, draft, tokens, uniform = inputs()
+        tokens[1] = wrong
+        got = run_verify(L, start, logits, draft, tokens, uniform, vocab, temperature)
+        fails(L, "outside the vocabulary")
+        tokens[1] = 0
+        assert got == [(-1, -1)] + ru.verify(start, logits, draft, tokens, uniform, temperature)[1:]
+    start, logits, draft, tokens, uniform = inputs()
+    got = run_verify(L, np.array([0, 2, 6], np.int32), logits, draft, tokens, uniform, vocab, temperature)
+    fails(L, "outside the batch's buffers")
+    assert got[1] == (-9, -9) and got[0] == ru.verify(start[:2], logits, draft, tokens, uniform, temperature)[0]
+
+
+def test_verify_emits_the_targets_distribution(L):
+    """20000 requests' worth of draws over six tokens: the emitted first tokens' frequencies are the target's within five
+    standard deviations, whatever the draft's distribution."""
+    rng = np.random.default_rng(9)
+    vocab, count, t = 6, 1000, 1.0
+    target, other = np.array([0.1, 1.0, -0.5, 0.7, -2.0, 0.3], F), np.array([1.0, -1.0, 0.5, 0.0, 0.5, -0.7], F)
+    p, q = ru.softmax(target.astype(np.float64)), ru.softmax(other.astype(np.float64))
+    seen = np.zeros(vocab)
+    start = np.arange(0, 2 * count + 1, 2).astype(np.int32)
+    logits, draft = np.tile(target, (2 * count, 1)), np.tile(other, (2 * count, 1))
+    for _ in range(20):
+        tokens = np.zeros(2 * count, np.int32)
+        tokens[1::2] = rng.choice(vocab, count, p=q)
+        got = run_verify(L, start, logits, draft, tokens, rng.random((2 * count, 2)).astype(F), vocab, t)
+        first = [tokens[2 * i + 1] if a else n for i, (a, n) in enumerate(got)]
+        seen += np.bincount(first, minlength=vocab)
+    n = 20 * count
+    assert (np.abs(seen - n * p) < 5 * np.sqrt(n * p * (1 - p))).all(), (seen / n, p)
+
+
+# ---- captured calls ---------------------------------------------------------------------------------------------------
+
+
+def test_captured_calls_follow_their_arrays(L):
+    """All four captured in one graph and replayed while the arrays, lengths and logits change, with eager work between the
+    replays; every replay equals the eager calls."""
+    T = hu.torch()
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(21)
+    heads, kv, hd, vocab, k = 8, 2, 64, 4000, 512
+    b = ru.Batch(hu.dev, [1, 3, 1], [5, 0, 60], prefix=100, prefix_seq_len=100, seq_len=80, slot=[2, 0, 1], slots=3)
+    q, kn, vn = (rng.standard_normal((b.rows, n * hd), dtype=F) for n in (heads, kv, kv))
+    table = rng.standard_normal((180, 2 * hd), dtype=F)
+    pk, pv = (rng.standard_normal((kv, 100, hd), dtype=F) for _ in range(2))
+    kc, vc = (rng.standard_normal((3, kv, 80, hd), dtype=F) for _ in range(2))
+    dev = {n: hu.dev(a) for n, a in (("q", q), ("k", kn), ("v", vn), ("t", table), ("pk", pk), ("pv", pv))}
+    cache = [hu.dev(kc), hu.dev(vc)]
+    rot, out = hu.dev(np.zeros_like(q)), hu.dev(np.zeros_like(q))
+    lora = Adapters(rng, b.rows, k, 96, 16, 4, True, False)
+    x, ids = hu.dev(rng.standard_normal((b.rows, k), dtype=F)), hu.dev(np.array([0, 1, 1, 3, -1], np.int32))
+    seg = ru.array([lora.struct])
+    start, logits, draft, tokens, uniform = verify_inputs(rng, [1, 3, 1], vocab, 0.7, True)
+    vdev = [hu.dev(a) for a in (logits, draft, tokens, uniform)]
+    acc, nxt = hu.dev(np.zeros(3, np.int32)), hu.dev(np.zeros(3, np.int32))
+
+    def calls():
+        L.llhip_rope_kv_store_requests(lh.ptr(rot), lh.ptr(dev["q"]), heads * hd, lh.ptr(dev["k"]), lh.ptr(dev["v"]),
+                                       kv * hd, lh.ptr(dev["t"]), b.struct, heads, kv, hd, lh.ptr(cache[0]),
+                                       lh.ptr(cache[1]))
+        L.llhip_attention_requests(lh.ptr(out), lh.ptr(rot), lh.ptr(dev["pk"]), lh.ptr(dev["pv"]), lh.ptr(cache[0]),
+                                   lh.ptr(cache[1]), b.struct, heads, kv, hd)
+        L.llhip_lora_bf16(lh.ptr(x), k, b.rows, k, lh.ptr(ids), 4, seg, 1)
+        L.llhip_verify_drafts(lh.ptr(acc), lh.ptr(nxt), lh.ptr(vdev[0]), vocab, lh.ptr(vdev[1]), vocab, lh.ptr(vdev[2]),
+                              lh.ptr(vdev[3]), lh.ptr(b.keep[0]), 3, b.rows, vocab, 0.7)
+
+    def results():
+        return [hu.host(a).copy() for a in (rot, out, lora.c, acc, nxt, cache[0], cache[1])]
+
+    calls()  # workspaces grow outside of the capture
+    quiet(L)
+    assert L.llhip_graph_begin() == 0, lh.last_error()
+    calls()
+    graph = L.llhip_graph_end()
+    assert graph, lh.last_error()
+    for step, length in enumerate(([6, 3, 61], [70, 10, 0], [1, 77, 79])):
+        b.keep[1].copy_(T.from_numpy(np.asarray(length, np.int32)))
+        ids.copy_(T.from_numpy(np.roll(np.array([0, 1, 1, 3, -1], np.int32), step)))
+        vdev[3].copy_(T.from_numpy(rng.random((b.rows, 2)).astype(F)))
+        T.cuda.synchronize()
+        calls()
+        quiet(L)
+        want = results()
+        for a in (rot, out, lora.c, acc, nxt):
+            a.zero_()
+        T.cuda.synchronize()
+        assert L.llhip_graph_launch(graph) == 0
+        quiet(L)
+        for g, w in zip(results(), want):
+            assert np.array_equal(g, w)
+    L.llhip_graph_destroy(graph)
