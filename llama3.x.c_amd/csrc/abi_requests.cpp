@@ -60,6 +60,42 @@ size_t caches_bytes(const RequestBatch *b, int n_kv_heads, int head_dim) {
   return (size_t)b->slots * b->seq_len * n_kv_heads * head_dim * kFloat;
 }
 
+// The scratch of these calls, which the library stream orders: grown on demand (never during graph capture), kept for the
+// process. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows.
+void *scratch_memory = nullptr;
+size_t scratch_bytes = 0;
+bool scratch_captured = false;
+
+bool workspace(const char *name, size_t bytes, void **out) {
+  Device &dev = device();
+  if (bytes > scratch_bytes) {
+    if (dev.capturing)
+      return raise("%s needs %zu bytes of workspace during graph capture; run the call once before capturing", name, bytes);
+    if (scratch_memory && !scratch_captured) {
+      (void)hipStreamSynchronize(dev.stream);
+      (void)hipFree(scratch_memory);
+      hbm_release(scratch_bytes);
+    }
+    scratch_memory = nullptr;
+    scratch_bytes = 0;
+    scratch_captured = false;
+    const size_t want = bytes + bytes / 4 + 4096;
+    if (!hbm_claim(want, "the request workspace"))
+      return false;
+    if (hipMalloc(&scratch_memory, want) != hipSuccess) {
+      (void)hipGetLastError();
+      hbm_release(want);
+      scratch_memory = nullptr;
+      return raise("%s: allocating %zu bytes of workspace failed", name, want);
+    }
+    scratch_bytes = want;
+  }
+  if (dev.capturing)
+    scratch_captured = true;
+  *out = scratch_memory;
+  return true;
+}
+
 // One adapter call, F32 or BF16: the segment types differ in their adapters' element only.
 template <class Segment>
 void lora(const char *name, const float *x, int ldx, int m, int k, const int *adapter, int adapters,
@@ -268,7 +304,10 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
                            batch->prefix ? call.ptr<const float>(PV) : nullptr, call.ptr<const float>(K),
                            call.ptr<const float>(V), batch_dev(call, refs, batch, n_kv_heads, head_dim), n_heads,
                            n_kv_heads, head_dim};
-  if (launch_attention_requests(job, call.stream()))
+  void *scratch = nullptr;
+  if (!workspace(name, attention_requests_workspace(job), &scratch))
+    return;
+  if (launch_attention_requests(job, scratch, call.stream()))
     call.finish();
 }
 

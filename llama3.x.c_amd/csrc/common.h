@@ -286,7 +286,8 @@ struct AttentionRequestsJob {
   RequestsDev batch;
   int n_heads, n_kv_heads, head_dim;
 };
-bool launch_attention_requests(const AttentionRequestsJob &job, hipStream_t stream);
+size_t attention_requests_workspace(const AttentionRequestsJob &job); // bytes of scratch the launch takes
+bool launch_attention_requests(const AttentionRequestsJob &job, void *workspace, hipStream_t stream);
 
 struct LoraSegmentDev {
   float *c;

@@ -1,41 +1,16 @@
-// Many requests on one model (gfx950): RoPE and cache rows at each request's own position, and attention behind a
-// prefix that all requests share.
+// Many requests on one model (gfx950): RoPE and cache rows at each request's own position.
 //
 //   rope_requests   one thread per V dimensions of a row's two q heads or of one KV head.
-//   attn_rows       attention of one row and one KV head per block, any shape: the positions walked in chunks of 64 with
-//                   the running maximum and sum of the softmax.
-#include <cfloat>
-
-#include "common.h"
-#include "lanes.h"
+#include "requests_device.h"
 
 namespace llhip {
 namespace {
 
-constexpr int kWave = 64;
 constexpr int kThreads = 256;
-constexpr int kChunk = 64;
-constexpr int kMaxGroup = 16;
-constexpr int kMaxHeadDim = 256;
-constexpr int kMaxRequests = 1024;
 
 bool launch_ok(const char *what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess || raise("launching %s failed: %s", what, hipGetErrorString(e));
-}
-
-// Request r's rows, own length and slot; no rows (and bad set) where they leave the batch's buffers. A request without
-// rows may hold anything else.
-struct Request {
-  int first, rows, length, slot;
-};
-__device__ __forceinline__ Request request_at(const RequestsDev &b, int r, bool &bad) {
-  const int first = b.start[r], last = b.start[r + 1], length = b.length[r], slot = b.slot ? b.slot[r] : r;
-  const bool rows_ok = first >= 0 && first <= last && last <= b.rows;
-  const int n = rows_ok ? last - first : 0;
-  const bool ok = rows_ok && (n == 0 || (length >= 0 && length <= b.seq_len - n && slot >= 0 && slot < b.slots));
-  bad |= !ok;
-  return Request{first, ok ? n : 0, length, slot};
 }
 
 // ---- RoPE and cache rows ----------------------------------------------------------------------------------------------
@@ -145,141 +120,6 @@ template <int V> __global__ __launch_bounds__(kThreads) void rope_requests(RopeR
   }
 }
 
-// ---- attention --------------------------------------------------------------------------------------------------------
-
-struct RequestAttn {
-  float *out;
-  const float *q, *prefix_key, *prefix_value, *key, *value;
-  RequestsDev batch;
-  int n_heads, n_kv_heads, head_dim;
-  float divisor; // sqrtf(head_dim)
-  int *flags;
-};
-
-// Any shape: block (row, KV head), the positions (prefix, then own) in chunks of 64. Wave w scores positions w, w + 4,
-// ..: lane l holds dimensions l, l + 64, .. of the K row and of the group's query vectors, the wave's sum is the dot. Per
-// chunk and head the maximum, the exponentials and their sum join the running ones, and thread (share, dimension) rescales
-// its value sums by exp(m_old - m_new) and adds its share of the chunk's positions; the shares meet in LDS at the end.
-__global__ __launch_bounds__(kThreads) void attn_rows(RequestAttn p, int row0) {
-  __shared__ float score[kMaxGroup][kChunk];
-  __shared__ float run_max[kMaxGroup], run_sum[kMaxGroup], rescale[kMaxGroup];
-  __shared__ float acc[kThreads * kMaxGroup]; // [share][head][head_dim], shares * head_dim <= 256
-  __shared__ int mine[3];
-  const int g = blockIdx.x % p.n_kv_heads, row = row0 + blockIdx.x / p.n_kv_heads;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  if (tid == 0)
-    mine[0] = -1;
-  __syncthreads();
-  bool bad_batch = false, bad = false;
-  for (int r = tid; r < p.batch.count; r += kThreads) {
-    const Request q = request_at(p.batch, r, bad_batch);
-    if (row >= q.first && row < q.first + q.rows) {
-      mine[0] = r;
-      mine[1] = q.length + row - q.first;
-      mine[2] = q.slot;
-    }
-  }
-  if (bad_batch && blockIdx.x == 0 && row0 == 0)
-    p.flags[3] = 1;
-  __syncthreads();
-  if (mine[0] < 0)
-    return; // the row belongs to no request
-  const int positions = p.batch.prefix + mine[1] + 1, slot = mine[2];
-  const int kv_mul = p.n_heads / p.n_kv_heads, hd = p.head_dim;
-  const float *qrow = p.q + ((size_t)row * p.n_heads + (size_t)g * kv_mul) * hd;
-  constexpr int kDims = kMaxHeadDim / kWave;
-  float qv[kMaxGroup][kDims];
-#pragma unroll
-  for (int h = 0; h < kMaxGroup; h++)
-#pragma unroll
-    for (int e = 0; e < kDims; e++) {
-      const int d = lane + e * kWave;
-      qv[h][e] = h < kv_mul && d < hd ? qrow[(size_t)h * hd + d] : 0.0f;
-    }
-  if (tid < kv_mul)
-    run_max[tid] = -FLT_MAX, run_sum[tid] = 0.0f;
-  const size_t own = (size_t)slot * p.batch.slot_floats + (size_t)g * p.batch.head_base;
-  const size_t far = (size_t)g * p.batch.prefix_head_base;
-  auto row_at = [&](const float *prefix, const float *cache, int t) {
-    return t < p.batch.prefix ? prefix + far + (size_t)t * p.batch.prefix_pos_stride
-                              : cache + own + (size_t)(t - p.batch.prefix) * p.batch.pos_stride;
-  };
-  const int shares = kThreads / hd, share = tid / hd, d = tid % hd;
-  float o[kMaxGroup];
-#pragma unroll
-  for (int h = 0; h < kMaxGroup; h++)
-    o[h] = 0.0f;
-  for (int t0 = 0; t0 < positions; t0 += kChunk) {
-    const int n = min(kChunk, positions - t0);
-    for (int t = wave; t < n; t += kThreads / kWave) {
-      const float *krow = row_at(p.prefix_key, p.key, t0 + t);
-      float kd[kDims];
-#pragma unroll
-      for (int e = 0; e < kDims; e++) {
-        const int dd = lane + e * kWave;
-        kd[e] = dd < hd ? krow[dd] : 0.0f;
-      }
-#pragma unroll
-      for (int h = 0; h < kMaxGroup; h++)
-        if (h < kv_mul) {
-          float dot = 0.0f;
-#pragma unroll
-          for (int e = 0; e < kDims; e++)
-            dot = fmaf(qv[h][e], kd[e], dot);
-          const float s = wave_sum(dot) / p.divisor;
-          bad |= !isfinite(s);
-          if (lane == 0)
-            score[h][t] = s;
-        }
-    }
-    __syncthreads();
-    for (int h = wave; h < kv_mul; h += kThreads / kWave) {
-      const float s = lane < n ? score[h][lane] : -FLT_MAX;
-      const float m_old = run_max[h], m = fmaxf(m_old, wave_max(s));
-      const float e = lane < n ? expf(s - m) : 0.0f;
-      score[h][lane] = e;
-      const float l = wave_sum(e);
-      if (lane == 0) {
-        const float alpha = expf(m_old - m);
-        rescale[h] = alpha;
-        run_max[h] = m;
-        run_sum[h] = run_sum[h] * alpha + l;
-      }
-    }
-    __syncthreads();
-    if (share < shares) {
-#pragma unroll
-      for (int h = 0; h < kMaxGroup; h++)
-        if (h < kv_mul)
-          o[h] *= rescale[h];
-      for (int t = share; t < n; t += shares) {
-        const float v = row_at(p.prefix_value, p.value, t0 + t)[d];
-#pragma unroll
-        for (int h = 0; h < kMaxGroup; h++)
-          if (h < kv_mul)
-            o[h] = fmaf(score[h][t], v, o[h]);
-      }
-    }
-    __syncthreads(); // the next chunk's scores overwrite this one's
-  }
-  if (bad && lane == 0)
-    p.flags[1] = 1;
-  if (share < shares) {
-#pragma unroll
-    for (int h = 0; h < kMaxGroup; h++)
-      if (h < kv_mul)
-        acc[((size_t)share * kv_mul + h) * hd + d] = o[h];
-  }
-  __syncthreads();
-  float *dst = p.out + ((size_t)row * p.n_heads + (size_t)g * kv_mul) * hd;
-  for (int i = tid; i < kv_mul * hd; i += kThreads) {
-    float total = 0.0f;
-    for (int s2 = 0; s2 < shares; s2++)
-      total += acc[(size_t)s2 * kv_mul * hd + i];
-    dst[i] = total / run_sum[i / hd];
-  }
-}
-
 } // namespace
 
 bool launch_rope_requests(const RopeRequestsJob &job, hipStream_t stream) {
@@ -295,30 +135,6 @@ bool launch_rope_requests(const RopeRequestsJob &job, hipStream_t stream) {
   const auto kernel = vec4 ? rope_requests<4> : rope_requests<2>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, job, device().error_flags);
   return launch_ok("rope_requests");
-}
-
-bool launch_attention_requests(const AttentionRequestsJob &job, hipStream_t stream) {
-  RequestAttn p{};
-  p.out = job.out;
-  p.q = job.q;
-  p.prefix_key = job.prefix_key;
-  p.prefix_value = job.prefix_value;
-  p.key = job.key;
-  p.value = job.value;
-  p.batch = job.batch;
-  p.n_heads = job.n_heads;
-  p.n_kv_heads = job.n_kv_heads;
-  p.head_dim = job.head_dim;
-  p.divisor = sqrtf((float)job.head_dim);
-  p.flags = device().error_flags;
-  const int most = (1 << 23) / job.n_kv_heads; // rows of a launch, which holds fewer than 2^32 threads
-  for (int row0 = 0; row0 < job.batch.rows; row0 += most) {
-    const int n = job.batch.rows - row0 < most ? job.batch.rows - row0 : most;
-    hipLaunchKernelGGL(attn_rows, dim3((unsigned)n * (unsigned)job.n_kv_heads), dim3(kThreads), 0, stream, p, row0);
-    if (job.batch.rows - row0 <= most)
-      break;
-  }
-  return launch_ok("attn_rows");
 }
 
 } // namespace llhip

@@ -1,0 +1,1110 @@
+// Attention of many requests behind a prefix that all of them share (gfx950).
+#include <cfloat>
+
+#include "requests_device.h"
+
+#include "lanes.h"
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+
+namespace llhip {
+namespace {
+
+constexpr int kWave = 64;
+constexpr int kThreads = 256;
+constexpr int kChunk = 64;
+constexpr int kMaxGroup = 16;
+constexpr int kMaxHeadDim = 256;
+
+bool launch_ok(const char *what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess || raise("launching %s failed: %s", what, hipGetErrorString(e));
+}
+
+struct RequestAttn {
+  float *out;
+  const float *q, *prefix_key, *prefix_value, *key, *value;
+  RequestsDev batch;
+  int n_heads, n_kv_heads, head_dim;
+  float divisor; // sqrtf(head_dim)
+  int *flags;
+};
+
+// Any shape: block (row, KV head), the positions (prefix, then own) in chunks of 64. Wave w scores positions w, w + 4,
+// ..: lane l holds dimensions l, l + 64, .. of the K row and of the group's query vectors, the wave's sum is the dot. Per
+// chunk and head the maximum, the exponentials and their sum join the running ones, and thread (share, dimension) rescales
+// its value sums by exp(m_old - m_new) and adds its share of the chunk's positions; the shares meet in LDS at the end.
+__global__ __launch_bounds__(kThreads) void attn_rows(RequestAttn p, int row0) {
+  __shared__ float score[kMaxGroup][kChunk];
+  __shared__ float run_max[kMaxGroup], run_sum[kMaxGroup], rescale[kMaxGroup];
+  __shared__ float acc[kThreads * kMaxGroup]; // [share][head][head_dim], shares * head_dim <= 256
+  __shared__ int mine[3];
+  const int g = blockIdx.x % p.n_kv_heads, row = row0 + blockIdx.x / p.n_kv_heads;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  if (tid == 0)
+    mine[0] = -1;
+  __syncthreads();
+  bool bad_batch = false, bad = false;
+  for (int r = tid; r < p.batch.count; r += kThreads) {
+    const Request q = request_at(p.batch, r, bad_batch);
+    if (row >= q.first && row < q.first + q.rows) {
+      mine[0] = r;
+      mine[1] = q.length + row - q.first;
+      mine[2] = q.slot;
+    }
+  }
+  if (bad_batch && blockIdx.x == 0 && row0 == 0)
+    p.flags[3] = 1;
+  __syncthreads();
+  if (mine[0] < 0)
+    return; // the row belongs to no request
+  const int positions = p.batch.prefix + mine[1] + 1, slot = mine[2];
+  const int kv_mul = p.n_heads / p.n_kv_heads, hd = p.head_dim;
+  const float *qrow = p.q + ((size_t)row * p.n_heads + (size_t)g * kv_mul) * hd;
+  constexpr int kDims = kMaxHeadDim / kWave;
+  float qv[kMaxGroup][kDims];
+#pragma unroll
+  for (int h = 0; h < kMaxGroup; h++)
+#pragma unroll
+    for (int e = 0; e < kDims; e++) {
+      const int d = lane + e * kWave;
+      qv[h][e] = h < kv_mul && d < hd ? qrow[(size_t)h * hd + d] : 0.0f;
+    }
+  if (tid < kv_mul)
+    run_max[tid] = -FLT_MAX, run_sum[tid] = 0.0f;
+  const size_t own = (size_t)slot * p.batch.slot_floats + (size_t)g * p.batch.head_base;
+  const size_t far = (size_t)g * p.batch.prefix_head_base;
+  auto row_at = [&](const float *prefix, const float *cache, int t) {
+    return t < p.batch.prefix ? prefix + far + (size_t)t * p.batch.prefix_pos_stride
+                              : cache + own + (size_t)(t - p.batch.prefix) * p.batch.pos_stride;
+  };
+  const int shares = kThreads / hd, share = tid / hd, d = tid % hd;
+  float o[kMaxGroup];
+#pragma unroll
+  for (int h = 0; h < kMaxGroup; h++)
+    o[h] = 0.0f;
+  for (int t0 = 0; t0 < positions; t0 += kChunk) {
+    const int n = min(kChunk, positions - t0);
+    for (int t = wave; t < n; t += kThreads / kWave) {
+      const float *krow = row_at(p.prefix_key, p.key, t0 + t);
+      float kd[kDims];
+#pragma unroll
+      for (int e = 0; e < kDims; e++) {
+        const int dd = lane + e * kWave;
+        kd[e] = dd < hd ? krow[dd] : 0.0f;
+      }
+#pragma unroll
+      for (int h = 0; h < kMaxGroup; h++)
+        if (h < kv_mul) {
+          float dot = 0.0f;
+#pragma unroll
+          for (int e = 0; e < kDims; e++)
+            dot = fmaf(qv[h][e], kd[e], dot);
+          const float s = wave_sum(dot) / p.divisor;
+          bad |= !isfinite(s);
+          if (lane == 0)
+            score[h][t] = s;
+        }
+    }
+    __syncthreads();
+    for (int h = wave; h < kv_mul; h += kThreads / kWave) {
+      const float s = lane < n ? score[h][lane] : -FLT_MAX;
+      const float m_old = run_max[h], m = fmaxf(m_old, wave_max(s));
+      const float e = lane < n ? expf(s - m) : 0.0f;
+      score[h][lane] = e;
+      const float l = wave_sum(e);
+      if (lane == 0) {
+        const float alpha = expf(m_old - m);
+        rescale[h] = alpha;
+        run_max[h] = m;
+        run_sum[h] = run_sum[h] * alpha + l;
+      }
+    }
+    __syncthreads();
+    if (share < shares) {
+#pragma unroll
+      for (int h = 0; h < kMaxGroup; h++)
+        if (h < kv_mul)
+          o[h] *= rescale[h];
+      for (int t = share; t < n; t += shares) {
+        const float v = row_at(p.prefix_value, p.value, t0 + t)[d];
+#pragma unroll
+        for (int h = 0; h < kMaxGroup; h++)
+          if (h < kv_mul)
+            o[h] = fmaf(score[h][t], v, o[h]);
+      }
+    }
+    __syncthreads(); // the next chunk's scores overwrite this one's
+  }
+  if (bad && lane == 0)
+    p.flags[1] = 1;
+  if (share < shares) {
+#pragma unroll
+    for (int h = 0; h < kMaxGroup; h++)
+      if (h < kv_mul)
+        acc[((size_t)share * kv_mul + h) * hd + d] = o[h];
+  }
+  __syncthreads();
+  float *dst = p.out + ((size_t)row * p.n_heads + (size_t)g * kv_mul) * hd;
+  for (int i = tid; i < kv_mul * hd; i += kThreads) {
+    float total = 0.0f;
+    for (int s2 = 0; s2 < shares; s2++)
+      total += acc[(size_t)s2 * kv_mul * hd + i];
+    dst[i] = total / run_sum[i / hd];
+  }
+}
+
+// ---- the matrix-core form ---------------------------------------------------------------------------------------------
+
+constexpr int kUnit = 32;        // positions of a step
+constexpr int kTileVectors = 128; // query vectors of a wide tile
+constexpr int kNarrowVectors = 32; // at most, of a narrow one
+constexpr int kTargetItems = 1024; // work items aimed at: two for each block that the chip holds
+constexpr int kMinUnits = 4;     // a step for each wave of a narrow block
+constexpr int kMaxShares = 32;   // of one walk
+
+struct FastAttn {
+  float *out;
+  const float *q, *prefix_key, *prefix_value, *key, *value;
+  RequestsDev batch;
+  int n_heads, n_kv_heads, kv_mul, hd;
+  int tile_rows;    // rows of a wide tile
+  int prefix_tiles; // tiles of all rows over the prefix (1 when narrow)
+  bool prefix_narrow;
+  float scale2; // log2(e) / sqrtf(hd)
+  float *partial;
+  int2 *row_slots; // per row: first own slot, own shares (-1: the row belongs to no request)
+  int *header;     // [0] shares of the prefix
+  int *flags;
+};
+
+// What every block works out for itself from the batch's arrays: the walks (a tile of query vectors over a range of
+// positions), each cut into shares of about equal length so that all of them are about kTargetItems work items.
+struct Plan {
+  int first[kMaxRequests], rows[kMaxRequests], length[kMaxRequests], slot[kMaxRequests];
+  int shares[kMaxRequests];
+  int items[kMaxRequests]; // running sum, the request's own included
+  int slots[kMaxRequests]; // likewise
+  long long units;
+  int longest, prefix_shares, bad;
+  int wave_items[kThreads / kWave], wave_slots[kThreads / kWave];
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Tiles of a request's own walk: one narrow tile, or wide ones.
+__device__ __forceinline__ int own_tiles(const FastAttn &p, int rows) {
+  return rows * p.kv_mul <= kNarrowVectors ? 1 : ceil_div(rows, p.tile_rows);
+}
+
+__device__ void make_plan(const FastAttn &p, Plan &plan) {
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int per = ceil_div(p.batch.count, kThreads), r0 = tid * per;
+  if (tid == 0)
+    plan.units = 0, plan.longest = 0, plan.bad = 0;
+  __syncthreads();
+  long long units = 0;
+  int longest = 0;
+  bool bad = false;
+  for (int r = r0; r < min(r0 + per, p.batch.count); r++) {
+    const Request q = request_at(p.batch, r, bad);
+    plan.first[r] = q.first;
+    plan.rows[r] = q.rows;
+    plan.length[r] = q.length;
+    plan.slot[r] = q.slot;
+    if (q.rows) {
+      const int u = ceil_div(q.length + q.rows, kUnit);
+      units += (long long)own_tiles(p, q.rows) * u;
+      longest = max(longest, u);
+    }
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    units += __shfl_xor(units, o);
+    longest = max(longest, __shfl_xor(longest, o));
+  }
+  if (lane == 0) {
+    atomicAdd((unsigned long long *)&plan.units, (unsigned long long)units);
+    atomicMax(&plan.longest, longest);
+  }
+  if (bad)
+    plan.bad = 1;
+  __syncthreads();
+  const int prefix_units = ceil_div(p.batch.prefix, kUnit);
+  const long long total = (plan.units + (long long)p.prefix_tiles * prefix_units) * p.n_kv_heads;
+  const int aim = (int)((total + kTargetItems - 1) / kTargetItems);
+  const int step = max(max(kMinUnits, aim), ceil_div(max(plan.longest, prefix_units), kMaxShares));
+  int items = 0, slots = 0;
+  for (int r = r0; r < min(r0 + per, p.batch.count); r++) {
+    const int n = plan.rows[r], u = ceil_div(plan.length[r] + n, kUnit);
+    const int shares = n ? ceil_div(u, step) : 0;
+    plan.shares[r] = shares;
+    items += n ? own_tiles(p, n) * shares * p.n_kv_heads : 0;
+    slots += n * p.n_heads * shares;
+    plan.items[r] = items;
+    plan.slots[r] = slots;
+  }
+  // the sums of the threads before this one
+  int item_run = items, slot_run = slots;
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int a = __shfl_up(item_run, o), b = __shfl_up(slot_run, o);
+    if (lane >= o)
+      item_run += a, slot_run += b;
+  }
+  if (lane == kWave - 1)
+    plan.wave_items[wave] = item_run, plan.wave_slots[wave] = slot_run;
+  __syncthreads();
+  item_run -= items, slot_run -= slots;
+  for (int w = 0; w < wave; w++)
+    item_run += plan.wave_items[w], slot_run += plan.wave_slots[w];
+  for (int r = r0; r < min(r0 + per, p.batch.count); r++)
+    plan.items[r] += item_run, plan.slots[r] += slot_run;
+  if (tid == 0)
+    plan.prefix_shares = ceil_div(prefix_units, step);
+  __syncthreads();
+}
+
+// One block's work: query vectors (row row0 + v / kv_mul, head g * kv_mul + v % kv_mul for v < vectors) over positions
+// t0 .. t1 - 1 of one cache; row row0 + j sees positions up to last0 + j (the prefix: all).
+struct Item {
+  const float *key, *value;
+  size_t pos_stride;
+  int row0, vectors, g;
+  int t0, t1;
+  int last0; // INT_MAX: every position is seen by every row
+  size_t slot0;
+  int slot_step; // floats' slots between vectors: a vector's slot is slot0 + (row * n_heads + head) * slot_step
+};
+
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// A value that is infinite or no number must reach exactly the rows that see its position, and 0 * infinity would carry it
+// to those that do not. So the products take 0 in the place of such values, and this adds them, weight by weight: rare,
+// and as slow as it is. pv: the lane's weights of the step's 32 positions (16 t + 4 (lane / 16) + e in pv[4 t + e]), live
+// the bits of those its vector sees, dim(d, e) the dimension of o[d][e]; weights: the wave's 32 x 16 floats of LDS.
+template <int D, class Dim>
+__device__ __forceinline__ void add_nonfinite(v4f (&o)[D], const float (&pv)[8], unsigned live, const Item &it, int t0,
+                                              int hd, int lane, float *weights, Dim dim) {
+  const int lq = lane >> 4, lc = lane & 15;
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    weights[(16 * (i / 4) + 4 * lq + i % 4) * 16 + lc] = (live >> i) & 1 ? pv[i] : -1.0f;
+  __builtin_amdgcn_wave_barrier(); // the wave's own LDS writes and reads stay in order
+#pragma unroll 1
+  for (int t = t0; t < min(t0 + kUnit, it.t1); t++) {
+    const float w = weights[(t - t0) * 16 + lc];
+    const float *row = it.value + (size_t)t * it.pos_stride;
+#pragma unroll
+    for (int d = 0; d < D; d++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int at = dim(d, e);
+        const float v = at < hd ? row[at] : 0.0f;
+        if (w >= 0.0f && !finite(v))
+          o[d][e] += w * v;
+      }
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+// x = h + m + l exactly, each part 8 significant bits: the parts of eight values as three BF16 operands.
+__device__ __forceinline__ void bf16_parts(const float (&v)[8], v4i &ph, v4i &pm, v4i &pl) {
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    unsigned u[2][3];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const float x = v[2 * w + k];
+      u[k][0] = __float_as_uint(x);
+      const float r1 = x - __uint_as_float(u[k][0] & 0xFFFF0000u);
+      u[k][1] = __float_as_uint(r1);
+      u[k][2] = __float_as_uint(r1 - __uint_as_float(u[k][1] & 0xFFFF0000u));
+    }
+    ph[w] = (int)__builtin_amdgcn_perm(u[1][0], u[0][0], 0x07060302u);
+    pm[w] = (int)__builtin_amdgcn_perm(u[1][1], u[0][1], 0x07060302u);
+    pl[w] = (int)__builtin_amdgcn_perm(u[1][2], u[0][2], 0x07060302u);
+  }
+}
+
+__device__ __forceinline__ v4f mfma_bf16(const v4i &a, const v4i &b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma_f16(const v4i &a, const v4i &b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// x * scale = h + l to 22 bits and more, two FP16 parts, for |x * scale| <= 2^15: two values a dword.
+__device__ __forceinline__ void f16_pair(float a, float b, float scale, int &h, int &l) {
+  const v2f x = {a * scale, b * scale};
+  const v2h hi = __builtin_convertvector(x, v2h);
+  const v2f rest = {__builtin_fmaf(a, scale, -(float)hi[0]), __builtin_fmaf(b, scale, -(float)hi[1])};
+  h = __builtin_bit_cast(int, hi);
+  l = __builtin_bit_cast(int, __builtin_convertvector(rest, v2h));
+}
+
+// The power of two that brings values up to `top` to at most 2^15 (top in [2^e, 2^(e+1)): 2^(14 - e)), and e, which is at
+// least `least`; top must be finite.
+__device__ __forceinline__ float f16_scale(float top, int least, int &e) {
+  e = max((int)(__float_as_uint(top) >> 23) - 127, least);
+  return __uint_as_float((unsigned)(127 + 14 - e) << 23);
+}
+
+__device__ __forceinline__ float4 load4(const float *row, int d, int hd) {
+  return d < hd ? *reinterpret_cast<const float4 *>(row + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// Narrow: at most 16 vectors a wave. The four waves walk 32-position steps in turn when the item has one tile of 16
+// vectors; with two tiles (or four) each tile has two waves (one) that walk all the steps, the rows that another wave has
+// read coming from the caches. K and V rows go straight into registers in the order the matrix instructions take them,
+// with no copy in LDS, and the waves' sums meet at the end. Products are exact three-part BF16 splits, as in attn_flash3.
+template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it, unsigned char *lds) {
+  constexpr int kSteps = HD / 32, kDt = HD / 16, kWaves = kThreads / kWave, kRow = HD + 4;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
+  const int hd = p.hd;
+  const int tiles = it.vectors <= 16 ? 1 : it.vectors <= 32 ? 2 : 4, walkers = kWaves / tiles; // waves of a tile
+  const int v_mine = 16 * (wave / walkers) + lc; // this lane's vector
+  const bool active = v_mine < it.vectors;
+  v4i *qs = reinterpret_cast<v4i *>(lds) + (size_t)wave * kSteps * 3 * kWave + lane; // the wave's: [step][part][lane]
+  float *fix = reinterpret_cast<float *>(lds + (size_t)kWaves * kSteps * 3 * kWave * 16) + wave * kUnit * 16;
+  {
+    const float *src = p.q + ((size_t)(it.row0 + (active ? v_mine / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
+                              (active ? v_mine % p.kv_mul : 0)) * hd;
+    const float4 zero = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < kSteps; st++) {
+      const int d = 32 * st + 8 * lq;
+      const float4 a = active ? load4(src, d, hd) : zero, b = active ? load4(src, d + 4, hd) : zero;
+      const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      v4i h, m, l;
+      bf16_parts(x, h, m, l);
+      qs[(size_t)st * 3 * kWave] = h, qs[(size_t)(st * 3 + 1) * kWave] = m, qs[(size_t)(st * 3 + 2) * kWave] = l;
+    }
+  }
+  const int last = !active ? -1 : it.last0 == INT32_MAX ? INT32_MAX : it.last0 + v_mine / p.kv_mul;
+  v4f o[kDt];
+  float m_run = -FLT_MAX, l_run = 0.0f, odd = 0.0f;
+#pragma unroll
+  for (int d = 0; d < kDt; d++)
+    o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  float4 kr[2][kSteps][2], vr[2][4][HD / 64];
+  auto load_k = [&](int t0) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const float *row = it.key + (size_t)min(t0 + 16 * t + lc, it.t1 - 1) * it.pos_stride;
+#pragma unroll
+      for (int st = 0; st < kSteps; st++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          kr[t][st][h] = load4(row, 32 * st + 8 * lq + 4 * h, hd);
+    }
+  };
+  auto load_v = [&](int t0) {
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float *row = it.value + (size_t)min(t0 + 16 * t + 4 * lq + e, it.t1 - 1) * it.pos_stride;
+#pragma unroll
+        for (int j = 0; j < HD / 64; j++)
+          vr[t][e][j] = load4(row, 64 * j + 4 * lc, hd);
+      }
+  };
+  const int stride = walkers * kUnit;
+  const int end = 16 * (wave / walkers) < it.vectors ? it.t1 : it.t0; // a tile without vectors walks nothing
+  int t0 = it.t0 + wave % walkers * kUnit;
+  if (t0 < end) {
+    load_k(t0);
+    load_v(t0);
+  }
+  for (; t0 < end; t0 += stride) {
+    v4f sc[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+      sc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < kSteps; st++) {
+      const v4i qh = qs[(size_t)st * 3 * kWave], qm = qs[(size_t)(st * 3 + 1) * kWave],
+                ql = qs[(size_t)(st * 3 + 2) * kWave];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const float4 a = kr[t][st][0], b = kr[t][st][1];
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        v4i kh, km, kl;
+        bf16_parts(x, kh, km, kl);
+        sc[t] = mfma_bf16(kl, qh, sc[t]);
+        sc[t] = mfma_bf16(kh, ql, sc[t]);
+        sc[t] = mfma_bf16(km, qm, sc[t]);
+        sc[t] = mfma_bf16(km, qh, sc[t]);
+        sc[t] = mfma_bf16(kh, qm, sc[t]);
+        sc[t] = mfma_bf16(kh, qh, sc[t]);
+      }
+    }
+    if (t0 + stride < end)
+      load_k(t0 + stride);
+    float pv[8], top = -FLT_MAX;
+    unsigned live = 0;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int at = t0 + 16 * t + 4 * lq + e;
+        const bool sees = at < it.t1 && at <= last;
+        const float s = sc[t][e] * p.scale2;
+        odd = sees ? fmaf(s, 0.0f, odd) : odd;
+        live |= (unsigned)sees << (4 * t + e);
+        pv[4 * t + e] = sees ? s : -FLT_MAX;
+        top = fmaxf(top, pv[4 * t + e]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float m_new = fmaxf(m_run, top), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float w = (live >> i) & 1 ? __builtin_amdgcn_exp2f(pv[i] - m_new) : 0.0f;
+      pv[i] = w;
+      sum += w;
+    }
+    l_run = l_run * alpha + sum; // this lane's positions; the four lanes of a vector meet at the end
+    m_run = m_new;
+#pragma unroll
+    for (int d = 0; d < kDt; d++)
+      o[d] *= alpha;
+    float nonfinite = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int j = 0; j < HD / 64; j++) {
+          const float4 x = vr[t][e][j];
+          nonfinite = fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, fmaf(x.z, 0.0f, fmaf(x.w, 0.0f, nonfinite))));
+        }
+    const bool some = __any(nonfinite != 0.0f); // NaN: some value of the step is not finite
+    if (some) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int j = 0; j < HD / 64; j++) {
+            float4 &x = vr[t][e][j];
+            x = float4{finite(x.x) ? x.x : 0.0f, finite(x.y) ? x.y : 0.0f, finite(x.z) ? x.z : 0.0f,
+                       finite(x.w) ? x.w : 0.0f};
+          }
+    }
+    v4i ph, pm, pl;
+    bf16_parts(pv, ph, pm, pl);
+#pragma unroll
+    for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) { // tile 4 j + c: dimensions 64 j + 4 m + c
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float4 &v = vr[i / 4][i % 4][j];
+          x[i] = c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
+        }
+        v4i vh, vm, vl;
+        bf16_parts(x, vh, vm, vl);
+        const int d = 4 * j + c;
+        o[d] = mfma_bf16(vl, ph, o[d]);
+        o[d] = mfma_bf16(vh, pl, o[d]);
+        o[d] = mfma_bf16(vm, pm, o[d]);
+        o[d] = mfma_bf16(vm, ph, o[d]);
+        o[d] = mfma_bf16(vh, pm, o[d]);
+        o[d] = mfma_bf16(vh, ph, o[d]);
+      }
+    if (some)
+      add_nonfinite(o, pv, live, it, t0, hd, lane, fix, [&](int d, int e) { return 64 * (d / 4) + 4 * (4 * lq + e) + d % 4; });
+    if (t0 + stride < end)
+      load_v(t0 + stride);
+  }
+  if (odd != 0.0f)
+    p.flags[1] = 1;
+  // the waves' sums: [wave][vector][HD values, maximum, sum]
+  __syncthreads(); // every wave is done with its query parts
+  float *sums = reinterpret_cast<float *>(lds);
+  {
+    float l = l_run;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    float *dst = sums + (size_t)(wave * 16 + lc) * kRow;
+#pragma unroll
+    for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        *reinterpret_cast<float4 *>(dst + 64 * j + 4 * (4 * lq + e)) =
+            float4{o[4 * j][e], o[4 * j + 1][e], o[4 * j + 2][e], o[4 * j + 3][e]};
+    if (lq == 0)
+      dst[HD] = m_run, dst[HD + 1] = l;
+  }
+  __syncthreads();
+  const int hd4 = hd / 4;
+  for (int i = tid; i < it.vectors * hd4; i += kThreads) {
+    const int v = i / hd4, d4 = i % hd4;
+    const float *src = sums + (size_t)(v / 16 * walkers * 16 + v % 16) * kRow;
+    float m = -FLT_MAX;
+    for (int w = 0; w < walkers; w++)
+      m = fmaxf(m, src[(size_t)w * 16 * kRow + HD]);
+    float l = 0.0f;
+    float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w = 0; w < walkers; w++) {
+      const float *at = src + (size_t)w * 16 * kRow;
+      const float scale = __builtin_amdgcn_exp2f(at[HD] - m);
+      const float4 x = *reinterpret_cast<const float4 *>(at + 4 * d4);
+      l = fmaf(scale, at[HD + 1], l);
+      sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
+    }
+    const size_t vec = (size_t)(it.row0 + v / p.kv_mul) * p.n_heads + (size_t)it.g * p.kv_mul + v % p.kv_mul;
+    float *dst = p.partial + (it.slot0 + vec * it.slot_step) * (size_t)(hd + 4);
+    *reinterpret_cast<float4 *>(dst + 4 * d4) = sum;
+    if (d4 == 0)
+      dst[hd] = m, dst[hd + 1] = l;
+  }
+}
+
+// Wide: up to 128 query vectors, 32 a wave; a step's K and V rows are split once for the block and staged in LDS. A
+// product x y is taken as hh + hl + lh of two FP16 parts each (22 bits and more), three matrix instructions where exact
+// BF16 parts take six. The parts need values near 2^15: each query vector and each K row is scaled by a power of two of
+// its own, taken out of the score again; each group of four V rows likewise, and its exponent ev joins the score before
+// the exponential, so that the weights are exp2(s + ev - m) and meet V 2^-ev, with m the running maximum of s + ev. The
+// softmax's sum takes them times 2^-ev.
+template <int HD> struct WideStage {
+  static constexpr int kKRow = HD + 8, kVRow = kUnit + 8;
+  uint16_t k[2][kUnit * kKRow];
+  uint16_t v[2][HD * kVRow];
+  float k_back[kUnit];  // 2^(e - 14): undoes a K row's scale
+  float v_exp[kUnit];   // ev
+  float v_back[kUnit];  // 2^-ev
+  float fix[kThreads / kWave * kUnit * 16];
+  int nonfinite;
+};
+
+template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
+  typedef WideStage<HD> Stage;
+  Stage &sh = *reinterpret_cast<Stage *>(lds);
+  float *fix = sh.fix;
+  constexpr int kSteps = HD / 32, kDt = HD / 16, kLeastK = -100, kLeastV = -30;
+  constexpr int kItems = kUnit * HD / 8 / kThreads; // K staging items of eight values a thread
+  constexpr int kLanes = HD / 8;                    // a K row's
+  constexpr int kVLanes = HD / 4;
+  static_assert(kItems >= 1 && kUnit / 4 * kVLanes <= kThreads, "staging items");
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
+  const int hd = p.hd;
+  const bool v_stager = tid < kUnit / 4 * kVLanes;
+  const int vg = tid / kVLanes, vd = 4 * (tid % kVLanes); // V item: positions 4 vg .. + 3, dimensions vd .. + 3
+  float4 kr[kItems][2], vr[4];
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < kItems; u++) {
+      const int i = tid + u * kThreads, d = 8 * (i % kLanes);
+      const float *row = it.key + (size_t)min(t0 + i / kLanes, it.t1 - 1) * it.pos_stride;
+      kr[u][0] = load4(row, d, hd);
+      kr[u][1] = load4(row, d + 4, hd);
+    }
+    if (v_stager)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        vr[e] = load4(it.value + (size_t)min(t0 + 4 * vg + e, it.t1 - 1) * it.pos_stride, vd, hd);
+  };
+  auto peak = [](const float4 &x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
+  auto stage = [&]() {
+#pragma unroll
+    for (int u = 0; u < kItems; u++) {
+      const int i = tid + u * kThreads, row = i / kLanes, d = 8 * (i % kLanes);
+      const float4 a = kr[u][0], b = kr[u][1];
+      // a row with an infinity keeps it: its scores are not finite, whatever the scale
+      const float top = fminf(group_reduce_max(fmaxf(peak(a), peak(b)), kLanes), FLT_MAX);
+      int e;
+      const float scale = f16_scale(top, kLeastK, e);
+      v4i h, l;
+      int th, tl;
+      f16_pair(a.x, a.y, scale, th, tl), h[0] = th, l[0] = tl;
+      f16_pair(a.z, a.w, scale, th, tl), h[1] = th, l[1] = tl;
+      f16_pair(b.x, b.y, scale, th, tl), h[2] = th, l[2] = tl;
+      f16_pair(b.z, b.w, scale, th, tl), h[3] = th, l[3] = tl;
+      *reinterpret_cast<v4i *>(&sh.k[0][row * Stage::kKRow + d]) = h;
+      *reinterpret_cast<v4i *>(&sh.k[1][row * Stage::kKRow + d]) = l;
+      if (d == 0)
+        sh.k_back[row] = __uint_as_float((unsigned)(127 - 14 + e) << 23);
+    }
+    if (v_stager) {
+      float odd = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        odd = fmaf(vr[e].x, 0.0f, fmaf(vr[e].y, 0.0f, fmaf(vr[e].z, 0.0f, fmaf(vr[e].w, 0.0f, odd))));
+      if (odd != 0.0f) {
+        sh.nonfinite = 1;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          vr[e] = float4{finite(vr[e].x) ? vr[e].x : 0.0f, finite(vr[e].y) ? vr[e].y : 0.0f,
+                         finite(vr[e].z) ? vr[e].z : 0.0f, finite(vr[e].w) ? vr[e].w : 0.0f};
+      }
+      float top = fmaxf(fmaxf(peak(vr[0]), peak(vr[1])), fmaxf(peak(vr[2]), peak(vr[3])));
+      top = group_reduce_max(top, kVLanes);
+      int ev;
+      const float scale = f16_scale(top, kLeastV, ev);
+      const int at = 8 * (vg % 4) + 4 * (vg / 4); // slot of position 16 t + 4 q + e: 8 q + 4 t + e
+      auto put = [&](int d, float x0, float x1, float x2, float x3) {
+        int h0, l0, h1, l1;
+        f16_pair(x0, x1, scale, h0, l0);
+        f16_pair(x2, x3, scale, h1, l1);
+        *reinterpret_cast<int2 *>(&sh.v[0][(vd + d) * Stage::kVRow + at]) = int2{h0, h1};
+        *reinterpret_cast<int2 *>(&sh.v[1][(vd + d) * Stage::kVRow + at]) = int2{l0, l1};
+      };
+      put(0, vr[0].x, vr[1].x, vr[2].x, vr[3].x);
+      put(1, vr[0].y, vr[1].y, vr[2].y, vr[3].y);
+      put(2, vr[0].z, vr[1].z, vr[2].z, vr[3].z);
+      put(3, vr[0].w, vr[1].w, vr[2].w, vr[3].w);
+      if (vd < 16) { // one lane a position
+        const int e = vd / 4;
+        sh.v_exp[4 * vg + e] = (float)ev;
+        sh.v_back[4 * vg + e] = __uint_as_float((unsigned)max(127 - ev, 1) << 23);
+      }
+    }
+  };
+  // the wave's query vectors: parts of dimensions 32 st + 8 lq .. + 7 of vector 32 wave + 16 n + lc
+  v4i qh[2][kSteps], ql[2][kSteps];
+  float q_back[2], m_run[2], l_run[2], odd = 0.0f;
+  int last[2];
+  const bool busy = 32 * wave < it.vectors; // a wave without vectors only stages
+  v4f o[2][kDt];
+#pragma unroll
+  for (int n = 0; n < 2; n++) {
+    const int v = 32 * wave + 16 * n + lc;
+    const bool active = v < it.vectors;
+    last[n] = !active ? -1 : it.last0 == INT32_MAX ? INT32_MAX : it.last0 + v / p.kv_mul;
+    const float *src = p.q + ((size_t)(it.row0 + (active ? v / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
+                              (active ? v % p.kv_mul : 0)) * hd;
+    float4 x[kSteps][2];
+    float top = 0.0f;
+#pragma unroll
+    for (int st = 0; st < kSteps; st++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        x[st][k] = active ? load4(src, 32 * st + 8 * lq + 4 * k, hd) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+        top = fmaxf(top, peak(x[st][k]));
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fminf(fmaxf(top, __shfl_xor(top, 32)), FLT_MAX);
+    int e;
+    const float scale = f16_scale(top, kLeastK, e);
+    q_back[n] = __uint_as_float((unsigned)(127 - 14 + e) << 23) * p.scale2;
+#pragma unroll
+    for (int st = 0; st < kSteps; st++) {
+      int th, tl;
+      f16_pair(x[st][0].x, x[st][0].y, scale, th, tl), qh[n][st][0] = th, ql[n][st][0] = tl;
+      f16_pair(x[st][0].z, x[st][0].w, scale, th, tl), qh[n][st][1] = th, ql[n][st][1] = tl;
+      f16_pair(x[st][1].x, x[st][1].y, scale, th, tl), qh[n][st][2] = th, ql[n][st][2] = tl;
+      f16_pair(x[st][1].z, x[st][1].w, scale, th, tl), qh[n][st][3] = th, ql[n][st][3] = tl;
+    }
+    m_run[n] = -FLT_MAX, l_run[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDt; d++)
+      o[n][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // positions up to here are seen by every vector of the tile
+  const int seen_by_all = it.last0 == INT32_MAX ? it.t1 : min(it.t1, it.last0 + 1);
+  auto compute = [&](int t0) {
+    v4f sc[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+        sc[n][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < kSteps; st++) {
+      v4i kh[2], kl[2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const int at = (16 * t + lc) * Stage::kKRow + 32 * st + 8 * lq;
+        kh[t] = *reinterpret_cast<const v4i *>(&sh.k[0][at]);
+        kl[t] = *reinterpret_cast<const v4i *>(&sh.k[1][at]);
+      }
+#pragma unroll
+      for (int k = 0; k < 3; k++) // the three products in turn over four sums: none waits for the one before
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+            sc[n][t] = mfma_f16(k == 0 ? kl[t] : kh[t], k == 1 ? ql[n][st] : qh[n][st], sc[n][t]);
+    }
+    const bool all = t0 + kUnit <= seen_by_all; // uniform
+    v4i ph[2], pl[2];
+    float pv[2][8];
+    unsigned live[2] = {0, 0};
+    float4 k_back[2], v_exp[2], v_back[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      k_back[t] = *reinterpret_cast<const float4 *>(&sh.k_back[16 * t + 4 * lq]);
+      v_exp[t] = *reinterpret_cast<const float4 *>(&sh.v_exp[16 * t + 4 * lq]);
+      v_back[t] = *reinterpret_cast<const float4 *>(&sh.v_back[16 * t + 4 * lq]);
+    }
+    auto of = [](const float4 &x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      float top = -FLT_MAX;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float s = sc[n][t][e] * of(k_back[t], e) * q_back[n];
+          float x = s + of(v_exp[t], e);
+          if (all) {
+            odd = fmaf(s, 0.0f, odd);
+          } else {
+            const int at = t0 + 16 * t + 4 * lq + e;
+            const bool sees = at < it.t1 && at <= last[n];
+            odd = sees ? fmaf(s, 0.0f, odd) : odd;
+            x = sees ? x : -FLT_MAX;
+            live[n] |= (unsigned)sees << (4 * t + e);
+          }
+          pv[n][4 * t + e] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float m_new = fmaxf(m_run[n], top);
+      if (__any(m_new > m_run[n])) { // else nothing of the sums changes
+        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+        l_run[n] *= alpha;
+        m_run[n] = m_new;
+#pragma unroll
+        for (int d = 0; d < kDt; d++)
+          o[n][d] *= alpha;
+      }
+      const float base = m_new - 15.0f; // weights up to 2^15
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        float w = __builtin_amdgcn_exp2f(pv[n][i] - base);
+        if (!all)
+          w = (live[n] >> i) & 1 ? w : 0.0f;
+        pv[n][i] = w;
+        sum = fmaf(w, of(v_back[i / 4], i % 4), sum);
+      }
+      l_run[n] += sum;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        int th, tl;
+        f16_pair(pv[n][2 * i], pv[n][2 * i + 1], 1.0f, th, tl);
+        ph[n][i] = th, pl[n][i] = tl;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kDt; d++) {
+      const int at = (16 * d + lc) * Stage::kVRow + 8 * lq;
+      const v4i vh = *reinterpret_cast<const v4i *>(&sh.v[0][at]), vl = *reinterpret_cast<const v4i *>(&sh.v[1][at]);
+#pragma unroll
+      for (int k = 0; k < 3; k++)
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+          o[n][d] = mfma_f16(k == 0 ? vl : vh, k == 1 ? pl[n] : ph[n], o[n][d]);
+    }
+    if (sh.nonfinite)
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+        add_nonfinite(o[n], pv[n], all ? (last[n] >= 0 ? 0xFFu : 0u) : live[n], it, t0, hd, lane,
+                      fix + wave * kUnit * 16, [&](int d, int e) { return 16 * d + 4 * lq + e; });
+  };
+  if (it.t0 < it.t1)
+    load(it.t0);
+  for (int t0 = it.t0; t0 < it.t1; t0 += kUnit) {
+    if (tid == 0)
+      sh.nonfinite = 0;
+    __syncthreads(); // the step before is done with the staged rows, and the mark is clear
+    stage();
+    if (t0 + kUnit < it.t1)
+      load(t0 + kUnit);
+    __syncthreads();
+    if (busy)
+      compute(t0);
+    __syncthreads();
+  }
+  if (odd != 0.0f && (last[0] >= 0 || last[1] >= 0))
+    p.flags[1] = 1;
+#pragma unroll
+  for (int n = 0; n < 2; n++) {
+    float l = l_run[n];
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const int v = 32 * wave + 16 * n + lc;
+    if (v >= it.vectors)
+      continue;
+    const size_t vec = (size_t)(it.row0 + v / p.kv_mul) * p.n_heads + (size_t)it.g * p.kv_mul + v % p.kv_mul;
+    float *dst = p.partial + (it.slot0 + vec * it.slot_step) * (size_t)(hd + 4);
+    const float back = 0x1p-29f; // 2^14 of the V rows, 2^15 of the weights
+#pragma unroll
+    for (int d = 0; d < kDt; d++)
+      if (16 * d + 4 * lq < hd)
+        *reinterpret_cast<float4 *>(dst + 16 * d + 4 * lq) =
+            float4{o[n][d][0] * back, o[n][d][1] * back, o[n][d][2] * back, o[n][d][3] * back};
+    if (lq == 0)
+      dst[hd] = m_run[n], dst[hd + 1] = l * 0x1p-15f;
+  }
+}
+
+template <int HD> constexpr size_t fast_lds() {
+  constexpr size_t narrow_q = (size_t)(kThreads / kWave) * ((HD / 32) * 3 * kWave * 16 + kUnit * 16 * 4);
+  constexpr size_t narrow_sums = (size_t)(kThreads / kWave) * 16 * (HD + 4) * 4;
+  size_t most = sizeof(Plan);
+  most = narrow_q > most ? narrow_q : most;
+  most = narrow_sums > most ? narrow_sums : most;
+  return sizeof(WideStage<HD>) > most ? sizeof(WideStage<HD>) : most;
+}
+
+// Blocks: ceil(rows / 256) that write down each row's slots for the merge, then the prefix's items (KV head fastest, so
+// that consecutive blocks, which go to the XCDs in turn, give an XCD the same heads' rows), then the requests' own.
+template <int HD> __global__ __launch_bounds__(kThreads, 2) void attn_requests(FastAttn p) {
+  extern __shared__ __align__(16) unsigned char lds[];
+  Plan &plan = *reinterpret_cast<Plan *>(lds);
+  make_plan(p, plan);
+  const int tid = threadIdx.x, row_blocks = ceil_div(p.batch.rows, kThreads);
+  const int prefix_shares = plan.prefix_shares, own_items = plan.items[p.batch.count - 1];
+  if ((int)blockIdx.x < row_blocks) {
+    if (blockIdx.x == 0 && tid == 0) {
+      p.header[0] = prefix_shares;
+      if (plan.bad)
+        p.flags[3] = 1;
+    }
+    __shared__ int2 mine[kThreads];
+    const int r0 = blockIdx.x * kThreads;
+    mine[tid] = int2{0, -1};
+    __syncthreads();
+    for (int r = tid; r < p.batch.count; r += kThreads) {
+      const int n = plan.rows[r], first = plan.first[r], shares = plan.shares[r];
+      const int slot0 = plan.slots[r] - n * p.n_heads * shares;
+      for (int i = max(first, r0); i < min(first + n, r0 + kThreads); i++)
+        mine[i - r0] = int2{slot0 + (i - first) * p.n_heads * shares, shares};
+    }
+    __syncthreads();
+    if (r0 + tid < p.batch.rows)
+      p.row_slots[r0 + tid] = mine[tid];
+    return;
+  }
+  int i = blockIdx.x - row_blocks;
+  const int prefix_items = p.prefix_tiles * prefix_shares * p.n_kv_heads;
+  const size_t prefix_slots = (size_t)p.batch.rows * p.n_heads * prefix_shares;
+  Item it;
+  bool narrow;
+  if (i < prefix_items) {
+    it.g = i % p.n_kv_heads;
+    i /= p.n_kv_heads;
+    const int tile = i % p.prefix_tiles, share = i / p.prefix_tiles;
+    const int units = ceil_div(p.batch.prefix, kUnit), length = ceil_div(units, prefix_shares) * kUnit;
+    const int rows = p.prefix_narrow ? p.batch.rows : p.tile_rows;
+    // rows that belong to no request before the first and behind the last one stay out
+    const int first = min(max(p.batch.start[0], 0), p.batch.rows);
+    const int end = min(max(p.batch.start[p.batch.count], 0), p.batch.rows);
+    it.row0 = max(tile * rows, first);
+    it.vectors = (min(tile * rows + rows, end) - it.row0) * p.kv_mul;
+    if (it.vectors <= 0)
+      return;
+    it.key = p.prefix_key + (size_t)it.g * p.batch.prefix_head_base;
+    it.value = p.prefix_value + (size_t)it.g * p.batch.prefix_head_base;
+    it.pos_stride = p.batch.prefix_pos_stride;
+    it.t0 = min(share * length, p.batch.prefix);
+    it.t1 = min(it.t0 + length, p.batch.prefix);
+    it.last0 = INT32_MAX;
+    it.slot0 = share;
+    it.slot_step = prefix_shares;
+    narrow = p.prefix_narrow;
+  } else {
+    i -= prefix_items;
+    if (i >= own_items)
+      return;
+    int lo = 0, hi = p.batch.count - 1; // the first request whose running sum passes i
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (plan.items[mid] > i)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    const int r = lo, n = plan.rows[r], shares = plan.shares[r], tiles = own_tiles(p, n);
+    i -= plan.items[r] - tiles * shares * p.n_kv_heads;
+    it.g = i % p.n_kv_heads;
+    i /= p.n_kv_heads;
+    const int tile = i % tiles, share = i / tiles;
+    narrow = n * p.kv_mul <= kNarrowVectors;
+    const int j0 = narrow ? 0 : tile * p.tile_rows, rows = narrow ? n : min(p.tile_rows, n - j0);
+    const int end = plan.length[r] + j0 + rows;
+    const int length = ceil_div(ceil_div(end, kUnit), shares) * kUnit;
+    const size_t cache = (size_t)plan.slot[r] * p.batch.slot_floats + (size_t)it.g * p.batch.head_base;
+    it.row0 = plan.first[r] + j0;
+    it.vectors = rows * p.kv_mul;
+    it.key = p.key + cache;
+    it.value = p.value + cache;
+    it.pos_stride = p.batch.pos_stride;
+    it.t0 = min(share * length, end);
+    it.t1 = min(it.t0 + length, end);
+    it.last0 = plan.length[r] + j0;
+    // the request's slots are [row][head][share]; slot0 makes up for vec counting from row 0 of the batch
+    it.slot0 = prefix_slots + (size_t)(plan.slots[r] - n * p.n_heads * shares) + share -
+               (size_t)plan.first[r] * p.n_heads * shares;
+    it.slot_step = shares;
+  }
+  __syncthreads(); // the plan's place is taken by the walk
+  if (narrow)
+    walk_narrow<HD>(p, it, lds);
+  else
+    walk_wide<HD>(p, it, lds);
+}
+
+// A thread per (row, head, four dimensions): the row's shares of the prefix and its own, rescaled to their largest maximum
+// and added in order.
+__global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
+  const int hd4 = p.hd / 4;
+  const long long idx = (long long)blockIdx.x * kThreads + threadIdx.x;
+  if (idx >= (long long)p.batch.rows * p.n_heads * hd4)
+    return;
+  const int d4 = (int)(idx % hd4);
+  const long long vec = idx / hd4;
+  const int row = (int)(vec / p.n_heads), head = (int)(vec % p.n_heads);
+  const int2 mine = p.row_slots[row];
+  if (mine.y < 0)
+    return;
+  const int shared = p.header[0], count = shared + mine.y;
+  const size_t slot = (size_t)(p.hd + 4);
+  const float *far = p.partial + (size_t)vec * shared * slot;
+  const float *own = p.partial + ((size_t)p.batch.rows * p.n_heads * shared + (size_t)mine.x + (size_t)head * mine.y) * slot;
+  float m = -FLT_MAX, l = 0.0f;
+  float4 o = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int kAhead = 4; // shares whose loads are in flight together
+  for (int s0 = 0; s0 < count; s0 += kAhead) {
+    float ms[kAhead], ls[kAhead];
+    float4 x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+      const int s = min(s0 + k, count - 1);
+      const float *src = s < shared ? far + (size_t)s * slot : own + (size_t)(s - shared) * slot;
+      ms[k] = s0 + k < count ? src[p.hd] : -FLT_MAX;
+      ls[k] = s0 + k < count ? src[p.hd + 1] : 0.0f;
+      x[k] = *reinterpret_cast<const float4 *>(src + 4 * d4);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+      top = fmaxf(top, ms[k]);
+    const float alpha = __builtin_amdgcn_exp2f(m - top);
+    l *= alpha;
+    o = float4{o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha};
+    m = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++)
+      if (s0 + k < count) {
+        const float w = __builtin_amdgcn_exp2f(ms[k] - m);
+        l = fmaf(w, ls[k], l);
+        o = float4{fmaf(w, x[k].x, o.x), fmaf(w, x[k].y, o.y), fmaf(w, x[k].z, o.z), fmaf(w, x[k].w, o.w)};
+      }
+  }
+  *reinterpret_cast<float4 *>(p.out + (size_t)vec * p.hd + 4 * d4) = float4{o.x / l, o.y / l, o.z / l, o.w / l};
+}
+
+} // namespace
+
+// The matrix-core form takes head dimensions up to 128 in whole groups of four, with 16-byte aligned rows.
+bool attention_requests_fast(const AttentionRequestsJob &job) {
+  const RequestsDev &b = job.batch;
+  const uintptr_t all = (uintptr_t)job.out | (uintptr_t)job.q | (uintptr_t)job.prefix_key | (uintptr_t)job.prefix_value |
+                        (uintptr_t)job.key | (uintptr_t)job.value;
+  return job.head_dim <= 128 && job.head_dim % 4 == 0 && (all & 15) == 0 && b.rows <= (1 << 20) && job.n_heads <= 1024;
+}
+
+// The most blocks and slots that a plan can ask for, whatever the arrays hold: every walk is cut into units / step + 1
+// shares at most, and step is at least 1 / kTargetItems of all units.
+struct FastBounds {
+  long long prefix_tiles, items, slots;
+  bool prefix_narrow;
+  int tile_rows;
+};
+FastBounds fast_bounds(const AttentionRequestsJob &job) {
+  const RequestsDev &b = job.batch;
+  const int kv_mul = job.n_heads / job.n_kv_heads;
+  FastBounds f{};
+  f.tile_rows = kTileVectors / kv_mul;
+  f.prefix_narrow = b.rows * kv_mul <= kNarrowVectors;
+  f.prefix_tiles = !b.prefix ? 0 : f.prefix_narrow ? 1 : (b.rows + f.tile_rows - 1) / f.tile_rows;
+  const long long own_tiles = (b.count < b.rows ? b.count : b.rows) + b.rows / f.tile_rows;
+  f.items = kTargetItems + job.n_kv_heads * (f.prefix_tiles + own_tiles);
+  const long long vectors = (long long)b.rows * job.n_heads;
+  // rows times shares, over the prefix and over the requests' own: see the plan; and no walk has more than kMaxShares
+  const long long capped = 2 * vectors * kMaxShares, spread = 2 * vectors + (long long)kTileVectors * kTargetItems * 2;
+  f.slots = capped < spread ? capped : spread;
+  return f;
+}
+
+size_t attention_requests_workspace(const AttentionRequestsJob &job) {
+  if (!attention_requests_fast(job))
+    return 0;
+  return (size_t)fast_bounds(job).slots * (size_t)(job.head_dim + 4) * sizeof(float) +
+         (size_t)job.batch.rows * sizeof(int2) + 256;
+}
+
+bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hipStream_t stream) {
+  const FastBounds f = fast_bounds(job);
+  FastAttn p{};
+  p.out = job.out;
+  p.q = job.q;
+  p.prefix_key = job.prefix_key;
+  p.prefix_value = job.prefix_value;
+  p.key = job.key;
+  p.value = job.value;
+  p.batch = job.batch;
+  p.n_heads = job.n_heads;
+  p.n_kv_heads = job.n_kv_heads;
+  p.kv_mul = job.n_heads / job.n_kv_heads;
+  p.hd = job.head_dim;
+  p.tile_rows = f.tile_rows;
+  p.prefix_tiles = (int)f.prefix_tiles;
+  p.prefix_narrow = f.prefix_narrow;
+  p.scale2 = 1.4426950408889634f / sqrtf((float)job.head_dim);
+  p.header = (int *)workspace;
+  p.row_slots = (int2 *)((char *)workspace + 16);
+  p.partial = (float *)((char *)workspace + ((16 + (size_t)job.batch.rows * sizeof(int2) + 15) & ~(size_t)15));
+  p.flags = device().error_flags;
+  const long long blocks = f.items + (job.batch.rows + kThreads - 1) / kThreads;
+  if (job.head_dim <= 64)
+    hipLaunchKernelGGL(attn_requests<64>, dim3((unsigned)blocks), dim3(kThreads), fast_lds<64>(), stream, p);
+  else
+    hipLaunchKernelGGL(attn_requests<128>, dim3((unsigned)blocks), dim3(kThreads), fast_lds<128>(), stream, p);
+  if (!launch_ok("attn_requests"))
+    return false;
+  const long long threads = (long long)job.batch.rows * job.n_heads * (job.head_dim / 4);
+  hipLaunchKernelGGL(attn_requests_merge, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream,
+                     p);
+  return launch_ok("attn_requests_merge");
+}
+
+bool launch_attention_requests(const AttentionRequestsJob &job, void *workspace, hipStream_t stream) {
+  if (attention_requests_fast(job))
+    return launch_attention_fast(job, workspace, stream);
+  RequestAttn p{};
+  p.out = job.out;
+  p.q = job.q;
+  p.prefix_key = job.prefix_key;
+  p.prefix_value = job.prefix_value;
+  p.key = job.key;
+  p.value = job.value;
+  p.batch = job.batch;
+  p.n_heads = job.n_heads;
+  p.n_kv_heads = job.n_kv_heads;
+  p.head_dim = job.head_dim;
+  p.divisor = sqrtf((float)job.head_dim);
+  p.flags = device().error_flags;
+  const int most = (1 << 23) / job.n_kv_heads; // rows of a launch, which holds fewer than 2^32 threads
+  for (int row0 = 0; row0 < job.batch.rows; row0 += most) {
+    const int n = job.batch.rows - row0 < most ? job.batch.rows - row0 : most;
+    hipLaunchKernelGGL(attn_rows, dim3((unsigned)n * (unsigned)job.n_kv_heads), dim3(kThreads), 0, stream, p, row0);
+    if (job.batch.rows - row0 <= most)
+      break;
+  }
+  return launch_ok("attn_rows");
+}
+
+} // namespace llhip
