@@ -164,9 +164,11 @@ __global__ __launch_bounds__(kThreads) void attn_rows(RequestAttn p, int row0) {
 constexpr int kUnit = 32;        // positions of a step
 constexpr int kTileVectors = 128; // query vectors of a wide tile
 constexpr int kNarrowVectors = 32; // at most, of a narrow one
-constexpr int kTargetItems = 1024; // work items aimed at: two for each block that the chip holds
+constexpr int kTargetItems = 512; // work items aimed at: one for each block that the chip holds
 constexpr int kMinUnits = 4;     // a step for each wave of a narrow block
 constexpr int kMaxShares = 32;   // of one walk
+constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far below that its weight is zero, also where a
+                                     // lane has seen nothing else
 
 struct FastAttn {
   float *out;
@@ -178,7 +180,7 @@ struct FastAttn {
   bool prefix_narrow;
   float scale2; // log2(e) / sqrtf(hd)
   float *partial;
-  int2 *row_slots; // per row: first own slot, own shares (-1: the row belongs to no request)
+  int4 *row_slots; // per row: first own slot, own shares (-1: the row belongs to no request), cache slot, own position
   int *header;     // [0] shares of the prefix
   int *flags;
 };
@@ -280,35 +282,17 @@ struct Item {
   int slot_step; // floats' slots between vectors: a vector's slot is slot0 + (row * n_heads + head) * slot_step
 };
 
+// Nothing moves across: each phase's registers are free before the next one's are taken (moved freely, the phases of a
+// step need more than the 256 registers that two waves a SIMD leave each).
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// A value that is infinite or no number must reach exactly the rows that see its position, and 0 * infinity would carry it
-// to those that do not. So the products take 0 in the place of such values, and this adds them, weight by weight: rare,
-// and as slow as it is. pv: the lane's weights of the step's 32 positions (16 t + 4 (lane / 16) + e in pv[4 t + e]), live
-// the bits of those its vector sees, dim(d, e) the dimension of o[d][e]; weights: the wave's 32 x 16 floats of LDS.
-template <int D, class Dim>
-__device__ __forceinline__ void add_nonfinite(v4f (&o)[D], const float (&pv)[8], unsigned live, const Item &it, int t0,
-                                              int hd, int lane, float *weights, Dim dim) {
-  const int lq = lane >> 4, lc = lane & 15;
-#pragma unroll
-  for (int i = 0; i < 8; i++)
-    weights[(16 * (i / 4) + 4 * lq + i % 4) * 16 + lc] = (live >> i) & 1 ? pv[i] : -1.0f;
-  __builtin_amdgcn_wave_barrier(); // the wave's own LDS writes and reads stay in order
-#pragma unroll 1
-  for (int t = t0; t < min(t0 + kUnit, it.t1); t++) {
-    const float w = weights[(t - t0) * 16 + lc];
-    const float *row = it.value + (size_t)t * it.pos_stride;
-#pragma unroll
-    for (int d = 0; d < D; d++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int at = dim(d, e);
-        const float v = at < hd ? row[at] : 0.0f;
-        if (w >= 0.0f && !finite(v))
-          o[d][e] += w * v;
-      }
-  }
-  __builtin_amdgcn_wave_barrier();
+// The end of a partial sum's slot: maximum (base 2), sum of the weights, and, where the item met a V value that is not
+// finite, its positions t0 .. t1 - 1 (else t1 = 0). Such a value must reach exactly the rows that see its position, and 0 *
+// infinity would carry it to those that do not; so the products take 0 in its place, and the merge adds it.
+__device__ __forceinline__ float4 slot_end(float m, float l, bool met, const Item &it) {
+  return float4{m, l, __int_as_float(it.t0), __int_as_float(met ? it.t1 : 0)};
 }
 
 // x = h + m + l exactly, each part 8 significant bits: the parts of eight values as three BF16 operands.
@@ -353,8 +337,16 @@ __device__ __forceinline__ float f16_scale(float top, int least, int &e) {
   return __uint_as_float((unsigned)(127 + 14 - e) << 23);
 }
 
+// Four values of a query vector, zero past the head's dimensions.
 __device__ __forceinline__ float4 load4(const float *row, int d, int hd) {
   return d < hd ? *reinterpret_cast<const float4 *>(row + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+// Four values of a K or V row. Past the head's dimensions the row's first ones, so that the load is unconditional (a
+// branch a load would have each wait for the one before): the query's zeros take them out of a score, and a value sum's
+// dimensions there are not stored.
+__device__ __forceinline__ float4 row4(const float *row, int d, int hd) {
+  return *reinterpret_cast<const float4 *>(row + (d < hd ? d : 0));
 }
 
 // Narrow: at most 16 vectors a wave. The four waves walk 32-position steps in turn when the item has one tile of 16
@@ -369,7 +361,6 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
   const int v_mine = 16 * (wave / walkers) + lc; // this lane's vector
   const bool active = v_mine < it.vectors;
   v4i *qs = reinterpret_cast<v4i *>(lds) + (size_t)wave * kSteps * 3 * kWave + lane; // the wave's: [step][part][lane]
-  float *fix = reinterpret_cast<float *>(lds + (size_t)kWaves * kSteps * 3 * kWave * 16) + wave * kUnit * 16;
   {
     const float *src = p.q + ((size_t)(it.row0 + (active ? v_mine / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
                               (active ? v_mine % p.kv_mul : 0)) * hd;
@@ -387,6 +378,7 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
   const int last = !active ? -1 : it.last0 == INT32_MAX ? INT32_MAX : it.last0 + v_mine / p.kv_mul;
   v4f o[kDt];
   float m_run = -FLT_MAX, l_run = 0.0f, odd = 0.0f;
+  bool met = false; // a value that is not finite
 #pragma unroll
   for (int d = 0; d < kDt; d++)
     o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
@@ -399,7 +391,7 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
       for (int st = 0; st < kSteps; st++)
 #pragma unroll
         for (int h = 0; h < 2; h++)
-          kr[t][st][h] = load4(row, 32 * st + 8 * lq + 4 * h, hd);
+          kr[t][st][h] = row4(row, 32 * st + 8 * lq + 4 * h, hd);
     }
   };
   auto load_v = [&](int t0) {
@@ -410,7 +402,7 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
         const float *row = it.value + (size_t)min(t0 + 16 * t + 4 * lq + e, it.t1 - 1) * it.pos_stride;
 #pragma unroll
         for (int j = 0; j < HD / 64; j++)
-          vr[t][e][j] = load4(row, 64 * j + 4 * lc, hd);
+          vr[t][e][j] = row4(row, 64 * j + 4 * lc, hd);
       }
   };
   const int stride = walkers * kUnit;
@@ -442,32 +434,29 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
         sc[t] = mfma_bf16(kh, qm, sc[t]);
         sc[t] = mfma_bf16(kh, qh, sc[t]);
       }
+      fence();
     }
-    if (t0 + stride < end)
-      load_k(t0 + stride);
+    load_k(t0 + stride); // past the end the last row again: a branch would have the next wait take these loads in
+    fence();
     float pv[8], top = -FLT_MAX;
-    unsigned live = 0;
+    const int seen = min(it.t1 - 1, last) - t0 - 4 * lq; // of the lane's positions 16 t + e
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int at = t0 + 16 * t + 4 * lq + e;
-        const bool sees = at < it.t1 && at <= last;
-        const float s = sc[t][e] * p.scale2;
-        odd = sees ? fmaf(s, 0.0f, odd) : odd;
-        live |= (unsigned)sees << (4 * t + e);
-        pv[4 * t + e] = sees ? s : -FLT_MAX;
+        pv[4 * t + e] = 16 * t + e <= seen ? sc[t][e] * p.scale2 : -FLT_MAX;
+        odd = fmaf(pv[4 * t + e], 0.0f, odd);
         top = fmaxf(top, pv[4 * t + e]);
       }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float m_new = fmaxf(m_run, top), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    const float base = fmaxf(m_new, kMasked);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float w = (live >> i) & 1 ? __builtin_amdgcn_exp2f(pv[i] - m_new) : 0.0f;
-      pv[i] = w;
-      sum += w;
+      pv[i] = __builtin_amdgcn_exp2f(pv[i] - base);
+      sum += pv[i];
     }
     l_run = l_run * alpha + sum; // this lane's positions; the four lanes of a vector meet at the end
     m_run = m_new;
@@ -484,8 +473,8 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
           const float4 x = vr[t][e][j];
           nonfinite = fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, fmaf(x.z, 0.0f, fmaf(x.w, 0.0f, nonfinite))));
         }
-    const bool some = __any(nonfinite != 0.0f); // NaN: some value of the step is not finite
-    if (some) {
+    if (__any(nonfinite != 0.0f)) { // NaN: some value of the step is not finite
+      met = true;
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -499,6 +488,7 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
     }
     v4i ph, pm, pl;
     bf16_parts(pv, ph, pm, pl);
+    fence();
 #pragma unroll
     for (int j = 0; j < HD / 64; j++)
 #pragma unroll
@@ -518,11 +508,12 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
         o[d] = mfma_bf16(vm, ph, o[d]);
         o[d] = mfma_bf16(vh, pm, o[d]);
         o[d] = mfma_bf16(vh, ph, o[d]);
+        if (c % 2)
+          fence();
       }
-    if (some)
-      add_nonfinite(o, pv, live, it, t0, hd, lane, fix, [&](int d, int e) { return 64 * (d / 4) + 4 * (4 * lq + e) + d % 4; });
-    if (t0 + stride < end)
-      load_v(t0 + stride);
+    fence();
+    load_v(t0 + stride);
+    fence();
   }
   if (odd != 0.0f)
     p.flags[1] = 1;
@@ -543,7 +534,7 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
     if (lq == 0)
       dst[HD] = m_run, dst[HD + 1] = l;
   }
-  __syncthreads();
+  met = __syncthreads_or(met);
   const int hd4 = hd / 4;
   for (int i = tid; i < it.vectors * hd4; i += kThreads) {
     const int v = i / hd4, d4 = i % hd4;
@@ -564,7 +555,7 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
     float *dst = p.partial + (it.slot0 + vec * it.slot_step) * (size_t)(hd + 4);
     *reinterpret_cast<float4 *>(dst + 4 * d4) = sum;
     if (d4 == 0)
-      dst[hd] = m, dst[hd + 1] = l;
+      *reinterpret_cast<float4 *>(dst + hd) = slot_end(m, l, met, it);
   }
 }
 
@@ -581,14 +572,11 @@ template <int HD> struct WideStage {
   float k_back[kUnit];  // 2^(e - 14): undoes a K row's scale
   float v_exp[kUnit];   // ev
   float v_back[kUnit];  // 2^-ev
-  float fix[kThreads / kWave * kUnit * 16];
-  int nonfinite;
 };
 
 template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
   typedef WideStage<HD> Stage;
   Stage &sh = *reinterpret_cast<Stage *>(lds);
-  float *fix = sh.fix;
   constexpr int kSteps = HD / 32, kDt = HD / 16, kLeastK = -100, kLeastV = -30;
   constexpr int kItems = kUnit * HD / 8 / kThreads; // K staging items of eight values a thread
   constexpr int kLanes = HD / 8;                    // a K row's
@@ -599,18 +587,19 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
   const bool v_stager = tid < kUnit / 4 * kVLanes;
   const int vg = tid / kVLanes, vd = 4 * (tid % kVLanes); // V item: positions 4 vg .. + 3, dimensions vd .. + 3
   float4 kr[kItems][2], vr[4];
+  bool met = false; // a value that is not finite
   auto load = [&](int t0) {
 #pragma unroll
     for (int u = 0; u < kItems; u++) {
       const int i = tid + u * kThreads, d = 8 * (i % kLanes);
       const float *row = it.key + (size_t)min(t0 + i / kLanes, it.t1 - 1) * it.pos_stride;
-      kr[u][0] = load4(row, d, hd);
-      kr[u][1] = load4(row, d + 4, hd);
+      kr[u][0] = row4(row, d, hd);
+      kr[u][1] = row4(row, d + 4, hd);
     }
     if (v_stager)
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        vr[e] = load4(it.value + (size_t)min(t0 + 4 * vg + e, it.t1 - 1) * it.pos_stride, vd, hd);
+        vr[e] = row4(it.value + (size_t)min(t0 + 4 * vg + e, it.t1 - 1) * it.pos_stride, vd, hd);
   };
   auto peak = [](const float4 &x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
   auto stage = [&]() {
@@ -639,7 +628,7 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
       for (int e = 0; e < 4; e++)
         odd = fmaf(vr[e].x, 0.0f, fmaf(vr[e].y, 0.0f, fmaf(vr[e].z, 0.0f, fmaf(vr[e].w, 0.0f, odd))));
       if (odd != 0.0f) {
-        sh.nonfinite = 1;
+        met = true;
 #pragma unroll
         for (int e = 0; e < 4; e++)
           vr[e] = float4{finite(vr[e].x) ? vr[e].x : 0.0f, finite(vr[e].y) ? vr[e].y : 0.0f,
@@ -708,8 +697,6 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
     for (int d = 0; d < kDt; d++)
       o[n][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  // positions up to here are seen by every vector of the tile
-  const int seen_by_all = it.last0 == INT32_MAX ? it.t1 : min(it.t1, it.last0 + 1);
   auto compute = [&](int t0) {
     v4f sc[2][2];
 #pragma unroll
@@ -733,40 +720,27 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
 #pragma unroll
           for (int n = 0; n < 2; n++)
             sc[n][t] = mfma_f16(k == 0 ? kl[t] : kh[t], k == 1 ? ql[n][st] : qh[n][st], sc[n][t]);
+      if (st % 2)
+        fence();
     }
-    const bool all = t0 + kUnit <= seen_by_all; // uniform
     v4i ph[2], pl[2];
-    float pv[2][8];
-    unsigned live[2] = {0, 0};
-    float4 k_back[2], v_exp[2], v_back[2];
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-      k_back[t] = *reinterpret_cast<const float4 *>(&sh.k_back[16 * t + 4 * lq]);
-      v_exp[t] = *reinterpret_cast<const float4 *>(&sh.v_exp[16 * t + 4 * lq]);
-      v_back[t] = *reinterpret_cast<const float4 *>(&sh.v_back[16 * t + 4 * lq]);
-    }
     auto of = [](const float4 &x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-      float top = -FLT_MAX;
+      float pv[8], top = -FLT_MAX;
+      const int seen = min(it.t1 - 1, last[n]) - t0 - 4 * lq; // of the lane's positions 16 t + e
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+      for (int t = 0; t < 2; t++) {
+        const float4 k_back = *reinterpret_cast<const float4 *>(&sh.k_back[16 * t + 4 * lq]);
+        const float4 v_exp = *reinterpret_cast<const float4 *>(&sh.v_exp[16 * t + 4 * lq]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float s = sc[n][t][e] * of(k_back[t], e) * q_back[n];
-          float x = s + of(v_exp[t], e);
-          if (all) {
-            odd = fmaf(s, 0.0f, odd);
-          } else {
-            const int at = t0 + 16 * t + 4 * lq + e;
-            const bool sees = at < it.t1 && at <= last[n];
-            odd = sees ? fmaf(s, 0.0f, odd) : odd;
-            x = sees ? x : -FLT_MAX;
-            live[n] |= (unsigned)sees << (4 * t + e);
-          }
-          pv[n][4 * t + e] = x;
-          top = fmaxf(top, x);
+          const float x = fmaf(sc[n][t][e] * of(k_back, e), q_back[n], of(v_exp, e));
+          pv[4 * t + e] = 16 * t + e <= seen ? x : -FLT_MAX;
+          odd = fmaf(pv[4 * t + e], 0.0f, odd);
+          top = fmaxf(top, pv[4 * t + e]);
         }
+      }
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float m_new = fmaxf(m_run[n], top);
@@ -778,23 +752,25 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
         for (int d = 0; d < kDt; d++)
           o[n][d] *= alpha;
       }
-      const float base = m_new - 15.0f; // weights up to 2^15
+      const float base = fmaxf(m_new, kMasked) - 15.0f; // weights up to 2^15
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        float w = __builtin_amdgcn_exp2f(pv[n][i] - base);
-        if (!all)
-          w = (live[n] >> i) & 1 ? w : 0.0f;
-        pv[n][i] = w;
-        sum = fmaf(w, of(v_back[i / 4], i % 4), sum);
+      for (int t = 0; t < 2; t++) {
+        const float4 v_back = *reinterpret_cast<const float4 *>(&sh.v_back[16 * t + 4 * lq]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          pv[4 * t + e] = __builtin_amdgcn_exp2f(pv[4 * t + e] - base);
+          sum = fmaf(pv[4 * t + e], of(v_back, e), sum);
+        }
       }
       l_run[n] += sum;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         int th, tl;
-        f16_pair(pv[n][2 * i], pv[n][2 * i + 1], 1.0f, th, tl);
+        f16_pair(pv[2 * i], pv[2 * i + 1], 1.0f, th, tl);
         ph[n][i] = th, pl[n][i] = tl;
       }
+      fence();
     }
 #pragma unroll
     for (int d = 0; d < kDt; d++) {
@@ -805,29 +781,24 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
 #pragma unroll
         for (int n = 0; n < 2; n++)
           o[n][d] = mfma_f16(k == 0 ? vl : vh, k == 1 ? pl[n] : ph[n], o[n][d]);
+      if (d % 4 == 3)
+        fence();
     }
-    if (sh.nonfinite)
-#pragma unroll
-      for (int n = 0; n < 2; n++)
-        add_nonfinite(o[n], pv[n], all ? (last[n] >= 0 ? 0xFFu : 0u) : live[n], it, t0, hd, lane,
-                      fix + wave * kUnit * 16, [&](int d, int e) { return 16 * d + 4 * lq + e; });
   };
   if (it.t0 < it.t1)
     load(it.t0);
   for (int t0 = it.t0; t0 < it.t1; t0 += kUnit) {
-    if (tid == 0)
-      sh.nonfinite = 0;
-    __syncthreads(); // the step before is done with the staged rows, and the mark is clear
+    __syncthreads(); // the step before is done with the staged rows
     stage();
     if (t0 + kUnit < it.t1)
       load(t0 + kUnit);
     __syncthreads();
     if (busy)
       compute(t0);
-    __syncthreads();
   }
   if (odd != 0.0f && (last[0] >= 0 || last[1] >= 0))
     p.flags[1] = 1;
+  met = __syncthreads_or(met);
 #pragma unroll
   for (int n = 0; n < 2; n++) {
     float l = l_run[n];
@@ -845,12 +816,12 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
         *reinterpret_cast<float4 *>(dst + 16 * d + 4 * lq) =
             float4{o[n][d][0] * back, o[n][d][1] * back, o[n][d][2] * back, o[n][d][3] * back};
     if (lq == 0)
-      dst[hd] = m_run[n], dst[hd + 1] = l * 0x1p-15f;
+      *reinterpret_cast<float4 *>(dst + hd) = slot_end(m_run[n], l * 0x1p-15f, met, it);
   }
 }
 
 template <int HD> constexpr size_t fast_lds() {
-  constexpr size_t narrow_q = (size_t)(kThreads / kWave) * ((HD / 32) * 3 * kWave * 16 + kUnit * 16 * 4);
+  constexpr size_t narrow_q = (size_t)(kThreads / kWave) * (HD / 32) * 3 * kWave * 16;
   constexpr size_t narrow_sums = (size_t)(kThreads / kWave) * 16 * (HD + 4) * 4;
   size_t most = sizeof(Plan);
   most = narrow_q > most ? narrow_q : most;
@@ -872,15 +843,15 @@ template <int HD> __global__ __launch_bounds__(kThreads, 2) void attn_requests(F
       if (plan.bad)
         p.flags[3] = 1;
     }
-    __shared__ int2 mine[kThreads];
+    __shared__ int4 mine[kThreads];
     const int r0 = blockIdx.x * kThreads;
-    mine[tid] = int2{0, -1};
+    mine[tid] = int4{0, -1, 0, 0};
     __syncthreads();
     for (int r = tid; r < p.batch.count; r += kThreads) {
       const int n = plan.rows[r], first = plan.first[r], shares = plan.shares[r];
       const int slot0 = plan.slots[r] - n * p.n_heads * shares;
       for (int i = max(first, r0); i < min(first + n, r0 + kThreads); i++)
-        mine[i - r0] = int2{slot0 + (i - first) * p.n_heads * shares, shares};
+        mine[i - r0] = int4{slot0 + (i - first) * p.n_heads * shares, shares, plan.slot[r], plan.length[r] + i - first};
     }
     __syncthreads();
     if (r0 + tid < p.batch.rows)
@@ -966,7 +937,7 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
   const int d4 = (int)(idx % hd4);
   const long long vec = idx / hd4;
   const int row = (int)(vec / p.n_heads), head = (int)(vec % p.n_heads);
-  const int2 mine = p.row_slots[row];
+  const int4 mine = p.row_slots[row];
   if (mine.y < 0)
     return;
   const int shared = p.header[0], count = shared + mine.y;
@@ -975,22 +946,21 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
   const float *own = p.partial + ((size_t)p.batch.rows * p.n_heads * shared + (size_t)mine.x + (size_t)head * mine.y) * slot;
   float m = -FLT_MAX, l = 0.0f;
   float4 o = float4{0.0f, 0.0f, 0.0f, 0.0f};
+  bool met = false;
   constexpr int kAhead = 4; // shares whose loads are in flight together
   for (int s0 = 0; s0 < count; s0 += kAhead) {
-    float ms[kAhead], ls[kAhead];
-    float4 x[kAhead];
+    float4 end[kAhead], x[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; k++) {
       const int s = min(s0 + k, count - 1);
       const float *src = s < shared ? far + (size_t)s * slot : own + (size_t)(s - shared) * slot;
-      ms[k] = s0 + k < count ? src[p.hd] : -FLT_MAX;
-      ls[k] = s0 + k < count ? src[p.hd + 1] : 0.0f;
+      end[k] = *reinterpret_cast<const float4 *>(src + p.hd);
       x[k] = *reinterpret_cast<const float4 *>(src + 4 * d4);
     }
     float top = m;
 #pragma unroll
     for (int k = 0; k < kAhead; k++)
-      top = fmaxf(top, ms[k]);
+      top = fmaxf(top, end[k].x); // the last share again past the count: the same maximum
     const float alpha = __builtin_amdgcn_exp2f(m - top);
     l *= alpha;
     o = float4{o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha};
@@ -998,10 +968,27 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
 #pragma unroll
     for (int k = 0; k < kAhead; k++)
       if (s0 + k < count) {
-        const float w = __builtin_amdgcn_exp2f(ms[k] - m);
-        l = fmaf(w, ls[k], l);
+        const float w = __builtin_amdgcn_exp2f(end[k].x - m);
+        l = fmaf(w, end[k].y, l);
         o = float4{fmaf(w, x[k].x, o.x), fmaf(w, x[k].y, o.y), fmaf(w, x[k].z, o.z), fmaf(w, x[k].w, o.w)};
+        met |= __float_as_int(end[k].w) != 0;
       }
+  }
+  if (met) { // V values that are not finite, whatever their weights: a positive one changes neither infinity nor NaN
+    const int g = head / p.kv_mul;
+    for (int s = 0; s < count; s++) {
+      const float *src = s < shared ? far + (size_t)s * slot : own + (size_t)(s - shared) * slot;
+      const bool prefix = s < shared;
+      const int t0 = __float_as_int(src[p.hd + 2]), t1 = __float_as_int(src[p.hd + 3]);
+      const float *v = prefix ? p.prefix_value + (size_t)g * p.batch.prefix_head_base
+                              : p.value + (size_t)mine.z * p.batch.slot_floats + (size_t)g * p.batch.head_base;
+      const size_t stride = prefix ? p.batch.prefix_pos_stride : p.batch.pos_stride;
+      for (int t = t0; t < (prefix ? t1 : min(t1, mine.w + 1)); t++) {
+        const float4 y = *reinterpret_cast<const float4 *>(v + (size_t)t * stride + 4 * d4);
+        o = float4{finite(y.x) ? o.x : o.x + y.x, finite(y.y) ? o.y : o.y + y.y, finite(y.z) ? o.z : o.z + y.z,
+                   finite(y.w) ? o.w : o.w + y.w};
+      }
+    }
   }
   *reinterpret_cast<float4 *>(p.out + (size_t)vec * p.hd + 4 * d4) = float4{o.x / l, o.y / l, o.z / l, o.w / l};
 }
@@ -1031,7 +1018,10 @@ FastBounds fast_bounds(const AttentionRequestsJob &job) {
   f.prefix_narrow = b.rows * kv_mul <= kNarrowVectors;
   f.prefix_tiles = !b.prefix ? 0 : f.prefix_narrow ? 1 : (b.rows + f.tile_rows - 1) / f.tile_rows;
   const long long own_tiles = (b.count < b.rows ? b.count : b.rows) + b.rows / f.tile_rows;
-  f.items = kTargetItems + job.n_kv_heads * (f.prefix_tiles + own_tiles);
+  const long long units = f.prefix_tiles * ((b.prefix + kUnit - 1) / kUnit) +
+                          own_tiles * (((long long)b.seq_len + kUnit - 1) / kUnit);
+  const long long shares = (units * job.n_kv_heads + kMinUnits - 1) / kMinUnits;
+  f.items = (shares < kTargetItems ? shares : kTargetItems) + job.n_kv_heads * (f.prefix_tiles + own_tiles);
   const long long vectors = (long long)b.rows * job.n_heads;
   // rows times shares, over the prefix and over the requests' own: see the plan; and no walk has more than kMaxShares
   const long long capped = 2 * vectors * kMaxShares, spread = 2 * vectors + (long long)kTileVectors * kTargetItems * 2;
@@ -1043,7 +1033,7 @@ size_t attention_requests_workspace(const AttentionRequestsJob &job) {
   if (!attention_requests_fast(job))
     return 0;
   return (size_t)fast_bounds(job).slots * (size_t)(job.head_dim + 4) * sizeof(float) +
-         (size_t)job.batch.rows * sizeof(int2) + 256;
+         (size_t)job.batch.rows * sizeof(int4) + 256;
 }
 
 bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hipStream_t stream) {
@@ -1065,8 +1055,8 @@ bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hip
   p.prefix_narrow = f.prefix_narrow;
   p.scale2 = 1.4426950408889634f / sqrtf((float)job.head_dim);
   p.header = (int *)workspace;
-  p.row_slots = (int2 *)((char *)workspace + 16);
-  p.partial = (float *)((char *)workspace + ((16 + (size_t)job.batch.rows * sizeof(int2) + 15) & ~(size_t)15));
+  p.row_slots = (int4 *)((char *)workspace + 16);
+  p.partial = (float *)((char *)workspace + ((16 + (size_t)job.batch.rows * sizeof(int4) + 15) & ~(size_t)15));
   p.flags = device().error_flags;
   const long long blocks = f.items + (job.batch.rows + kThreads - 1) / kThreads;
   if (job.head_dim <= 64)

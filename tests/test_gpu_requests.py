@@ -219,11 +219,12 @@ def test_attention_sharp_scores(L):
     attention_case(L, 10, 8, 2, 128, "head", b, scale=30.0)
 
 
-def test_attention_spread_values(L):
+@pytest.mark.parametrize("rows_of", [[1, 3], [40, 20]])
+def test_attention_spread_values(L, rows_of):
     """Keys and values of very different sizes from position to position and dimension to dimension."""
     L.kernels_kv_layout_select(b"head")
     heads, kv, hd = 8, 2, 128
-    b = ru.Batch(hu.dev, [1, 3], [90, 0], prefix=200, prefix_seq_len=200, seq_len=100)
+    b = ru.Batch(hu.dev, rows_of, [90 - rows_of[0], 0], prefix=200, prefix_seq_len=200, seq_len=100)
     rng = np.random.default_rng(11)
     spread = lambda shape: (rng.standard_normal(shape) * 10.0 ** rng.uniform(-6, 4, shape)).astype(F)  # noqa: E731
     q = (1e-3 * rng.standard_normal((b.rows, heads * hd))).astype(F)
@@ -235,6 +236,36 @@ def test_attention_spread_values(L):
     quiet(L)
     want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
     within(hu.host(out), want, bound)
+
+
+@pytest.mark.parametrize("rows", [3, 20, 45])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_attention_nonfinite_values_reach_only_the_rows_that_see_them(L, rows, value):
+    """V of an own position that only the last row sees, V of a prefix position in one dimension, K behind the diagonal: the
+    other rows and dimensions are as without them (one tile of a wave, and tiles of a block)."""
+    L.kernels_kv_layout_select(b"head")
+    heads, kv, hd = 8, 2, 128
+    rng = np.random.default_rng(rows)
+    b = ru.Batch(hu.dev, [rows, 1], [30, 2], prefix=90, prefix_seq_len=90, seq_len=100)
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    pk, pv = (rng.standard_normal((kv, 90, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((2, kv, 100, hd), dtype=F) for _ in range(2))
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
+    pv[1, 40, 7] = value
+    v[0, 0, 30 + rows - 1, 64:] = value
+    k[0, :, 30 + rows:] = value
+    out = hu.dev(np.zeros_like(q))
+    dev = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in dev], b.struct, heads, kv, hd)
+    quiet(L)
+    got = hu.host(out).reshape(b.rows, heads, hd)
+    hit = np.zeros(got.shape, bool)
+    hit[:, heads // 2:, 7] = True
+    hit[rows - 1, :heads // 2, 64:] = True
+    same = np.isnan(got[hit]) if np.isnan(value) else got[hit] == value
+    assert same.all()
+    rest = ~hit
+    within(got[rest], want.reshape(got.shape)[rest], bound.reshape(got.shape)[rest])
 
 
 def test_attention_refuses_what_lies_outside(L):
