@@ -61,7 +61,7 @@ size_t caches_bytes(const RequestBatch *b, int n_kv_heads, int head_dim) {
 }
 
 // The scratch of these calls, which the library stream orders: grown on demand (never during graph capture), kept for the
-// process. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows.
+// process. Its first 256 bytes are counters, zero between the calls. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows.
 void *scratch_memory = nullptr;
 size_t scratch_bytes = 0;
 bool scratch_captured = false;
@@ -87,6 +87,13 @@ bool workspace(const char *name, size_t bytes, void **out) {
       hbm_release(want);
       scratch_memory = nullptr;
       return raise("%s: allocating %zu bytes of workspace failed", name, want);
+    }
+    if (hipMemset(scratch_memory, 0, 256) != hipSuccess || hipDeviceSynchronize() != hipSuccess) { // counters
+      (void)hipGetLastError();
+      (void)hipFree(scratch_memory);
+      hbm_release(want);
+      scratch_memory = nullptr;
+      return raise("%s: clearing the workspace failed", name);
     }
     scratch_bytes = want;
   }

@@ -10,7 +10,6 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 namespace llhip {
 namespace {
@@ -167,6 +166,7 @@ constexpr int kNarrowVectors = 32; // at most, of a narrow one
 constexpr int kTargetItems = 512; // work items aimed at: one for each block that the chip holds
 constexpr int kMinUnits = 4;     // a step for each wave of a narrow block
 constexpr int kMaxShares = 32;   // of one walk
+constexpr int kWideCost = 2;     // a wide step takes about as long as this many narrow ones
 constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far below that its weight is zero, also where a
                                      // lane has seen nothing else
 
@@ -188,67 +188,93 @@ struct FastAttn {
 // What every block works out for itself from the batch's arrays: the walks (a tile of query vectors over a range of
 // positions), each cut into shares of about equal length so that all of them are about kTargetItems work items.
 struct Plan {
-  int first[kMaxRequests], rows[kMaxRequests], length[kMaxRequests], slot[kMaxRequests];
-  int shares[kMaxRequests];
   int items[kMaxRequests]; // running sum, the request's own included
   int slots[kMaxRequests]; // likewise
   long long units;
-  int longest, prefix_shares, bad;
+  int longest, step, bad;
+  int total_rows, first_row, end_row; // of the requests: their number, the lowest, one past the highest
   int wave_items[kThreads / kWave], wave_slots[kThreads / kWave];
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Tiles of a request's own walk: one narrow tile, or wide ones.
+// A request's own walk is one narrow tile, or wide ones.
+__device__ __forceinline__ bool own_narrow(const FastAttn &p, int rows) { return rows * p.kv_mul <= kNarrowVectors; }
 __device__ __forceinline__ int own_tiles(const FastAttn &p, int rows) {
-  return rows * p.kv_mul <= kNarrowVectors ? 1 : ceil_div(rows, p.tile_rows);
+  return own_narrow(p, rows) ? 1 : ceil_div(rows, p.tile_rows);
+}
+// Shares of a walk: as many as bring one down to `step` in narrow steps' time.
+__device__ __forceinline__ int own_shares(const FastAttn &p, const Request &q, int step) {
+  return q.rows ? ceil_div(ceil_div(q.length + q.rows, kUnit) * (own_narrow(p, q.rows) ? 1 : kWideCost), step) : 0;
+}
+__device__ __forceinline__ int prefix_cost(const FastAttn &p) {
+  return ceil_div(p.batch.prefix, kUnit) * (p.prefix_narrow ? 1 : kWideCost);
 }
 
 __device__ void make_plan(const FastAttn &p, Plan &plan) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  constexpr int kPer = kMaxRequests / kThreads; // requests of a thread, at most
   const int per = ceil_div(p.batch.count, kThreads), r0 = tid * per;
   if (tid == 0)
-    plan.units = 0, plan.longest = 0, plan.bad = 0;
+    plan.units = 0, plan.longest = 0, plan.bad = 0, plan.total_rows = 0, plan.first_row = p.batch.rows, plan.end_row = 0;
   __syncthreads();
   long long units = 0;
-  int longest = 0;
+  int longest = 0, total_rows = 0, first_row = p.batch.rows, end_row = 0, rows[kPer], u[kPer];
   bool bad = false;
-  for (int r = r0; r < min(r0 + per, p.batch.count); r++) {
-    const Request q = request_at(p.batch, r, bad);
-    plan.first[r] = q.first;
-    plan.rows[r] = q.rows;
-    plan.length[r] = q.length;
-    plan.slot[r] = q.slot;
-    if (q.rows) {
-      const int u = ceil_div(q.length + q.rows, kUnit);
-      units += (long long)own_tiles(p, q.rows) * u;
-      longest = max(longest, u);
+#pragma unroll
+  for (int k = 0; k < kPer; k++) {
+    rows[k] = u[k] = 0;
+    if (k < per && r0 + k < p.batch.count) {
+      const Request q = request_at(p.batch, r0 + k, bad);
+      rows[k] = q.rows;
+      total_rows = min(total_rows + q.rows, INT32_MAX / kThreads);
+      if (q.rows) {
+        first_row = min(first_row, q.first);
+        end_row = max(end_row, q.first + q.rows);
+      }
+      u[k] = q.rows ? ceil_div(q.length + q.rows, kUnit) : 0;
+      if (own_narrow(p, q.rows)) {
+        units += u[k];
+      } else {
+        units += (long long)own_tiles(p, q.rows) * u[k] * kWideCost;
+        u[k] *= kWideCost;
+      }
+      longest = max(longest, u[k]);
     }
   }
   for (int o = 32; o > 0; o >>= 1) {
     units += __shfl_xor(units, o);
     longest = max(longest, __shfl_xor(longest, o));
+    total_rows += __shfl_xor(total_rows, o);
+    first_row = min(first_row, __shfl_xor(first_row, o));
+    end_row = max(end_row, __shfl_xor(end_row, o));
   }
   if (lane == 0) {
     atomicAdd((unsigned long long *)&plan.units, (unsigned long long)units);
     atomicMax(&plan.longest, longest);
+    atomicAdd(&plan.total_rows, total_rows);
+    atomicMin(&plan.first_row, first_row);
+    atomicMax(&plan.end_row, end_row);
   }
   if (bad)
     plan.bad = 1;
   __syncthreads();
-  const int prefix_units = ceil_div(p.batch.prefix, kUnit);
+  if (plan.total_rows > p.batch.rows) { // requests over each other's rows (and some start above the next, so bad is set):
+    // none is taken, the launch and its workspace hold for rows that lie apart
+#pragma unroll
+    for (int k = 0; k < kPer; k++)
+      rows[k] = u[k] = 0;
+  }
+  const int prefix_units = prefix_cost(p);
   const long long total = (plan.units + (long long)p.prefix_tiles * prefix_units) * p.n_kv_heads;
   const int aim = (int)((total + kTargetItems - 1) / kTargetItems);
   const int step = max(max(kMinUnits, aim), ceil_div(max(plan.longest, prefix_units), kMaxShares));
   int items = 0, slots = 0;
-  for (int r = r0; r < min(r0 + per, p.batch.count); r++) {
-    const int n = plan.rows[r], u = ceil_div(plan.length[r] + n, kUnit);
-    const int shares = n ? ceil_div(u, step) : 0;
-    plan.shares[r] = shares;
-    items += n ? own_tiles(p, n) * shares * p.n_kv_heads : 0;
-    slots += n * p.n_heads * shares;
-    plan.items[r] = items;
-    plan.slots[r] = slots;
+#pragma unroll
+  for (int k = 0; k < kPer; k++) {
+    const int shares = ceil_div(u[k], step);
+    items += own_tiles(p, rows[k]) * shares * p.n_kv_heads;
+    slots += rows[k] * p.n_heads * shares;
   }
   // the sums of the threads before this one
   int item_run = items, slot_run = slots;
@@ -263,10 +289,15 @@ __device__ void make_plan(const FastAttn &p, Plan &plan) {
   item_run -= items, slot_run -= slots;
   for (int w = 0; w < wave; w++)
     item_run += plan.wave_items[w], slot_run += plan.wave_slots[w];
-  for (int r = r0; r < min(r0 + per, p.batch.count); r++)
-    plan.items[r] += item_run, plan.slots[r] += slot_run;
+#pragma unroll
+  for (int k = 0; k < kPer; k++)
+    if (k < per && r0 + k < p.batch.count) {
+      const int shares = ceil_div(u[k], step);
+      plan.items[r0 + k] = item_run += own_tiles(p, rows[k]) * shares * p.n_kv_heads;
+      plan.slots[r0 + k] = slot_run += rows[k] * p.n_heads * shares;
+    }
   if (tid == 0)
-    plan.prefix_shares = ceil_div(prefix_units, step);
+    plan.step = step;
   __syncthreads();
 }
 
@@ -286,6 +317,15 @@ struct Item {
 // step need more than the 256 registers that two waves a SIMD leave each).
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
+// The region's matrix instructions each followed by five others, which run while the matrix cores work.
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int i = 0; i < 48; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix
+    __builtin_amdgcn_sched_group_barrier(0x002, 5, 0); // vector
+  }
+}
+
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // The end of a partial sum's slot: maximum (base 2), sum of the weights, and, where the item met a V value that is not
@@ -295,28 +335,6 @@ __device__ __forceinline__ float4 slot_end(float m, float l, bool met, const Ite
   return float4{m, l, __int_as_float(it.t0), __int_as_float(met ? it.t1 : 0)};
 }
 
-// x = h + m + l exactly, each part 8 significant bits: the parts of eight values as three BF16 operands.
-__device__ __forceinline__ void bf16_parts(const float (&v)[8], v4i &ph, v4i &pm, v4i &pl) {
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    unsigned u[2][3];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-      const float x = v[2 * w + k];
-      u[k][0] = __float_as_uint(x);
-      const float r1 = x - __uint_as_float(u[k][0] & 0xFFFF0000u);
-      u[k][1] = __float_as_uint(r1);
-      u[k][2] = __float_as_uint(r1 - __uint_as_float(u[k][1] & 0xFFFF0000u));
-    }
-    ph[w] = (int)__builtin_amdgcn_perm(u[1][0], u[0][0], 0x07060302u);
-    pm[w] = (int)__builtin_amdgcn_perm(u[1][1], u[0][1], 0x07060302u);
-    pl[w] = (int)__builtin_amdgcn_perm(u[1][2], u[0][2], 0x07060302u);
-  }
-}
-
-__device__ __forceinline__ v4f mfma_bf16(const v4i &a, const v4i &b, v4f c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-}
 __device__ __forceinline__ v4f mfma_f16(const v4i &a, const v4i &b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
@@ -342,38 +360,68 @@ __device__ __forceinline__ float4 load4(const float *row, int d, int hd) {
   return d < hd ? *reinterpret_cast<const float4 *>(row + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-// Four values of a K or V row. Past the head's dimensions the row's first ones, so that the load is unconditional (a
-// branch a load would have each wait for the one before): the query's zeros take them out of a score, and a value sum's
-// dimensions there are not stored.
-__device__ __forceinline__ float4 row4(const float *row, int d, int hd) {
-  return *reinterpret_cast<const float4 *>(row + (d < hd ? d : 0));
+// K or V rows t0 .. t1 - 1 of an item as a buffer: a load past them reads zero, and a row's place is a 32-bit offset that a
+// step advances by one addition (a 64-bit address a load took a third of a step's vector instructions).
+struct Rows {
+  __amdgpu_buffer_rsrc_t rsrc;
+  unsigned stride; // bytes
+};
+__device__ __forceinline__ Rows rows_of(const float *cache, const Item &it, int hd) {
+  const uint64_t base = (uint64_t)(uintptr_t)(cache + (size_t)it.t0 * it.pos_stride);
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)base);
+  const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)(base >> 32));
+  const unsigned stride = __builtin_amdgcn_readfirstlane((unsigned)it.pos_stride * 4u);
+  const int n = __builtin_amdgcn_readfirstlane(it.t1 - it.t0);
+  const int bytes = n > 0 ? (n - 1) * (int)stride + hd * 4 : 0;
+  return Rows{__builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)(((uint64_t)hi << 32) | lo), (short)0, bytes, 0x00020000),
+              stride};
+}
+// Dimensions d .. d + 3 at byte offset `at` of its row's start, `rows` rows further; zero past the head's dimensions.
+template <bool FULL> __device__ __forceinline__ float4 row4(const Rows &r, unsigned at, int rows, int d, int hd) {
+  const unsigned off = at + 4u * (unsigned)d;
+  return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(r.rsrc, FULL || d < hd ? off : 0x7FFFFFF0u,
+                                                                          (unsigned)rows * r.stride, 0));
+}
+
+// The largest or the sum of a query vector's four lanes (lane, and 16, 32 and 48 lanes away), on the vector unit.
+__device__ __forceinline__ float four_max(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float four_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
 }
 
 // Narrow: at most 16 vectors a wave. The four waves walk 32-position steps in turn when the item has one tile of 16
 // vectors; with two tiles (or four) each tile has two waves (one) that walk all the steps, the rows that another wave has
 // read coming from the caches. K and V rows go straight into registers in the order the matrix instructions take them,
-// with no copy in LDS, and the waves' sums meet at the end. Products are exact three-part BF16 splits, as in attn_flash3.
-template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it, unsigned char *lds) {
+// with no copy in LDS, and the waves' sums meet at the end. The products are FP32 ones on the matrix cores, the cheapest
+// form where a K or V value meets so few vectors: the 128 instructions of a step take 4096 cycles, while BF16 parts take
+// 1536 and 3800 on the vector unit to split the values.
+template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, const Item &it, unsigned char *lds) {
   constexpr int kSteps = HD / 32, kDt = HD / 16, kWaves = kThreads / kWave, kRow = HD + 4;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
   const int hd = p.hd;
   const int tiles = it.vectors <= 16 ? 1 : it.vectors <= 32 ? 2 : 4, walkers = kWaves / tiles; // waves of a tile
   const int v_mine = 16 * (wave / walkers) + lc; // this lane's vector
   const bool active = v_mine < it.vectors;
-  v4i *qs = reinterpret_cast<v4i *>(lds) + (size_t)wave * kSteps * 3 * kWave + lane; // the wave's: [step][part][lane]
+  float qr[kSteps][8]; // dimensions 32 st + 8 lq .. + 7
   {
     const float *src = p.q + ((size_t)(it.row0 + (active ? v_mine / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
                               (active ? v_mine % p.kv_mul : 0)) * hd;
-    const float4 zero = float4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int st = 0; st < kSteps; st++) {
-      const int d = 32 * st + 8 * lq;
-      const float4 a = active ? load4(src, d, hd) : zero, b = active ? load4(src, d + 4, hd) : zero;
-      const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      v4i h, m, l;
-      bf16_parts(x, h, m, l);
-      qs[(size_t)st * 3 * kWave] = h, qs[(size_t)(st * 3 + 1) * kWave] = m, qs[(size_t)(st * 3 + 2) * kWave] = l;
-    }
+    for (int st = 0; st < kSteps; st++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int d = 32 * st + 8 * lq + 4 * h;
+        const float4 x = *reinterpret_cast<const float4 *>(src + (FULL || d < hd ? d : 0));
+        const float scale = active && (FULL || d < hd) ? p.scale2 : 0.0f;
+        qr[st][4 * h] = x.x * scale, qr[st][4 * h + 1] = x.y * scale, qr[st][4 * h + 2] = x.z * scale,
+        qr[st][4 * h + 3] = x.w * scale;
+      }
   }
   const int last = !active ? -1 : it.last0 == INT32_MAX ? INT32_MAX : it.last0 + v_mine / p.kv_mul;
   v4f o[kDt];
@@ -383,60 +431,51 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
   for (int d = 0; d < kDt; d++)
     o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   float4 kr[2][kSteps][2], vr[2][4][HD / 64];
-  auto load_k = [&](int t0) {
+  const Rows keys = rows_of(it.key, it, hd), values = rows_of(it.value, it, hd);
+  unsigned k_at = (unsigned)(wave % walkers * kUnit + lc) * keys.stride, v_at = (unsigned)(wave % walkers * kUnit + 4 * lq) * values.stride;
+  auto load_k = [&]() {
 #pragma unroll
-    for (int t = 0; t < 2; t++) {
-      const float *row = it.key + (size_t)min(t0 + 16 * t + lc, it.t1 - 1) * it.pos_stride;
+    for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int st = 0; st < kSteps; st++)
 #pragma unroll
         for (int h = 0; h < 2; h++)
-          kr[t][st][h] = row4(row, 32 * st + 8 * lq + 4 * h, hd);
-    }
+          kr[t][st][h] = row4<FULL>(keys, k_at, 16 * t, 32 * st + 8 * lq + 4 * h, hd);
+    k_at += (unsigned)(walkers * kUnit) * keys.stride;
   };
-  auto load_v = [&](int t0) {
+  auto load_v = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float *row = it.value + (size_t)min(t0 + 16 * t + 4 * lq + e, it.t1 - 1) * it.pos_stride;
+      for (int e = 0; e < 4; e++)
 #pragma unroll
         for (int j = 0; j < HD / 64; j++)
-          vr[t][e][j] = row4(row, 64 * j + 4 * lc, hd);
-      }
+          vr[t][e][j] = row4<FULL>(values, v_at, 16 * t + e, 64 * j + 4 * lc, hd);
+    v_at += (unsigned)(walkers * kUnit) * values.stride;
   };
   const int stride = walkers * kUnit;
   const int end = 16 * (wave / walkers) < it.vectors ? it.t1 : it.t0; // a tile without vectors walks nothing
   int t0 = it.t0 + wave % walkers * kUnit;
   if (t0 < end) {
-    load_k(t0);
-    load_v(t0);
+    load_k();
+    load_v();
   }
+  auto of = [](const float4 &x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
   for (; t0 < end; t0 += stride) {
-    v4f sc[2];
+    // S^T = K Q^T: instruction (st, i) takes dimension 32 st + 8 lq + i from lane group lq; two sums a position tile
+    v4f sc[2][2];
 #pragma unroll
     for (int t = 0; t < 2; t++)
-      sc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      sc[t][0] = sc[t][1] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int st = 0; st < kSteps; st++) {
-      const v4i qh = qs[(size_t)st * 3 * kWave], qm = qs[(size_t)(st * 3 + 1) * kWave],
-                ql = qs[(size_t)(st * 3 + 2) * kWave];
+    for (int st = 0; st < kSteps; st++)
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const float4 a = kr[t][st][0], b = kr[t][st][1];
-        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        v4i kh, km, kl;
-        bf16_parts(x, kh, km, kl);
-        sc[t] = mfma_bf16(kl, qh, sc[t]);
-        sc[t] = mfma_bf16(kh, ql, sc[t]);
-        sc[t] = mfma_bf16(km, qm, sc[t]);
-        sc[t] = mfma_bf16(km, qh, sc[t]);
-        sc[t] = mfma_bf16(kh, qm, sc[t]);
-        sc[t] = mfma_bf16(kh, qh, sc[t]);
-      }
-      fence();
-    }
-    load_k(t0 + stride); // past the end the last row again: a branch would have the next wait take these loads in
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+          sc[t][i & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(of(kr[t][st][i / 4], i % 4), qr[st][i], sc[t][i & 1], 0, 0, 0);
+    fence();
+    load_k(); // zeros past the end: a branch would have the next wait take these loads in
     fence();
     float pv[8], top = -FLT_MAX;
     const int seen = min(it.t1 - 1, last) - t0 - 4 * lq; // of the lane's positions 16 t + e
@@ -444,25 +483,26 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        pv[4 * t + e] = 16 * t + e <= seen ? sc[t][e] * p.scale2 : -FLT_MAX;
+        pv[4 * t + e] = 16 * t + e <= seen ? sc[t][0][e] + sc[t][1][e] : -FLT_MAX;
         odd = fmaf(pv[4 * t + e], 0.0f, odd);
         top = fmaxf(top, pv[4 * t + e]);
       }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float m_new = fmaxf(m_run, top), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    top = four_max(top);
+    const float m_new = fmaxf(m_run, top);
+    if (__any(m_new > m_run)) { // else nothing of the sums changes
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+      m_run = m_new;
+#pragma unroll
+      for (int d = 0; d < kDt; d++)
+        o[d] *= alpha;
+    }
     const float base = fmaxf(m_new, kMasked);
-    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       pv[i] = __builtin_amdgcn_exp2f(pv[i] - base);
-      sum += pv[i];
+      l_run += pv[i]; // this lane's positions; the four lanes of a vector meet at the end
     }
-    l_run = l_run * alpha + sum; // this lane's positions; the four lanes of a vector meet at the end
-    m_run = m_new;
-#pragma unroll
-    for (int d = 0; d < kDt; d++)
-      o[d] *= alpha;
     float nonfinite = 0.0f;
 #pragma unroll
     for (int t = 0; t < 2; t++)
@@ -486,44 +526,25 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
                        finite(x.w) ? x.w : 0.0f};
           }
     }
-    v4i ph, pm, pl;
-    bf16_parts(pv, ph, pm, pl);
+    // O^T += V^T P^T: instruction (t, e) takes position 16 t + 4 lq + e from lane group lq, which is where the weights
+    // are; tile 4 j + c holds dimensions 64 j + 4 m + c
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int d = 0; d < kDt; d++)
+          o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(of(vr[t][e][d / 4], d % 4), pv[4 * t + e], o[d], 0, 0, 0);
     fence();
-#pragma unroll
-    for (int j = 0; j < HD / 64; j++)
-#pragma unroll
-      for (int c = 0; c < 4; c++) { // tile 4 j + c: dimensions 64 j + 4 m + c
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float4 &v = vr[i / 4][i % 4][j];
-          x[i] = c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
-        }
-        v4i vh, vm, vl;
-        bf16_parts(x, vh, vm, vl);
-        const int d = 4 * j + c;
-        o[d] = mfma_bf16(vl, ph, o[d]);
-        o[d] = mfma_bf16(vh, pl, o[d]);
-        o[d] = mfma_bf16(vm, pm, o[d]);
-        o[d] = mfma_bf16(vm, ph, o[d]);
-        o[d] = mfma_bf16(vh, pm, o[d]);
-        o[d] = mfma_bf16(vh, ph, o[d]);
-        if (c % 2)
-          fence();
-      }
-    fence();
-    load_v(t0 + stride);
+    load_v();
     fence();
   }
   if (odd != 0.0f)
     p.flags[1] = 1;
   // the waves' sums: [wave][vector][HD values, maximum, sum]
-  __syncthreads(); // every wave is done with its query parts
   float *sums = reinterpret_cast<float *>(lds);
   {
-    float l = l_run;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    const float l = four_sum(l_run);
     float *dst = sums + (size_t)(wave * 16 + lc) * kRow;
 #pragma unroll
     for (int j = 0; j < HD / 64; j++)
@@ -565,18 +586,24 @@ template <int HD> __device__ void walk_narrow(const FastAttn &p, const Item &it,
 // its own, taken out of the score again; each group of four V rows likewise, and its exponent ev joins the score before
 // the exponential, so that the weights are exp2(s + ev - m) and meet V 2^-ev, with m the running maximum of s + ev. The
 // softmax's sum takes them times 2^-ev.
+// V parts lie transposed, a dimension's 32 slots in 64 bytes, its 16-byte units where v_unit puts them: a matrix operand's
+// read takes one unit of 16 dimensions, a staging write half a unit of every fourth one, and both spread over the banks.
 template <int HD> struct WideStage {
-  static constexpr int kKRow = HD + 8, kVRow = kUnit + 8;
+  static constexpr int kKRow = HD + 8;
   uint16_t k[2][kUnit * kKRow];
-  uint16_t v[2][HD * kVRow];
-  float k_back[kUnit];  // 2^(e - 14): undoes a K row's scale
-  float v_exp[kUnit];   // ev
-  float v_back[kUnit];  // 2^-ev
+  uint16_t v[2][HD * kUnit];
+  float k_back[kUnit]; // 2^(e - 14): undoes a K row's scale
+  float v_exp[kUnit];  // ev
+  float v_back[kUnit]; // 2^-ev
 };
+__device__ __forceinline__ int v_unit(int dim, int unit) { // in halves
+  const int four = dim >> 2;
+  return ((four << 2) | ((dim ^ four) & 3)) * kUnit + 8 * ((unit ^ four ^ (dim >> 4)) & 3);
+}
 
-template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
+template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
   typedef WideStage<HD> Stage;
-  Stage &sh = *reinterpret_cast<Stage *>(lds);
+  Stage *const stages = reinterpret_cast<Stage *>(lds); // two: a step is staged while the one before is computed
   constexpr int kSteps = HD / 32, kDt = HD / 16, kLeastK = -100, kLeastV = -30;
   constexpr int kItems = kUnit * HD / 8 / kThreads; // K staging items of eight values a thread
   constexpr int kLanes = HD / 8;                    // a K row's
@@ -584,25 +611,29 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
   static_assert(kItems >= 1 && kUnit / 4 * kVLanes <= kThreads, "staging items");
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
   const int hd = p.hd;
-  const bool v_stager = tid < kUnit / 4 * kVLanes;
+  constexpr bool kAllStage = kUnit / 4 * kVLanes == kThreads;
+  const bool v_stager = kAllStage || tid < kUnit / 4 * kVLanes;
   const int vg = tid / kVLanes, vd = 4 * (tid % kVLanes); // V item: positions 4 vg .. + 3, dimensions vd .. + 3
   float4 kr[kItems][2], vr[4];
   bool met = false; // a value that is not finite
-  auto load = [&](int t0) {
+  const Rows keys = rows_of(it.key, it, hd), values = rows_of(it.value, it, hd);
+  unsigned k_at = (unsigned)(tid / kLanes) * keys.stride, v_at = (unsigned)(4 * vg) * values.stride;
+  auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < kItems; u++) {
-      const int i = tid + u * kThreads, d = 8 * (i % kLanes);
-      const float *row = it.key + (size_t)min(t0 + i / kLanes, it.t1 - 1) * it.pos_stride;
-      kr[u][0] = row4(row, d, hd);
-      kr[u][1] = row4(row, d + 4, hd);
+      const int d = 8 * (tid % kLanes);
+      kr[u][0] = row4<FULL>(keys, k_at, u * (kThreads / kLanes), d, hd);
+      kr[u][1] = row4<FULL>(keys, k_at, u * (kThreads / kLanes), d + 4, hd);
     }
     if (v_stager)
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        vr[e] = row4(it.value + (size_t)min(t0 + 4 * vg + e, it.t1 - 1) * it.pos_stride, vd, hd);
+        vr[e] = row4<FULL>(values, v_at, e, vd, hd);
+    k_at += kUnit * keys.stride;
+    v_at += kUnit * values.stride;
   };
   auto peak = [](const float4 &x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
-  auto stage = [&]() {
+  auto stage = [&](Stage &sh) {
 #pragma unroll
     for (int u = 0; u < kItems; u++) {
       const int i = tid + u * kThreads, row = i / kLanes, d = 8 * (i % kLanes);
@@ -619,42 +650,43 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
       f16_pair(b.z, b.w, scale, th, tl), h[3] = th, l[3] = tl;
       *reinterpret_cast<v4i *>(&sh.k[0][row * Stage::kKRow + d]) = h;
       *reinterpret_cast<v4i *>(&sh.k[1][row * Stage::kKRow + d]) = l;
-      if (d == 0)
-        sh.k_back[row] = __uint_as_float((unsigned)(127 - 14 + e) << 23);
+      sh.k_back[row] = __uint_as_float((unsigned)(127 - 14 + e) << 23); // by all of the row's lanes: no branch
     }
     if (v_stager) {
-      float odd = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        odd = fmaf(vr[e].x, 0.0f, fmaf(vr[e].y, 0.0f, fmaf(vr[e].z, 0.0f, fmaf(vr[e].w, 0.0f, odd))));
-      if (odd != 0.0f) {
-        met = true;
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          vr[e] = float4{finite(vr[e].x) ? vr[e].x : 0.0f, finite(vr[e].y) ? vr[e].y : 0.0f,
-                         finite(vr[e].z) ? vr[e].z : 0.0f, finite(vr[e].w) ? vr[e].w : 0.0f};
-      }
       float top = fmaxf(fmaxf(peak(vr[0]), peak(vr[1])), fmaxf(peak(vr[2]), peak(vr[3])));
       top = group_reduce_max(top, kVLanes);
       int ev;
       const float scale = f16_scale(top, kLeastV, ev);
-      const int at = 8 * (vg % 4) + 4 * (vg / 4); // slot of position 16 t + 4 q + e: 8 q + 4 t + e
+      // slot of position 16 t + 4 q + e: 8 q + 4 t + e, so the four of this item are half of unit vg % 4
       auto put = [&](int d, float x0, float x1, float x2, float x3) {
         int h0, l0, h1, l1;
         f16_pair(x0, x1, scale, h0, l0);
         f16_pair(x2, x3, scale, h1, l1);
-        *reinterpret_cast<int2 *>(&sh.v[0][(vd + d) * Stage::kVRow + at]) = int2{h0, h1};
-        *reinterpret_cast<int2 *>(&sh.v[1][(vd + d) * Stage::kVRow + at]) = int2{l0, l1};
+        const int at = v_unit(vd + d, vg % 4) + 4 * (vg / 4);
+        *reinterpret_cast<int2 *>(&sh.v[0][at]) = int2{h0, h1};
+        *reinterpret_cast<int2 *>(&sh.v[1][at]) = int2{l0, l1};
       };
       put(0, vr[0].x, vr[1].x, vr[2].x, vr[3].x);
       put(1, vr[0].y, vr[1].y, vr[2].y, vr[3].y);
       put(2, vr[0].z, vr[1].z, vr[2].z, vr[3].z);
       put(3, vr[0].w, vr[1].w, vr[2].w, vr[3].w);
-      if (vd < 16) { // one lane a position
-        const int e = vd / 4;
-        sh.v_exp[4 * vg + e] = (float)ev;
-        sh.v_back[4 * vg + e] = __uint_as_float((unsigned)max(127 - ev, 1) << 23);
-      }
+      const int e = 4 * vg + tid % 4;
+      sh.v_exp[e] = (float)ev;
+      sh.v_back[e] = __uint_as_float((unsigned)max(127 - ev, 1) << 23);
+    }
+  };
+  // the loaded V values that are not finite become 0
+  auto check = [&]() {
+    float odd = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      odd = fmaf(vr[e].x, 0.0f, fmaf(vr[e].y, 0.0f, fmaf(vr[e].z, 0.0f, fmaf(vr[e].w, 0.0f, odd))));
+    if (__any(v_stager && odd != 0.0f)) {
+      met = true;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        vr[e] = float4{finite(vr[e].x) ? vr[e].x : 0.0f, finite(vr[e].y) ? vr[e].y : 0.0f,
+                       finite(vr[e].z) ? vr[e].z : 0.0f, finite(vr[e].w) ? vr[e].w : 0.0f};
     }
   };
   // the wave's query vectors: parts of dimensions 32 st + 8 lq .. + 7 of vector 32 wave + 16 n + lc
@@ -679,8 +711,7 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
         x[st][k] = active ? load4(src, 32 * st + 8 * lq + 4 * k, hd) : float4{0.0f, 0.0f, 0.0f, 0.0f};
         top = fmaxf(top, peak(x[st][k]));
       }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fminf(fmaxf(top, __shfl_xor(top, 32)), FLT_MAX);
+    top = fminf(four_max(top), FLT_MAX);
     int e;
     const float scale = f16_scale(top, kLeastK, e);
     q_back[n] = __uint_as_float((unsigned)(127 - 14 + e) << 23) * p.scale2;
@@ -697,8 +728,8 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
     for (int d = 0; d < kDt; d++)
       o[n][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  auto compute = [&](int t0) {
-    v4f sc[2][2];
+  v4f sc[2][2];
+  auto score = [&](const Stage &sh) {
 #pragma unroll
     for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -720,9 +751,9 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
 #pragma unroll
           for (int n = 0; n < 2; n++)
             sc[n][t] = mfma_f16(k == 0 ? kl[t] : kh[t], k == 1 ? ql[n][st] : qh[n][st], sc[n][t]);
-      if (st % 2)
-        fence();
     }
+  };
+  auto weigh_and_add = [&](const Stage &sh, int t0) {
     v4i ph[2], pl[2];
     auto of = [](const float4 &x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
 #pragma unroll
@@ -741,18 +772,17 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
           top = fmaxf(top, pv[4 * t + e]);
         }
       }
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float m_new = fmaxf(m_run[n], top);
-      if (__any(m_new > m_run[n])) { // else nothing of the sums changes
-        const float alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
+      // the running maximum moves only when a score passes it by 2^8, which the weights' range leaves room for: nearly
+      // all steps then need no exchange between lanes and no rescale
+      if (__any(top > m_run[n] + 8.0f)) {
+        const float m_new = fmaxf(m_run[n], four_max(top)), alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
         l_run[n] *= alpha;
         m_run[n] = m_new;
 #pragma unroll
         for (int d = 0; d < kDt; d++)
           o[n][d] *= alpha;
       }
-      const float base = fmaxf(m_new, kMasked) - 15.0f; // weights up to 2^15
+      const float base = fmaxf(m_run[n], kMasked) - 7.0f; // weights up to 2^15
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 2; t++) {
@@ -770,88 +800,115 @@ template <int HD> __device__ void walk_wide(const FastAttn &p, const Item &it, u
         f16_pair(pv[2 * i], pv[2 * i + 1], 1.0f, th, tl);
         ph[n][i] = th, pl[n][i] = tl;
       }
-      fence();
     }
+    fence();
 #pragma unroll
-    for (int d = 0; d < kDt; d++) {
-      const int at = (16 * d + lc) * Stage::kVRow + 8 * lq;
-      const v4i vh = *reinterpret_cast<const v4i *>(&sh.v[0][at]), vl = *reinterpret_cast<const v4i *>(&sh.v[1][at]);
+    for (int d = 0; d < kDt; d += 2) { // the products in turn over four sums, as above
+      v4i vh[2], vl[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int at = v_unit(16 * (d + i) + lc, lq);
+        vh[i] = *reinterpret_cast<const v4i *>(&sh.v[0][at]);
+        vl[i] = *reinterpret_cast<const v4i *>(&sh.v[1][at]);
+      }
 #pragma unroll
       for (int k = 0; k < 3; k++)
 #pragma unroll
-        for (int n = 0; n < 2; n++)
-          o[n][d] = mfma_f16(k == 0 ? vl : vh, k == 1 ? pl[n] : ph[n], o[n][d]);
-      if (d % 4 == 3)
-        fence();
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+            o[n][d + i] = mfma_f16(k == 0 ? vl[i] : vh[i], k == 1 ? pl[n] : ph[n], o[n][d + i]);
+      fence();
     }
   };
-  if (it.t0 < it.t1)
-    load(it.t0);
-  for (int t0 = it.t0; t0 < it.t1; t0 += kUnit) {
-    __syncthreads(); // the step before is done with the staged rows
-    stage();
-    if (t0 + kUnit < it.t1)
-      load(t0 + kUnit);
+  if (it.t0 < it.t1) {
+    load();
+    check();
+    stage(stages[0]);
+    load(); // zeros past the end
     __syncthreads();
-    if (busy)
-      compute(t0);
+  }
+  int turn = 0;
+  for (int t0 = it.t0; t0 < it.t1; t0 += kUnit, turn ^= 1) {
+    check();
+    fence();
+    if (busy) {
+      // the scores' matrix instructions with the next step's staging between them (its stage was read before the last
+      // barrier; past the end it takes zeros that nobody reads)
+      score(stages[turn]);
+      stage(stages[turn ^ 1]);
+      interleave();
+      fence();
+      load();
+      fence();
+      weigh_and_add(stages[turn], t0);
+    } else {
+      stage(stages[turn ^ 1]);
+      load();
+    }
+    __syncthreads();
   }
   if (odd != 0.0f && (last[0] >= 0 || last[1] >= 0))
     p.flags[1] = 1;
   met = __syncthreads_or(met);
 #pragma unroll
   for (int n = 0; n < 2; n++) {
-    float l = l_run[n];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    const float l = four_sum(l_run[n]);
     const int v = 32 * wave + 16 * n + lc;
     if (v >= it.vectors)
       continue;
     const size_t vec = (size_t)(it.row0 + v / p.kv_mul) * p.n_heads + (size_t)it.g * p.kv_mul + v % p.kv_mul;
     float *dst = p.partial + (it.slot0 + vec * it.slot_step) * (size_t)(hd + 4);
-    const float back = 0x1p-29f; // 2^14 of the V rows, 2^15 of the weights
+    const float back = 0x1p-21f; // 2^14 of the V rows, 2^7 of the weights
 #pragma unroll
     for (int d = 0; d < kDt; d++)
       if (16 * d + 4 * lq < hd)
         *reinterpret_cast<float4 *>(dst + 16 * d + 4 * lq) =
             float4{o[n][d][0] * back, o[n][d][1] * back, o[n][d][2] * back, o[n][d][3] * back};
     if (lq == 0)
-      *reinterpret_cast<float4 *>(dst + hd) = slot_end(m_run[n], l * 0x1p-15f, met, it);
+      *reinterpret_cast<float4 *>(dst + hd) = slot_end(m_run[n], l * 0x1p-7f, met, it);
   }
 }
 
 template <int HD> constexpr size_t fast_lds() {
-  constexpr size_t narrow_q = (size_t)(kThreads / kWave) * (HD / 32) * 3 * kWave * 16;
   constexpr size_t narrow_sums = (size_t)(kThreads / kWave) * 16 * (HD + 4) * 4;
   size_t most = sizeof(Plan);
-  most = narrow_q > most ? narrow_q : most;
   most = narrow_sums > most ? narrow_sums : most;
-  return sizeof(WideStage<HD>) > most ? sizeof(WideStage<HD>) : most;
+  return 2 * sizeof(WideStage<HD>) > most ? 2 * sizeof(WideStage<HD>) : most;
 }
 
-// Blocks: ceil(rows / 256) that write down each row's slots for the merge, then the prefix's items (KV head fastest, so
-// that consecutive blocks, which go to the XCDs in turn, give an XCD the same heads' rows), then the requests' own.
-template <int HD> __global__ __launch_bounds__(kThreads, 2) void attn_requests(FastAttn p) {
+// Blocks: ceil(rows / 256) that write down each row's slots for the merge, then one for each item, the prefix's first (KV
+// head fastest, so that consecutive blocks, which go to the XCDs in turn, give an XCD the same heads' rows), then the
+// requests' own. (Blocks that stay and take items from a counter were slower: 512 of them asking one counter wait for each
+// other, and their loads behind the answer with them.)
+template <int HD, bool FULL> __global__ __launch_bounds__(kThreads, 2) void attn_requests(FastAttn p) {
   extern __shared__ __align__(16) unsigned char lds[];
   Plan &plan = *reinterpret_cast<Plan *>(lds);
   make_plan(p, plan);
-  const int tid = threadIdx.x, row_blocks = ceil_div(p.batch.rows, kThreads);
-  const int prefix_shares = plan.prefix_shares, own_items = plan.items[p.batch.count - 1];
+  const int tid = threadIdx.x, step = plan.step;
+  const int row_blocks = ceil_div(p.batch.rows, kThreads);
+  const int prefix_shares = ceil_div(prefix_cost(p), step);
+  const int prefix_items = p.prefix_tiles * prefix_shares * p.n_kv_heads;
+  const size_t prefix_slots = (size_t)p.batch.rows * p.n_heads * prefix_shares;
+  if (blockIdx.x == 0 && tid == 0) {
+    p.header[0] = prefix_shares;
+    if (plan.bad)
+      p.flags[3] = 1;
+  }
   if ((int)blockIdx.x < row_blocks) {
-    if (blockIdx.x == 0 && tid == 0) {
-      p.header[0] = prefix_shares;
-      if (plan.bad)
-        p.flags[3] = 1;
-    }
     __shared__ int4 mine[kThreads];
     const int r0 = blockIdx.x * kThreads;
     mine[tid] = int4{0, -1, 0, 0};
     __syncthreads();
+    bool bad = false;
     for (int r = tid; r < p.batch.count; r += kThreads) {
-      const int n = plan.rows[r], first = plan.first[r], shares = plan.shares[r];
-      const int slot0 = plan.slots[r] - n * p.n_heads * shares;
-      for (int i = max(first, r0); i < min(first + n, r0 + kThreads); i++)
-        mine[i - r0] = int4{slot0 + (i - first) * p.n_heads * shares, shares, plan.slot[r], plan.length[r] + i - first};
+      const Request q = request_at(p.batch, r, bad);
+      if (plan.total_rows > p.batch.rows)
+        continue;
+      const int shares = own_shares(p, q, step);
+      const int slot0 = plan.slots[r] - q.rows * p.n_heads * shares;
+      for (int i = max(q.first, r0); i < min(q.first + q.rows, r0 + kThreads); i++)
+        mine[i - r0] = int4{slot0 + (i - q.first) * p.n_heads * shares, shares, q.slot, q.length + i - q.first};
     }
     __syncthreads();
     if (r0 + tid < p.batch.rows)
@@ -859,23 +916,19 @@ template <int HD> __global__ __launch_bounds__(kThreads, 2) void attn_requests(F
     return;
   }
   int i = blockIdx.x - row_blocks;
-  const int prefix_items = p.prefix_tiles * prefix_shares * p.n_kv_heads;
-  const size_t prefix_slots = (size_t)p.batch.rows * p.n_heads * prefix_shares;
+  if (i >= prefix_items + plan.items[p.batch.count - 1])
+    return;
   Item it;
   bool narrow;
   if (i < prefix_items) {
     it.g = i % p.n_kv_heads;
     i /= p.n_kv_heads;
     const int tile = i % p.prefix_tiles, share = i / p.prefix_tiles;
-    const int units = ceil_div(p.batch.prefix, kUnit), length = ceil_div(units, prefix_shares) * kUnit;
+    const int length = ceil_div(ceil_div(p.batch.prefix, kUnit), prefix_shares) * kUnit;
     const int rows = p.prefix_narrow ? p.batch.rows : p.tile_rows;
     // rows that belong to no request before the first and behind the last one stay out
-    const int first = min(max(p.batch.start[0], 0), p.batch.rows);
-    const int end = min(max(p.batch.start[p.batch.count], 0), p.batch.rows);
-    it.row0 = max(tile * rows, first);
-    it.vectors = (min(tile * rows + rows, end) - it.row0) * p.kv_mul;
-    if (it.vectors <= 0)
-      return;
+    it.row0 = max(tile * rows, plan.first_row);
+    it.vectors = max(min(tile * rows + rows, plan.end_row) - it.row0, 0) * p.kv_mul;
     it.key = p.prefix_key + (size_t)it.g * p.batch.prefix_head_base;
     it.value = p.prefix_value + (size_t)it.g * p.batch.prefix_head_base;
     it.pos_stride = p.batch.prefix_pos_stride;
@@ -887,8 +940,6 @@ template <int HD> __global__ __launch_bounds__(kThreads, 2) void attn_requests(F
     narrow = p.prefix_narrow;
   } else {
     i -= prefix_items;
-    if (i >= own_items)
-      return;
     int lo = 0, hi = p.batch.count - 1; // the first request whose running sum passes i
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
@@ -897,34 +948,37 @@ template <int HD> __global__ __launch_bounds__(kThreads, 2) void attn_requests(F
       else
         lo = mid + 1;
     }
-    const int r = lo, n = plan.rows[r], shares = plan.shares[r], tiles = own_tiles(p, n);
+    bool bad = false;
+    const int r = lo;
+    const Request q = request_at(p.batch, r, bad);
+    const int shares = own_shares(p, q, step), tiles = own_tiles(p, q.rows);
     i -= plan.items[r] - tiles * shares * p.n_kv_heads;
     it.g = i % p.n_kv_heads;
     i /= p.n_kv_heads;
     const int tile = i % tiles, share = i / tiles;
-    narrow = n * p.kv_mul <= kNarrowVectors;
-    const int j0 = narrow ? 0 : tile * p.tile_rows, rows = narrow ? n : min(p.tile_rows, n - j0);
-    const int end = plan.length[r] + j0 + rows;
+    narrow = own_narrow(p, q.rows);
+    const int j0 = narrow ? 0 : tile * p.tile_rows, rows = narrow ? q.rows : min(p.tile_rows, q.rows - j0);
+    const int end = q.length + j0 + rows;
     const int length = ceil_div(ceil_div(end, kUnit), shares) * kUnit;
-    const size_t cache = (size_t)plan.slot[r] * p.batch.slot_floats + (size_t)it.g * p.batch.head_base;
-    it.row0 = plan.first[r] + j0;
+    const size_t cache = (size_t)q.slot * p.batch.slot_floats + (size_t)it.g * p.batch.head_base;
+    it.row0 = q.first + j0;
     it.vectors = rows * p.kv_mul;
     it.key = p.key + cache;
     it.value = p.value + cache;
     it.pos_stride = p.batch.pos_stride;
     it.t0 = min(share * length, end);
     it.t1 = min(it.t0 + length, end);
-    it.last0 = plan.length[r] + j0;
+    it.last0 = q.length + j0;
     // the request's slots are [row][head][share]; slot0 makes up for vec counting from row 0 of the batch
-    it.slot0 = prefix_slots + (size_t)(plan.slots[r] - n * p.n_heads * shares) + share -
-               (size_t)plan.first[r] * p.n_heads * shares;
+    it.slot0 = prefix_slots + (size_t)(plan.slots[r] - q.rows * p.n_heads * shares) + share -
+               (size_t)q.first * p.n_heads * shares;
     it.slot_step = shares;
   }
   __syncthreads(); // the plan's place is taken by the walk
   if (narrow)
-    walk_narrow<HD>(p, it, lds);
+    walk_narrow<HD, FULL>(p, it, lds);
   else
-    walk_wide<HD>(p, it, lds);
+    walk_wide<HD, FULL>(p, it, lds);
 }
 
 // A thread per (row, head, four dimensions): the row's shares of the prefix and its own, rescaled to their largest maximum
@@ -979,11 +1033,11 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
     for (int s = 0; s < count; s++) {
       const float *src = s < shared ? far + (size_t)s * slot : own + (size_t)(s - shared) * slot;
       const bool prefix = s < shared;
-      const int t0 = __float_as_int(src[p.hd + 2]), t1 = __float_as_int(src[p.hd + 3]);
+      const int t0 = max(__float_as_int(src[p.hd + 2]), 0), t1 = __float_as_int(src[p.hd + 3]);
       const float *v = prefix ? p.prefix_value + (size_t)g * p.batch.prefix_head_base
                               : p.value + (size_t)mine.z * p.batch.slot_floats + (size_t)g * p.batch.head_base;
       const size_t stride = prefix ? p.batch.prefix_pos_stride : p.batch.pos_stride;
-      for (int t = t0; t < (prefix ? t1 : min(t1, mine.w + 1)); t++) {
+      for (int t = t0; t < min(t1, prefix ? p.batch.prefix : mine.w + 1); t++) {
         const float4 y = *reinterpret_cast<const float4 *>(v + (size_t)t * stride + 4 * d4);
         o = float4{finite(y.x) ? o.x : o.x + y.x, finite(y.y) ? o.y : o.y + y.y, finite(y.z) ? o.z : o.z + y.z,
                    finite(y.w) ? o.w : o.w + y.w};
@@ -1000,7 +1054,9 @@ bool attention_requests_fast(const AttentionRequestsJob &job) {
   const RequestsDev &b = job.batch;
   const uintptr_t all = (uintptr_t)job.out | (uintptr_t)job.q | (uintptr_t)job.prefix_key | (uintptr_t)job.prefix_value |
                         (uintptr_t)job.key | (uintptr_t)job.value;
-  return job.head_dim <= 128 && job.head_dim % 4 == 0 && (all & 15) == 0 && b.rows <= (1 << 20) && job.n_heads <= 1024;
+  // a walk's rows lie within 2^31 bytes, which its loads' 32-bit offsets reach
+  const bool near = (size_t)b.prefix * b.prefix_pos_stride < (1u << 29) && (size_t)b.seq_len * b.pos_stride < (1u << 29);
+  return job.head_dim <= 128 && job.head_dim % 4 == 0 && (all & 15) == 0 && b.rows <= (1 << 20) && job.n_heads <= 1024 && near;
 }
 
 // The most blocks and slots that a plan can ask for, whatever the arrays hold: every walk is cut into units / step + 1
@@ -1018,8 +1074,8 @@ FastBounds fast_bounds(const AttentionRequestsJob &job) {
   f.prefix_narrow = b.rows * kv_mul <= kNarrowVectors;
   f.prefix_tiles = !b.prefix ? 0 : f.prefix_narrow ? 1 : (b.rows + f.tile_rows - 1) / f.tile_rows;
   const long long own_tiles = (b.count < b.rows ? b.count : b.rows) + b.rows / f.tile_rows;
-  const long long units = f.prefix_tiles * ((b.prefix + kUnit - 1) / kUnit) +
-                          own_tiles * (((long long)b.seq_len + kUnit - 1) / kUnit);
+  const long long units = kWideCost * (f.prefix_tiles * ((b.prefix + kUnit - 1) / kUnit) +
+                                       own_tiles * (((long long)b.seq_len + kUnit - 1) / kUnit));
   const long long shares = (units * job.n_kv_heads + kMinUnits - 1) / kMinUnits;
   f.items = (shares < kTargetItems ? shares : kTargetItems) + job.n_kv_heads * (f.prefix_tiles + own_tiles);
   const long long vectors = (long long)b.rows * job.n_heads;
@@ -1055,14 +1111,29 @@ bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hip
   p.prefix_narrow = f.prefix_narrow;
   p.scale2 = 1.4426950408889634f / sqrtf((float)job.head_dim);
   p.header = (int *)workspace;
-  p.row_slots = (int4 *)((char *)workspace + 16);
-  p.partial = (float *)((char *)workspace + ((16 + (size_t)job.batch.rows * sizeof(int4) + 15) & ~(size_t)15));
+  p.row_slots = (int4 *)((char *)workspace + 256);
+  p.partial = (float *)((char *)workspace + 256 + (size_t)job.batch.rows * sizeof(int4));
   p.flags = device().error_flags;
   const long long blocks = f.items + (job.batch.rows + kThreads - 1) / kThreads;
-  if (job.head_dim <= 64)
-    hipLaunchKernelGGL(attn_requests<64>, dim3((unsigned)blocks), dim3(kThreads), fast_lds<64>(), stream, p);
-  else
-    hipLaunchKernelGGL(attn_requests<128>, dim3((unsigned)blocks), dim3(kThreads), fast_lds<128>(), stream, p);
+  const bool full = job.head_dim == 64 || job.head_dim == 128;
+  const auto kernel = job.head_dim <= 64 ? (full ? attn_requests<64, true> : attn_requests<64, false>)
+                                         : (full ? attn_requests<128, true> : attn_requests<128, false>);
+  const size_t lds = job.head_dim <= 64 ? fast_lds<64>() : fast_lds<128>();
+  static const hipError_t allowed = [] {
+    hipError_t e = hipSuccess;
+    auto allow = [&](const void *k, size_t bytes) {
+      if (e == hipSuccess)
+        e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    };
+    allow((const void *)attn_requests<64, true>, fast_lds<64>());
+    allow((const void *)attn_requests<64, false>, fast_lds<64>());
+    allow((const void *)attn_requests<128, true>, fast_lds<128>());
+    allow((const void *)attn_requests<128, false>, fast_lds<128>());
+    return e;
+  }();
+  if (allowed != hipSuccess)
+    return raise("allowing the attention kernel its LDS failed: %s", hipGetErrorString(allowed));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kThreads), lds, stream, p);
   if (!launch_ok("attn_requests"))
     return false;
   const long long threads = (long long)job.batch.rows * job.n_heads * (job.head_dim / 4);

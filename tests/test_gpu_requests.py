@@ -302,6 +302,14 @@ def test_attention_refuses_what_lies_outside(L):
     out = call(start=[-1, 2, 4])
     fails(L, "outside the batch's buffers")
     assert np.array_equal(hu.host(out)[2:], want[2:]) and (hu.host(out)[:2] == 0).all()
+    # requests over each other's rows, each whole in itself: nothing is done
+    out = call(rows_of=[1] * 9, length=[0] * 9, slot=[0] * 9, start=[0, 4, 0, 4, 0, 4, 0, 4, 0, 4])
+    fails(L, "outside the batch's buffers")
+    assert (hu.host(out) == 0).all()
+    # rows of a whole request behind start[count]
+    out = call(rows_of=[1] * 3, length=[0, 0, 3], slot=[0, 0, 1], start=[0, 0, 2, 0])
+    fails(L, "outside the batch's buffers")
+    assert np.array_equal(hu.host(out)[:2], want[:2]) and (hu.host(out)[2:] == 0).all()
     worse = q.copy()
     worse[3, 5] = np.inf
     call(q=worse)
