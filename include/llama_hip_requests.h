@@ -109,7 +109,8 @@ void llhip_lora_bf16(const float *x, int ldx, int m, int k, const int *adapter, 
  * accepted[r] receives the number of accepted drafts and next[r] the token after them; a request without rows keeps
  * both. Logits of -infinity are tokens masked out. A row that decides with a NaN, +infinity or no token left, and a
  * draft outside the vocabulary, set both to -1 and fail at the next host-visible point. Probabilities, sums and the
- * borders between tokens are FP64; uniform lies in [0, 1). At most LLHIP_MAX_REQUESTS requests. */
+ * borders between tokens are FP64; uniform lies in [0, 1). At most LLHIP_MAX_REQUESTS requests, 2^20
+ * rows and 2^22 tokens. */
 void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t ld, const float *draft_logits,
                          size_t draft_ld, const int *tokens, const float *uniform, const int *start, int count, int rows,
                          int vocab, float temperature);

@@ -349,6 +349,10 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
     raise("%s: rows of %d logits at strides %zu and %zu", name, vocab, ld, draft_logits ? draft_ld : ld);
     return;
   }
+  if (!verify_shape_ok(rows, vocab)) {
+    raise("%s: %d rows of %d tokens, at most 2^20 rows of 2^22 tokens are taken", name, rows, vocab);
+    return;
+  }
   if (!accepted || !next || !logits || !tokens || !start || (!greedy && !uniform)) {
     raise("%s: null buffer", name);
     return;
@@ -371,7 +375,10 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
                       draft_logits ? call.ptr<const float>(D) : nullptr, ld, draft_ld, call.ptr<const int>(T),
                       call.ptr<const int>(S), greedy ? nullptr : call.ptr<const float>(U), count, rows, vocab,
                       temperature};
-  if (launch_verify(job, call.stream()))
+  void *scratch = nullptr;
+  if (!workspace(name, verify_workspace(job), &scratch))
+    return;
+  if (launch_verify(job, scratch, call.stream()))
     call.finish();
 }
 

@@ -315,7 +315,9 @@ struct VerifyJob {
   int count, rows, vocab;
   float temperature;
 };
-bool launch_verify(const VerifyJob &job, hipStream_t stream);
+bool verify_shape_ok(int rows, int vocab);
+size_t verify_workspace(const VerifyJob &job); // bytes of scratch the launch takes
+bool launch_verify(const VerifyJob &job, void *workspace, hipStream_t stream);
 
 struct GemmSegmentDev {
   float *c;
