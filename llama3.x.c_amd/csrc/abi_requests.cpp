@@ -199,7 +199,10 @@ void lora(const char *name, const float *x, int ldx, int m, int k, const int *ad
                                 swiglu ? call.ptr<const void>(W[i][3]) : nullptr,
                                 s.scale ? call.ptr<const float>(S[i]) : nullptr, s.ldc, s.n, s.rank, swiglu};
   }
-  if (launch_lora(job, call.stream()))
+  void *scratch = nullptr;
+  if (!workspace(name, lora_workspace(job), &scratch))
+    return;
+  if (launch_lora(job, scratch, call.stream()))
     call.finish();
 }
 

@@ -304,7 +304,8 @@ struct LoraJob {
   bool bf16;
   LoraSegmentDev seg[3];
 };
-bool launch_lora(const LoraJob &job, hipStream_t stream);
+size_t lora_workspace(const LoraJob &job); // bytes of scratch the launch takes
+bool launch_lora(const LoraJob &job, void *workspace, hipStream_t stream);
 
 struct VerifyJob {
   int *accepted, *next;
