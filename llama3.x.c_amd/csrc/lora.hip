@@ -4,7 +4,7 @@
 //   lora_shrink   block (share of K, tile of 32 rows with one adapter, eight 16-entry tiles of A): the share's part of A x on
 //                 the BF16 matrix cores. The tiles are found in the adapter array by the blocks themselves.
 //   lora_join     the shares' parts added, for batches whose columns would each read them again.
-//   lora_expand   block (256 columns, tile of rows): base + scale B (A x), and for W1 and W3 their gate, read and written once.
+//   lora_expand   block (columns, tile of rows): base + scale B (A x), and for W1 and W3 their gate, read and written once.
 //   lora_rows     any shape: one block per row and segment, A x kept in LDS.
 //
 // The products are FP32-accurate: a value x is split exactly into three BF16 parts (8 bits each), and x y is taken as the
@@ -86,7 +86,6 @@ template <class T> __global__ __launch_bounds__(kThreads) void lora_rows(LoraJob
 
 constexpr int kTileRows = 32;
 constexpr int kMaxAdapters = 4096; // of the tiled form: their rows are counted in LDS
-constexpr int kColumns = 256;      // of an lora_expand block
 
 // The launch: A's of all segments (and A3's) as one list of matrices, their rows in 16-entry tiles side by side in A x.
 struct Tiled {
@@ -98,6 +97,7 @@ struct Tiled {
   bool skip_plain;            // rows without an adapter stay as they are
   int tiles;                  // row tiles at most
   int width;                  // floats of a row of A x: 16 * first_tile[matrices]
+  int columns;                // of an lora_expand block: a multiple of 128
   struct Tile {
     int adapter, rows;        // -1: none; 0 rows: no tile
     int row[kTileRows];
@@ -208,8 +208,40 @@ struct ShrinkLds {
   Tiled::Tile tile;
 };
 
-// The batch's tile number b: rows of one adapter in their order, 32 a tile, the adapters in theirs and the rows without one
-// last. Rows with an id outside the table are in none (bad).
+// The batch's tile number b, of at most 64 rows: a lane a row. A row whose place among its adapter's rows is 0 or 32 begins
+// a tile; tile b begins with the b-th such row. (Counting as below took 1.4 us more.)
+__device__ void find_tile_of_64(const Tiled &p, ShrinkLds &sh, int b, bool &bad) {
+  const int lane = threadIdx.x & (kWave - 1), m = p.job.m;
+  const int id = lane < m ? p.job.adapter[lane] : INT32_MIN;
+  const bool known = id >= -1 && id < p.job.adapters;
+  bad = lane < m && !known;
+  unsigned long long same = 0;
+#pragma unroll
+  for (int j = 0; j < kWave; j++)
+    same |= (unsigned long long)(__builtin_amdgcn_readlane(id, j) == id) << j;
+  const int place = __popcll(same & ((1ull << lane) - 1));
+  const bool begins = known && place % kTileRows == 0 && !(id == -1 && p.skip_plain);
+  unsigned long long begin = __ballot(begins);
+  for (int i = 0; i < b && begin; i++)
+    begin &= begin - 1;
+  if (threadIdx.x == 0)
+    sh.tile.rows = 0;
+  __syncthreads();
+  if (begin == 0)
+    return; // fewer tiles
+  const int first = __builtin_ctzll(begin), from = __shfl(place, first);
+  const bool mine = known && id == __builtin_amdgcn_readlane(id, first) && place >= from && place < from + kTileRows;
+  const unsigned long long rows = __ballot(mine);
+  if (threadIdx.x < kWave) { // one wave writes
+    if (mine)
+      sh.tile.row[place - from] = lane;
+    if (lane == first)
+      sh.tile.adapter = id, sh.tile.rows = __popcll(rows);
+  }
+}
+
+// Of any number of rows: the rows of one adapter in their order, 32 a tile, the adapters in theirs and the rows without one
+// last. Rows with an id outside the table are in none (bad). A thread looks through a run of rows.
 __device__ void find_tile(const Tiled &p, ShrinkLds &sh, int b, bool &bad) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, m = p.job.m, bins = p.job.adapters + 1;
   for (int i = tid; i < bins; i += kThreads)
@@ -225,6 +257,22 @@ __device__ void find_tile(const Tiled &p, ShrinkLds &sh, int b, bool &bad) {
       atomicAdd(&sh.count[bin], 1);
   }
   __syncthreads();
+  // a sum over the threads before this one
+  auto before = [&](int v) {
+    int run = v;
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int u = __shfl_up(run, o);
+      if (lane >= o)
+        run += u;
+    }
+    if (lane == kWave - 1)
+      sh.wave_sum[wave] = run;
+    __syncthreads();
+    run -= v;
+    for (int w = 0; w < wave; w++)
+      run += sh.wave_sum[w];
+    return run;
+  };
   const int per = (bins + kThreads - 1) / kThreads, b0 = min(tid * per, bins), b1 = min(b0 + per, bins);
   auto tiles_of = [&](int bin) {
     return bin == bins - 1 && p.skip_plain ? 0 : (sh.count[bin] + kTileRows - 1) / kTileRows;
@@ -232,18 +280,7 @@ __device__ void find_tile(const Tiled &p, ShrinkLds &sh, int b, bool &bad) {
   int tiles = 0;
   for (int i = b0; i < b1; i++)
     tiles += tiles_of(i);
-  int run = tiles;
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int v = __shfl_up(run, o);
-    if (lane >= o)
-      run += v;
-  }
-  if (lane == kWave - 1)
-    sh.wave_sum[wave] = run;
-  __syncthreads();
-  run -= tiles;
-  for (int w = 0; w < wave; w++)
-    run += sh.wave_sum[w];
+  int run = before(tiles);
   if (b >= run && b < run + tiles) // one thread's adapters hold the tile
     for (int i = b0; i < b1; i++) {
       const int n = tiles_of(i);
@@ -258,24 +295,18 @@ __device__ void find_tile(const Tiled &p, ShrinkLds &sh, int b, bool &bad) {
   const int from = sh.hit[1] * kTileRows, rows = min(kTileRows, sh.count[bin] - from);
   if (tid == 0)
     sh.tile.adapter = bin == bins - 1 ? -1 : bin, sh.tile.rows = rows;
-  int before = 0;
-  for (int i0 = 0; i0 < m && before < from + rows; i0 += kThreads) {
-    const int i = i0 + tid;
-    const bool mine = i < m && bin_of(p.job.adapter[i]) == bin;
-    const unsigned long long votes = __ballot(mine);
-    if (lane == 0)
-      sh.wave_sum[wave] = __popcll(votes);
-    __syncthreads();
-    int at = before + __popcll(votes & ((1ull << lane) - 1));
-    for (int w = 0; w < kThreads / kWave; w++) {
-      if (w < wave)
-        at += sh.wave_sum[w];
-      before += sh.wave_sum[w];
-    }
-    if (mine && at >= from && at < from + rows)
-      sh.tile.row[at - from] = i;
-    __syncthreads();
-  }
+  const int each = (m + kThreads - 1) / kThreads, i0 = min(tid * each, m), i1 = min(i0 + each, m);
+  int found = 0;
+  for (int i = i0; i < i1; i++)
+    found += bin_of(p.job.adapter[i]) == bin;
+  int at = before(found);
+  if (at < from + rows && at + found > from)
+    for (int i = i0; i < i1; i++)
+      if (bin_of(p.job.adapter[i]) == bin) {
+        if (at >= from && at < from + rows)
+          sh.tile.row[at - from] = i;
+        at++;
+      }
 }
 
 // One block's part of A x for RT * 16 rows and NR 16-entry tiles of A (the last ones repeated past the launch's number).
@@ -306,31 +337,53 @@ __device__ __forceinline__ void shrink(const Tiled &p, const Tiled::Tile &tile, 
       acc[i][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   const int parts = p.shares * (kThreads / kWave), part = share * (kThreads / kWave) + wave;
   const int s0 = (int)((long long)p.steps * part / parts), s1 = (int)((long long)p.steps * (part + 1) / parts);
-  for (int s = s0; s < s1; s++) {
-    const bool inside = 32 * s + 8 * lq < p.job.k;
-    const int at = inside ? 32 * s : 0;
+  // a step's operands, the next one's on their way while this one's products are formed
+  struct Step {
     Operand<T> w[NR];
     float4 xa[RT], xb[RT];
+  };
+  auto load = [&](Step &st, int s) {
+    const bool inside = 32 * s + 8 * lq < p.job.k;
+    const int at = inside ? 32 * s : -8 * lq; // past K the row's first values: A's are set to zero
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+      st.xa[t] = *reinterpret_cast<const float4 *>(x[t] + at), st.xb[t] = *reinterpret_cast<const float4 *>(x[t] + at + 4);
 #pragma unroll
     for (int i = 0; i < NR; i++)
-      w[i].load(a[i] + (inside ? at : -8 * lq));
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-      const float *src = x[t] + (inside ? at : -8 * lq);
-      xa[t] = *reinterpret_cast<const float4 *>(src), xb[t] = *reinterpret_cast<const float4 *>(src + 4);
-    }
+      st.w[i].load(a[i] + at);
+  };
+  auto add = [&](Step &st, int s) {
     if (p.job.k % 32) // uniform
 #pragma unroll
       for (int i = 0; i < NR; i++)
-        w[i].keep(inside);
+        st.w[i].keep(32 * s + 8 * lq < p.job.k);
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-      const float v[8] = {xa[t].x, xa[t].y, xa[t].z, xa[t].w, xb[t].x, xb[t].y, xb[t].z, xb[t].w};
+      const float v[8] = {st.xa[t].x, st.xa[t].y, st.xa[t].z, st.xa[t].w, st.xb[t].x, st.xb[t].y, st.xb[t].z, st.xb[t].w};
       v4i h, m, l;
       parts_of(v, h, m, l);
 #pragma unroll
       for (int i = 0; i < NR; i++)
-        acc[i][t] = w[i].times(h, m, l, acc[i][t]);
+        acc[i][t] = st.w[i].times(h, m, l, acc[i][t]);
+    }
+  };
+  Step one;
+  if constexpr (NR <= 4) {
+    Step two;
+    if (s0 < s1) {
+      load(one, s0);
+      for (int s = s0; s < s1; s += 2) {
+        load(two, min(s + 1, s1 - 1)); // unconditional: a branch would have the products wait for these loads too
+        add(one, s);
+        load(one, min(s + 2, s1 - 1));
+        if (s + 1 < s1)
+          add(two, s + 1);
+      }
+    }
+  } else { // two steps' operands would leave one wave to a SIMD
+    for (int s = s0; s < s1; s++) {
+      load(one, s);
+      add(one, s);
     }
   }
   // the waves' sums: 2 and 3 to 0 and 1, then 1 to 0
@@ -367,7 +420,10 @@ template <class T, int NR> __global__ __launch_bounds__(kThreads) void lora_shri
   __shared__ __align__(16) float red[2 * NR * 2 * 4 * kWave];
   const int share = blockIdx.x, b = blockIdx.y, t0 = blockIdx.z * NR;
   bool bad = false;
-  find_tile(p, sh, b, bad);
+  if (p.job.m <= kWave)
+    find_tile_of_64(p, sh, b, bad);
+  else
+    find_tile(p, sh, b, bad);
   if (bad && share == 0 && b == 0 && t0 == 0)
     p.flags[5] = 1;
   __syncthreads();
@@ -394,9 +450,8 @@ __global__ __launch_bounds__(kThreads) void lora_join(Tiled p) {
   *reinterpret_cast<v4f *>(p.joined + at) = sum;
 }
 
-// Block (256 columns of a segment, tile of rows). The tile's A x goes into LDS as its three parts; a wave takes 64 columns
-// in pairs of 16-column tiles, columns 8 q + e and 8 q + 4 + e of the pair in its first and second, so that a lane ends
-// with eight consecutive columns of its row and a row's accesses are whole cache lines.
+// Block (p.columns of a segment, tile of rows). The tile's A x goes into LDS as its three parts; a wave takes 32 columns
+// at a time, two 16-column tiles; the base rows are asked for before anything else.
 template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) void lora_expand(Tiled p) {
   extern __shared__ __align__(16) unsigned char lds[];
   const Tiled::Tile &tile = p.tile[blockIdx.y];
@@ -405,14 +460,20 @@ template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) 
     return;
   int chunk = blockIdx.x, s = 0, first_matrix = 0;
   LoraSegmentDev seg = pick(p.job, 0);
-  while (chunk >= (seg.n + kColumns - 1) / kColumns) { // the segment of this block's columns
-    chunk -= (seg.n + kColumns - 1) / kColumns;
+  while (chunk >= (seg.n + p.columns - 1) / p.columns) { // the segment of this block's columns
+    chunk -= (seg.n + p.columns - 1) / p.columns;
     first_matrix += seg.swiglu ? 2 : 1;
     seg = pick(p.job, ++s);
   }
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
   const int parts = seg.swiglu ? 2 : 1, pad = (seg.rank + 31) / 32 * 32, stride = pad + 8;
   uint16_t *low = reinterpret_cast<uint16_t *>(lds); // [matrix][part][32][stride]
+  int row_of[2]; // the lane's rows; past the tile's last, that one
+#pragma unroll
+  for (int t = 0; t < 2; t++)
+    row_of[t] = tile.row[min(16 * t + lc, rows - 1)];
+  const float scale = adapter >= 0 && seg.scale ? seg.scale[adapter] : 1.0f;
+  bool staged = false;
   if (adapter >= 0) {
     // sums of the shares, split: eight entries of a row an item, zeros past the rank
     for (int i = tid; i < parts * rows * (pad / 8); i += kThreads) {
@@ -439,11 +500,32 @@ template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) 
       *reinterpret_cast<v4i *>(dst + kTileRows * stride) = m;
       *reinterpret_cast<v4i *>(dst + 2 * kTileRows * stride) = l;
     }
-    __syncthreads();
   }
-  const float scale = adapter >= 0 && seg.scale ? seg.scale[adapter] : 1.0f;
-  const int end = min(seg.n, (chunk + 1) * kColumns);
-  for (int n0 = chunk * kColumns + 32 * wave; n0 < end; n0 += 32 * (kThreads / kWave)) {
+  const int end = min(seg.n, (chunk + 1) * p.columns);
+  for (int n0 = chunk * p.columns + 32 * wave; n0 < end; n0 += 32 * (kThreads / kWave)) {
+    // the base rows first: they come from far
+    float4 y[2][2], z[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+      if (16 * t < rows) // uniform
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const int n = n0 + 16 * c + 4 * lq;
+          const size_t at = (size_t)row_of[t] * seg.ldc + (VEC ? min(n, seg.n - 4) : 0);
+          if (VEC) {
+            y[t][c] = *reinterpret_cast<const float4 *>(seg.base + at);
+            if (seg.swiglu)
+              z[t][c] = *reinterpret_cast<const float4 *>(seg.base3 + at);
+          } else {
+            float u[4], v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              u[e] = seg.base[at + min(n + e, seg.n - 1)];
+              v[e] = seg.swiglu ? seg.base3[at + min(n + e, seg.n - 1)] : 0.0f;
+            }
+            y[t][c] = float4{u[0], u[1], u[2], u[3]}, z[t][c] = float4{v[0], v[1], v[2], v[3]};
+          }
+        }
     v4f acc[2][2][2]; // [matrix][row tile][column tile]
 #pragma unroll
     for (int part = 0; part < 2; part++)
@@ -453,22 +535,30 @@ template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) 
     if (adapter >= 0)
       for (int r0 = 0; r0 < seg.rank; r0 += 32) {
         const int r = r0 + 8 * lq;
+        Operand<T> w[2][2];
 #pragma unroll
         for (int part = 0; part < 2; part++)
           if (part < parts) {
             const T *b = (const T *)(part ? seg.b3 : seg.b) + (size_t)adapter * seg.n * seg.rank;
-            Operand<T> w[2];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-              const int n = min(n0 + 8 * (lc / 4) + 4 * c + lc % 4, seg.n - 1);
+              const int n = min(n0 + 16 * c + lc, seg.n - 1);
               const T *src = b + (size_t)n * seg.rank;
               if constexpr (RANK8) {
-                w[c].load(src + (r < seg.rank ? r : 0));
-                w[c].keep(r < seg.rank);
+                w[part][c].load(src + (r < seg.rank ? r : 0));
+                w[part][c].keep(r < seg.rank);
               } else {
-                w[c].load_some(src + (r < seg.rank ? r : 0), r < seg.rank ? seg.rank - r : 0);
+                w[part][c].load_some(src + (r < seg.rank ? r : 0), r < seg.rank ? seg.rank - r : 0);
               }
             }
+          }
+        if (!staged) { // the block's first products: the parts are whole behind this barrier
+          __syncthreads();
+          staged = true;
+        }
+#pragma unroll
+        for (int part = 0; part < 2; part++)
+          if (part < parts) {
             const uint16_t *src = low + (size_t)part * 3 * kTileRows * stride + r;
 #pragma unroll
             for (int t = 0; t < 2; t++)
@@ -478,7 +568,7 @@ template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) 
                           l = *reinterpret_cast<const v4i *>(at + 2 * kTileRows * stride);
 #pragma unroll
                 for (int c = 0; c < 2; c++)
-                  acc[part][t][c] = w[c].times(h, m, l, acc[part][t][c]);
+                  acc[part][t][c] = w[part][c].times(h, m, l, acc[part][t][c]);
               }
           }
       }
@@ -486,41 +576,32 @@ template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) 
     for (int t = 0; t < 2; t++) {
       if (16 * t + lc >= rows)
         continue;
-      const size_t row = (size_t)tile.row[16 * t + lc] * seg.ldc;
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        const int n = n0 + 8 * lq + 4 * c;
-        float y[4], z[4];
-        if (VEC) {
-          if (n >= end)
-            continue;
-          *reinterpret_cast<float4 *>(y) = *reinterpret_cast<const float4 *>(seg.base + row + n);
-          if (seg.swiglu)
-            *reinterpret_cast<float4 *>(z) = *reinterpret_cast<const float4 *>(seg.base3 + row + n);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            y[e] = n + e < end ? seg.base[row + n + e] : 0.0f;
-            z[e] = seg.swiglu && n + e < end ? seg.base3[row + n + e] : 0.0f;
-          }
-        }
+        const int n = n0 + 16 * c + 4 * lq;
+        float u[4] = {y[t][c].x, y[t][c].y, y[t][c].z, y[t][c].w};
+        const float v[4] = {z[t][c].x, z[t][c].y, z[t][c].z, z[t][c].w};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          y[e] = fmaf(scale, acc[0][t][c][e], y[e]);
+          u[e] = fmaf(scale, acc[0][t][c][e], u[e]);
           if (seg.swiglu)
-            y[e] = silu(y[e]) * fmaf(scale, acc[1][t][c][e], z[e]);
+            u[e] = silu(u[e]) * fmaf(scale, acc[1][t][c][e], v[e]);
         }
+        float *dst = seg.c + (size_t)row_of[t] * seg.ldc + n;
         if (VEC) {
-          *reinterpret_cast<float4 *>(seg.c + row + n) = *reinterpret_cast<const float4 *>(y);
+          if (n < end)
+            *reinterpret_cast<float4 *>(dst) = float4{u[0], u[1], u[2], u[3]};
         } else {
 #pragma unroll
           for (int e = 0; e < 4; e++)
             if (n + e < end)
-              seg.c[row + n + e] = y[e];
+              dst[e] = u[e];
         }
       }
     }
   }
+  if (adapter >= 0 && !staged)
+    __syncthreads(); // a wave without columns of its own meets the others'
 }
 
 } // namespace
@@ -550,10 +631,10 @@ LoraShape lora_shape(const LoraJob &job) {
   f.width = 16 * f.first_tile[f.matrices];
   const int groups = job.adapters + 1 < job.m ? job.adapters + 1 : job.m;
   f.tiles = job.m / kTileRows + groups;
-  // shares of K: two blocks a CU, each wave at least two steps of 32 values
+  // shares of K: four blocks a CU (one: 82 us for 1100 rows beside W1 and W3, two 83, four 81), each wave at least two steps of 32 values
   const int cus = device().cu_count > 0 ? device().cu_count : 256, steps = (job.k + 31) / 32;
   const int most = steps / (2 * kThreads / kWave) > 1 ? steps / (2 * kThreads / kWave) : 1;
-  const int want = (2 * cus + f.tiles - 1) / f.tiles;
+  const int want = (4 * cus + f.tiles - 1) / f.tiles;
   f.shares = want < most ? want : most;
   f.join = job.m > 64 && f.shares > 1;
   return f;
@@ -597,13 +678,19 @@ template <class T> bool launch_tiled(const LoraJob &job, void *workspace, hipStr
     if (!launch_ok("lora_join"))
       return false;
   }
+  // Blocks of 128 columns where few rows leave the chip idle with 256 (10 instead of 11 us for one row, 13.0 instead of 13.6
+  // for 32 beside QKV); of 256 else, which stage A x half as often (1100 rows beside W1 and W3: 86 us, 88 with 128, 89 with 512).
+  long wide = 0;
+  for (int s = 0; s < job.nseg; s++)
+    wide += (long)((job.seg[s].n + 255) / 256) * f.tiles;
+  p.columns = wide >= 1024 ? 256 : 128;
   bool vec = true, rank8 = true;
   int chunks = 0, pad = 0;
   for (int s = 0; s < job.nseg; s++) {
     const LoraSegmentDev &g = job.seg[s];
     vec &= g.n % 4 == 0 && g.ldc % 4 == 0 && (((uintptr_t)g.c | (uintptr_t)g.base | (uintptr_t)g.base3) & 15) == 0;
     rank8 &= g.rank % 8 == 0 && (((uintptr_t)g.b | (uintptr_t)g.b3) & 15) == 0;
-    chunks += (g.n + kColumns - 1) / kColumns;
+    chunks += (g.n + p.columns - 1) / p.columns;
     const int mine = (g.swiglu ? 2 : 1) * ((g.rank + 31) / 32 * 32 + 8);
     pad = mine > pad ? mine : pad;
   }
