@@ -32,6 +32,15 @@ float *engine_forward(Model *model, int token, int position);
  * last row, ALL count x vocab_size in row order, NONE returns NULL; the storage belongs to the model and is
  * invalidated by the next forward. */
 float *engine_forward_batch(Model *model, const int *tokens, int count, int pos0, LogitsWanted want);
+/* A decode step over drafted tokens: tokens[0] is the token at pos0 (the prefix [0, pos0) run before), tokens[1 ..
+ * count - 1] were drafted for the positions behind it, 1 <= count <= engine_max_batch. The rows run as
+ * engine_forward_batch's with every row's logits, which stay on the device, and llhip_verify_drafts (llama_hip_requests.h:
+ * draft_logits, draft_ld, uniform and temperature are its arguments, in host or device memory) judges the drafts.
+ * Returns how many were accepted, n of 0 .. count - 1, and in *next the token behind them; the next call takes *next at
+ * pos0 + n + 1, which overwrites the refused drafts' cache rows. -1 when the call failed in record mode; *next is then
+ * unchanged. */
+int llhip_engine_verify(Model *model, const int *tokens, int count, int pos0, const float *draft_logits, size_t draft_ld,
+                        const float *uniform, float temperature, int *next);
 void engine_free(Model *model);   /* runtime.h:114 */
 int engine_group_size(void);      /* runtime.h:116: the last loaded checkpoint's group size (0 for FP32) */
 /* runtime.h:115 (src/engine.c:191-195) for the last loaded checkpoint: "int8_q8_0", "int8_q8_0_w8a32" (Q8_0 with

@@ -30,6 +30,7 @@
 #include "llama_hip_engine.h"
 #include "llama_hip_forward.h"
 #include "llama_hip_gemm.h"
+#include "llama_hip_requests.h"
 
 namespace llhip {
 namespace {
@@ -471,8 +472,9 @@ Engine *open_engine(Model *model, const char *path, int context, bool a32) {
 // RoPE, the K/V cache (head-major: staged rows then k_kv_store; rows layout: written in place), attention, quantize,
 // Wo + residual, RMSNorm, quantize, W1/W3 SwiGLU, quantize, W2 + residual; then the final RMSNorm in place, quantize
 // and the classifier. W8A32 hands the FP32 rows to the GEMVs instead of quantizing; FP32 runs the FP32 GEMVs. The
-// classifier runs only when the logits are wanted (src/engine.c:75-77); they land in e->host_logits.
-bool forward(Engine *e, int token, int pos, bool want_logits) {
+// classifier runs only when the logits are wanted (src/engine.c:75-77); they land in e->host_logits, or stay on the
+// device at `stay`.
+bool forward(Engine *e, int token, int pos, bool want_logits, float *stay = nullptr) {
   const Config &c = e->c;
   const int d = c.dim, hidden = c.hidden_dim, hd = c.head_dim, gs = e->gs, nh = c.n_heads, nkv = c.n_kv_heads;
   const size_t kvl = (size_t)hd * nkv;
@@ -538,13 +540,14 @@ bool forward(Engine *e, int token, int pos, bool want_logits) {
   if (want_logits) {
     k_rmsnorm(e->x, e->x, e->rms_final, d, c.norm_eps);
     quantize(e->xq, e->xs, e->x, d);
+    float *logits = stay ? stay : e->logits;
     if (e->q8)
-      k_matmul_q8(e->logits, &in_x, e->cls.k8(), d, c.vocab_size, gs);
+      k_matmul_q8(logits, &in_x, e->cls.k8(), d, c.vocab_size, gs);
     else
-      k_matmul(e->logits, e->x, e->cls.f(), d, c.vocab_size);
+      k_matmul(logits, e->x, e->cls.f(), d, c.vocab_size);
     if (!flush_pending_quantize() ||
-        hipMemcpyAsync(e->host_logits, e->logits, (size_t)c.vocab_size * sizeof(float), hipMemcpyDeviceToHost,
-                       device().stream) != hipSuccess)
+        (!stay && hipMemcpyAsync(e->host_logits, logits, (size_t)c.vocab_size * sizeof(float), hipMemcpyDeviceToHost,
+                                  device().stream) != hipSuccess))
       return fail_after_wait("engine_forward: copying the logits to the host failed");
   }
   llhip_synchronize(); // the logits have landed; reports a non-finite activation or score of this token
@@ -659,8 +662,9 @@ bool logits_all_q8(Engine *e, int count) {
 // and RoPE tables, per layer RMSNorm of the rows, (quantize,) the QKV GEMM, RoPE, the cache rows, batched causal
 // attention, (quantize,) Wo + residual, RMSNorm, (quantize,) W1/W3 SwiGLU, (quantize,) W2 + residual; then the final
 // RMSNorm and classifier of the last row (LAST) or of every row (ALL; in BF16 mode one BF16 GEMM on the packed
-// classifier).
-float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int pos0, LogitsWanted want) {
+// classifier). stay: ALL's logits are left in e->blogits, which is returned; the work on them is still queued.
+float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int pos0, LogitsWanted want,
+                    bool stay = false) {
   const Config &c = e->c;
   const int d = c.dim, hidden = c.hidden_dim, hd = c.head_dim, gs = e->gs, nh = c.n_heads, nkv = c.n_kv_heads;
   const int kvl = hd * nkv;
@@ -772,6 +776,12 @@ float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int p
     // budget (tests/q8.c:158-183), and the classifier streams once per batch instead of once per row.
     if (e->q8) {
       norm_rows(e->rms_final);
+      if (stay) { // bit for bit the pieces' logits
+        const GemmQ8Segment seg{e->blogits, c.vocab_size, e->cls.k8(), K8Weight{}, nullptr, nullptr, c.vocab_size,
+                                GEMM_STORE};
+        k_gemm_q8(e->bxq, e->bxs, count, d, gs, &seg, 1);
+        return llhip_last_error()[0] ? nullptr : e->blogits;
+      }
       if (!logits_all_q8(e, count))
         return nullptr;
       llhip_synchronize();
@@ -792,6 +802,8 @@ float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int p
       k_matmul(e->logits, x, e->cls.f(), d, c.vocab_size);
     }
   }
+  if (stay)
+    return llhip_last_error()[0] ? nullptr : e->blogits;
   float *host;
   if (want == LOGITS_ALL) {
     if (!host_batch_room(e, (size_t)count * vocab))
@@ -825,6 +837,23 @@ float *forward_batch(Model *model, Engine *e, const int *tokens, int count, int 
       memcpy(e->host_batch + (size_t)i * vocab, e->host_logits, vocab * sizeof(float));
   }
   return want == LOGITS_NONE ? nullptr : want == LOGITS_ALL ? e->host_batch : e->host_logits;
+}
+
+// Every row's logits as forward_batch makes them, left on the device.
+float *forward_batch_on_device(Model *model, Engine *e, const int *tokens, int count, int pos0) {
+  prefill_validate(model, tokens, count, pos0, LOGITS_ALL);
+  if (llhip_last_error()[0])
+    return nullptr;
+  if (model->prefill_gemm && (count > 1 || e->bf16))
+    return forward_rows(model, e, tokens, count, pos0, LOGITS_ALL, true);
+  const size_t vocab = e->c.vocab_size;
+  if (count > 1 && !e->blogits && !device_array(&e->blogits, (size_t)model->max_batch * vocab))
+    return nullptr;
+  float *logits = count > 1 ? e->blogits : e->logits;
+  for (int i = 0; i < count; i++)
+    if (!forward(e, tokens[i], pos0 + i, true, logits + (size_t)i * vocab))
+      return nullptr;
+  return logits;
 }
 
 } // namespace
@@ -890,6 +919,44 @@ float *engine_forward_batch(Model *model, const int *tokens, int count, int pos0
   }
   llhip_clear_error();
   return forward_batch(model, e, tokens, count, pos0, want);
+}
+
+int llhip_engine_verify(Model *model, const int *tokens, int count, int pos0, const float *draft_logits, size_t draft_ld,
+                        const float *uniform, float temperature, int *next) {
+  Engine *e = model ? (Engine *)model->implementation : nullptr;
+  if (!e) {
+    raise("llhip_engine_verify: no model loaded");
+    return -1;
+  }
+  llhip_clear_error();
+  const int vocab = e->c.vocab_size;
+  if (!(temperature >= 0.0f) || !std::isfinite(temperature)) {
+    raise("llhip_engine_verify: temperature %g must be finite and not negative", (double)temperature);
+    return -1;
+  }
+  if (!next || (temperature > 0.0f && !uniform)) {
+    raise("llhip_engine_verify: null buffer");
+    return -1;
+  }
+  if (temperature > 0.0f && draft_logits && draft_ld < (size_t)vocab) {
+    raise("llhip_engine_verify: rows of %d logits at a stride of %zu", vocab, draft_ld);
+    return -1;
+  }
+  if (count > 0 && !verify_shape_ok(count, vocab)) {
+    raise("llhip_engine_verify: %d rows of %d tokens, at most 2^20 rows of 2^22 tokens are taken", count, vocab);
+    return -1;
+  }
+  const float *logits = forward_batch_on_device(model, e, tokens, count, pos0);
+  if (!logits)
+    return -1;
+  const int start[2] = {0, count};
+  int accepted = -1, after = -1;
+  llhip_verify_drafts(&accepted, &after, logits, (size_t)vocab, draft_logits, draft_ld, tokens, uniform, start, 1, count,
+                      vocab, temperature);
+  if (llhip_last_error()[0])
+    return -1;
+  *next = after;
+  return accepted;
 }
 
 void engine_kv_stats(Model *model, int position, int verify, KvStats *out) {

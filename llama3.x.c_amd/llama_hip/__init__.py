@@ -161,6 +161,7 @@ _SIGNATURES = {
     "engine_forward_batch": (ctypes.POINTER(ctypes.c_float), [P, P, I32, I32, I32]),
     "engine_group_size": (I32, []),
     "engine_precision": (ctypes.c_char_p, []),
+    "llhip_engine_verify": (I32, [P, P, I32, I32, P, SZ, P, ctypes.c_float, P]),
     "engine_kv_stats": (None, [P, I32, I32, P]),
     "llhip_hbm_claimed": (SZ, []),
     "k_attention_init": (None, [P, I32, I32, I32, I32]),

@@ -1,9 +1,13 @@
 """Many requests on one model, on the GPU: each operator against its plain float64 form (tests/requests_util.py, the bounds
 derived there), its index checks, host buffers and captured calls; and a small model served by all of them together."""
+import ctypes
+import os
+
 import numpy as np
 import pytest
 
 import llama_hip as lh
+from llama_hip import checkpoint as ck
 from tests import hip_util as hu
 from tests import requests_util as ru
 
@@ -751,3 +755,268 @@ def test_captured_calls_follow_their_arrays(L):
         for g, w in zip(results(), want):
             assert np.array_equal(g, w)
     L.llhip_graph_destroy(graph)
+
+
+# ---- the engine's step over drafts ------------------------------------------------------------------------------------
+
+
+ENGINE = dict(dim=128, hidden_dim=256, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=1500, seq_len=96, rope_theta=10000.0)
+
+
+def engine_model(path, kind):
+    gs = 64
+    norms, t = ck.synthetic(ENGINE, gs, 17)
+    if kind.startswith("q8"):
+        ck.write_q8_v3(path, ENGINE, gs, norms, t)
+    else:
+        f32 = {n: q.astype(F) * np.repeat(s.reshape(-1), gs).reshape(q.shape).astype(F) for n, (q, s) in t.items()}
+        ck.write_f32_v3(path, ENGINE, norms, f32)
+
+
+@pytest.mark.parametrize("kind", ["q8", "q8_fp32_activations", "f32", "bf16", "q8_no_gemm"])
+def test_engine_verify(L, tmp_path, monkeypatch, kind):
+    """llhip_engine_verify's decisions are the plain form's on the logits that engine_forward_batch gives for the same rows
+    at the same place, drawn and greedy, with a draft model and without, for one row and many; a model goes on from the
+    accepted drafts; and its refusals, which leave the model usable."""
+    if kind == "q8_fp32_activations":
+        monkeypatch.setenv("LLAMA_Q8_ACTIVATIONS", "fp32")
+    if kind == "bf16":
+        monkeypatch.setenv("LLAMA_PRECISION", "bf16")
+    if kind == "q8_no_gemm":
+        monkeypatch.setenv("LLAMA_PREFILL_GEMM", "off")
+    if kind in ("q8_fp32_activations", "q8_no_gemm"):  # rows run one at a time; a batch is one row unless asked for
+        monkeypatch.setenv("LLAMA_PREFILL_BATCH", "24")
+    L.kernels_kv_layout_select(b"head")
+    path = os.path.join(tmp_path, "tiny.bin")
+    engine_model(path, kind)
+    vocab = ENGINE["vocab_size"]
+    rng = np.random.default_rng(8)
+    model, following = lh.Model(), ctypes.c_int(-7)
+    at = ctypes.byref(model)
+
+    def verify(tokens, pos, draft, uniform, temperature):
+        return L.llhip_engine_verify(at, lh.ptr(tokens), len(tokens), pos, lh.ptr(draft), 0 if draft is None else vocab,
+                                     lh.ptr(uniform), temperature, ctypes.byref(following))
+
+    try:
+        L.engine_load(at, path.encode())
+        assert model.implementation, lh.last_error()
+        prompt = rng.integers(0, vocab, 20).astype(np.int32)
+        assert L.engine_forward_batch(at, lh.ptr(prompt), 20, 0, lh.LOGITS_LAST), lh.last_error()
+        known, pos, accepted_any = int(prompt[0]), 20, 0
+        for n, temperature, drawn in ((1, 0.0, False), (5, 0.0, False), (4, 0.8, True), (6, 1.3, False), (1, 0.7, False),
+                                      (8, 0.5, True)):
+            tokens = rng.integers(0, vocab, n).astype(np.int32)
+            tokens[0] = known
+            for i in range(1, n):  # the model's own choice, but for the last
+                p = L.engine_forward_batch(at, lh.ptr(tokens[:i]), i, pos, lh.LOGITS_ALL)
+                row = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (i, vocab))[i - 1]
+                if i < n - 1:
+                    tokens[i] = int(row.argmax())
+            p = L.engine_forward_batch(at, lh.ptr(tokens), n, pos, lh.LOGITS_ALL)
+            logits = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (n, vocab)).copy()
+            draft = (logits + 0.3 * rng.standard_normal(logits.shape)).astype(F) if drawn else None
+            uniform = rng.random((n, 2)).astype(F) if temperature else None
+            want = ru.verify([0, n], logits, draft, tokens, uniform, temperature)[0]
+            got = verify(tokens, pos, draft, uniform, temperature)
+            assert not lh.last_error(), lh.last_error()
+            assert (got, following.value) == want, (n, temperature)
+            if drawn:  # from device memory
+                keep = hu.dev(draft), hu.dev(uniform)
+                assert verify(tokens, pos, keep[0], keep[1], temperature) == want[0] and following.value == want[1]
+            pos, known, accepted_any = pos + got + 1, following.value, accepted_any + got
+        assert accepted_any >= 3  # greedy accepts the model's own choices: 3 of its 4 at least
+        u = np.zeros((2, 2), F)
+        following.value = -7
+        two = np.array([1, 2], np.int32)
+        for call, words in ((lambda: verify(two, 95, None, u, 0.5), "batch input out of range"),
+                            (lambda: verify(np.array([1, vocab], np.int32), 20, None, u, 0.5), "out of range: token="),
+                            (lambda: verify(two, 20, None, None, 0.5), "null buffer"),
+                            (lambda: verify(two, 20, None, u, -1.0), "not negative"),
+                            (lambda: L.llhip_engine_verify(at, lh.ptr(two), 2, 20, lh.ptr(u), vocab - 1, lh.ptr(u), 0.5,
+                                                           ctypes.byref(following)), "at a stride of"),
+                            (lambda: L.llhip_engine_verify(at, lh.ptr(two), 0, 20, None, 0, None, 0.0,
+                                                           ctypes.byref(following)), "batch input out of range"),
+                            (lambda: L.llhip_engine_verify(at, None, 2, 20, None, 0, None, 0.0,
+                                                           ctypes.byref(following)), "batch input out of range"),
+                            (lambda: L.llhip_engine_verify(at, lh.ptr(two), 2, 20, None, 0, None, 0.0, None), "null buffer")):
+            assert call() == -1 and following.value == -7
+            assert words in lh.last_error(), lh.last_error()
+        assert verify(two, 20, None, None, 0.0) >= 0 and not lh.last_error()
+    finally:
+        L.engine_free(at)
+
+
+# ---- a small model served by all of them ------------------------------------------------------------------------------
+
+
+class Served:
+    """Two layers with their adapters: the float64 forward of one request's whole sequence, and the operands on the
+    device."""
+    dim, heads, kv, hd, hidden, vocab, layers, rank, adapters = 256, 4, 2, 64, 352, 700, 2, 8, 3
+
+    def __init__(self, rng):
+        kvl = self.kv * self.hd
+        shapes = {"q": (self.dim, self.dim), "k": (kvl, self.dim), "v": (kvl, self.dim), "o": (self.dim, self.dim),
+                  "1": (self.hidden, self.dim), "3": (self.hidden, self.dim), "2": (self.dim, self.hidden)}
+        normal = lambda *s: (rng.standard_normal(s) / np.sqrt(s[-1])).astype(F)
+        self.embed, self.cls = rng.standard_normal((self.vocab, self.dim), dtype=F), 4 * normal(self.vocab, self.dim)
+        self.norm = np.ones(self.dim, F)
+        self.w, self.a, self.b, self.scale = [], [], [], rng.uniform(0.5, 1.5, self.adapters).astype(F)
+        for _ in range(self.layers):
+            self.w.append({n: normal(*s) for n, s in shapes.items()})
+            self.a.append({n: normal(self.adapters, self.rank, s[1]) for n, s in shapes.items()})
+            self.b.append({n: normal(self.adapters, s[0], self.rank) for n, s in shapes.items()})
+        self.dev = [{n: tuple(hu.dev(x) for x in (w[n], a[n], b[n])) for n in shapes}
+                    for w, a, b in zip(self.w, self.a, self.b)]
+        self.head = hu.dev(self.norm), hu.dev(self.cls), hu.dev(self.scale)
+
+    def tables(self, positions):
+        freq = 10000.0 ** (-np.arange(0, self.hd, 2) / self.hd)
+        angle = np.arange(positions)[:, None] * freq
+        return np.cos(angle).astype(F), np.sin(angle).astype(F)
+
+    def plain(self, prefix, own, adapter):
+        """The own tokens' logits in float64; the prefix has no adapter."""
+        n, total = len(prefix), len(prefix) + len(own)
+        x = self.embed[np.concatenate((prefix, own)).astype(int)].astype(np.float64)
+        ids = np.array([-1] * n + [adapter] * len(own))
+        cos, sin = (t.astype(np.float64) for t in self.tables(total))
+
+        def project(l, name, x):
+            y = x @ self.w[l][name].T.astype(np.float64)
+            if adapter >= 0:
+                low = x[n:] @ self.a[l][name][adapter].T.astype(np.float64)
+                y[n:] += float(self.scale[adapter]) * (low @ self.b[l][name][adapter].T.astype(np.float64))
+            return y
+
+        def turn(y):
+            y = y.reshape(total, -1, self.hd // 2, 2)
+            c, s = cos[:, None], sin[:, None]
+            return np.stack((y[..., 0] * c - y[..., 1] * s, y[..., 0] * s + y[..., 1] * c), -1).reshape(total, -1, self.hd)
+
+        norm = lambda x: x / np.sqrt((x * x).mean(1, keepdims=True) + 1e-5)
+        mul = self.heads // self.kv
+        for l in range(self.layers):
+            y = norm(x)
+            q, k = turn(project(l, "q", y)), np.repeat(turn(project(l, "k", y)), mul, 1)
+            v = np.repeat(project(l, "v", y).reshape(total, self.kv, self.hd), mul, 1)
+            s = np.einsum("ihd,jhd->hij", q, k) / np.sqrt(self.hd)
+            s[:, np.triu_indices(total, 1)[0], np.triu_indices(total, 1)[1]] = -np.inf
+            p = np.exp(s - s.max(2, keepdims=True))
+            p /= p.sum(2, keepdims=True)
+            x = x + project(l, "o", np.einsum("hij,jhd->ihd", p, v).reshape(total, -1))
+            y = norm(x)
+            gate = project(l, "1", y)
+            x = x + project(l, "2", gate / (1.0 + np.exp(-gate)) * project(l, "3", y))
+        return (norm(x) @ self.cls.T.astype(np.float64))[n:]
+
+    def run(self, L, tokens, b, ids, caches, prefix_caches, table, rows_of_logits=None):
+        """The batch's logits on the device, by the library alone; caches [layer][key, value]."""
+        T, m, kvl = hu.torch(), b.rows, self.kv * self.hd
+        x = hu.dev(self.embed[np.asarray(tokens)])
+        buf = {n: hu.dev(np.zeros((m, w), F)) for n, w in (("y", self.dim), ("q", self.dim), ("k", kvl), ("v", kvl),
+                                                            ("at", self.dim), ("1", self.hidden), ("3", self.hidden))}
+        idd = hu.dev(np.asarray(ids, np.int32))
+        norm, cls, scale = self.head
+
+        def gemm(x, k, *segments):
+            L.k_gemm_f32(lh.ptr(x), k, m, k, ru.array([lh.GemmSegment(lh.ptr(c), w.shape[0], lh.ptr(w), None, k, w.shape[0],
+                                                                      kind) for c, w, kind in segments]), len(segments))
+
+        def lora(x, k, *segments):
+            if b.count:
+                L.llhip_lora_f32(lh.ptr(x), k, m, k, lh.ptr(idd), self.adapters, ru.array(segments), len(segments))
+
+        def beside(l, name, c, **third):
+            w, a, bb = self.dev[l][name]
+            return ru.lora_segment(False, c, w.shape[0], c, a, bb, scale, w.shape[0], self.rank, **third)
+
+        for l in range(self.layers):
+            d = self.dev[l]
+            L.k_rmsnorm_rows(lh.ptr(buf["y"]), lh.ptr(x), lh.ptr(norm), m, self.dim, 1e-5)
+            gemm(buf["y"], self.dim, *[(buf[n], d[n][0], lh.GEMM_STORE) for n in "qkv"])
+            lora(buf["y"], self.dim, *[beside(l, n, buf[n]) for n in "qkv"])
+            L.llhip_rope_kv_store_requests(lh.ptr(buf["q"]), lh.ptr(buf["q"]), self.dim, lh.ptr(buf["k"]),
+                                           lh.ptr(buf["v"]), kvl, lh.ptr(table), b.struct, self.heads, self.kv, self.hd,
+                                           lh.ptr(caches[l][0]), lh.ptr(caches[l][1]))
+            pk, pv = prefix_caches[l] if prefix_caches else (None, None)
+            L.llhip_attention_requests(lh.ptr(buf["at"]), lh.ptr(buf["q"]), lh.ptr(pk), lh.ptr(pv), lh.ptr(caches[l][0]),
+                                       lh.ptr(caches[l][1]), b.struct, self.heads, self.kv, self.hd)
+            gemm(buf["at"], self.dim, (x, d["o"][0], lh.GEMM_ADD))
+            lora(buf["at"], self.dim, beside(l, "o", x))
+            L.k_rmsnorm_rows(lh.ptr(buf["y"]), lh.ptr(x), lh.ptr(norm), m, self.dim, 1e-5)
+            gemm(buf["y"], self.dim, (buf["1"], d["1"][0], lh.GEMM_STORE), (buf["3"], d["3"][0], lh.GEMM_STORE))
+            lora(buf["y"], self.dim, beside(l, "1", buf["1"], base3=buf["3"], a3=d["3"][1], b3=d["3"][2]))
+            gemm(buf["1"], self.hidden, (x, d["2"][0], lh.GEMM_ADD))
+            lora(buf["1"], self.hidden, beside(l, "2", x))
+        L.k_rmsnorm_rows(lh.ptr(buf["y"]), lh.ptr(x), lh.ptr(norm), m, self.dim, 1e-5)
+        quiet(L)
+        last = buf["y"] if rows_of_logits is None else buf["y"][T.as_tensor(rows_of_logits, device="cuda")].contiguous()
+        T.cuda.synchronize()
+        m = len(last)
+        logits = hu.dev(np.zeros((m, self.vocab), F))
+        gemm(last, self.dim, (logits, cls, lh.GEMM_STORE))
+        quiet(L)
+        return logits
+
+
+@pytest.mark.parametrize("layout", ["head", "rows"])
+def test_a_model_served_by_all_of_them(L, layout):
+    """A prefix computed once, then three requests with adapters 2, none and 0: their prompts, a step with drafts, and one
+    more from where the drafts were left, whose cache rows replace the refused ones'. Logits against the whole sequences in
+    float64, the decisions against those logits.
+
+    Tolerance: each of the 2 * 9 products, sums and norms adds at most (dim / 32 + 48) U = 56 U of the sum of its terms'
+    magnitudes, which here are at most 8 times the result's size; normed rows of size 1 carry it on unchanged, so that the
+    logits, of size 4, are off by less than 18 * 56 * 8 * 4 U = 2e-3."""
+    L.kernels_kv_layout_select(layout.encode())
+    rng = np.random.default_rng(31)
+    s = Served(rng)
+    prefix, seq_len, slots, adapter, slot = rng.integers(0, s.vocab, 37), 40, 5, [2, -1, 0], [3, 0, 4]
+    cos, sin = s.tables(len(prefix) + seq_len)
+    table = hu.dev(np.concatenate((np.repeat(cos, 2, 1), np.stack((-sin, sin), 2).reshape(len(cos), -1)), 1).astype(F))
+    made = lambda n, lead: [[hu.dev(np.full(lead + ru.cache_shape(layout, n, s.kv, s.hd), np.nan, F)) for _ in range(2)]
+                            for _ in range(s.layers)]
+    shared, caches = made(len(prefix), (1,)), made(seq_len, (slots,))
+    alone = ru.Batch(hu.dev, [len(prefix)], [0], seq_len=len(prefix), slots=1)
+    got = hu.host(s.run(L, prefix, alone, [-1] * len(prefix), shared, None, table))
+    assert np.abs(got - s.plain([], prefix, -1)).max() < 2e-3
+    own = [list(rng.integers(0, s.vocab, n)) for n in (7, 1, 12)]
+    start = np.array([0, 7, 8, 20], np.int32)
+
+    def batch(rows_of, length):
+        return ru.Batch(hu.dev, rows_of, length, slot=slot, slots=slots, prefix=len(prefix), seq_len=seq_len)
+
+    ids = lambda rows_of: np.repeat(adapter, rows_of)
+    prompts = [len(o) for o in own]
+    logits = s.run(L, sum(own, []), batch(prompts, [0, 0, 0]), ids(prompts), caches, shared, table, start[1:] - 1)
+    got = hu.host(logits)
+    want = [s.plain(prefix, o, a) for o, a in zip(own, adapter)]
+    for r in range(3):
+        assert np.abs(got[r] - want[r][-1]).max() < 2e-3, r
+    decided = run_verify(L, np.arange(4, dtype=np.int32), got, None, np.zeros(3, np.int32), None, s.vocab, 0.0)
+    assert decided == [(0, int(w.argmax())) for w in got]
+    known = [n for _, n in decided]
+    for rows_of, temperature in (([4, 1, 3], 0.0), ([2, 5, 3], 0.9), ([1, 2, 1], 0.0)):
+        tokens, full = [], []
+        for r in range(3):
+            mine = [known[r]]
+            while len(mine) < rows_of[r]:  # the model's own next token, but a wrong one last in the third request
+                z = s.plain(prefix, own[r] + mine, adapter[r])[-1]
+                mine.append(int(z.argmin() if r == 2 and len(mine) == rows_of[r] - 1 else z.argmax()))
+            tokens += mine
+            full.append(mine)
+        b = batch(rows_of, [len(o) for o in own])
+        got = hu.host(s.run(L, tokens, b, ids(rows_of), caches, shared, table))
+        for r in range(3):
+            want = s.plain(prefix, own[r] + full[r], adapter[r])[len(own[r]):]
+            assert np.abs(got[b.start[r]:b.start[r + 1]] - want).max() < 2e-3, (r, rows_of)
+        uniform = rng.random((b.rows, 2)).astype(F) if temperature else None
+        tokens = np.asarray(tokens, np.int32)
+        decided = run_verify(L, b.start, got, None, tokens, uniform, s.vocab, temperature)
+        assert decided == ru.verify(b.start, got, None, tokens, uniform, temperature)
+        for r, (n, following) in enumerate(decided):
+            own[r] += full[r][:n + 1]
+            known[r] = following
+    quiet(L)

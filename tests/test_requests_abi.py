@@ -208,3 +208,12 @@ def test_verify_refusals(L):
     refused(L, "must not overlap")
     verify_call(L, count=0, logits=None)
     assert not lh.last_error()
+
+
+def test_engine_verify_without_a_model(L):
+    following = ctypes.c_int(7)
+    model = lh.Model()
+    for m in (None, ctypes.byref(model)):
+        got = L.llhip_engine_verify(m, lh.ptr(np.zeros(2, np.int32)), 2, 0, None, 0, None, 0.0, ctypes.byref(following))
+        assert got == -1 and following.value == 7
+        refused(L, "no model loaded")
