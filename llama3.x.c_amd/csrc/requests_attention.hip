@@ -163,155 +163,167 @@ __global__ __launch_bounds__(kThreads) void attn_rows(RequestAttn p, int row0) {
 constexpr int kUnit = 32;        // positions of a step
 constexpr int kTileVectors = 128; // query vectors of a wide tile
 constexpr int kNarrowVectors = 32; // at most, of a narrow one
-constexpr int kTargetItems = 512; // work items aimed at: one for each block that the chip holds
-constexpr int kMinUnits = 4;     // a step for each wave of a narrow block
-constexpr int kMaxShares = 32;   // of one walk
-constexpr int kWideCost = 2;     // a wide step takes about as long as this many narrow ones
+constexpr int kBlocksPerCu = 2;
+constexpr int kTable = 128;      // requests that a block keeps in LDS; it reads the others again
+constexpr int kMinSlice = 1024; // of a block
 constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far below that its weight is zero, also where a
                                      // lane has seen nothing else
+
+// Where a row's partial sums lie: those of its tile over the prefix, and over its own positions, by the blocks first ..
+// last that took the tile's walk.
+struct RowSlots {
+  int prefix_first, prefix_last, prefix_v;
+  int own_first, own_last, own_v; // own_first -1: the row belongs to no request
+  int slot, last;                 // cache slot and last own position
+};
 
 struct FastAttn {
   float *out;
   const float *q, *prefix_key, *prefix_value, *key, *value;
   RequestsDev batch;
   int n_heads, n_kv_heads, kv_mul, hd;
-  int tile_rows;    // rows of a wide tile
-  int prefix_tiles; // tiles of all rows over the prefix (1 when narrow)
-  bool prefix_narrow;
-  float scale2; // log2(e) / sqrtf(hd)
+  int tile_rows; // rows of a wide tile
+  int blocks;    // of a KV head
+  float scale2;  // log2(e) / sqrtf(hd)
+  // slots of hd + 4 floats: [prefix, own][row][head] where a walk begins, [KV head][block][vector of the tile] where a
+  // block goes on with the walk of the one before
   float *partial;
-  int4 *row_slots; // per row: first own slot, own shares (-1: the row belongs to no request), cache slot, own position
-  int *header;     // [0] shares of the prefix
+  RowSlots *rows;
   int *flags;
 };
 
-// What every block works out for itself from the batch's arrays: the walks (a tile of query vectors over a range of
-// positions), each cut into shares of about equal length so that all of them are about kTargetItems work items.
+// What every block works out for itself from the batch's arrays. The walks of a KV head (a tile of query vectors over the
+// prefix, or over a request's own positions) lie one behind the other on a line, each as long as it takes in time, and
+// the line is cut into slices of one length, one for a block: all blocks start together and end together. (Walks cut into
+// about equal shares of their own, one to a block, left a third of the blocks' time idle behind the first round.)
 struct Plan {
-  int items[kMaxRequests]; // running sum, the request's own included
-  int slots[kMaxRequests]; // likewise
-  long long units;
-  int longest, step, bad;
-  int total_rows, first_row, end_row; // of the requests: their number, the lowest, one past the highest
-  int wave_items[kThreads / kWave], wave_slots[kThreads / kWave];
+  long long line[kMaxRequests]; // where request r's own walks end
+  long long prefix, full;       // the prefix's part of the line, and of one full tile in it
+  long long slice, total;
+  int total_rows, first_row, end_row; // of the requests: their rows' number, the lowest, one past the highest
+  long long wave_sum[kThreads / kWave];
+  Request table[kTable]; // the first requests, for the blocks' walks
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// A request's own walk is one narrow tile, or wide ones.
-__device__ __forceinline__ bool own_narrow(const FastAttn &p, int rows) { return rows * p.kv_mul <= kNarrowVectors; }
+// How long a walk over so many positions takes a block, two of them on a CU, in quarters of what a narrow walk with up to 16
+// vectors takes for one position (8 ns).
+struct WalkTime {
+  int begin, position;
+};
+__device__ __host__ __forceinline__ constexpr WalkTime walk_time_of(int vectors) {
+  return vectors <= 16 ? WalkTime{680, 4} : vectors <= kNarrowVectors ? WalkTime{920, 6} : WalkTime{1120, 12};
+}
+__device__ __forceinline__ long long walk_time(int vectors, int positions) {
+  const WalkTime t = walk_time_of(vectors);
+  return t.begin + (long long)t.position * positions;
+}
+// A request's own walks: one narrow tile, or full wide ones and the rest, tile t over the positions up to its last row's.
 __device__ __forceinline__ int own_tiles(const FastAttn &p, int rows) {
-  return own_narrow(p, rows) ? 1 : ceil_div(rows, p.tile_rows);
+  return rows * p.kv_mul <= kNarrowVectors ? 1 : ceil_div(rows, p.tile_rows);
 }
-// Shares of a walk: as many as bring one down to `step` in narrow steps' time.
-__device__ __forceinline__ int own_shares(const FastAttn &p, const Request &q, int step) {
-  return q.rows ? ceil_div(ceil_div(q.length + q.rows, kUnit) * (own_narrow(p, q.rows) ? 1 : kWideCost), step) : 0;
+__device__ __forceinline__ long long tile_start(const FastAttn &p, int length, long long t) {
+  constexpr WalkTime wide = walk_time_of(kTileVectors);
+  return t * wide.begin + wide.position * (t * length + p.tile_rows * (t * (t + 1) / 2));
 }
-__device__ __forceinline__ int prefix_cost(const FastAttn &p) {
-  return ceil_div(p.batch.prefix, kUnit) * (p.prefix_narrow ? 1 : kWideCost);
+__device__ __forceinline__ long long own_time(const FastAttn &p, const Request &q) {
+  if (q.rows == 0)
+    return 0;
+  const int t = own_tiles(p, q.rows) - 1;
+  return tile_start(p, q.length, t) + walk_time((q.rows - t * p.tile_rows) * p.kv_mul, q.length + q.rows);
 }
+
+// x / y of the line's lengths (below 2^50, where the double quotient's whole part is exact), a third of the time that the
+// compiler's division takes.
+__device__ __forceinline__ long long whole(long long x, long long y) { return (long long)((double)x / (double)y); }
 
 __device__ void make_plan(const FastAttn &p, Plan &plan) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   constexpr int kPer = kMaxRequests / kThreads; // requests of a thread, at most
   const int per = ceil_div(p.batch.count, kThreads), r0 = tid * per;
-  if (tid == 0)
-    plan.units = 0, plan.longest = 0, plan.bad = 0, plan.total_rows = 0, plan.first_row = p.batch.rows, plan.end_row = 0;
-  __syncthreads();
-  long long units = 0;
-  int longest = 0, total_rows = 0, first_row = p.batch.rows, end_row = 0, rows[kPer], u[kPer];
+  if (tid == 0) { // as the arrays say, if they are right
+    plan.first_row = p.batch.start[0];
+    plan.end_row = p.batch.start[p.batch.count];
+    plan.total_rows = 0;
+  }
+  long long sum = 0, time[kPer];
+  int total_rows = 0, first_row = p.batch.rows, end_row = 0;
   bool bad = false;
 #pragma unroll
   for (int k = 0; k < kPer; k++) {
-    rows[k] = u[k] = 0;
+    time[k] = 0;
     if (k < per && r0 + k < p.batch.count) {
       const Request q = request_at(p.batch, r0 + k, bad);
-      rows[k] = q.rows;
+      if (r0 + k < kTable)
+        plan.table[r0 + k] = q;
       total_rows = min(total_rows + q.rows, INT32_MAX / kThreads);
       if (q.rows) {
         first_row = min(first_row, q.first);
         end_row = max(end_row, q.first + q.rows);
       }
-      u[k] = q.rows ? ceil_div(q.length + q.rows, kUnit) : 0;
-      if (own_narrow(p, q.rows)) {
-        units += u[k];
-      } else {
-        units += (long long)own_tiles(p, q.rows) * u[k] * kWideCost;
-        u[k] *= kWideCost;
-      }
-      longest = max(longest, u[k]);
+      sum += time[k] = own_time(p, q);
     }
   }
-  for (int o = 32; o > 0; o >>= 1) {
-    units += __shfl_xor(units, o);
-    longest = max(longest, __shfl_xor(longest, o));
-    total_rows += __shfl_xor(total_rows, o);
-    first_row = min(first_row, __shfl_xor(first_row, o));
-    end_row = max(end_row, __shfl_xor(end_row, o));
+  long long run = sum; // the threads' up to this one
+  for (int o = 1; o < kWave; o <<= 1) {
+    const long long v = __shfl_up(run, o);
+    if (lane >= o)
+      run += v;
   }
-  if (lane == 0) {
-    atomicAdd((unsigned long long *)&plan.units, (unsigned long long)units);
-    atomicMax(&plan.longest, longest);
+  if (lane == kWave - 1)
+    plan.wave_sum[wave] = run;
+  if (__syncthreads_or(bad)) { // what is left of them
+    if (blockIdx.x == 0 && tid == 0)
+      p.flags[3] = 1;
+    if (tid == 0)
+      plan.first_row = p.batch.rows, plan.end_row = 0;
+    __syncthreads();
     atomicAdd(&plan.total_rows, total_rows);
     atomicMin(&plan.first_row, first_row);
     atomicMax(&plan.end_row, end_row);
+    __syncthreads();
   }
-  if (bad)
-    plan.bad = 1;
-  __syncthreads();
-  if (plan.total_rows > p.batch.rows) { // requests over each other's rows (and some start above the next, so bad is set):
-    // none is taken, the launch and its workspace hold for rows that lie apart
-#pragma unroll
-    for (int k = 0; k < kPer; k++)
-      rows[k] = u[k] = 0;
+  // requests over each other's rows (and some start above the next, so bad is set): none is taken
+  const bool none = plan.total_rows > p.batch.rows;
+  const int rows = none || !p.batch.prefix ? 0 : max(plan.end_row - plan.first_row, 0);
+  const int tiles = ceil_div(rows, p.tile_rows);
+  const long long full = walk_time(p.tile_rows * p.kv_mul, p.batch.prefix);
+  const long long prefix =
+      tiles ? (tiles - 1) * full + walk_time((rows - (tiles - 1) * p.tile_rows) * p.kv_mul, p.batch.prefix) : 0;
+  long long at = prefix + run - sum, total = prefix;
+  for (int w = 0; w < kThreads / kWave; w++) {
+    if (w < wave)
+      at += plan.wave_sum[w];
+    total += plan.wave_sum[w];
   }
-  const int prefix_units = prefix_cost(p);
-  const long long total = (plan.units + (long long)p.prefix_tiles * prefix_units) * p.n_kv_heads;
-  const int aim = (int)((total + kTargetItems - 1) / kTargetItems);
-  const int step = max(max(kMinUnits, aim), ceil_div(max(plan.longest, prefix_units), kMaxShares));
-  int items = 0, slots = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; k++) {
-    const int shares = ceil_div(u[k], step);
-    items += own_tiles(p, rows[k]) * shares * p.n_kv_heads;
-    slots += rows[k] * p.n_heads * shares;
-  }
-  // the sums of the threads before this one
-  int item_run = items, slot_run = slots;
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int a = __shfl_up(item_run, o), b = __shfl_up(slot_run, o);
-    if (lane >= o)
-      item_run += a, slot_run += b;
-  }
-  if (lane == kWave - 1)
-    plan.wave_items[wave] = item_run, plan.wave_slots[wave] = slot_run;
-  __syncthreads();
-  item_run -= items, slot_run -= slots;
-  for (int w = 0; w < wave; w++)
-    item_run += plan.wave_items[w], slot_run += plan.wave_slots[w];
 #pragma unroll
   for (int k = 0; k < kPer; k++)
-    if (k < per && r0 + k < p.batch.count) {
-      const int shares = ceil_div(u[k], step);
-      plan.items[r0 + k] = item_run += own_tiles(p, rows[k]) * shares * p.n_kv_heads;
-      plan.slots[r0 + k] = slot_run += rows[k] * p.n_heads * shares;
-    }
-  if (tid == 0)
-    plan.step = step;
+    if (k < per && r0 + k < p.batch.count)
+      plan.line[r0 + k] = none ? 0 : at += time[k];
+  if (tid == 0) {
+    plan.prefix = prefix;
+    plan.full = full;
+    plan.total = none ? 0 : total;
+    plan.slice = max(whole(total + p.blocks - 1, p.blocks), (long long)kMinSlice);
+  }
   __syncthreads();
 }
 
-// One block's work: query vectors (row row0 + v / kv_mul, head g * kv_mul + v % kv_mul for v < vectors) over positions
-// t0 .. t1 - 1 of one cache; row row0 + j sees positions up to last0 + j (the prefix: all).
+// Query vectors (row row0 + v / kv_mul, head g * kv_mul + v % kv_mul for v < vectors) over positions t0 .. t1 - 1 of one
+// cache; row row0 + j sees positions up to last0 + j (the prefix: all).
 struct Item {
   const float *key, *value;
   size_t pos_stride;
   int row0, vectors, g;
   int t0, t1;
   int last0; // INT_MAX: every position is seen by every row
-  size_t slot0;
-  int slot_step; // floats' slots between vectors: a vector's slot is slot0 + (row * n_heads + head) * slot_step
+  size_t slot0; // vector v's slot is slot0 + (v / kv_mul) * slot_row + v % kv_mul
+  int slot_row;
 };
+__device__ __forceinline__ float *slot_of(const FastAttn &p, const Item &it, int v) {
+  return p.partial + (it.slot0 + (size_t)(v / p.kv_mul) * it.slot_row + v % p.kv_mul) * (size_t)(p.hd + 4);
+}
 
 // Nothing moves across: each phase's registers are free before the next one's are taken (moved freely, the phases of a
 // step need more than the 256 registers that two waves a SIMD leave each).
@@ -324,6 +336,14 @@ __device__ __forceinline__ void interleave() {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix
     __builtin_amdgcn_sched_group_barrier(0x002, 5, 0); // vector
   }
+}
+
+// The thread's number, new to the compiler at each walk: else it keeps what both walks derive from it in registers all along
+// a block's walks (43 of them spilled).
+__device__ __forceinline__ int own_thread() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
 }
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
@@ -403,26 +423,22 @@ __device__ __forceinline__ float four_sum(float x) {
 // 1536 and 3800 on the vector unit to split the values.
 template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, const Item &it, unsigned char *lds) {
   constexpr int kSteps = HD / 32, kDt = HD / 16, kWaves = kThreads / kWave, kRow = HD + 4;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
+  const int tid = own_thread(), lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
   const int hd = p.hd;
   const int tiles = it.vectors <= 16 ? 1 : it.vectors <= 32 ? 2 : 4, walkers = kWaves / tiles; // waves of a tile
   const int v_mine = 16 * (wave / walkers) + lc; // this lane's vector
   const bool active = v_mine < it.vectors;
-  float qr[kSteps][8]; // dimensions 32 st + 8 lq .. + 7
-  {
-    const float *src = p.q + ((size_t)(it.row0 + (active ? v_mine / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
-                              (active ? v_mine % p.kv_mul : 0)) * hd;
+  float4 x[kSteps][2]; // dimensions 32 st + 8 lq .. + 7, on their way with the first step's rows
+  const float *src = p.q + ((size_t)(it.row0 + (active ? v_mine / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
+                            (active ? v_mine % p.kv_mul : 0)) * hd;
 #pragma unroll
-    for (int st = 0; st < kSteps; st++)
+  for (int st = 0; st < kSteps; st++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const int d = 32 * st + 8 * lq + 4 * h;
-        const float4 x = *reinterpret_cast<const float4 *>(src + (FULL || d < hd ? d : 0));
-        const float scale = active && (FULL || d < hd) ? p.scale2 : 0.0f;
-        qr[st][4 * h] = x.x * scale, qr[st][4 * h + 1] = x.y * scale, qr[st][4 * h + 2] = x.z * scale,
-        qr[st][4 * h + 3] = x.w * scale;
-      }
-  }
+    for (int h = 0; h < 2; h++) {
+      const int d = 32 * st + 8 * lq + 4 * h;
+      x[st][h] = *reinterpret_cast<const float4 *>(src + (FULL || d < hd ? d : 0));
+    }
+  fence();
   const int last = !active ? -1 : it.last0 == INT32_MAX ? INT32_MAX : it.last0 + v_mine / p.kv_mul;
   v4f o[kDt];
   float m_run = -FLT_MAX, l_run = 0.0f, odd = 0.0f;
@@ -432,7 +448,8 @@ template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, cons
     o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   float4 kr[2][kSteps][2], vr[2][4][HD / 64];
   const Rows keys = rows_of(it.key, it, hd), values = rows_of(it.value, it, hd);
-  unsigned k_at = (unsigned)(wave % walkers * kUnit + lc) * keys.stride, v_at = (unsigned)(wave % walkers * kUnit + 4 * lq) * values.stride;
+  unsigned k_at = (unsigned)(wave % walkers * kUnit + lc) * keys.stride;
+  unsigned v_at = (unsigned)(wave % walkers * kUnit + 4 * lq) * values.stride;
   auto load_k = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; t++)
@@ -456,10 +473,18 @@ template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, cons
   const int stride = walkers * kUnit;
   const int end = 16 * (wave / walkers) < it.vectors ? it.t1 : it.t0; // a tile without vectors walks nothing
   int t0 = it.t0 + wave % walkers * kUnit;
-  if (t0 < end) {
-    load_k();
-    load_v();
-  }
+  load_k(); // zeros past the end
+  load_v();
+  fence();
+  float qr[kSteps][8];
+#pragma unroll
+  for (int st = 0; st < kSteps; st++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const float scale = active && (FULL || 32 * st + 8 * lq + 4 * h < hd) ? p.scale2 : 0.0f;
+      qr[st][4 * h] = x[st][h].x * scale, qr[st][4 * h + 1] = x[st][h].y * scale, qr[st][4 * h + 2] = x[st][h].z * scale,
+      qr[st][4 * h + 3] = x[st][h].w * scale;
+    }
   auto of = [](const float4 &x, int e) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
   for (; t0 < end; t0 += stride) {
     // S^T = K Q^T: instruction (st, i) takes dimension 32 st + 8 lq + i from lane group lq; two sums a position tile
@@ -572,8 +597,7 @@ template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, cons
       l = fmaf(scale, at[HD + 1], l);
       sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
     }
-    const size_t vec = (size_t)(it.row0 + v / p.kv_mul) * p.n_heads + (size_t)it.g * p.kv_mul + v % p.kv_mul;
-    float *dst = p.partial + (it.slot0 + vec * it.slot_step) * (size_t)(hd + 4);
+    float *dst = slot_of(p, it, v);
     *reinterpret_cast<float4 *>(dst + 4 * d4) = sum;
     if (d4 == 0)
       *reinterpret_cast<float4 *>(dst + hd) = slot_end(m, l, met, it);
@@ -609,7 +633,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
   constexpr int kLanes = HD / 8;                    // a K row's
   constexpr int kVLanes = HD / 4;
   static_assert(kItems >= 1 && kUnit / 4 * kVLanes <= kThreads, "staging items");
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
+  const int tid = own_thread(), lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
   const int hd = p.hd;
   constexpr bool kAllStage = kUnit / 4 * kVLanes == kThreads;
   const bool v_stager = kAllStage || tid < kUnit / 4 * kVLanes;
@@ -689,12 +713,10 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
                        finite(vr[e].z) ? vr[e].z : 0.0f, finite(vr[e].w) ? vr[e].w : 0.0f};
     }
   };
-  // the wave's query vectors: parts of dimensions 32 st + 8 lq .. + 7 of vector 32 wave + 16 n + lc
-  v4i qh[2][kSteps], ql[2][kSteps];
-  float q_back[2], m_run[2], l_run[2], odd = 0.0f;
+  // the wave's query vectors, dimensions 32 st + 8 lq .. + 7 of vector 32 wave + 16 n + lc: on their way with the first
+  // step's rows, then their parts
+  float4 x[2][kSteps][2];
   int last[2];
-  const bool busy = 32 * wave < it.vectors; // a wave without vectors only stages
-  v4f o[2][kDt];
 #pragma unroll
   for (int n = 0; n < 2; n++) {
     const int v = 32 * wave + 16 * n + lc;
@@ -702,26 +724,37 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     last[n] = !active ? -1 : it.last0 == INT32_MAX ? INT32_MAX : it.last0 + v / p.kv_mul;
     const float *src = p.q + ((size_t)(it.row0 + (active ? v / p.kv_mul : 0)) * p.n_heads + (size_t)it.g * p.kv_mul +
                               (active ? v % p.kv_mul : 0)) * hd;
-    float4 x[kSteps][2];
-    float top = 0.0f;
 #pragma unroll
     for (int st = 0; st < kSteps; st++)
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        x[st][k] = active ? load4(src, 32 * st + 8 * lq + 4 * k, hd) : float4{0.0f, 0.0f, 0.0f, 0.0f};
-        top = fmaxf(top, peak(x[st][k]));
-      }
+      for (int k = 0; k < 2; k++)
+        x[n][st][k] = load4(src, active ? 32 * st + 8 * lq + 4 * k : hd, hd);
+  }
+  fence();
+  load(); // zeros past the end
+  fence();
+  v4i qh[2][kSteps], ql[2][kSteps];
+  float q_back[2], m_run[2], l_run[2], odd = 0.0f;
+  const bool busy = 32 * wave < it.vectors; // a wave without vectors only stages
+  v4f o[2][kDt];
+#pragma unroll
+  for (int n = 0; n < 2; n++) {
+    float top = 0.0f;
+#pragma unroll
+    for (int st = 0; st < kSteps; st++)
+      top = fmaxf(top, fmaxf(peak(x[n][st][0]), peak(x[n][st][1])));
     top = fminf(four_max(top), FLT_MAX);
     int e;
     const float scale = f16_scale(top, kLeastK, e);
     q_back[n] = __uint_as_float((unsigned)(127 - 14 + e) << 23) * p.scale2;
 #pragma unroll
     for (int st = 0; st < kSteps; st++) {
+      const float4 a = x[n][st][0], b = x[n][st][1];
       int th, tl;
-      f16_pair(x[st][0].x, x[st][0].y, scale, th, tl), qh[n][st][0] = th, ql[n][st][0] = tl;
-      f16_pair(x[st][0].z, x[st][0].w, scale, th, tl), qh[n][st][1] = th, ql[n][st][1] = tl;
-      f16_pair(x[st][1].x, x[st][1].y, scale, th, tl), qh[n][st][2] = th, ql[n][st][2] = tl;
-      f16_pair(x[st][1].z, x[st][1].w, scale, th, tl), qh[n][st][3] = th, ql[n][st][3] = tl;
+      f16_pair(a.x, a.y, scale, th, tl), qh[n][st][0] = th, ql[n][st][0] = tl;
+      f16_pair(a.z, a.w, scale, th, tl), qh[n][st][1] = th, ql[n][st][1] = tl;
+      f16_pair(b.x, b.y, scale, th, tl), qh[n][st][2] = th, ql[n][st][2] = tl;
+      f16_pair(b.z, b.w, scale, th, tl), qh[n][st][3] = th, ql[n][st][3] = tl;
     }
     m_run[n] = -FLT_MAX, l_run[n] = 0.0f;
 #pragma unroll
@@ -822,10 +855,9 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     }
   };
   if (it.t0 < it.t1) {
-    load();
     check();
     stage(stages[0]);
-    load(); // zeros past the end
+    load();
     __syncthreads();
   }
   int turn = 0;
@@ -857,8 +889,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     const int v = 32 * wave + 16 * n + lc;
     if (v >= it.vectors)
       continue;
-    const size_t vec = (size_t)(it.row0 + v / p.kv_mul) * p.n_heads + (size_t)it.g * p.kv_mul + v % p.kv_mul;
-    float *dst = p.partial + (it.slot0 + vec * it.slot_step) * (size_t)(hd + 4);
+    float *dst = slot_of(p, it, v);
     const float back = 0x1p-21f; // 2^14 of the V rows, 2^7 of the weights
 #pragma unroll
     for (int d = 0; d < kDt; d++)
@@ -870,119 +901,167 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
   }
 }
 
+// LDS: the plan, then the walk's.
+constexpr size_t kPlanLds = (sizeof(Plan) + 15) / 16 * 16;
 template <int HD> constexpr size_t fast_lds() {
-  constexpr size_t narrow_sums = (size_t)(kThreads / kWave) * 16 * (HD + 4) * 4;
-  size_t most = sizeof(Plan);
-  most = narrow_sums > most ? narrow_sums : most;
-  return 2 * sizeof(WideStage<HD>) > most ? 2 * sizeof(WideStage<HD>) : most;
+  constexpr size_t narrow_sums = (size_t)(kThreads / kWave) * 16 * (HD + 4) * 4, stages = 2 * sizeof(WideStage<HD>);
+  return kPlanLds + (narrow_sums > stages ? narrow_sums : stages);
+}
+static_assert(kBlocksPerCu * fast_lds<128>() <= 160 * 1024, "blocks of a CU");
+
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uniform(long long x) {
+  return (long long)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
 }
 
-// Blocks: ceil(rows / 256) that write down each row's slots for the merge, then one for each item, the prefix's first (KV
-// head fastest, so that consecutive blocks, which go to the XCDs in turn, give an XCD the same heads' rows), then the
-// requests' own. (Blocks that stay and take items from a counter were slower: 512 of them asking one counter wait for each
-// other, and their loads behind the answer with them.)
-template <int HD, bool FULL> __global__ __launch_bounds__(kThreads, 2) void attn_requests(FastAttn p) {
+// Positions 0 .. e - 1 of a walk that lies at a .. a + time - 1 on the line: the first one behind the cut at x.
+__device__ __forceinline__ int cut_at(long long x, long long a, long long time, int e) {
+  return x <= a ? 0 : x >= a + time ? e : (int)((double)(x - a) / (double)time * e) / kUnit * kUnit;
+}
+
+// Where row `row` finds its partial sums, for the merge.
+__device__ void find_slots(const FastAttn &p, const Plan &plan, int r0) {
+  __shared__ int owner[kThreads];
+  const int tid = threadIdx.x, row = r0 + tid;
+  owner[tid] = -1;
+  __syncthreads();
+  bool bad = false;
+  if (plan.total > 0)
+    for (int r = tid; r < p.batch.count; r += kThreads) {
+      const Request q = request_at(p.batch, r, bad);
+      for (int i = max(q.first, r0); i < min(q.first + q.rows, r0 + kThreads); i++)
+        owner[i - r0] = r;
+    }
+  __syncthreads();
+  if (row >= p.batch.rows)
+    return;
+  RowSlots at{};
+  at.own_first = -1;
+  if (owner[tid] >= 0) {
+    const Request q = request_at(p.batch, owner[tid], bad);
+    const int j = row - q.first, tile = own_tiles(p, q.rows) == 1 ? 0 : j / p.tile_rows;
+    const int rows = min(p.tile_rows, q.rows - tile * p.tile_rows), end = q.length + tile * p.tile_rows + rows;
+    const long long a = plan.line[owner[tid]] - own_time(p, q) + tile_start(p, q.length, tile);
+    at.own_first = (int)whole(a, plan.slice);
+    at.own_last = (int)whole(a + walk_time(rows * p.kv_mul, end) - 1, plan.slice);
+    at.own_v = (j - tile * p.tile_rows) * p.kv_mul;
+    at.slot = q.slot;
+    at.last = q.length + j;
+    if (p.batch.prefix) {
+      const int i = row - plan.first_row, t = i / p.tile_rows;
+      const long long b = t * plan.full, e = min(b + plan.full, plan.prefix);
+      at.prefix_first = (int)whole(b, plan.slice);
+      at.prefix_last = (int)whole(e - 1, plan.slice);
+      at.prefix_v = (i - t * p.tile_rows) * p.kv_mul;
+    }
+  }
+  p.rows[row] = at;
+}
+
+// Blocks: p.blocks for each KV head (the head fastest, so that consecutive blocks, which go to the XCDs in turn, give an XCD
+// the same heads' rows, and that the two blocks of a CU come from different parts of the line), then ceil(rows / 256) that
+// write down each row's slots for the merge (in front they kept blocks with slices from starting with the others).
+template <int HD, bool FULL> __global__ __launch_bounds__(kThreads, kBlocksPerCu) void attn_requests(FastAttn p) {
   extern __shared__ __align__(16) unsigned char lds[];
   Plan &plan = *reinterpret_cast<Plan *>(lds);
   make_plan(p, plan);
-  const int tid = threadIdx.x, step = plan.step;
-  const int row_blocks = ceil_div(p.batch.rows, kThreads);
-  const int prefix_shares = ceil_div(prefix_cost(p), step);
-  const int prefix_items = p.prefix_tiles * prefix_shares * p.n_kv_heads;
-  const size_t prefix_slots = (size_t)p.batch.rows * p.n_heads * prefix_shares;
-  if (blockIdx.x == 0 && tid == 0) {
-    p.header[0] = prefix_shares;
-    if (plan.bad)
-      p.flags[3] = 1;
-  }
-  if ((int)blockIdx.x < row_blocks) {
-    __shared__ int4 mine[kThreads];
-    const int r0 = blockIdx.x * kThreads;
-    mine[tid] = int4{0, -1, 0, 0};
-    __syncthreads();
-    bool bad = false;
-    for (int r = tid; r < p.batch.count; r += kThreads) {
-      const Request q = request_at(p.batch, r, bad);
-      if (plan.total_rows > p.batch.rows)
-        continue;
-      const int shares = own_shares(p, q, step);
-      const int slot0 = plan.slots[r] - q.rows * p.n_heads * shares;
-      for (int i = max(q.first, r0); i < min(q.first + q.rows, r0 + kThreads); i++)
-        mine[i - r0] = int4{slot0 + (i - q.first) * p.n_heads * shares, shares, q.slot, q.length + i - q.first};
-    }
-    __syncthreads();
-    if (r0 + tid < p.batch.rows)
-      p.row_slots[r0 + tid] = mine[tid];
+  const int tid = threadIdx.x;
+  const int i = blockIdx.x, g = i % p.n_kv_heads, block = i / p.n_kv_heads;
+  if (block >= p.blocks) {
+    find_slots(p, plan, (i - p.blocks * p.n_kv_heads) * kThreads);
     return;
   }
-  int i = blockIdx.x - row_blocks;
-  if (i >= prefix_items + plan.items[p.batch.count - 1])
-    return;
-  Item it;
-  bool narrow;
-  if (i < prefix_items) {
-    it.g = i % p.n_kv_heads;
-    i /= p.n_kv_heads;
-    const int tile = i % p.prefix_tiles, share = i / p.prefix_tiles;
-    const int length = ceil_div(ceil_div(p.batch.prefix, kUnit), prefix_shares) * kUnit;
-    const int rows = p.prefix_narrow ? p.batch.rows : p.tile_rows;
-    // rows that belong to no request before the first and behind the last one stay out
-    it.row0 = max(tile * rows, plan.first_row);
-    it.vectors = max(min(tile * rows + rows, plan.end_row) - it.row0, 0) * p.kv_mul;
-    it.key = p.prefix_key + (size_t)it.g * p.batch.prefix_head_base;
-    it.value = p.prefix_value + (size_t)it.g * p.batch.prefix_head_base;
-    it.pos_stride = p.batch.prefix_pos_stride;
-    it.t0 = min(share * length, p.batch.prefix);
-    it.t1 = min(it.t0 + length, p.batch.prefix);
-    it.last0 = INT32_MAX;
-    it.slot0 = share;
-    it.slot_step = prefix_shares;
-    narrow = p.prefix_narrow;
-  } else {
-    i -= prefix_items;
-    int lo = 0, hi = p.batch.count - 1; // the first request whose running sum passes i
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (plan.items[mid] > i)
-        hi = mid;
-      else
-        lo = mid + 1;
+  const long long x0 = uniform(block * plan.slice), x1 = uniform(min(block * plan.slice + plan.slice, plan.total));
+  const size_t begins = (size_t)p.batch.rows * p.n_heads; // slots of the walks that begin in a block, prefix and own each
+  int r = -1;
+  for (long long x = x0; x < x1;) {
+    Item it;
+    long long a, time; // the walk's place
+    int end;           // its positions
+    const bool prefix = x < plan.prefix;
+    if (prefix) {
+      const int tile = (int)whole(x, plan.full);
+      a = tile * plan.full;
+      time = min(plan.full, plan.prefix - a);
+      end = p.batch.prefix;
+      it.row0 = plan.first_row + tile * p.tile_rows;
+      it.vectors = min(p.tile_rows, plan.end_row - it.row0) * p.kv_mul;
+      it.key = p.prefix_key + (size_t)g * p.batch.prefix_head_base;
+      it.value = p.prefix_value + (size_t)g * p.batch.prefix_head_base;
+      it.pos_stride = p.batch.prefix_pos_stride;
+      it.last0 = INT32_MAX;
+    } else {
+      if (r < 0) {
+        int lo = 0, hi = p.batch.count - 1; // the first request whose walks end behind x
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (plan.line[mid] > x)
+            hi = mid;
+          else
+            lo = mid + 1;
+        }
+        r = lo;
+      }
+      while (plan.line[r] <= x) // requests without rows; the last one's end is the line's
+        r++;
+      bool bad = false;
+      const Request q = r < kTable ? plan.table[r] : request_at(p.batch, r, bad);
+      const long long begin = plan.line[r] - own_time(p, q);
+      int tile = 0;
+      for (int hi = own_tiles(p, q.rows) - 1; tile < hi;) { // the last tile that begins at or before x
+        const int mid = (tile + hi + 1) / 2;
+        if (begin + tile_start(p, q.length, mid) <= x)
+          tile = mid;
+        else
+          hi = mid - 1;
+      }
+      const int j0 = tile * p.tile_rows, rows = min(p.tile_rows, q.rows - j0);
+      const size_t cache = (size_t)q.slot * p.batch.slot_floats + (size_t)g * p.batch.head_base;
+      end = q.length + j0 + rows;
+      a = begin + tile_start(p, q.length, tile);
+      time = walk_time(rows * p.kv_mul, end);
+      it.row0 = q.first + j0;
+      it.vectors = rows * p.kv_mul;
+      it.key = p.key + cache;
+      it.value = p.value + cache;
+      it.pos_stride = p.batch.pos_stride;
+      it.last0 = q.length + j0;
     }
-    bool bad = false;
-    const int r = lo;
-    const Request q = request_at(p.batch, r, bad);
-    const int shares = own_shares(p, q, step), tiles = own_tiles(p, q.rows);
-    i -= plan.items[r] - tiles * shares * p.n_kv_heads;
-    it.g = i % p.n_kv_heads;
-    i /= p.n_kv_heads;
-    const int tile = i % tiles, share = i / tiles;
-    narrow = own_narrow(p, q.rows);
-    const int j0 = narrow ? 0 : tile * p.tile_rows, rows = narrow ? q.rows : min(p.tile_rows, q.rows - j0);
-    const int end = q.length + j0 + rows;
-    const int length = ceil_div(ceil_div(end, kUnit), shares) * kUnit;
-    const size_t cache = (size_t)q.slot * p.batch.slot_floats + (size_t)it.g * p.batch.head_base;
-    it.row0 = q.first + j0;
-    it.vectors = rows * p.kv_mul;
-    it.key = p.key + cache;
-    it.value = p.value + cache;
-    it.pos_stride = p.batch.pos_stride;
-    it.t0 = min(share * length, end);
-    it.t1 = min(it.t0 + length, end);
-    it.last0 = q.length + j0;
-    // the request's slots are [row][head][share]; slot0 makes up for vec counting from row 0 of the batch
-    it.slot0 = prefix_slots + (size_t)(plan.slots[r] - q.rows * p.n_heads * shares) + share -
-               (size_t)q.first * p.n_heads * shares;
-    it.slot_step = shares;
+    a = uniform(a);
+    time = uniform(time);
+    r = uniform(r);
+    it.g = g;
+    it.row0 = uniform(it.row0);
+    it.vectors = uniform(it.vectors);
+    it.last0 = uniform(it.last0);
+    it.t0 = uniform(cut_at(x, a, time, end));
+    it.t1 = uniform(cut_at(x1, a, time, end));
+    if (a >= x0) {
+      it.slot0 = (prefix ? 0 : begins) + (size_t)it.row0 * p.n_heads + (size_t)g * p.kv_mul;
+      it.slot_row = p.n_heads;
+    } else {
+      it.slot0 = 2 * begins + ((size_t)g * p.blocks + block) * kTileVectors;
+      it.slot_row = p.kv_mul;
+    }
+    if (x != x0)
+      __syncthreads(); // the walk before is done with its LDS
+    if (it.t0 == it.t1) { // a cut within the first step's positions: nothing is left for this side of it
+      const int quads = p.hd / 4 + 1;
+      for (int e = tid; e < it.vectors * quads; e += kThreads)
+        *reinterpret_cast<float4 *>(slot_of(p, it, e / quads) + 4 * (e % quads)) =
+            float4{e % quads == quads - 1 ? -FLT_MAX : 0.0f, 0.0f, 0.0f, 0.0f};
+    } else if (it.vectors <= kNarrowVectors) {
+      walk_narrow<HD, FULL>(p, it, lds + kPlanLds);
+    } else {
+      walk_wide<HD, FULL>(p, it, lds + kPlanLds);
+    }
+    x = a + time;
   }
-  __syncthreads(); // the plan's place is taken by the walk
-  if (narrow)
-    walk_narrow<HD, FULL>(p, it, lds);
-  else
-    walk_wide<HD, FULL>(p, it, lds);
 }
 
-// A thread per (row, head, four dimensions): the row's shares of the prefix and its own, rescaled to their largest maximum
-// and added in order.
+// A thread per (row, head, four dimensions): the row's partial sums over the prefix and over its own positions, rescaled to
+// their largest maximum and added in order.
 __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
   const int hd4 = p.hd / 4;
   const long long idx = (long long)blockIdx.x * kThreads + threadIdx.x;
@@ -990,24 +1069,31 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
     return;
   const int d4 = (int)(idx % hd4);
   const long long vec = idx / hd4;
-  const int row = (int)(vec / p.n_heads), head = (int)(vec % p.n_heads);
-  const int4 mine = p.row_slots[row];
-  if (mine.y < 0)
+  const int row = (int)(vec / p.n_heads), head = (int)(vec % p.n_heads), g = head / p.kv_mul, h = head % p.kv_mul;
+  const RowSlots mine = p.rows[row];
+  if (mine.own_first < 0)
     return;
-  const int shared = p.header[0], count = shared + mine.y;
-  const size_t slot = (size_t)(p.hd + 4);
-  const float *far = p.partial + (size_t)vec * shared * slot;
-  const float *own = p.partial + ((size_t)p.batch.rows * p.n_heads * shared + (size_t)mine.x + (size_t)head * mine.y) * slot;
+  const int shared = p.batch.prefix ? mine.prefix_last - mine.prefix_first + 1 : 0;
+  const int count = shared + mine.own_last - mine.own_first + 1;
+  const size_t slot = (size_t)(p.hd + 4), begins = (size_t)p.batch.rows * p.n_heads;
+  auto slot_at = [&](int s) {
+    const bool prefix = s < shared;
+    const int k = prefix ? s : s - shared, block = (prefix ? mine.prefix_first : mine.own_first) + k;
+    const size_t at = k == 0 ? (prefix ? 0 : begins) + (size_t)vec
+                             : 2 * begins + ((size_t)g * p.blocks + block) * kTileVectors +
+                                   (prefix ? mine.prefix_v : mine.own_v) + h;
+    return p.partial + at * slot;
+  };
   float m = -FLT_MAX, l = 0.0f;
   float4 o = float4{0.0f, 0.0f, 0.0f, 0.0f};
   bool met = false;
-  constexpr int kAhead = 4; // shares whose loads are in flight together
+  constexpr int kAhead = 8; // shares whose loads are in flight together
   for (int s0 = 0; s0 < count; s0 += kAhead) {
     float4 end[kAhead], x[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; k++) {
       const int s = min(s0 + k, count - 1);
-      const float *src = s < shared ? far + (size_t)s * slot : own + (size_t)(s - shared) * slot;
+      const float *src = slot_at(s);
       end[k] = *reinterpret_cast<const float4 *>(src + p.hd);
       x[k] = *reinterpret_cast<const float4 *>(src + 4 * d4);
     }
@@ -1029,15 +1115,14 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
       }
   }
   if (met) { // V values that are not finite, whatever their weights: a positive one changes neither infinity nor NaN
-    const int g = head / p.kv_mul;
     for (int s = 0; s < count; s++) {
-      const float *src = s < shared ? far + (size_t)s * slot : own + (size_t)(s - shared) * slot;
+      const float *src = slot_at(s);
       const bool prefix = s < shared;
       const int t0 = max(__float_as_int(src[p.hd + 2]), 0), t1 = __float_as_int(src[p.hd + 3]);
       const float *v = prefix ? p.prefix_value + (size_t)g * p.batch.prefix_head_base
-                              : p.value + (size_t)mine.z * p.batch.slot_floats + (size_t)g * p.batch.head_base;
+                              : p.value + (size_t)mine.slot * p.batch.slot_floats + (size_t)g * p.batch.head_base;
       const size_t stride = prefix ? p.batch.prefix_pos_stride : p.batch.pos_stride;
-      for (int t = t0; t < min(t1, prefix ? p.batch.prefix : mine.w + 1); t++) {
+      for (int t = t0; t < min(t1, prefix ? p.batch.prefix : mine.last + 1); t++) {
         const float4 y = *reinterpret_cast<const float4 *>(v + (size_t)t * stride + 4 * d4);
         o = float4{finite(y.x) ? o.x : o.x + y.x, finite(y.y) ? o.y : o.y + y.y, finite(y.z) ? o.z : o.z + y.z,
                    finite(y.w) ? o.w : o.w + y.w};
@@ -1059,41 +1144,33 @@ bool attention_requests_fast(const AttentionRequestsJob &job) {
   return job.head_dim <= 128 && job.head_dim % 4 == 0 && (all & 15) == 0 && b.rows <= (1 << 20) && job.n_heads <= 1024 && near;
 }
 
-// The most blocks and slots that a plan can ask for, whatever the arrays hold: every walk is cut into units / step + 1
-// shares at most, and step is at least 1 / kTargetItems of all units.
-struct FastBounds {
-  long long prefix_tiles, items, slots;
-  bool prefix_narrow;
-  int tile_rows;
-};
-FastBounds fast_bounds(const AttentionRequestsJob &job) {
+// Blocks of a KV head: what the chip holds at once, or as many as the longest line that the buffers' sizes allow gives
+// slices of kMinSlice.
+static int fast_blocks(const AttentionRequestsJob &job) {
   const RequestsDev &b = job.batch;
-  const int kv_mul = job.n_heads / job.n_kv_heads;
-  FastBounds f{};
-  f.tile_rows = kTileVectors / kv_mul;
-  f.prefix_narrow = b.rows * kv_mul <= kNarrowVectors;
-  f.prefix_tiles = !b.prefix ? 0 : f.prefix_narrow ? 1 : (b.rows + f.tile_rows - 1) / f.tile_rows;
-  const long long own_tiles = (b.count < b.rows ? b.count : b.rows) + b.rows / f.tile_rows;
-  const long long units = kWideCost * (f.prefix_tiles * ((b.prefix + kUnit - 1) / kUnit) +
-                                       own_tiles * (((long long)b.seq_len + kUnit - 1) / kUnit));
-  const long long shares = (units * job.n_kv_heads + kMinUnits - 1) / kMinUnits;
-  f.items = (shares < kTargetItems ? shares : kTargetItems) + job.n_kv_heads * (f.prefix_tiles + own_tiles);
-  const long long vectors = (long long)b.rows * job.n_heads;
-  // rows times shares, over the prefix and over the requests' own: see the plan; and no walk has more than kMaxShares
-  const long long capped = 2 * vectors * kMaxShares, spread = 2 * vectors + (long long)kTileVectors * kTargetItems * 2;
-  f.slots = capped < spread ? capped : spread;
-  return f;
+  const long long cus = device().cu_count > 0 ? device().cu_count : 256, kv_mul = job.n_heads / job.n_kv_heads;
+  const long long tile_rows = kTileVectors / kv_mul, tiles = (b.rows + tile_rows - 1) / tile_rows;
+  const long long own = (b.count < b.rows ? b.count : b.rows) + tiles; // own tiles
+  constexpr WalkTime wide = walk_time_of(kTileVectors);                // the longest
+  const long long line = (b.prefix ? tiles * (wide.begin + (long long)wide.position * b.prefix) : 0) +
+                         own * (wide.begin + (long long)wide.position * b.seq_len);
+  const long long most = (line + kMinSlice - 1) / kMinSlice, held = kBlocksPerCu * cus / job.n_kv_heads;
+  return (int)(most < held ? most : held > 1 ? held : 1);
+}
+
+// Slots: one for each vector of the prefix's walks and of the requests' own, and a tile's for each block, which goes on with
+// one walk at most.
+static size_t fast_slots(const AttentionRequestsJob &job) {
+  return 2 * (size_t)job.batch.rows * job.n_heads + (size_t)job.n_kv_heads * fast_blocks(job) * kTileVectors;
 }
 
 size_t attention_requests_workspace(const AttentionRequestsJob &job) {
   if (!attention_requests_fast(job))
     return 0;
-  return (size_t)fast_bounds(job).slots * (size_t)(job.head_dim + 4) * sizeof(float) +
-         (size_t)job.batch.rows * sizeof(int4) + 256;
+  return 256 + fast_slots(job) * (size_t)(job.head_dim + 4) * sizeof(float) + (size_t)job.batch.rows * sizeof(RowSlots);
 }
 
 bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hipStream_t stream) {
-  const FastBounds f = fast_bounds(job);
   FastAttn p{};
   p.out = job.out;
   p.q = job.q;
@@ -1106,15 +1183,13 @@ bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hip
   p.n_kv_heads = job.n_kv_heads;
   p.kv_mul = job.n_heads / job.n_kv_heads;
   p.hd = job.head_dim;
-  p.tile_rows = f.tile_rows;
-  p.prefix_tiles = (int)f.prefix_tiles;
-  p.prefix_narrow = f.prefix_narrow;
+  p.tile_rows = kTileVectors / p.kv_mul;
+  p.blocks = fast_blocks(job);
   p.scale2 = 1.4426950408889634f / sqrtf((float)job.head_dim);
-  p.header = (int *)workspace;
-  p.row_slots = (int4 *)((char *)workspace + 256);
-  p.partial = (float *)((char *)workspace + 256 + (size_t)job.batch.rows * sizeof(int4));
+  p.rows = (RowSlots *)((char *)workspace + 256);
+  p.partial = (float *)(p.rows + job.batch.rows);
   p.flags = device().error_flags;
-  const long long blocks = f.items + (job.batch.rows + kThreads - 1) / kThreads;
+  const long long blocks = (long long)p.blocks * p.n_kv_heads + (job.batch.rows + kThreads - 1) / kThreads;
   const bool full = job.head_dim == 64 || job.head_dim == 128;
   const auto kernel = job.head_dim <= 64 ? (full ? attn_requests<64, true> : attn_requests<64, false>)
                                          : (full ? attn_requests<128, true> : attn_requests<128, false>);
