@@ -329,15 +329,6 @@ __device__ __forceinline__ float *slot_of(const FastAttn &p, const Item &it, int
 // step need more than the 256 registers that two waves a SIMD leave each).
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
-// The region's matrix instructions each followed by five others, which run while the matrix cores work.
-__device__ __forceinline__ void interleave() {
-#pragma unroll
-  for (int i = 0; i < 48; i++) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix
-    __builtin_amdgcn_sched_group_barrier(0x002, 5, 0); // vector
-  }
-}
-
 // The thread's number, new to the compiler at each walk: else it keeps what both walks derive from it in registers all along
 // a block's walks (43 of them spilled).
 __device__ __forceinline__ int own_thread() {
@@ -835,22 +826,30 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
       }
     }
     fence();
-#pragma unroll
-    for (int d = 0; d < kDt; d += 2) { // the products in turn over four sums, as above
-      v4i vh[2], vl[2];
+    // the products in turn over four sums, as above; the next operands are on their way meanwhile
+    v4i vh[2][2], vl[2][2];
+    auto fetch = [&](int d, int buffer) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         const int at = v_unit(16 * (d + i) + lc, lq);
-        vh[i] = *reinterpret_cast<const v4i *>(&sh.v[0][at]);
-        vl[i] = *reinterpret_cast<const v4i *>(&sh.v[1][at]);
+        vh[buffer][i] = *reinterpret_cast<const v4i *>(&sh.v[0][at]);
+        vl[buffer][i] = *reinterpret_cast<const v4i *>(&sh.v[1][at]);
       }
+    };
+    fetch(0, 0);
+#pragma unroll
+    for (int d = 0; d < kDt; d += 2) {
+      const int now = d / 2 % 2;
+      if (d + 2 < kDt)
+        fetch(d + 2, now ^ 1);
+      fence();
 #pragma unroll
       for (int k = 0; k < 3; k++)
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int n = 0; n < 2; n++)
-            o[n][d + i] = mfma_f16(k == 0 ? vl[i] : vh[i], k == 1 ? pl[n] : ph[n], o[n][d + i]);
+            o[n][d + i] = mfma_f16(k == 0 ? vl[now][i] : vh[now][i], k == 1 ? pl[n] : ph[n], o[n][d + i]);
       fence();
     }
   };
@@ -865,11 +864,9 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     check();
     fence();
     if (busy) {
-      // the scores' matrix instructions with the next step's staging between them (its stage was read before the last
-      // barrier; past the end it takes zeros that nobody reads)
       score(stages[turn]);
+      // the next step's stage was read before the last barrier; past the end it takes zeros that nobody reads
       stage(stages[turn ^ 1]);
-      interleave();
       fence();
       load();
       fence();
