@@ -55,9 +55,12 @@ void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride,
  * request r attends to positions 0 .. prefix - 1 of prefix_key / prefix_value and to own positions 0 .. length[r] + j of
  * its slot (whose last rows llhip_rope_kv_store_requests stored). q and out hold rows of n_heads * head_dim floats;
  * scores, softmax and value sums as in k_attention (FP32-accurate; a non-finite score fails with "nonfinite value in
- * softmax"). The prefix is read once for all requests, not once for each. prefix_key and prefix_value may be NULL where
- * prefix is 0; requests may share a slot here. out must not overlap q or a cache. The shapes are k_attention's: n_heads
- * a multiple of n_kv_heads, at most 16 per KV head, head_dim at most 256. */
+ * softmax"). The sums are divided by the weights' at the end, so n positions' values must stay below 3e38 / n, as there;
+ * products with values far below 2^-30 of their K row's largest, or of the largest in four V rows, are exact to about 2^-36
+ * of that, and V rows of very different sizes keep this up to 2^80. The prefix is read once for all requests, not once for
+ * each. prefix_key and prefix_value may be NULL where prefix is 0; requests may share a slot here. out must not overlap q
+ * or a cache. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16 per KV head, head_dim at most
+ * 256. */
 void llhip_attention_requests(float *out, const float *q, const float *prefix_key, const float *prefix_value,
                               const float *key_cache, const float *value_cache, const RequestBatch *batch, int n_heads,
                               int n_kv_heads, int head_dim);
@@ -70,7 +73,8 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
  * A row without an adapter has P = 0. base and base3 have c's leading dimension, and either may be c itself. A is
  * adapters x rank x k and B adapters x n x rank, row-major; rank 1 .. LLHIP_MAX_LORA_RANK, the same for the segment's
  * adapters (smaller ones padded with zeros). Sums are FP32 throughout, also over BF16 adapters (the activations are not
- * rounded). c must not overlap x, the adapters, or another segment's c or base. */
+ * rounded); a row of x, or an adapter, that holds an infinity or a NaN gives its rows' columns NaN or infinity. c must not
+ * overlap x, the adapters, or another segment's c or base. */
 typedef struct {
   float *c;
   int ldc;
@@ -109,8 +113,8 @@ void llhip_lora_bf16(const float *x, int ldx, int m, int k, const int *adapter, 
  * accepted[r] receives the number of accepted drafts and next[r] the token after them; a request without rows keeps
  * both. Logits of -infinity are tokens masked out. A row that decides with a NaN, +infinity or no token left, and a
  * draft outside the vocabulary, set both to -1 and fail at the next host-visible point. Probabilities, sums and the
- * borders between tokens are FP64; uniform lies in [0, 1). At most LLHIP_MAX_REQUESTS requests, 2^20
- * rows and 2^22 tokens. */
+ * borders between tokens are FP64; uniform lies in [0, 1). accepted and next must not overlap each other or an input. At
+ * most LLHIP_MAX_REQUESTS requests, 2^20 rows and 2^22 tokens. */
 void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t ld, const float *draft_logits,
                          size_t draft_ld, const int *tokens, const float *uniform, const int *start, int count, int rows,
                          int vocab, float temperature);

@@ -2,6 +2,7 @@
 // as for the other calls, one stream-ordered operation per call.
 #include <cmath>
 #include <cstring>
+#include <mutex>
 
 #include "common.h"
 #include "llama_hip_requests.h"
@@ -61,7 +62,9 @@ size_t caches_bytes(const RequestBatch *b, int n_kv_heads, int head_dim) {
 }
 
 // The scratch of these calls, which the library stream orders: grown on demand (never during graph capture), kept for the
-// process. Its first 256 bytes are counters, zero between the calls. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows.
+// process. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows. A call
+// holds the lock until its kernels are queued, so that another thread's do not come between them.
+std::mutex scratch_mutex;
 void *scratch_memory = nullptr;
 size_t scratch_bytes = 0;
 bool scratch_captured = false;
@@ -87,13 +90,6 @@ bool workspace(const char *name, size_t bytes, void **out) {
       hbm_release(want);
       scratch_memory = nullptr;
       return raise("%s: allocating %zu bytes of workspace failed", name, want);
-    }
-    if (hipMemset(scratch_memory, 0, 256) != hipSuccess || hipDeviceSynchronize() != hipSuccess) { // counters
-      (void)hipGetLastError();
-      (void)hipFree(scratch_memory);
-      hbm_release(want);
-      scratch_memory = nullptr;
-      return raise("%s: clearing the workspace failed", name);
     }
     scratch_bytes = want;
   }
@@ -199,11 +195,14 @@ void lora(const char *name, const float *x, int ldx, int m, int k, const int *ad
                                 swiglu ? call.ptr<const void>(W[i][3]) : nullptr,
                                 s.scale ? call.ptr<const float>(S[i]) : nullptr, s.ldc, s.n, s.rank, swiglu};
   }
+  std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
   if (!workspace(name, lora_workspace(job), &scratch))
     return;
-  if (launch_lora(job, scratch, call.stream()))
-    call.finish();
+  if (!launch_lora(job, scratch, call.stream()))
+    return;
+  lock.unlock();
+  call.finish();
 }
 
 } // namespace
@@ -314,11 +313,14 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
                            batch->prefix ? call.ptr<const float>(PV) : nullptr, call.ptr<const float>(K),
                            call.ptr<const float>(V), batch_dev(call, refs, batch, n_kv_heads, head_dim), n_heads,
                            n_kv_heads, head_dim};
+  std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
   if (!workspace(name, attention_requests_workspace(job), &scratch))
     return;
-  if (launch_attention_requests(job, scratch, call.stream()))
-    call.finish();
+  if (!launch_attention_requests(job, scratch, call.stream()))
+    return;
+  lock.unlock();
+  call.finish();
 }
 
 void llhip_lora_f32(const float *x, int ldx, int m, int k, const int *adapter, int adapters, const LoraSegment *segments,
@@ -365,6 +367,16 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
     raise("%s: accepted and next must not overlap", name);
     return;
   }
+  const size_t logits_bytes = ((size_t)(rows - 1) * ld + vocab) * kFloat;
+  const size_t draft_bytes = ((size_t)(rows - 1) * draft_ld + vocab) * kFloat;
+  for (const int *out : {accepted, next})
+    if (overlaps(out, out_bytes, logits, logits_bytes) || overlaps(out, out_bytes, draft_logits, draft_bytes) ||
+        overlaps(out, out_bytes, tokens, (size_t)rows * sizeof(int)) ||
+        overlaps(out, out_bytes, start, ((size_t)count + 1) * sizeof(int)) ||
+        (!greedy && overlaps(out, out_bytes, uniform, (size_t)rows * 2 * kFloat))) {
+      raise("%s: accepted and next must not overlap an input", name);
+      return;
+    }
   Call call(name);
   const size_t row = (size_t)vocab * kFloat;
   Ref A = call.out(accepted, out_bytes, true), N = call.out(next, out_bytes, true); // requests without rows keep both
@@ -378,11 +390,14 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
                       draft_logits ? call.ptr<const float>(D) : nullptr, ld, draft_ld, call.ptr<const int>(T),
                       call.ptr<const int>(S), greedy ? nullptr : call.ptr<const float>(U), count, rows, vocab,
                       temperature};
+  std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
   if (!workspace(name, verify_workspace(job), &scratch))
     return;
-  if (launch_verify(job, scratch, call.stream()))
-    call.finish();
+  if (!launch_verify(job, scratch, call.stream()))
+    return;
+  lock.unlock();
+  call.finish();
 }
 
 } // extern "C"

@@ -631,7 +631,8 @@ LoraShape lora_shape(const LoraJob &job) {
   f.width = 16 * f.first_tile[f.matrices];
   const int groups = job.adapters + 1 < job.m ? job.adapters + 1 : job.m;
   f.tiles = job.m / kTileRows + groups;
-  // shares of K: four blocks a CU (one: 82 us for 1100 rows beside W1 and W3, two 83, four 81), each wave at least two steps of 32 values
+  // shares of K: four blocks a CU (one: 82 us for 1100 rows beside W1 and W3, two 83, four 81), each wave at least two
+  // steps of 32 values
   const int cus = device().cu_count > 0 ? device().cu_count : 256, steps = (job.k + 31) / 32;
   const int most = steps / (2 * kThreads / kWave) > 1 ? steps / (2 * kThreads / kWave) : 1;
   const int want = (4 * cus + f.tiles - 1) / f.tiles;
@@ -645,7 +646,8 @@ size_t lora_workspace(const LoraJob &job) {
   if (!lora_tiled(job))
     return 0;
   const LoraShape f = lora_shape(job);
-  return 256 + (size_t)f.tiles * (sizeof(Tiled::Tile) + (size_t)(f.shares + (f.join ? 1 : 0)) * kTileRows * f.width * sizeof(float)) + 64;
+  const size_t sums = (size_t)(f.shares + (f.join ? 1 : 0)) * kTileRows * f.width * sizeof(float);
+  return (size_t)f.tiles * (sizeof(Tiled::Tile) + sums) + 64;
 }
 
 namespace {
@@ -661,7 +663,7 @@ template <class T> bool launch_tiled(const LoraJob &job, void *workspace, hipStr
   p.skip_plain = f.skip_plain;
   p.tiles = f.tiles;
   p.width = f.width;
-  p.tile = (Tiled::Tile *)((char *)workspace + 256);
+  p.tile = (Tiled::Tile *)workspace;
   p.low = (float *)(((uintptr_t)(p.tile + f.tiles) + 15) & ~(uintptr_t)15);
   p.joined = f.join ? p.low + (size_t)f.shares * f.tiles * kTileRows * f.width : p.low;
   p.flags = device().error_flags;

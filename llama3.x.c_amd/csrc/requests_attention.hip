@@ -416,7 +416,7 @@ template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, cons
   constexpr int kSteps = HD / 32, kDt = HD / 16, kWaves = kThreads / kWave, kRow = HD + 4;
   const int tid = own_thread(), lane = tid & (kWave - 1), wave = tid / kWave, lq = lane >> 4, lc = lane & 15;
   const int hd = p.hd;
-  const int tiles = it.vectors <= 16 ? 1 : it.vectors <= 32 ? 2 : 4, walkers = kWaves / tiles; // waves of a tile
+  const int tiles = it.vectors <= 16 ? 1 : 2, walkers = kWaves / tiles; // waves of a tile
   const int v_mine = 16 * (wave / walkers) + lc; // this lane's vector
   const bool active = v_mine < it.vectors;
   float4 x[kSteps][2]; // dimensions 32 st + 8 lq .. + 7, on their way with the first step's rows
@@ -600,7 +600,8 @@ template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, cons
 // BF16 parts take six. The parts need values near 2^15: each query vector and each K row is scaled by a power of two of
 // its own, taken out of the score again; each group of four V rows likewise, and its exponent ev joins the score before
 // the exponential, so that the weights are exp2(s + ev - m) and meet V 2^-ev, with m the running maximum of s + ev. The
-// softmax's sum takes them times 2^-ev.
+// softmax's sum takes them times 2^-ev. A product is so exact to about 2^-36 of its row's largest value (for V of the
+// largest in four rows), and the sum holds groups up to 2^140 apart: between 2^-60, which smaller values take, and 2^80.
 // V parts lie transposed, a dimension's 32 slots in 64 bytes, its 16-byte units where v_unit puts them: a matrix operand's
 // read takes one unit of 16 dimensions, a staging write half a unit of every fourth one, and both spread over the banks.
 template <int HD> struct WideStage {
@@ -619,7 +620,7 @@ __device__ __forceinline__ int v_unit(int dim, int unit) { // in halves
 template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
   typedef WideStage<HD> Stage;
   Stage *const stages = reinterpret_cast<Stage *>(lds); // two: a step is staged while the one before is computed
-  constexpr int kSteps = HD / 32, kDt = HD / 16, kLeastK = -100, kLeastV = -30;
+  constexpr int kSteps = HD / 32, kDt = HD / 16, kLeastK = -100, kLeastV = -60;
   constexpr int kItems = kUnit * HD / 8 / kThreads; // K staging items of eight values a thread
   constexpr int kLanes = HD / 8;                    // a K row's
   constexpr int kVLanes = HD / 4;
@@ -671,7 +672,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
       float top = fmaxf(fmaxf(peak(vr[0]), peak(vr[1])), fmaxf(peak(vr[2]), peak(vr[3])));
       top = group_reduce_max(top, kVLanes);
       int ev;
-      const float scale = f16_scale(top, kLeastV, ev);
+      const float scale = f16_scale(top > 0.0f ? top : 1.0f, kLeastV, ev); // rows of zeros take no extreme exponent
       // slot of position 16 t + 4 q + e: 8 q + 4 t + e, so the four of this item are half of unit vg % 4
       auto put = [&](int d, float x0, float x1, float x2, float x3) {
         int h0, l0, h1, l1;
@@ -687,7 +688,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
       put(3, vr[0].w, vr[1].w, vr[2].w, vr[3].w);
       const int e = 4 * vg + tid % 4;
       sh.v_exp[e] = (float)ev;
-      sh.v_back[e] = __uint_as_float((unsigned)max(127 - ev, 1) << 23);
+      sh.v_back[e] = __uint_as_float(ev < 127 ? (unsigned)(127 - ev) << 23 : 1u << 22);
     }
   };
   // the loaded V values that are not finite become 0
@@ -790,7 +791,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
         const float4 v_exp = *reinterpret_cast<const float4 *>(&sh.v_exp[16 * t + 4 * lq]);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float x = fmaf(sc[n][t][e] * of(k_back, e), q_back[n], of(v_exp, e));
+          const float x = fmaf(sc[n][t][e], of(k_back, e) * q_back[n], of(v_exp, e));
           pv[4 * t + e] = 16 * t + e <= seen ? x : -FLT_MAX;
           odd = fmaf(pv[4 * t + e], 0.0f, odd);
           top = fmaxf(top, pv[4 * t + e]);
@@ -1138,7 +1139,10 @@ bool attention_requests_fast(const AttentionRequestsJob &job) {
                         (uintptr_t)job.key | (uintptr_t)job.value;
   // a walk's rows lie within 2^31 bytes, which its loads' 32-bit offsets reach
   const bool near = (size_t)b.prefix * b.prefix_pos_stride < (1u << 29) && (size_t)b.seq_len * b.pos_stride < (1u << 29);
-  return job.head_dim <= 128 && job.head_dim % 4 == 0 && (all & 15) == 0 && b.rows <= (1 << 20) && job.n_heads <= 1024 && near;
+  // the merge's launch holds fewer than 2^32 threads
+  const bool few = (uint64_t)b.rows * job.n_heads * job.head_dim / 4 <= (1u << 31);
+  return job.head_dim <= 128 && job.head_dim % 4 == 0 && (all & 15) == 0 && b.rows <= (1 << 20) && job.n_heads <= 1024 &&
+         near && few;
 }
 
 // Blocks of a KV head: what the chip holds at once, or as many as the longest line that the buffers' sizes allow gives
@@ -1164,7 +1168,7 @@ static size_t fast_slots(const AttentionRequestsJob &job) {
 size_t attention_requests_workspace(const AttentionRequestsJob &job) {
   if (!attention_requests_fast(job))
     return 0;
-  return 256 + fast_slots(job) * (size_t)(job.head_dim + 4) * sizeof(float) + (size_t)job.batch.rows * sizeof(RowSlots);
+  return fast_slots(job) * (size_t)(job.head_dim + 4) * sizeof(float) + (size_t)job.batch.rows * sizeof(RowSlots);
 }
 
 bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hipStream_t stream) {
@@ -1183,7 +1187,7 @@ bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hip
   p.tile_rows = kTileVectors / p.kv_mul;
   p.blocks = fast_blocks(job);
   p.scale2 = 1.4426950408889634f / sqrtf((float)job.head_dim);
-  p.rows = (RowSlots *)((char *)workspace + 256);
+  p.rows = (RowSlots *)workspace;
   p.partial = (float *)(p.rows + job.batch.rows);
   p.flags = device().error_flags;
   const long long blocks = (long long)p.blocks * p.n_kv_heads + (job.batch.rows + kThreads - 1) / kThreads;

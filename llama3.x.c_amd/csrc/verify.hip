@@ -396,7 +396,6 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick(Verify p) {
       break;
     refused = false;
   }
-  // the chunk's tokens, 16 consecutive ones a thread
   // the chunk's tokens, consecutive ones a thread
   const int i0 = max(chunk, 0) * kChunk + tid * kTokens, end = min(p.job.vocab, i0 + kTokens);
   double w[kTokens], sum = 0.0;
@@ -448,7 +447,7 @@ bool verify_shape_ok(int rows, int vocab) { return vocab <= kChunk * kMaxChunks 
 
 size_t verify_workspace(const VerifyJob &job) {
   const size_t chunks = ((size_t)job.vocab + kChunk - 1) / kChunk;
-  return 256 + (size_t)job.count * sizeof(Decision) + (size_t)job.rows * chunks * sizeof(Stat) * (job.draft ? 2 : 1) +
+  return (size_t)job.count * sizeof(Decision) + (size_t)job.rows * chunks * sizeof(Stat) * (job.draft ? 2 : 1) +
          (size_t)job.count * chunks * sizeof(double);
 }
 
@@ -456,7 +455,7 @@ bool launch_verify(const VerifyJob &job, void *workspace, hipStream_t stream) {
   Verify p{};
   p.job = job;
   p.chunks = (job.vocab + kChunk - 1) / kChunk;
-  p.decisions = (Decision *)((char *)workspace + 256);
+  p.decisions = (Decision *)workspace;
   p.target = (Stat *)(p.decisions + job.count);
   p.draft = p.target + (size_t)job.rows * p.chunks;
   p.rest = (double *)(job.draft ? p.draft + (size_t)job.rows * p.chunks : p.draft);

@@ -242,6 +242,28 @@ def test_attention_spread_values(L, rows_of):
     within(hu.host(out), want, bound)
 
 
+@pytest.mark.parametrize("rows_of", [[1, 3], [40, 20]])
+@pytest.mark.parametrize("sizes", [(1e35,), (1e-20,), (1e24, 1.0, 0.0), (1e10, 1e-15, 0.0), (0.0,)])
+def test_attention_value_sizes(L, rows_of, sizes):
+    """V rows of extreme sizes, position by position, and of zeros; keys and queries whose scores stay ordinary. (The sums
+    are divided by the weights' at the end, so the values of n positions with weights near the largest must stay below
+    3.4e38 / n, here 3.4e38 / 290 = 1.2e36; 1e38 overflows, in k_attention too.)"""
+    L.kernels_kv_layout_select(b"head")
+    heads, kv, hd = 8, 2, 128
+    b = ru.Batch(hu.dev, rows_of, [90 - rows_of[0], 0], prefix=200, prefix_seq_len=200, seq_len=100)
+    rng = np.random.default_rng(12)
+    size = lambda n: np.asarray(sizes, F)[np.arange(n) // 8 % len(sizes)][:, None]  # noqa: E731
+    q = (1e-30 * rng.standard_normal((b.rows, heads * hd))).astype(F)
+    pk, k = ((1e30 * rng.standard_normal(s)).astype(F) for s in ((kv, 200, hd), (2, kv, 100, hd)))
+    pv, v = (size(s[-2]) * rng.uniform(0.5, 1.5, s).astype(F) for s in ((kv, 200, hd), (2, kv, 100, hd)))
+    out = hu.dev(np.zeros_like(q))
+    args = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in args], b.struct, heads, kv, hd)
+    quiet(L)
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
+    within(hu.host(out), want, bound)
+
+
 @pytest.mark.parametrize("rows", [3, 20, 45])
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 def test_attention_nonfinite_values_reach_only_the_rows_that_see_them(L, rows, value):
@@ -755,6 +777,245 @@ def test_captured_calls_follow_their_arrays(L):
         for g, w in zip(results(), want):
             assert np.array_equal(g, w)
     L.llhip_graph_destroy(graph)
+
+
+def test_two_graphs_share_the_workspace(L):
+    """Two graphs of the same operators over other operands, replayed in turn with a larger eager call between, which takes
+    another workspace; a call that would need a larger one while it is captured is refused."""
+    T = hu.torch()
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(5)
+    heads, kv, hd = 8, 2, 128
+
+    def make(rows_of, length, prefix):
+        b = ru.Batch(hu.dev, rows_of, length, prefix=prefix, prefix_seq_len=prefix, seq_len=200)
+        a = [rng.standard_normal(n, dtype=F) for n in ((b.rows, heads * hd), (kv, prefix, hd), (kv, prefix, hd),
+                                                       (b.slots, kv, 200, hd), (b.slots, kv, 200, hd))]
+        want, bound = ru.attention(b, *a, heads, kv, hd, "head")
+        return b, [hu.dev(x) for x in a], hu.dev(np.zeros_like(a[0])), want, bound
+
+    def call(m):
+        L.llhip_attention_requests(lh.ptr(m[2]), *[lh.ptr(x) for x in m[1]], m[0].struct, heads, kv, hd)
+
+    one, two = make([1] * 9, rng.integers(0, 199, 9), 700), make([30, 1, 5], [100, 5, 190], 90)
+    graphs = []
+    for m in (one, two):
+        call(m)
+        quiet(L)
+        assert L.llhip_graph_begin() == 0
+        call(m)
+        graphs.append(L.llhip_graph_end())
+        assert graphs[-1], lh.last_error()
+    m, k, n, rank = 60000, 64, 16, 256
+    x = hu.dev(rng.standard_normal((m, k), dtype=F))
+    big = Adapters(rng, 1, k, n, rank, 1, True, False)
+    c = hu.dev(np.zeros((m, n), F))
+    seg = ru.array([ru.lora_segment(True, c, n, c, big.keep[0][0][0], big.keep[0][0][1], None, n, rank)] * 1)
+    ids = hu.dev(np.zeros(m, np.int32))
+    assert L.llhip_graph_begin() == 0
+    L.llhip_lora_bf16(lh.ptr(x), k, m, k, lh.ptr(ids), 1, seg, 1)
+    message = lh.last_error()
+    refused = "during graph capture" in message
+    L.llhip_clear_error()
+    empty = L.llhip_graph_end()
+    if empty:
+        L.llhip_graph_destroy(empty)
+    L.llhip_clear_error()
+    assert refused, message
+    for turn in range(3):
+        if turn == 1:
+            L.llhip_lora_bf16(lh.ptr(x), k, m, k, lh.ptr(ids), 1, seg, 1)
+        for a in (one, two):
+            a[2].zero_()
+        T.cuda.synchronize()
+        for g in graphs + graphs[::-1]:
+            assert L.llhip_graph_launch(g) == 0
+        quiet(L)
+        for a in (one, two):
+            within(hu.host(a[2]), a[3], a[4], turn)
+    for g in graphs:
+        L.llhip_graph_destroy(g)
+
+
+def test_calls_from_two_threads(L):
+    """Attention and verification from two threads at once, whose kernels share one workspace."""
+    import threading
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(6)
+    heads, kv, hd = 8, 2, 64
+    b = ru.Batch(hu.dev, [1] * 20, rng.integers(0, 100, 20), prefix=300, prefix_seq_len=300, seq_len=128)
+    a = [rng.standard_normal(n, dtype=F) for n in ((b.rows, heads * hd), (kv, 300, hd), (kv, 300, hd),
+                                                   (b.slots, kv, 128, hd), (b.slots, kv, 128, hd))]
+    want, bound = ru.attention(b, *a, heads, kv, hd, "head")
+    dev, out = [hu.dev(x) for x in a], hu.dev(np.zeros_like(a[0]))
+    start, logits, draft, tokens, uniform = verify_inputs(rng, [3] * 20, 4000, 0.7, True)
+    vdev = [hu.dev(x) for x in (logits, draft, tokens, uniform, start)]
+    acc, nxt = hu.dev(np.zeros(20, np.int32)), hu.dev(np.zeros(20, np.int32))
+
+    def attend():
+        for _ in range(200):
+            L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(x) for x in dev], b.struct, heads, kv, hd)
+
+    def judge():
+        for _ in range(200):
+            L.llhip_verify_drafts(lh.ptr(acc), lh.ptr(nxt), lh.ptr(vdev[0]), 4000, lh.ptr(vdev[1]), 4000, lh.ptr(vdev[2]),
+                                  lh.ptr(vdev[3]), lh.ptr(vdev[4]), 20, 60, 4000, 0.7)
+
+    attend(), judge()
+    quiet(L)
+    team = [threading.Thread(target=f) for f in (attend, judge)]
+    for t in team:
+        t.start()
+    for t in team:
+        t.join()
+    quiet(L)
+    within(hu.host(out), want, bound)
+    assert list(zip(hu.host(acc).tolist(), hu.host(nxt).tolist())) == ru.verify(start, logits, draft, tokens, uniform, 0.7)
+
+
+# ---- the largest numbers ----------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("count", [64, 65, 128, 129, 300, 1024])
+def test_attention_many_requests(L, count):
+    """As many requests as a call takes, some without rows, behind a prefix and without one; vectors of one row, drafts."""
+    rng = np.random.default_rng(count)
+    rows_of = rng.choice([0, 1, 1, 1, 4, 9], count)
+    for prefix in (0, 70):
+        b = ru.Batch(hu.dev, rows_of, rng.integers(0, 40, count), slot=rng.permutation(count), prefix=prefix, seq_len=49,
+                     first=1, spare=2)
+        attention_case(L, count, 4, 2, 64, "head", b)
+
+
+def test_attention_without_rows(L):
+    b = ru.Batch(hu.dev, [0, 0, 0], [0, 5, 9], prefix=9, seq_len=16, first=2, spare=5)
+    attention_case(L, 1, 4, 2, 64, "head", b)
+
+
+@pytest.mark.parametrize("count", [257, 1024])
+def test_rope_many_requests(L, count):
+    L.kernels_kv_layout_select(b"rows")
+    rng = np.random.default_rng(count)
+    heads, kv, hd = 3, 1, 8
+    rows_of = rng.choice([0, 1, 1, 3], count)
+    b = ru.Batch(hu.dev, rows_of, rng.integers(0, 20, count), slot=rng.permutation(count), prefix=3, seq_len=24)
+    q, k, v = (rng.standard_normal((b.rows, n * hd), dtype=F) for n in (heads, kv, kv))
+    angle = rng.standard_normal((27, hd // 2))
+    cos, sin = np.cos(angle).astype(F), np.sin(angle).astype(F)
+    table = np.concatenate((np.repeat(cos, 2, 1), np.stack((-sin, sin), 2).reshape(27, -1)), 1)
+    out, kc, vc = hu.dev(np.zeros_like(q)), hu.dev(np.zeros((count, 24, hd), F)), hu.dev(np.zeros((count, 24, hd), F))
+    keep = [hu.dev(x) for x in (q, k, v, table)]
+    L.llhip_rope_kv_store_requests(lh.ptr(out), lh.ptr(keep[0]), heads * hd, lh.ptr(keep[1]), lh.ptr(keep[2]), hd,
+                                   lh.ptr(keep[3]), b.struct, heads, kv, hd, lh.ptr(kc), lh.ptr(vc))
+    quiet(L)
+    at = np.zeros(b.rows, int)
+    want_k, want_v = np.zeros((count, 24, hd), F), np.zeros((count, 24, hd), F)
+
+    def turn(x, at):
+        x = x.reshape(len(x), -1, hd // 2, 2)
+        c, s = cos[at][:, None], sin[at][:, None]
+        return np.stack((x[..., 0] * c - x[..., 1] * s, x[..., 0] * s + x[..., 1] * c), -1).reshape(len(x), -1)
+
+    for _, rows, length, _ in b.requests():
+        at[rows] = 3 + length + np.arange(rows.stop - rows.start)
+    turned = turn(k, at)
+    for _, rows, length, slot in b.requests():
+        n = rows.stop - rows.start
+        want_k[slot, length:length + n], want_v[slot, length:length + n] = turned[rows], v[rows]
+    assert np.array_equal(hu.host(out), turn(q, at))
+    assert np.array_equal(hu.host(kc), want_k) and np.array_equal(hu.host(vc), want_v)
+
+
+def test_verify_1024_requests(L):
+    rng = np.random.default_rng(4)
+    inputs = verify_inputs(rng, rng.integers(0, 4, 1024), 50, 0.9, True)
+    got = run_verify(L, *inputs, 50, 0.9)
+    assert not lh.last_error(), lh.last_error()
+    assert got == [(-9, -9) if w is None else w for w in ru.verify(*inputs, 0.9)]
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_lora_many_adapters(L, m):
+    """More adapters than the tiles' search takes, and as many."""
+    for adapters in (4096, 4097):
+        rng = np.random.default_rng(m)
+        k, n, rank = 16, 24, 4
+        x = rng.standard_normal((m, k), dtype=F)
+        ids = rng.integers(-1, adapters, m)
+        ids[-1] = adapters - 1
+        s = Adapters(rng, m, k, n, rank, adapters, False, False)
+        keep = run_lora(L, x, k, k, ids, adapters, [s], False)
+        quiet(L)
+        s.check(x, ids)
+        del keep
+
+
+def test_caches_past_32_bits(L):
+    """Slots that begin past 2^32 values and bytes, stored into and read."""
+    T = hu.torch()
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(7)
+    heads, kv, hd, seq_len, slots = 4, 1, 64, 1 << 20, 66
+    key, value = (T.empty(slots, kv, seq_len, hd, device="cuda") for _ in range(2))
+    lengths, slot, rows_of = [300, seq_len - 3, 7], [65, 64, 0], [2, 3, 1]
+    b = ru.Batch(hu.dev, rows_of, lengths, slot=slot, slots=slots, prefix=0, seq_len=seq_len)
+    q, k, v = (rng.standard_normal((b.rows, n * hd), dtype=F) for n in (heads, kv, kv))
+    table = T.zeros(seq_len, 2 * hd, device="cuda")
+    table[:, :hd] = 1.0  # no turn
+    old = {s: rng.standard_normal((2, 300, hd), dtype=F) for s in (65, 0)}
+    for s, x in old.items():
+        key[s, 0, :300].copy_(T.from_numpy(x[0]))
+        value[s, 0, :300].copy_(T.from_numpy(x[1]))
+    key[64].zero_()
+    value[64].zero_()
+    # the last own rows of slot 64 take all of the weight
+    q[2:5] = 1.0
+    k[2:5] = 60.0 / 8.0
+    T.cuda.synchronize()
+    rot, out = hu.dev(np.zeros_like(q)), hu.dev(np.zeros_like(q))
+    keep = [hu.dev(x) for x in (q, k, v)]
+    L.llhip_rope_kv_store_requests(lh.ptr(rot), lh.ptr(keep[0]), heads * hd, lh.ptr(keep[1]), lh.ptr(keep[2]),
+                                   kv * hd, lh.ptr(table), b.struct, heads, kv, hd, lh.ptr(key), lh.ptr(value))
+    L.llhip_attention_requests(lh.ptr(out), lh.ptr(rot), None, None, lh.ptr(key), lh.ptr(value), b.struct, heads, kv, hd)
+    quiet(L)
+    got = hu.host(out)
+    small = ru.Batch(hu.dev, [2, 1], [300, 7], seq_len=302)
+    cache = np.zeros((2, 2, 1, 302, hd), F)
+    for i, (s, rows) in enumerate(((65, slice(0, 2)), (0, slice(5, 6)))):
+        cache[:, i, 0, :300] = old[s]
+        at = lengths[slot.index(s)]
+        cache[0, i, 0, at:at + rows.stop - rows.start], cache[1, i, 0, at:at + rows.stop - rows.start] = k[rows], v[rows]
+    none = np.zeros((1, 0, hd), F)
+    want, bound = ru.attention(small, q[[0, 1, 5]], none, none, cache[0], cache[1], heads, kv, hd, "head")
+    within(got[[0, 1, 5]], want, bound)
+    # equal scores of 60 over the positions stored: 2^20 others weigh exp(-60) each, below 1e-19 together; three sums' and a
+    # division's roundings, and the weights' of scores near 60 (72 U of the score), stay below 5000 U
+    for j in range(3):
+        mean = v[2:3 + j].astype(np.float64).mean(0)
+        assert np.abs(got[2 + j].reshape(heads, hd) - mean).max() < 5000 * ru.U * np.abs(v[2:5]).max()
+    assert T.equal(key[65, 0, 300:302].cpu(), T.from_numpy(k[:2]))
+    assert T.equal(value[64, 0, seq_len - 3:].cpu(), T.from_numpy(v[2:5]))
+
+
+def test_attention_walk_past_2_gib(L):
+    """Positions whose rows lie more than 2^31 bytes into a slot: the form for any shape."""
+    T = hu.torch()
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(8)
+    hd, seq_len = 256, (1 << 21) + 64
+    key, value = (T.zeros(1, 1, seq_len, hd, device="cuda") for _ in range(2))
+    b = ru.Batch(hu.dev, [2], [seq_len - 2], seq_len=seq_len)
+    q = np.ones((2, hd), F)
+    v = rng.standard_normal((2, hd), dtype=F)
+    key[0, 0, -2:] = 60.0 / 16.0
+    value[0, 0, -2:].copy_(T.from_numpy(v))
+    T.cuda.synchronize()
+    out, qd = hu.dev(np.zeros((2, hd), F)), hu.dev(q)
+    L.llhip_attention_requests(lh.ptr(out), lh.ptr(qd), None, None, lh.ptr(key), lh.ptr(value), b.struct, 1, 1, hd)
+    quiet(L)
+    got = hu.host(out)
+    for j in range(2):  # as above
+        assert np.abs(got[j] - v[:1 + j].astype(np.float64).mean(0)).max() < 5000 * ru.U * np.abs(v).max()
 
 
 # ---- the engine's step over drafts ------------------------------------------------------------------------------------

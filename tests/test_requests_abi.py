@@ -206,6 +206,14 @@ def test_verify_refusals(L):
     same = np.zeros(3, np.int32)
     verify_call(L, accepted=same, next=same[1:])
     refused(L, "must not overlap")
+    for name in ("accepted", "next"):
+        tokens, start, uniform = np.zeros(4, np.int32), np.array([0, 2, 4], np.int32), np.zeros((4, 2), np.float32)
+        logits, draft = np.zeros((4, 10), np.float32), np.zeros((4, 10), np.float32)
+        for over in ({"tokens": tokens, name: tokens[2:]}, {"start": start, name: start[1:]},
+                     {"uniform": uniform, name: uniform.view(np.int32)[1:]}, {"logits": logits, name: logits[3, 8:]},
+                     {"draft": draft, name: draft[3, 8:]}):
+            verify_call(L, **over)
+            refused(L, "must not overlap an input")
     verify_call(L, count=0, logits=None)
     assert not lh.last_error()
 
