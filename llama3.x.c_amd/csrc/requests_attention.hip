@@ -1076,13 +1076,12 @@ template <int HD, bool FULL> __global__ __launch_bounds__(kThreads, kBlocksPerCu
 // A thread per (row, head, four dimensions): the row's partial sums over the prefix and over its own positions, rescaled to
 // their largest maximum and added in order.
 __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
-  const int hd4 = p.hd / 4;
-  const long long idx = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (idx >= (long long)p.batch.rows * p.n_heads * hd4)
+  const unsigned hd4 = (unsigned)p.hd / 4;
+  const unsigned idx = blockIdx.x * kThreads + threadIdx.x, vec = idx / hd4; // at most 2^31: 32-bit divisions
+  const int d4 = (int)(idx % hd4), row = (int)(vec / (unsigned)p.n_heads), head = (int)(vec % (unsigned)p.n_heads);
+  if (row >= p.batch.rows)
     return;
-  const int d4 = (int)(idx % hd4);
-  const long long vec = idx / hd4;
-  const int row = (int)(vec / p.n_heads), head = (int)(vec % p.n_heads), g = head / p.kv_mul, h = head % p.kv_mul;
+  const int g = head / p.kv_mul, h = head % p.kv_mul;
   const RowSlots mine = p.rows[row];
   if (mine.own_first < 0)
     return;
