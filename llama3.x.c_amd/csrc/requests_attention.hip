@@ -9,8 +9,9 @@
 //
 // Measured at 32 heads over 8 KV heads of dimension 128, both launches: 32 requests of one row behind 2048 positions, 502 own
 // ones on average, 49 us (148 MB of K and V: 3.0 TB/s); 64 behind 8192 with 594 100 us (378 MB: 3.8 TB/s); 16 with two to
-// seven rows behind 4096 with 916 69 us; five prompts, 923 rows, behind 1024 94 us. Wide walks are bound by their
-// dependencies (vector unit 50% busy, matrix cores 30%, LDS less), narrow ones by HBM.
+// seven rows behind 4096 with 916 66 us; five prompts, 923 rows, behind 1024 94 us. Wide walks are bound by their
+// instructions: a step takes the two waves of a SIMD 5600 cycles, 4300 of vector and 3100 of matrix instructions, which overlap
+// little (over the whole kernel the vector unit is 50% busy, the matrix cores 30%, LDS less); narrow ones by HBM.
 #include <cfloat>
 
 #include "requests_device.h"
