@@ -776,7 +776,7 @@ float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int p
     // budget (tests/q8.c:158-183), and the classifier streams once per batch instead of once per row.
     if (e->q8) {
       norm_rows(e->rms_final);
-      if (stay) { // bit for bit the pieces' logits
+      if (stay) { // the pieces' logits, up to the rounding of the tiles that a larger batch may take
         const GemmQ8Segment seg{e->blogits, c.vocab_size, e->cls.k8(), K8Weight{}, nullptr, nullptr, c.vocab_size,
                                 GEMM_STORE};
         k_gemm_q8(e->bxq, e->bxs, count, d, gs, &seg, 1);
