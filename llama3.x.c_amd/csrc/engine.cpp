@@ -87,6 +87,7 @@ struct Engine {
   int batch_rows = 0;
   float *bx = nullptr, *bxb = nullptr, *bq = nullptr, *bk = nullptr, *bv = nullptr, *bhb = nullptr, *bxs = nullptr;
   float *bhs = nullptr, *blogits = nullptr;
+  int logits_rows = 0;                   // that blogits holds
   int8_t *bxq = nullptr, *bhq = nullptr; // quantized rows of dim (xb) and of hidden_dim (hb) values
   int *btokens = nullptr;
   // a batch's logits on the host: pinned, so the copy of every row's logits (1 GB for 2048 rows of 128256) runs at
@@ -133,7 +134,7 @@ void free_batch(Engine *e) {
   drop(e->bxq), drop(e->bhq), drop(e->bhs), drop(e->btokens), drop(e->blogits);
   if (e->panel.base)
     aligned_buffer_free(&e->panel);
-  e->batch_rows = 0;
+  e->batch_rows = e->logits_rows = 0;
 }
 
 void release(Engine *e) {
@@ -580,6 +581,19 @@ bool allocate_batch(Engine *e, int rows) {
   return true;
 }
 
+// Room for `rows` rows of logits in blogits: grown where the model was configured for larger batches since (llhip_free
+// waits for the stream).
+bool batch_logits_room(Engine *e, int rows) {
+  if (rows <= e->logits_rows)
+    return true;
+  drop(e->blogits);
+  e->logits_rows = 0;
+  if (!device_array(&e->blogits, (size_t)rows * e->c.vocab_size))
+    return false;
+  e->logits_rows = rows;
+  return true;
+}
+
 // One product on FP32 activations (src/tp.c:475-490): the FP32 GEMM, or in BF16 mode the same segments on the packed
 // copies of layer l's matrices `index` (and `index3` for the SwiGLU pair).
 void gemm_f32_or_bf16(Engine *e, const float *a, int lda, int m, int k, const GemmSegment *seg, int count, int l,
@@ -757,7 +771,7 @@ float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int p
     return nullptr;
   }
   const size_t vocab = c.vocab_size;
-  if (want == LOGITS_ALL && !e->blogits && !device_array(&e->blogits, (size_t)e->batch_rows * vocab))
+  if (want == LOGITS_ALL && !batch_logits_room(e, e->batch_rows))
     return nullptr;
   if (want == LOGITS_ALL && e->bf16) { // src/tp.c:601-609: a BF16 GEMM on the packed classifier
     if (!e->cls_packed) {
@@ -847,7 +861,7 @@ float *forward_batch_on_device(Model *model, Engine *e, const int *tokens, int c
   if (model->prefill_gemm && (count > 1 || e->bf16))
     return forward_rows(model, e, tokens, count, pos0, LOGITS_ALL, true);
   const size_t vocab = e->c.vocab_size;
-  if (count > 1 && !e->blogits && !device_array(&e->blogits, (size_t)model->max_batch * vocab))
+  if (count > 1 && !batch_logits_room(e, model->max_batch))
     return nullptr;
   float *logits = count > 1 ? e->blogits : e->logits;
   for (int i = 0; i < count; i++)

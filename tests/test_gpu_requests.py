@@ -1108,6 +1108,58 @@ def test_engine_verify(L, tmp_path, monkeypatch, kind):
         L.engine_free(at)
 
 
+def reconfigured(L, tmp_path, monkeypatch, kind, gemm):
+    """A q8 or f32 model loaded for batches of 4, with its GEMM `gemm`, verified once, then configured for batches of 24 with
+    the GEMM on: (the model, the tokens of 24 rows, uniforms for them, and the logits of a model loaded for 24)."""
+    L.kernels_kv_layout_select(b"head")
+    path = os.path.join(tmp_path, "tiny.bin")
+    engine_model(path, kind)
+    vocab, rng = ENGINE["vocab_size"], np.random.default_rng(31)
+    tokens, uniform = rng.integers(0, vocab, 24).astype(np.int32), rng.random((24, 2)).astype(F)
+    monkeypatch.setenv("LLAMA_PREFILL_BATCH", "24")
+    fresh, model, following = lh.Model(), lh.Model(), ctypes.c_int(-7)
+    L.engine_load(ctypes.byref(fresh), path.encode())
+    p = L.engine_forward_batch(ctypes.byref(fresh), lh.ptr(tokens), 24, 0, lh.LOGITS_ALL)
+    assert p, lh.last_error()
+    logits = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (24, vocab)).copy()
+    L.engine_free(ctypes.byref(fresh))
+    monkeypatch.setenv("LLAMA_PREFILL_BATCH", "4")
+    monkeypatch.setenv("LLAMA_PREFILL_GEMM", gemm)
+    L.engine_load(ctypes.byref(model), path.encode())
+    at = ctypes.byref(model)
+    assert L.llhip_engine_verify(at, lh.ptr(tokens), 4, 0, None, 0, None, 0.0, ctypes.byref(following)) >= 0, lh.last_error()
+    monkeypatch.setenv("LLAMA_PREFILL_BATCH", "24")
+    monkeypatch.setenv("LLAMA_PREFILL_GEMM", "on")
+    L.prefill_configure_engine(at, 24, kind == "q8")
+    assert not lh.last_error() and L.engine_max_batch(at) == 24
+    return model, tokens, uniform, logits
+
+
+@pytest.mark.parametrize("kind", ["q8", "f32"])
+def test_engine_verify_holds_the_logits_of_a_larger_batch(L, tmp_path, monkeypatch, kind):
+    """Rows one at a time with room for 4 rows' logits, then the GEMM with 24: the logits' buffer grows by both paths."""
+    model, tokens, uniform, logits = reconfigured(L, tmp_path, monkeypatch, kind, "off")
+    at, vocab, following = ctypes.byref(model), ENGINE["vocab_size"], ctypes.c_int(-7)
+    try:
+        claimed = L.llhip_hbm_claimed()
+        got = L.llhip_engine_verify(at, lh.ptr(tokens), 24, 0, None, 0, lh.ptr(uniform), 0.8, ctypes.byref(following))
+        assert not lh.last_error(), lh.last_error()
+        assert (got, following.value) == ru.verify([0, 24], logits, None, tokens, uniform, 0.8)[0]
+        # the 24 rows of the GEMMs and 20 rows of logits more
+        assert L.llhip_hbm_claimed() - claimed >= 4 * (20 * vocab + 24 * 3 * ENGINE["dim"])
+        p = L.engine_forward_batch(at, lh.ptr(tokens), 24, 0, lh.LOGITS_ALL)
+        assert (np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (24, vocab)) == logits).all()
+        monkeypatch.setenv("LLAMA_PREFILL_BATCH", "40")  # and by rows one at a time
+        monkeypatch.setenv("LLAMA_PREFILL_GEMM", "off")
+        L.prefill_configure_engine(at, 40, kind == "q8")
+        forty = np.resize(tokens, 40)
+        claimed = L.llhip_hbm_claimed()
+        assert L.llhip_engine_verify(at, lh.ptr(forty), 40, 0, None, 0, None, 0.0, ctypes.byref(following)) >= 0
+        assert not lh.last_error() and L.llhip_hbm_claimed() - claimed == 4 * 16 * vocab
+    finally:
+        L.engine_free(at)
+
+
 # ---- a small model served by all of them ------------------------------------------------------------------------------
 
 
