@@ -83,7 +83,7 @@ struct Engine {
   int *token_host = nullptr;
   float *host_logits = nullptr;
   AttentionWork work{};
-  // the batched forward's rows (max_batch of each, allocated on its first call)
+  // the batched forward's rows (max_batch of each, allocated on its first call, and again for a larger batch)
   int batch_rows = 0;
   float *bx = nullptr, *bxb = nullptr, *bq = nullptr, *bk = nullptr, *bv = nullptr, *bhb = nullptr, *bxs = nullptr;
   float *bhs = nullptr, *blogits = nullptr;
@@ -555,8 +555,10 @@ bool forward(Engine *e, int token, int pos, bool want_logits, float *stay = null
   return llhip_last_error()[0] == 0;
 }
 
-// The batched forward's rows, max_batch of each, on its first call; all or nothing.
+// The batched forward's rows, max_batch of each, on its first call and where the model was configured for larger batches
+// since; all or nothing.
 bool allocate_batch(Engine *e, int rows) {
+  free_batch(e);
   const Config &c = e->c;
   const size_t m = rows, d = c.dim, kv = (size_t)c.head_dim * c.n_kv_heads, h = c.hidden_dim;
   const size_t groups = e->q8 ? (size_t)e->gs : 1;
@@ -682,7 +684,7 @@ float *forward_rows(Model *model, Engine *e, const int *tokens, int count, int p
   const Config &c = e->c;
   const int d = c.dim, hidden = c.hidden_dim, hd = c.head_dim, gs = e->gs, nh = c.n_heads, nkv = c.n_kv_heads;
   const int kvl = hd * nkv;
-  if (!e->batch_rows && !allocate_batch(e, model->max_batch))
+  if (e->batch_rows < count && !allocate_batch(e, model->max_batch))
     return nullptr;
   const float *brope = e->rope_all + (size_t)pos0 * 2 * hd; // rows pos0 .. pos0 + count - 1
   llhip_memcpy_h2d(e->btokens, tokens, (size_t)count * sizeof(int));

@@ -1160,6 +1160,31 @@ def test_engine_verify_holds_the_logits_of_a_larger_batch(L, tmp_path, monkeypat
         L.engine_free(at)
 
 
+@pytest.mark.parametrize("kind", ["q8", "f32", "bf16"])
+def test_engine_verify_holds_the_rows_of_a_larger_batch(L, tmp_path, monkeypatch, kind):
+    """The GEMM's rows allocated for batches of 4 grow for a batch of 24, and stay for one of 3."""
+    if kind == "bf16":
+        monkeypatch.setenv("LLAMA_PRECISION", "bf16")
+    model, tokens, uniform, logits = reconfigured(L, tmp_path, monkeypatch, kind, "on")
+    at, vocab, following = ctypes.byref(model), ENGINE["vocab_size"], ctypes.c_int(-7)
+    try:
+        claimed = L.llhip_hbm_claimed()
+        got = L.llhip_engine_verify(at, lh.ptr(tokens), 24, 0, None, 0, lh.ptr(uniform), 0.8, ctypes.byref(following))
+        assert not lh.last_error(), lh.last_error()
+        assert (got, following.value) == ru.verify([0, 24], logits, None, tokens, uniform, 0.8)[0]
+        claimed = L.llhip_hbm_claimed() - claimed
+        assert claimed >= 4 * 20 * (vocab + 3 * ENGINE["dim"] + ENGINE["hidden_dim"])
+        p = L.engine_forward_batch(at, lh.ptr(tokens), 24, 0, lh.LOGITS_ALL)
+        assert (np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (24, vocab)) == logits).all()
+        monkeypatch.setenv("LLAMA_PREFILL_BATCH", "3")
+        L.prefill_configure_engine(at, 3, kind == "q8")
+        claimed = L.llhip_hbm_claimed()
+        assert L.llhip_engine_verify(at, lh.ptr(tokens), 3, 0, None, 0, None, 0.0, ctypes.byref(following)) >= 0
+        assert not lh.last_error() and L.llhip_hbm_claimed() == claimed
+    finally:
+        L.engine_free(at)
+
+
 # ---- a small model served by all of them ------------------------------------------------------------------------------
 
 
