@@ -35,7 +35,8 @@ float *engine_forward_batch(Model *model, const int *tokens, int count, int pos0
 /* A decode step over drafted tokens: tokens[0] is the token at pos0 (the prefix [0, pos0) run before), tokens[1 ..
  * count - 1] were drafted for the positions behind it, 1 <= count <= engine_max_batch. The rows run as
  * engine_forward_batch's with every row's logits, which stay on the device, and llhip_verify_drafts (llama_hip_requests.h:
- * draft_logits, draft_ld, uniform and temperature are its arguments, in host or device memory) judges the drafts.
+ * draft_logits, draft_ld, uniform and temperature are its arguments, in host or device memory: count - 1 rows of
+ * draft_logits, row i the one that tokens[i + 1] was drawn from, and count pairs of uniforms) judges the drafts.
  * Returns how many were accepted, n of 0 .. count - 1, and in *next the token behind them; the next call takes *next at
  * pos0 + n + 1, which overwrites the refused drafts' cache rows. -1 when the call failed in record mode; *next is then
  * unchanged. */

@@ -104,17 +104,18 @@ void llhip_lora_bf16(const float *x, int ldx, int m, int k, const int *adapter, 
 /* Drafted tokens checked against the model (speculative sampling). Request r's rows start[r] .. start[r + 1] - 1 are as
  * in RequestBatch: the first row's token is known, row i's token tokens[i] of the others was drafted, and row i's
  * logits (vocab floats at logits + i * ld) judge row i + 1's token. With p = softmax(logits / temperature) of row i and q
- * the same of draft_logits' row i (the distribution the draft was drawn from; draft_logits NULL: the draft was not
- * drawn, q is 1 at it), the drafts are accepted in turn while uniform[2 i] * q(x) < p(x). At the first refusal the next
- * token is drawn from max(0, p - q) (from p should that be empty); with every draft accepted, from the last row's p:
+ * the same of draft_logits' row i (the distribution that row i + 1's draft was drawn from; draft_logits NULL: the draft
+ * was not drawn, q is 1 at it), the drafts are accepted in turn while uniform[2 i] * q(x) < p(x). At the first refusal the
+ * next token is drawn from max(0, p - q) (from p should that be empty); with every draft accepted, from the last row's p:
  * the first token, in ascending order, at which the running sum passes uniform[2 i + 1] times the whole sum. The tokens
  * so emitted are distributed as the model's own. temperature 0 is greedy: a draft is accepted where it is the row's
  * largest logit (the lowest such token), which is also the next token; uniform and draft_logits are then not read.
  * accepted[r] receives the number of accepted drafts and next[r] the token after them; a request without rows keeps
  * both. Logits of -infinity are tokens masked out. A row that decides with a NaN, +infinity or no token left, and a
  * draft outside the vocabulary, set both to -1 and fail at the next host-visible point. Probabilities, sums and the
- * borders between tokens are FP64; uniform lies in [0, 1). accepted and next must not overlap each other or an input. At
- * most LLHIP_MAX_REQUESTS requests, 2^20 rows and 2^22 tokens. */
+ * borders between tokens are FP64; uniform lies in [0, 1). draft_logits holds rows - 1 rows: a request's last row has no
+ * draft behind it, and the buffer's last row is not read. accepted and next must not overlap each other or an input,
+ * draft_logits taken as `rows` rows. At most LLHIP_MAX_REQUESTS requests, 2^20 rows and 2^22 tokens. */
 void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t ld, const float *draft_logits,
                          size_t draft_ld, const int *tokens, const float *uniform, const int *start, int count, int rows,
                          int vocab, float temperature);

@@ -377,11 +377,14 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
       raise("%s: accepted and next must not overlap an input", name);
       return;
     }
+  if (rows == 1)
+    draft_logits = nullptr; // nothing is drafted
   Call call(name);
   const size_t row = (size_t)vocab * kFloat;
   Ref A = call.out(accepted, out_bytes, true), N = call.out(next, out_bytes, true); // requests without rows keep both
   Ref L = call.in2d(logits, row, ld * kFloat, (size_t)rows);
-  Ref D = draft_logits ? call.in2d(draft_logits, row, draft_ld * kFloat, (size_t)rows) : Ref{};
+  // the buffer's last row judges nothing: its draft_logits row need not be there
+  Ref D = draft_logits ? call.in2d(draft_logits, row, draft_ld * kFloat, (size_t)rows - 1) : Ref{};
   Ref T = call.in(tokens, (size_t)rows * sizeof(int)), S = call.in(start, ((size_t)count + 1) * sizeof(int));
   Ref U = greedy ? Ref{} : call.in(uniform, (size_t)rows * 2 * kFloat);
   if (!call.ready())

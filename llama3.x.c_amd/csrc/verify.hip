@@ -130,8 +130,8 @@ template <bool GREEDY> __global__ __launch_bounds__(kThreads) void verify_stats(
   __shared__ double powers[kPowers];
   const int row = row0 + blockIdx.y, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const bool drafted = blockIdx.z;
-  if (row < p.job.start[0] || row >= p.job.start[p.job.count])
-    return;
+  if (row < p.job.start[0] || row >= p.job.start[p.job.count] || (drafted && row == p.job.rows - 1))
+    return; // the last row of all judges nothing, and the draft's may not be there
   const float *src = drafted ? p.job.draft + (size_t)row * p.job.draft_ld : p.job.logits + (size_t)row * p.job.ld;
   auto place = [&](int j) { return p.vec4 ? 4 * (lane + j / 4 * kWave) + j % 4 : lane + j * kWave; }; // of x[j]
   const int chunk = blockIdx.x * kWaves + wave, i0 = chunk * kChunk, n = min(kChunk, p.job.vocab - i0);

@@ -1,6 +1,7 @@
 """Many requests on one model, on the GPU: each operator against its plain float64 form (tests/requests_util.py, the bounds
 derived there), its index checks, host buffers and captured calls; and a small model served by all of them together."""
 import ctypes
+import mmap
 import os
 
 import numpy as np
@@ -697,6 +698,44 @@ def test_verify_refuses_rows_that_decide_nothing(L, temperature):
     assert got[1] == (-9, -9) and got[0] == ru.verify(start[:2], logits, draft, tokens, uniform, temperature)[0]
 
 
+def at_a_mappings_end(a):
+    """A host copy of `a` whose last byte is its mapping's: the page behind cannot be read."""
+    page = mmap.PAGESIZE
+    room = (a.nbytes + page - 1) // page * page
+    m = mmap.mmap(-1, room + page)
+    libc = ctypes.CDLL(None, use_errno=True)
+    libc.mprotect.argtypes = [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int]
+    view = np.frombuffer(m, a.dtype, a.size, room - a.nbytes).reshape(a.shape)
+    view[...] = a
+    assert libc.mprotect(view.ctypes.data + a.nbytes, page, 0) == 0, ctypes.get_errno()
+    return view
+
+
+@pytest.mark.parametrize("ld", [5000, 5008])
+@pytest.mark.parametrize("rows_of,spare", [([1], 0), ([4], 0), ([3, 1, 2], 0), ([3, 2], 2)])
+def test_verify_reads_no_draft_row_behind_the_last(L, rows_of, spare, ld):
+    """draft_logits of rows - 1 rows: on the device an allocation that ends with them, on the host a mapping."""
+    vocab, rng = 5000, np.random.default_rng(ld + sum(rows_of))
+    start, logits, draft, tokens, uniform = verify_inputs(rng, rows_of + [spare], vocab, 0.9, True, ld=ld)
+    start, rows, count = start[:-1].copy(), len(logits), len(rows_of)
+    want = ru.verify(start, logits[:, :vocab], draft[:, :vocab], tokens, uniform, 0.9)
+    exact = at_a_mappings_end(draft[:-1].reshape(-1)[:max((rows - 2) * ld + vocab, 0)])
+    device = L.llhip_malloc(exact.nbytes) if exact.nbytes else None
+    try:
+        if exact.nbytes:
+            L.llhip_memcpy_h2d(device, lh.ptr(exact), exact.nbytes)
+        for place in ("host", "device"):
+            accepted, following = np.full(count, -9, np.int32), np.full(count, -9, np.int32)
+            L.llhip_verify_drafts(lh.ptr(accepted), lh.ptr(following), lh.ptr(logits), ld,
+                                  exact.ctypes.data if place == "host" else device, ld, lh.ptr(tokens), lh.ptr(uniform),
+                                  lh.ptr(start), count, rows, vocab, 0.9)
+            assert not lh.last_error(), lh.last_error()
+            assert list(zip(accepted.tolist(), following.tolist())) == want
+    finally:
+        if device:
+            L.llhip_free(device)
+
+
 def test_verify_emits_the_targets_distribution(L):
     """20000 requests' worth of draws over six tokens: the emitted first tokens' frequencies are the target's within five
     standard deviations, whatever the draft's distribution."""
@@ -1105,6 +1144,39 @@ def test_engine_verify(L, tmp_path, monkeypatch, kind):
             assert words in lh.last_error(), lh.last_error()
         assert verify(two, 20, None, None, 0.0) >= 0 and not lh.last_error()
     finally:
+        L.engine_free(at)
+
+
+def test_engine_verify_reads_a_draft_row_for_each_draft(L, tmp_path):
+    """count - 1 rows of draft_logits, at the end of a mapping and of a device allocation; none for one row."""
+    L.kernels_kv_layout_select(b"head")
+    path = os.path.join(tmp_path, "tiny.bin")
+    engine_model(path, "q8")
+    vocab, rng = ENGINE["vocab_size"], np.random.default_rng(12)
+    model, following, device = lh.Model(), ctypes.c_int(-7), None
+    at = ctypes.byref(model)
+    try:
+        L.engine_load(at, path.encode())
+        for n in (5, 2, 1):
+            tokens, uniform = rng.integers(0, vocab, n).astype(np.int32), rng.random((n, 2)).astype(F)
+            p = L.engine_forward_batch(at, lh.ptr(tokens), n, 0, lh.LOGITS_ALL)
+            logits = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (n, vocab)).copy()
+            draft = (logits + rng.standard_normal(logits.shape)).astype(F)
+            want = ru.verify([0, n], logits, draft, tokens, uniform, 0.9)[0]
+            exact = at_a_mappings_end(draft[:-1])
+            device = L.llhip_malloc(max(exact.nbytes, 4))
+            if exact.nbytes:
+                L.llhip_memcpy_h2d(device, lh.ptr(exact), exact.nbytes)
+            for place in (exact.ctypes.data, device):
+                got = L.llhip_engine_verify(at, lh.ptr(tokens), n, 0, place, vocab, lh.ptr(uniform), 0.9,
+                                            ctypes.byref(following))
+                assert not lh.last_error(), lh.last_error()
+                assert (got, following.value) == want
+            L.llhip_free(device)
+            device = None
+    finally:
+        if device:
+            L.llhip_free(device)
         L.engine_free(at)
 
 
