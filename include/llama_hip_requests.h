@@ -55,12 +55,14 @@ void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride,
  * request r attends to positions 0 .. prefix - 1 of prefix_key / prefix_value and to own positions 0 .. length[r] + j of
  * its slot (whose last rows llhip_rope_kv_store_requests stored). q and out hold rows of n_heads * head_dim floats;
  * scores, softmax and value sums as in k_attention (FP32-accurate; a non-finite score fails with "nonfinite value in
- * softmax"). The sums are divided by the weights' at the end, so n positions' values must stay below 3e38 / n, as there;
- * products with values far below 2^-30 of their K row's largest, or of the largest in four V rows, are exact to about 2^-36
- * of that, and V rows of very different sizes keep this up to 2^80. The prefix is read once for all requests, not once for
- * each. prefix_key and prefix_value may be NULL where prefix is 0; requests may share a slot here. out must not overlap q
- * or a cache. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16 per KV head, head_dim at most
- * 256. */
+ * softmax"). The sums are divided by the weights' at the end, so n positions' values must stay below 3e38 / n, as there.
+ * Where a tile has more than 32 query vectors (a KV head's heads of its rows), the products are of two FP16 parts, with FP32
+ * sums: a factor is exact to 2^-22 of itself or, where that is more, to 2^-39 of the largest of its query vector, its K row
+ * (both taken as at least 2^-100) or its group of four V rows, and a weight to 2^-24 of its row's largest, or 2^-36 over V
+ * rows of about one size; V rows further apart in size than that, and smaller tiles, take FP32 products. The prefix is read
+ * once for all requests, not once for each. prefix_key and prefix_value may be NULL where prefix is 0; requests may share a
+ * slot here. out must not overlap q or a cache. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16
+ * per KV head, head_dim at most 256. */
 void llhip_attention_requests(float *out, const float *q, const float *prefix_key, const float *prefix_value,
                               const float *key_cache, const float *value_cache, const RequestBatch *batch, int n_heads,
                               int n_kv_heads, int head_dim);

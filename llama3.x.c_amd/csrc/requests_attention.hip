@@ -13,6 +13,7 @@
 // instructions: a step takes the two waves of a SIMD 5600 cycles, 4300 of vector and 3100 of matrix instructions, which overlap
 // little (over the whole kernel the vector unit is 50% busy, the matrix cores 30%, LDS less); narrow ones by HBM.
 #include <cfloat>
+#include <type_traits>
 
 #include "requests_device.h"
 
@@ -198,9 +199,9 @@ struct FastAttn {
   const float *q, *prefix_key, *prefix_value, *key, *value;
   RequestsDev batch;
   int n_heads, n_kv_heads, kv_mul, hd;
-  int tile_rows; // rows of a wide tile
-  int blocks;    // of a KV head
-  float scale2;  // log2(e) / sqrtf(hd)
+  int tile_rows, narrow_rows; // rows of a wide tile, and at most of a narrow one
+  int blocks;                 // of a KV head
+  float scale2;               // log2(e) / sqrtf(hd)
   // slots of hd + 4 floats: [prefix, own][row][head] where a walk begins, [KV head][block][vector of the tile] where a
   // block goes on with the walk of the one before
   float *partial;
@@ -345,6 +346,12 @@ __device__ __forceinline__ float *slot_of(const FastAttn &p, const Item &it, int
 // Nothing moves across: each phase's registers are free before the next one's are taken (moved freely, the phases of a
 // step need more than the 256 registers that two waves a SIMD leave each).
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uniform(long long x) {
+  return (long long)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
 
 // The thread's number, new to the compiler at each walk: else it keeps what both walks derive from it in registers all along
 // a block's walks (43 of them spilled).
@@ -617,10 +624,22 @@ template <int HD, bool FULL> __device__ void walk_narrow(const FastAttn &p, cons
 // BF16 parts take six. The parts need values near 2^15: each query vector and each K row is scaled by a power of two of
 // its own, taken out of the score again; each group of four V rows likewise, and its exponent ev joins the score before
 // the exponential, so that the weights are exp2(s + ev - m) and meet V 2^-ev, with m the running maximum of s + ev. The
-// softmax's sum takes them times 2^-ev. A product is so exact to about 2^-36 of its row's largest value (for V of the
-// largest in four rows), and the sum holds groups up to 2^140 apart: between 2^-60, which smaller values take, and 2^80.
+// softmax's sum takes them times 2^-ev. A value is so exact to 2^-22 of itself, or to 2^-39 of the largest of its query
+// vector, K row or four V rows.
+//
+// A weight is exact to 2^-22 of itself, or to 2^-25 where the largest is 2^11 or more; so, with the ev of a walk within 3
+// kSpread of each other, to 2^(12 - 36) of the row's largest (to 2^-36 where they are the same). An element far above the
+// others would raise its rows' ev and leave the other rows' weights too few bits, in every dimension. So a wave compares the
+// exponents of its V rows with those of its first step, and at the end of a walk they are compared with each other: where
+// they lie further apart, or below what ev takes, the block does the walk again in narrow tiles, whose FP32 products have no
+// such limits. That takes longer (one element of 10^6 in a prefix: 923 prompt rows 94 -> 290 us, 64 requests 98 -> 180), and
+// is rare: the largest of four rows of a head differs by far less.
+// (Kept per walk as a smallest and a largest ev, in registers, scalars or LDS, the same check spilled 10 to 17 registers: 64
+// requests 98 -> 112 us.)
+//
 // V parts lie transposed, a dimension's 32 slots in 64 bytes, its 16-byte units where v_unit puts them: a matrix operand's
 // read takes one unit of 16 dimensions, a staging write half a unit of every fourth one, and both spread over the banks.
+constexpr int kSpread = 4, kNoExponent = -(1 << 20);
 template <int HD> struct WideStage {
   static constexpr int kKRow = HD + 8;
   uint16_t k[2][kUnit * kKRow];
@@ -634,7 +653,7 @@ __device__ __forceinline__ int v_unit(int dim, int unit) { // in halves
   return ((four << 2) | ((dim ^ four) & 3)) * kUnit + 8 * ((unit ^ four ^ (dim >> 4)) & 3);
 }
 
-template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
+template <int HD, bool FULL> __device__ bool walk_wide(const FastAttn &p, const Item &it, unsigned char *lds) {
   typedef WideStage<HD> Stage;
   Stage *const stages = reinterpret_cast<Stage *>(lds); // two: a step is staged while the one before is computed
   constexpr int kSteps = HD / 32, kDt = HD / 16, kLeastK = -100, kLeastV = -60;
@@ -648,7 +667,9 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
   const bool v_stager = kAllStage || tid < kUnit / 4 * kVLanes;
   const int vg = tid / kVLanes, vd = 4 * (tid % kVLanes); // V item: positions 4 vg .. + 3, dimensions vd .. + 3
   float4 kr[kItems][2], vr[4];
-  bool met = false; // a value that is not finite
+  bool met = false;           // a value that is not finite
+  int ev_first = kNoExponent; // the largest exponent of the wave's V rows of the first step that are not zero
+  bool spread = false;        // that of others lies further from it than kSpread
   const Rows keys = rows_of(it.key, it, hd), values = rows_of(it.value, it, hd);
   unsigned k_at = (unsigned)(tid / kLanes) * keys.stride, v_at = (unsigned)(4 * vg) * values.stride;
   auto load = [&]() {
@@ -666,7 +687,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     v_at += kUnit * values.stride;
   };
   auto peak = [](const float4 &x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); };
-  auto stage = [&](Stage &sh) {
+  auto stage = [&](Stage &sh, auto first) {
 #pragma unroll
     for (int u = 0; u < kItems; u++) {
       const int i = tid + u * kThreads, row = i / kLanes, d = 8 * (i % kLanes);
@@ -690,6 +711,16 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
       top = group_reduce_max(top, kVLanes);
       int ev;
       const float scale = f16_scale(top > 0.0f ? top : 1.0f, kLeastV, ev); // rows of zeros take no extreme exponent
+      const int exponent = (int)(__float_as_uint(top) >> 23) - 127; // ev, but not raised to kLeastV
+      if constexpr (decltype(first)::value) {
+        const int mine = top > 0.0f ? exponent : kNoExponent;
+#pragma unroll
+        for (int o = 0; o < kWave; o += kVLanes)
+          ev_first = max(ev_first, __builtin_amdgcn_readlane(mine, o));
+        spread = mine != kNoExponent && mine < ev_first - kSpread;
+      } else {
+        spread |= top > 0.0f && (unsigned)(exponent - ev_first + kSpread) > 2u * kSpread;
+      }
       // slot of position 16 t + 4 q + e: 8 q + 4 t + e, so the four of this item are half of unit vg % 4
       auto put = [&](int d, float x0, float x1, float x2, float x3) {
         int h0, l0, h1, l1;
@@ -814,9 +845,9 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
           top = fmaxf(top, pv[4 * t + e]);
         }
       }
-      // the running maximum moves only when a score passes it by 2^8, which the weights' range leaves room for: nearly
+      // the running maximum moves only when a score passes it by 2^4, which the weights' range leaves room for: nearly
       // all steps then need no exchange between lanes and no rescale
-      if (__any(top > m_run[n] + 8.0f)) {
+      if (__any(top > m_run[n] + 4.0f)) {
         const float m_new = fmaxf(m_run[n], four_max(top)), alpha = __builtin_amdgcn_exp2f(m_run[n] - m_new);
         l_run[n] *= alpha;
         m_run[n] = m_new;
@@ -824,7 +855,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
         for (int d = 0; d < kDt; d++)
           o[n][d] *= alpha;
       }
-      const float base = fmaxf(m_run[n], kMasked) - 7.0f; // weights up to 2^15
+      const float base = fmaxf(m_run[n], kMasked) - 11.0f; // weights up to 2^15, the largest at least 2^11
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < 2; t++) {
@@ -873,7 +904,7 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
   };
   if (it.t0 < it.t1) {
     check();
-    stage(stages[0]);
+    stage(stages[0], std::true_type());
     load();
     __syncthreads();
   }
@@ -884,20 +915,36 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     if (busy) {
       score(stages[turn]);
       // the next step's stage was read before the last barrier; past the end it takes zeros that nobody reads
-      stage(stages[turn ^ 1]);
+      stage(stages[turn ^ 1], std::false_type());
       fence();
       load();
       fence();
       weigh_and_add(stages[turn], t0);
     } else {
-      stage(stages[turn ^ 1]);
+      stage(stages[turn ^ 1], std::false_type());
       load();
     }
     __syncthreads();
   }
+  // the waves' findings, where the stages were
+  int2 *const found = reinterpret_cast<int2 *>(lds);
+  const bool apart = __any(spread);
+  if (lane == 0)
+    found[wave] = int2{ev_first, (apart ? 2 : 0) | (met ? 1 : 0)};
+  __syncthreads();
+  int low = INT32_MAX, high = kNoExponent, flags = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / kWave; w++) {
+    const int2 f = found[w];
+    low = min(low, f.x == kNoExponent ? INT32_MAX : f.x);
+    high = max(high, f.x);
+    flags |= f.y;
+  }
+  if (flags & 2 || high - kSpread > low || low - kSpread < kLeastV) // uniform
+    return false;
+  met = flags & 1;
   if (odd != 0.0f && (last[0] >= 0 || last[1] >= 0))
     p.flags[1] = 1;
-  met = __syncthreads_or(met);
 #pragma unroll
   for (int n = 0; n < 2; n++) {
     const float l = four_sum(l_run[n]);
@@ -905,15 +952,16 @@ template <int HD, bool FULL> __device__ void walk_wide(const FastAttn &p, const 
     if (v >= it.vectors)
       continue;
     float *dst = slot_of(p, it, v);
-    const float back = 0x1p-21f; // 2^14 of the V rows, 2^7 of the weights
+    const float back = 0x1p-25f; // 2^14 of the V rows, 2^11 of the weights
 #pragma unroll
     for (int d = 0; d < kDt; d++)
       if (16 * d + 4 * lq < hd)
         *reinterpret_cast<float4 *>(dst + 16 * d + 4 * lq) =
             float4{o[n][d][0] * back, o[n][d][1] * back, o[n][d][2] * back, o[n][d][3] * back};
     if (lq == 0)
-      *reinterpret_cast<float4 *>(dst + hd) = slot_end(m_run[n], l * 0x1p-7f, met, it);
+      *reinterpret_cast<float4 *>(dst + hd) = slot_end(m_run[n], l * 0x1p-11f, met, it);
   }
+  return true;
 }
 
 // LDS: the plan, then the walk's.
@@ -923,12 +971,6 @@ template <int HD> constexpr size_t fast_lds() {
   return kPlanLds + (narrow_sums > stages ? narrow_sums : stages);
 }
 static_assert(kBlocksPerCu * fast_lds<128>() <= 160 * 1024, "blocks of a CU");
-
-// A value that all lanes hold, in scalar registers.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long long uniform(long long x) {
-  return (long long)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
-}
 
 // Positions 0 .. e - 1 of a walk that lies at a .. a + time - 1 on the line: the first one behind the cut at x.
 __device__ __forceinline__ int cut_at(long long x, long long a, long long time, int e) {
@@ -989,7 +1031,7 @@ template <int HD, bool FULL> __global__ __launch_bounds__(kThreads, kBlocksPerCu
   }
   const long long x0 = uniform(block * plan.slice), x1 = uniform(min(block * plan.slice + plan.slice, plan.total));
   const size_t begins = (size_t)p.batch.rows * p.n_heads; // slots of the walks that begin in a block, prefix and own each
-  int r = -1;
+  int r = -1, part = -1; // the part of a wide tile that is done again in narrow ones, by its first row
   for (long long x = x0; x < x1;) {
     Item it;
     long long a, time; // the walk's place
@@ -1059,17 +1101,32 @@ template <int HD, bool FULL> __global__ __launch_bounds__(kThreads, kBlocksPerCu
       it.slot0 = 2 * begins + ((size_t)g * p.blocks + block) * kTileVectors;
       it.slot_row = p.kv_mul;
     }
-    if (x != x0)
+    if (x != x0 || part >= 0)
       __syncthreads(); // the walk before is done with its LDS
     if (it.t0 == it.t1) { // a cut within the first step's positions: nothing is left for this side of it
       const int quads = p.hd / 4 + 1;
       for (int e = tid; e < it.vectors * quads; e += kThreads)
         *reinterpret_cast<float4 *>(slot_of(p, it, e / quads) + 4 * (e % quads)) =
             float4{e % quads == quads - 1 ? -FLT_MAX : 0.0f, 0.0f, 0.0f, 0.0f};
-    } else if (it.vectors <= kNarrowVectors) {
-      walk_narrow<HD, FULL>(p, it, lds + kPlanLds);
+    } else if (it.vectors > kNarrowVectors && part < 0) {
+      if (!walk_wide<HD, FULL>(p, it, lds + kPlanLds)) {
+        part = 0; // V rows too far apart in size for its parts
+        continue;
+      }
     } else {
-      walk_wide<HD, FULL>(p, it, lds + kPlanLds);
+      int next = -1;
+      if (part >= 0) {
+        const int rows = uniform(it.vectors / p.kv_mul), n = min(rows - part, p.narrow_rows);
+        it.row0 += part;
+        it.vectors = n * p.kv_mul;
+        it.last0 = prefix ? INT32_MAX : it.last0 + part;
+        it.slot0 += (size_t)part * it.slot_row;
+        next = part + n < rows ? part + n : -1;
+      }
+      walk_narrow<HD, FULL>(p, it, lds + kPlanLds);
+      part = next;
+      if (part >= 0)
+        continue;
     }
     x = a + time;
   }
@@ -1201,6 +1258,7 @@ bool launch_attention_fast(const AttentionRequestsJob &job, void *workspace, hip
   p.kv_mul = job.n_heads / job.n_kv_heads;
   p.hd = job.head_dim;
   p.tile_rows = kTileVectors / p.kv_mul;
+  p.narrow_rows = kNarrowVectors / p.kv_mul;
   p.blocks = fast_blocks(job);
   p.scale2 = 1.4426950408889634f / sqrtf((float)job.head_dim);
   p.rows = (RowSlots *)workspace;

@@ -265,6 +265,80 @@ def test_attention_value_sizes(L, rows_of, sizes):
     within(hu.host(out), want, bound)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 2, 64), (10, 2, 80)])
+@pytest.mark.parametrize("form", ["element", "half", "own"])
+@pytest.mark.parametrize("raised", [1e2, 1e4, 1e7, 1e12, 1e30])
+def test_attention_large_value_elements(L, heads, kv, hd, form, raised):
+    """Tiles of a block over V rows of which some elements are far larger than the rest: one element of a prefix row, half
+    the dimensions of eight rows, one element of an own row that only the later rows see. The other dimensions' sums keep
+    their own accuracy."""
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(13)
+    b = ru.Batch(hu.dev, [40, 30], [37, 5], prefix=256, prefix_seq_len=256, seq_len=96)
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    pk, pv = (rng.standard_normal((kv, 256, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((2, kv, 96, hd), dtype=F) for _ in range(2))
+    if form == "element":
+        pv[:, 100, 3] = raised
+    elif form == "half":
+        pv[:, rng.choice(256, 8, replace=False), hd // 2:] *= F(raised)
+    else:
+        v[0, :, 50, hd - 1] = raised
+    out = hu.dev(np.zeros_like(q))
+    dev = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in dev], b.struct, heads, kv, hd)
+    quiet(L)
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
+    within(hu.host(out), want, bound)
+
+
+@pytest.mark.parametrize("sizes", [(1e-17, 1e-19), (1e-28,), (1e-28, 1.0), (1.0, 100.0, 0.0, 0.01)])
+def test_attention_small_values(L, sizes):
+    """Tiles of a block over V rows below what the FP16 parts' exponents take, and around the border; rows of zeros between
+    others; the first rows larger or smaller than the rest."""
+    L.kernels_kv_layout_select(b"head")
+    heads, kv, hd = 8, 2, 128
+    b = ru.Batch(hu.dev, [40, 30], [50, 0], prefix=200, prefix_seq_len=200, seq_len=100)
+    rng = np.random.default_rng(15)
+    size = lambda n: np.asarray(sizes, F)[np.arange(n) // 8 % len(sizes)][:, None]  # noqa: E731
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    pk, k = (rng.standard_normal(s, dtype=F) for s in ((kv, 200, hd), (2, kv, 100, hd)))
+    pv, v = (size(s[-2]) * rng.uniform(0.5, 1.5, s).astype(F) for s in ((kv, 200, hd), (2, kv, 100, hd)))
+    out = hu.dev(np.zeros_like(q))
+    args = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in args], b.struct, heads, kv, hd)
+    quiet(L)
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
+    within(hu.host(out), want, bound)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 2, 64)])
+@pytest.mark.parametrize("gap", [5.0, 12.0, 18.0])
+def test_attention_one_position_without_values(L, heads, kv, hd, gap):
+    """Nearly the whole weight, all but exp(-gap) or less, on a position whose V row is zero among ordinary ones, so that
+    the outputs are the small weights' sums. A weight is held to 2^-36 of the row's largest over V rows of one size, and the
+    exponents of four normal rows' largest differ by two at most: 2^-34 of each value beside the plain bound."""
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(14)
+    b = ru.Batch(hu.dev, [40, 30], [37, 5], prefix=256, prefix_seq_len=256, seq_len=96)
+    q = (0.5 * rng.standard_normal((b.rows, heads * hd))).astype(F)
+    pk, pv = (rng.standard_normal((kv, 256, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((2, kv, 96, hd), dtype=F) for _ in range(2))
+    q.reshape(b.rows, heads, hd)[:, :, 0] = 1.0
+    pk[:, :, 0], k[..., 0] = 0.0, 0.0
+    pk[:, 33] = 0.0
+    pk[:, 33, 0] = (gap + 3.0) * np.sqrt(hd)  # the other scores are below 3
+    pv[:, 33] = 0.0
+    out = hu.dev(np.zeros_like(q))
+    dev = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in dev], b.struct, heads, kv, hd)
+    quiet(L)
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, "head")
+    sums = np.abs(pv).sum(1)[None, :, None] + np.abs(v).sum(2).max(0)[None, :, None]
+    extra = np.broadcast_to(2.0 ** -34 * sums, (b.rows, kv, heads // kv, hd)).reshape(bound.shape)
+    within(hu.host(out), want, bound + extra)
+
+
 @pytest.mark.parametrize("rows", [3, 20, 45])
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 def test_attention_nonfinite_values_reach_only_the_rows_that_see_them(L, rows, value):
