@@ -76,7 +76,7 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
  * adapters x rank x k and B adapters x n x rank, row-major; rank 1 .. LLHIP_MAX_LORA_RANK, the same for the segment's
  * adapters (smaller ones padded with zeros). Sums are FP32 throughout, also over BF16 adapters (the activations are not
  * rounded); a row of x, or an adapter, that holds an infinity or a NaN gives its rows' columns NaN or infinity. c must not
- * overlap x, the adapters, or another segment's c or base. */
+ * overlap x, the ids, any segment's adapters or scales, or another segment's c or base. */
 typedef struct {
   float *c;
   int ldc;

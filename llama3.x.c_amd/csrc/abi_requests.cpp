@@ -131,26 +131,32 @@ void lora(const char *name, const float *x, int ldx, int m, int k, const int *ad
       raise("%s: segment %d has a null buffer", name, i);
       return;
     }
+  }
+  for (int i = 0; i < count; i++) {
+    const Segment &s = segments[i];
     const size_t out = ((size_t)(m - 1) * s.ldc + s.n) * kFloat;
-    const size_t a_bytes = (size_t)adapters * s.rank * k * element, b_bytes = (size_t)adapters * s.n * s.rank * element;
-    bool bad = overlaps(s.c, out, x, x_bytes) || overlaps(s.c, out, s.a, a_bytes) || overlaps(s.c, out, s.b, b_bytes) ||
+    bool bad = overlaps(s.c, out, x, x_bytes) || overlaps(s.c, out, adapter, (size_t)m * sizeof(int)) ||
                (s.base != s.c && overlaps(s.c, out, s.base, out));
-    if (swiglu)
-      bad |= overlaps(s.c, out, s.a3, a_bytes) || overlaps(s.c, out, s.b3, b_bytes) ||
-             (s.base3 != s.c && overlaps(s.c, out, s.base3, out));
+    if (s.kind == GEMM_SWIGLU)
+      bad |= s.base3 != s.c && overlaps(s.c, out, s.base3, out);
     for (int j = 0; j < count; j++) {
-      const size_t other = ((size_t)(m - 1) * segments[j].ldc + segments[j].n) * kFloat;
+      const Segment &t = segments[j];
+      const size_t other = ((size_t)(m - 1) * t.ldc + t.n) * kFloat;
+      const size_t a_bytes = (size_t)adapters * t.rank * k * element, b_bytes = (size_t)adapters * t.n * t.rank * element;
       // segments side by side in one row buffer (QKV rows) share an extent: their columns must differ
       auto apart = [&](const float *p) {
         if (!overlaps(s.c, out, p, other))
           return true;
         const ptrdiff_t gap = s.c - p;
-        return s.ldc == segments[j].ldc && ((gap >= segments[j].n && gap + s.n <= s.ldc) ||
-                                            (-gap >= s.n && -gap + segments[j].n <= s.ldc));
+        return s.ldc == t.ldc && ((gap >= t.n && gap + s.n <= s.ldc) || (-gap >= s.n && -gap + t.n <= s.ldc));
       };
+      const bool swiglu = t.kind == GEMM_SWIGLU;
       if (j != i)
-        bad |= !apart(segments[j].c) || !apart(segments[j].base) ||
-               (segments[j].kind == GEMM_SWIGLU && segments[j].base3 && !apart(segments[j].base3));
+        bad |= !apart(t.c) || !apart(t.base) || (swiglu && !apart(t.base3));
+      bad |= overlaps(s.c, out, t.a, a_bytes) || overlaps(s.c, out, t.b, b_bytes) ||
+             overlaps(s.c, out, t.scale, (size_t)adapters * kFloat);
+      if (swiglu)
+        bad |= overlaps(s.c, out, t.a3, a_bytes) || overlaps(s.c, out, t.b3, b_bytes);
     }
     if (bad) {
       raise("%s: segment %d's output overlaps an input or another segment", name, i);

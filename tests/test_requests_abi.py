@@ -179,6 +179,40 @@ def test_lora_refusals(L, bf16):
     assert not lh.last_error()
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("own", [False, True])
+def test_lora_refuses_outputs_over_any_segments_inputs(L, bf16, own):
+    """An output over the adapters, the second adapters or the scales of its own segment or another, or over the ids."""
+    kind = np.uint16 if bf16 else np.float32
+    memory = np.zeros(4096, np.float32)
+    c, base = memory[64:64 + 18].reshape(3, 6), np.zeros((3, 6), np.float32)
+    a, b, scale = np.zeros((2, 4, 8), kind), np.zeros((2, 6, 4), kind), np.ones(2, np.float32)
+    fn = L.llhip_lora_bf16 if bf16 else L.llhip_lora_f32
+    x, ids = np.zeros((3, 8), np.float32), np.zeros(3, np.int32)
+
+    def call(ids=ids, **over):
+        t = {"a": a, "b": b, "a3": a, "b3": b, "scale": scale}
+        t.update(over)
+        target = ru.lora_segment(bf16, c if own else np.zeros((3, 6), np.float32), 6, base, t["a"], t["b"], t["scale"], 6, 4,
+                                 base, t["a3"], t["b3"])
+        first = ru.lora_segment(bf16, c, 6, base, a, b, None, 6, 4)
+        segs = ru.array([target] if own else [first, target])
+        fn(lh.ptr(x), 8, 3, 8, lh.ptr(ids), 2, segs, len(segs))
+
+    units = memory.view(kind)
+    per = units.size // memory.size
+    for name, size in (("a", 64), ("b", 48), ("a3", 64), ("b3", 48)):
+        for at in (64 * per - size + 1, 64 * per + 5, (64 + 18) * per - 1):
+            call(**{name: units[at:at + size]})
+            refused(L, "overlaps an input")
+    for at in (63, 70, 81):
+        call(scale=memory[at:at + 2])
+        refused(L, "overlaps an input")
+    for at in (62, 70, 81):
+        call(ids=memory.view(np.int32)[at:at + 3])
+        refused(L, "overlaps an input")
+
+
 def verify_call(L, vocab=10, rows=4, count=2, temperature=1.0, ld=10, draft_ld=10, **over):
     a = {"accepted": np.zeros(2, np.int32), "next": np.zeros(2, np.int32), "logits": np.zeros((4, 10), np.float32),
          "draft": np.zeros((4, 10), np.float32), "tokens": np.zeros(4, np.int32), "uniform": np.zeros((4, 2), np.float32),
