@@ -45,8 +45,8 @@ enum { LLHIP_MAX_REQUESTS = 1024 };
  * as k_rope_apply rotates them (bitwise), k's n_kv_heads heads rotated and v copied into the request's slot at own
  * position length[r] + j. table: prefix + seq_len rows of k_rope_table, position by position. q_out has q's stride and
  * may be q itself; k and v stay as they are. No two requests of a call may share a slot (that fails at the next
- * host-visible point; the slot's rows are then one of them's). q_out, the rows and both caches must not overlap otherwise;
- * head_dim even and at most 256. */
+ * host-visible point; the slot's rows are then one of them's). q_out, the rows, both caches and the batch's arrays must not overlap
+ * otherwise; head_dim even and at most 256. */
 void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride, const float *k, const float *v,
                                   size_t kv_stride, const float *table, const RequestBatch *batch, int n_heads,
                                   int n_kv_heads, int head_dim, float *key_cache, float *value_cache);
@@ -61,7 +61,7 @@ void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride,
  * (both taken as at least 2^-100) or its group of four V rows, and a weight to 2^-24 of its row's largest, or 2^-36 over V
  * rows of about one size; V rows further apart in size than that, and smaller tiles, take FP32 products. The prefix is read
  * once for all requests, not once for each. prefix_key and prefix_value may be NULL where prefix is 0; requests may share a
- * slot here. out must not overlap q or a cache. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16
+ * slot here. out must not overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16
  * per KV head, head_dim at most 256. */
 void llhip_attention_requests(float *out, const float *q, const float *prefix_key, const float *prefix_value,
                               const float *key_cache, const float *value_cache, const RequestBatch *batch, int n_heads,

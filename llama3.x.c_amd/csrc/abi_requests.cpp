@@ -57,6 +57,13 @@ RequestsDev batch_dev(const Call &call, const BatchRefs &r, const RequestBatch *
   return d;
 }
 
+// Whether a call that writes these bytes would write over the batch's arrays, which its other blocks still read.
+bool over_arrays(const RequestBatch *b, const void *out, size_t bytes) {
+  const size_t n = (size_t)b->count * sizeof(int);
+  return overlaps(out, bytes, b->start, n + sizeof(int)) || overlaps(out, bytes, b->length, n) ||
+         overlaps(out, bytes, b->slot, n);
+}
+
 size_t caches_bytes(const RequestBatch *b, int n_kv_heads, int head_dim) {
   return (size_t)b->slots * b->seq_len * n_kv_heads * head_dim * kFloat;
 }
@@ -249,12 +256,12 @@ void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride,
                                      (-gap >= (ptrdiff_t)dkv && -gap + (ptrdiff_t)dq <= (ptrdiff_t)q_stride));
   };
   bool bad = overlaps(key_cache, cache, value_cache, cache) || (q_out != q && overlaps(q_out, q_bytes, q, q_bytes)) ||
-             !apart(k) || !apart(v) || overlaps(table, table_bytes, q_out, q_bytes);
+             !apart(k) || !apart(v) || overlaps(table, table_bytes, q_out, q_bytes) || over_arrays(batch, q_out, q_bytes);
   for (float *c : {key_cache, value_cache})
-    bad |= overlaps(c, cache, q, q_bytes) || overlaps(c, cache, q_out, q_bytes) || overlaps(c, cache, k, kv_bytes) ||
+    bad |= over_arrays(batch, c, cache) || overlaps(c, cache, q, q_bytes) || overlaps(c, cache, q_out, q_bytes) || overlaps(c, cache, k, kv_bytes) ||
            overlaps(c, cache, v, kv_bytes) || overlaps(c, cache, table, table_bytes);
   if (bad) {
-    raise("%s: q_out, the rows, the table and the caches must not overlap", name);
+    raise("%s: q_out, the rows, the table, the caches and the batch's arrays must not overlap", name);
     return;
   }
   Call call(name);
@@ -301,8 +308,8 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
                     : 0;
   if (overlaps(out, row_bytes, q, row_bytes) || overlaps(out, row_bytes, key_cache, cache) ||
       overlaps(out, row_bytes, value_cache, cache) || overlaps(out, row_bytes, prefix_key, prefix_bytes) ||
-      overlaps(out, row_bytes, prefix_value, prefix_bytes)) {
-    raise("%s: out must not overlap q or a cache", name);
+      overlaps(out, row_bytes, prefix_value, prefix_bytes) || over_arrays(batch, out, row_bytes)) {
+    raise("%s: out must not overlap q, a cache or the batch's arrays", name);
     return;
   }
   Call call(name);

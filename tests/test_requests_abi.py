@@ -135,6 +135,26 @@ def test_rope_refusals(L):
     refused(L, "must not overlap")
 
 
+@pytest.mark.parametrize("array", [0, 1, 2])
+def test_outputs_over_the_batchs_arrays_are_refused(L, array):
+    """An output over the first or last entry of start, length or slot, of which a slot may be missing."""
+    for entry, at in ((0, 0), (0, 95), (-1, 50)):
+        b = make(slot=[1, 0])
+        memory = np.zeros(4096, np.float32)
+        field = ("start", "length", "slot")[array]
+        ints = memory[1024:1024 + len(b.keep[array])].view(np.int32)
+        ints[:] = b.keep[array]
+        setattr(b.struct, field, lh.ptr(ints))
+        begin = 1024 + entry % ints.size - at
+        attention_call(L, b.struct, out=memory[begin:begin + 96].reshape(3, 32))
+        refused(L, "must not overlap")
+        rope_call(L, b.struct, o=memory[begin:begin + 96].reshape(3, 32))
+        refused(L, "must not overlap")
+        for cache in ("kc", "vc"):
+            rope_call(L, b.struct, **{cache: memory[begin:begin + 512]})
+            refused(L, "must not overlap")
+
+
 def lora_call(L, m=3, k=8, ldx=8, adapters=2, count=1, bf16=False, x=True, ids=True, edit=None, segments=None, **over):
     kind = np.uint16 if bf16 else np.float32
     c, base = np.zeros((m, 6), np.float32), np.zeros((m, 6), np.float32)
