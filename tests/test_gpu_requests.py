@@ -292,6 +292,32 @@ def test_attention_large_value_elements(L, heads, kv, hd, form, raised):
     within(hu.host(out), want, bound)
 
 
+@pytest.mark.parametrize("layout", ["head", "rows"])
+@pytest.mark.parametrize("heads,kv,hd", [(16, 1, 128), (6, 2, 64), (8, 2, 128)])
+def test_attention_large_elements_in_some_slices(L, layout, heads, kv, hd):
+    """A prefix cut into slices of which one holds a large element, an own walk that holds another beside a V value that is
+    not finite and only the last row sees; the parts with and without meet in the same rows."""
+    L.kernels_kv_layout_select(layout.encode())
+    rng = np.random.default_rng(heads)
+    b = ru.Batch(hu.dev, [45, 1, 20], [700, 3, 0], prefix=3000, prefix_seq_len=3001, seq_len=760)
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    pk, pv = (rng.standard_normal(ru.cache_shape(layout, 3001, kv, hd), dtype=F) for _ in range(2))
+    k, v = (rng.standard_normal((3,) + ru.cache_shape(layout, 760, kv, hd), dtype=F) for _ in range(2))
+    ru.by_head(pv, layout)[0, 1700, 5] = 1e12
+    ru.by_head(v[0], layout)[:, 650, hd - 2] = -1e9
+    want, bound = ru.attention(b, q, pk, pv, k, v, heads, kv, hd, layout)
+    ru.by_head(v[0], layout)[0, 744, 9] = np.inf  # request 0's last row's own position
+    out = hu.dev(np.zeros_like(q))
+    dev = [hu.dev(a) for a in (q, pk, pv, k, v)]
+    L.llhip_attention_requests(lh.ptr(out), *[lh.ptr(a) for a in dev], b.struct, heads, kv, hd)
+    quiet(L)
+    got = hu.host(out).reshape(b.rows, heads, hd)
+    hit = np.zeros(got.shape, bool)
+    hit[44, :heads // kv, 9] = True
+    assert (got[hit] == np.inf).all()
+    within(got[~hit], want.reshape(got.shape)[~hit], bound.reshape(got.shape)[~hit])
+
+
 @pytest.mark.parametrize("sizes", [(1e-17, 1e-19), (1e-28,), (1e-28, 1.0), (1.0, 100.0, 0.0, 0.01)])
 def test_attention_small_values(L, sizes):
     """Tiles of a block over V rows below what the FP16 parts' exponents take, and around the border; rows of zeros between
