@@ -45,8 +45,10 @@ enum { LLHIP_MAX_REQUESTS = 1024 };
  * as k_rope_apply rotates them (bitwise), k's n_kv_heads heads rotated and v copied into the request's slot at own
  * position length[r] + j. table: prefix + seq_len rows of k_rope_table, position by position. q_out has q's stride and
  * may be q itself; k and v stay as they are. No two requests of a call may share a slot (that fails at the next
- * host-visible point; the slot's rows are then one of them's). q_out, the rows, both caches and the batch's arrays must not overlap
- * otherwise; head_dim even and at most 256. */
+ * host-visible point; the slot's rows are then one of them's). q_out, the rows, both caches and the batch's arrays must
+ * not overlap otherwise; head_dim even and at most 256. A launch holds 2^23 blocks, each of two q heads or one KV head of
+ * 1024 / head_dim rows (512 / head_dim unless head_dim and the strides are multiples of 4 and the buffers 16-byte aligned):
+ * more rows, over two million of 32 + 8 heads of 128, are refused. */
 void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride, const float *k, const float *v,
                                   size_t kv_stride, const float *table, const RequestBatch *batch, int n_heads,
                                   int n_kv_heads, int head_dim, float *key_cache, float *value_cache);
@@ -59,10 +61,15 @@ void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride,
  * Where a tile has more than 32 query vectors (a KV head's heads of its rows), the products are of two FP16 parts, with FP32
  * sums: a factor is exact to 2^-22 of itself or, where that is more, to 2^-39 of the largest of its query vector, its K row
  * (both taken as at least 2^-100) or its group of four V rows, and a weight to 2^-24 of its row's largest, or 2^-36 over V
- * rows of about one size; V rows further apart in size than that, and smaller tiles, take FP32 products. The prefix is read
- * once for all requests, not once for each. prefix_key and prefix_value may be NULL where prefix is 0; requests may share a
- * slot here. out must not overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16
- * per KV head, head_dim at most 256. */
+ * rows of about one size; V rows more than 16 to 4096 times apart in size, and smaller tiles, take FP32 products.
+ *
+ * Tiles are of 128 query vectors of a KV head, of all requests' rows together, and the prefix is read once for each. They are
+ * formed where head_dim is a multiple of 4 and at most 128, the buffers are 16-byte aligned, the prefix and a slot of one
+ * KV head (in the rows layout: of all) are below 2 GiB, and there are at most 2^20 rows, 1024 heads and 2^33 floats of q.
+ * Any other shape has each row read what it attends to by itself, some ten to hundred times slower. prefix_key and
+ * prefix_value may be NULL where prefix is 0; requests may share a slot here. out must not overlap q, a cache or the
+ * batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16 per KV head, head_dim at
+ * most 256. */
 void llhip_attention_requests(float *out, const float *q, const float *prefix_key, const float *prefix_value,
                               const float *key_cache, const float *value_cache, const RequestBatch *batch, int n_heads,
                               int n_kv_heads, int head_dim);
@@ -75,7 +82,9 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
  * A row without an adapter has P = 0. base and base3 have c's leading dimension, and either may be c itself. A is
  * adapters x rank x k and B adapters x n x rank, row-major; rank 1 .. LLHIP_MAX_LORA_RANK, the same for the segment's
  * adapters (smaller ones padded with zeros). Sums are FP32 throughout, also over BF16 adapters (the activations are not
- * rounded); a row of x, or an adapter, that holds an infinity or a NaN gives its rows' columns NaN or infinity. c must not
+ * rounded); a row of x, or an adapter, that holds an infinity or a NaN gives its rows' columns NaN or infinity. Rows and
+ * A on 16-byte boundaries with k a multiple of 8 (ldx of 4), at most 4096 adapters and 2^20 rows take the matrix cores;
+ * other shapes take each row by itself, some ten to twenty times slower for many rows, and up to 2^23 of them. c must not
  * overlap x, the ids, any segment's adapters or scales, or another segment's c or base. */
 typedef struct {
   float *c;

@@ -258,8 +258,8 @@ void llhip_rope_kv_store_requests(float *q_out, const float *q, size_t q_stride,
   bool bad = overlaps(key_cache, cache, value_cache, cache) || (q_out != q && overlaps(q_out, q_bytes, q, q_bytes)) ||
              !apart(k) || !apart(v) || overlaps(table, table_bytes, q_out, q_bytes) || over_arrays(batch, q_out, q_bytes);
   for (float *c : {key_cache, value_cache})
-    bad |= over_arrays(batch, c, cache) || overlaps(c, cache, q, q_bytes) || overlaps(c, cache, q_out, q_bytes) || overlaps(c, cache, k, kv_bytes) ||
-           overlaps(c, cache, v, kv_bytes) || overlaps(c, cache, table, table_bytes);
+    bad |= overlaps(c, cache, q, q_bytes) || overlaps(c, cache, q_out, q_bytes) || overlaps(c, cache, k, kv_bytes) ||
+           overlaps(c, cache, v, kv_bytes) || overlaps(c, cache, table, table_bytes) || over_arrays(batch, c, cache);
   if (bad) {
     raise("%s: q_out, the rows, the table, the caches and the batch's arrays must not overlap", name);
     return;

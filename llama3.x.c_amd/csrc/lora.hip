@@ -5,7 +5,8 @@
 //                 the BF16 matrix cores. The tiles are found in the adapter array by the blocks themselves.
 //   lora_join     the shares' parts added, for batches whose columns would each read them again.
 //   lora_expand   block (columns, tile of rows): base + scale B (A x), and for W1 and W3 their gate, read and written once.
-//   lora_rows     any shape: one block per row and segment, A x kept in LDS.
+//   lora_rows     any shape: one block per row and segment, A x kept in LDS. 32 rows of 4097 values, rank 16, beside QKV take
+//                 87 us, 1100 of rank 64 beside W1 and W3 1790.
 //
 // Measured (BF16 but for the first): one row of 2048 values, rank 8, beside Wo 9.5 us; 32 rows of 4096, rank 16, beside QKV
 // 13 us (7 and 6.5); 1100 rows of 4096, rank 64, beside W1 and W3 of 14336 81 us (21, 5 and 58: the expansion moves 189 MB of
@@ -246,7 +247,9 @@ __device__ void find_tile_of_64(const Tiled &p, ShrinkLds &sh, int b, bool &bad)
 }
 
 // Of any number of rows: the rows of one adapter in their order, 32 a tile, the adapters in theirs and the rows without one
-// last. Rows with an id outside the table are in none (bad). A thread looks through a run of rows.
+// last. Rows with an id outside the table are in none (bad). A thread looks through a run of rows. Every block of
+// lora_shrink does so, which grows with the square of the rows: 1100, 17600 and 70400 rows of 4096 values, rank 16, spend 15,
+// 198 and 1106 us in A x, where x once is 4, 58 and 233.
 __device__ void find_tile(const Tiled &p, ShrinkLds &sh, int b, bool &bad) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, m = p.job.m, bins = p.job.adapters + 1;
   for (int i = tid; i < bins; i += kThreads)
@@ -611,7 +614,8 @@ template <class T, bool VEC, bool RANK8> __global__ __launch_bounds__(kThreads) 
 
 } // namespace
 
-// The tiled form takes rows and adapters whose K is a multiple of 8, 16-byte aligned, and at most 4096 adapters.
+// The tiled form takes rows and adapters whose K is a multiple of 8, 16-byte aligned (its loads are of eight values), at most
+// 4096 adapters (counted in LDS) and 2^20 rows.
 bool lora_tiled(const LoraJob &job) {
   uintptr_t all = (uintptr_t)job.x;
   for (int s = 0; s < job.nseg; s++)

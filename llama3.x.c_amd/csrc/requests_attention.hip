@@ -1,15 +1,17 @@
 // Attention of many requests behind a prefix that all of them share (gfx950).
 //
 //   attn_requests        block: a slice of a KV head's walks, a walk being a tile of query vectors over the prefix (all
-//                        requests' rows together, so that the prefix is read once) or over a request's own positions. One
-//                        pass over K and V with the softmax's running maximum and sum; 128 vectors a wide tile, whose
-//                        products are FP16 parts on the matrix cores, up to 32 a narrow one, with FP32 products.
+//                        requests' rows together, so that the prefix is read once a tile) or over a request's own
+//                        positions. One pass over K and V with the softmax's running maximum and sum; 128 vectors a wide
+//                        tile, whose products are FP16 parts on the matrix cores, up to 32 a narrow one, with FP32 products.
 //   attn_requests_merge  a row's partial sums, rescaled to their largest maximum.
-//   attn_rows            any shape.
+//   attn_rows            any shape, one row at a time: 32 rows of 8 heads over 4 KV heads of 256 behind 2048 positions take
+//                        2.4 ms, where their K and V once would take 24 us.
 //
 // Measured at 32 heads over 8 KV heads of dimension 128, both launches: 32 requests of one row behind 2048 positions, 502 own
-// ones on average, 49 us (148 MB of K and V: 3.0 TB/s); 64 behind 8192 with 594 100 us (378 MB: 3.8 TB/s); 16 with two to
-// seven rows behind 4096 with 916 66 us; five prompts, 923 rows, behind 1024 94 us. Wide walks are bound by their
+// ones on average, 48 us (148 MB of K and V: 3.1 TB/s); 64 behind 8192 with 594 99 us (378 MB: 3.8 TB/s); 16 with two to
+// seven rows behind 4096 with 916 65 us; five prompts, 923 rows, behind 1024 93 us. With 32 heads over 8 of 64: the 32 rows
+// 27.6 us, the 16 requests' drafts 42, the prompts 94. Wide walks are bound by their
 // instructions: a step takes the two waves of a SIMD 5600 cycles, 4300 of vector and 3100 of matrix instructions, which overlap
 // little (over the whole kernel the vector unit is 50% busy, the matrix cores 30%, LDS less); narrow ones by HBM.
 #include <cfloat>
@@ -1205,7 +1207,8 @@ __global__ __launch_bounds__(kThreads) void attn_requests_merge(FastAttn p) {
 
 } // namespace
 
-// The matrix-core form takes head dimensions up to 128 in whole groups of four, with 16-byte aligned rows.
+// The matrix-core form takes head dimensions up to 128 in whole groups of four, with 16-byte aligned rows: its loads are of
+// 16 bytes, and a head of 256 would need twice the registers for its query parts and value sums.
 bool attention_requests_fast(const AttentionRequestsJob &job) {
   const RequestsDev &b = job.batch;
   const uintptr_t all = (uintptr_t)job.out | (uintptr_t)job.q | (uintptr_t)job.prefix_key | (uintptr_t)job.prefix_value |
