@@ -131,6 +131,19 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
                          size_t draft_ld, const int *tokens, const float *uniform, const int *start, int count, int rows,
                          int vocab, float temperature);
 
+/* What rows of logits say of given tokens: row i's logits (vocab floats at logits + i * ld) at temperature T > 0, with z =
+ * (l - max l) / T and S the sum of exp z. logprob[i] = z - log S of tokens[i]; entropy[i] = log S - sum(z exp z) / S, where
+ * entropy is given; top_token[i * top ..] and top_logprob[i * top ..] the `top` (0 .. LLHIP_MAX_TOP) likeliest tokens and
+ * their log probabilities, the likeliest first, of equal logits the lower token first. Logits of -infinity are tokens masked
+ * out: their log probability is -infinity, and where fewer than `top` are left, the places behind them hold token -1 and
+ * -infinity. tokens[i] of -1 stands for none (the last row of a prompt): its logprob is 0. tokens NULL with logprob NULL
+ * leaves the log probabilities out. A row with a NaN, +infinity or no token left gets NaN in all places and tokens -1, and a
+ * token outside the vocabulary NaN; both fail at the next host-visible point. Exponentials are FP32, a row's sums of them
+ * FP64 over parts of 16 tokens. The outputs must not overlap each other or an input. At most 2^20 rows and 2^22 tokens. */
+enum { LLHIP_MAX_TOP = 32 };
+void llhip_token_logprobs(float *logprob, float *entropy, int *top_token, float *top_logprob, int top,
+                          const float *logits, size_t ld, const int *tokens, int rows, int vocab, float temperature);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,20 +2,60 @@
 // as for the other calls, one stream-ordered operation per call.
 #include <cmath>
 #include <cstring>
-#include <mutex>
 
 #include "common.h"
 #include "llama_hip_requests.h"
 
 using namespace llhip;
 
+namespace llhip {
+
+// The scratch of these calls and of those over pages, which the library stream orders: grown on demand (never during
+// graph capture), kept for the
+// process. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows. A call
+// holds the lock until its kernels are queued, so that another thread's do not come between them.
+std::mutex scratch_mutex;
+namespace {
+void *scratch_memory = nullptr;
+size_t scratch_bytes = 0;
+bool scratch_captured = false;
+} // namespace
+
+bool scratch_room(const char *name, size_t bytes, void **out) {
+  Device &dev = device();
+  if (bytes > scratch_bytes) {
+    if (dev.capturing)
+      return raise("%s needs %zu bytes of workspace during graph capture; run the call once before capturing", name, bytes);
+    if (scratch_memory && !scratch_captured) {
+      (void)hipStreamSynchronize(dev.stream);
+      (void)hipFree(scratch_memory);
+      hbm_release(scratch_bytes);
+    }
+    scratch_memory = nullptr;
+    scratch_bytes = 0;
+    scratch_captured = false;
+    const size_t want = bytes + bytes / 4 + 4096;
+    if (!hbm_claim(want, "the request workspace"))
+      return false;
+    if (hipMalloc(&scratch_memory, want) != hipSuccess) {
+      (void)hipGetLastError();
+      hbm_release(want);
+      scratch_memory = nullptr;
+      return raise("%s: allocating %zu bytes of workspace failed", name, want);
+    }
+    scratch_bytes = want;
+  }
+  if (dev.capturing)
+    scratch_captured = true;
+  *out = scratch_memory;
+  return true;
+}
+
+} // namespace llhip
+
 namespace {
 
 constexpr size_t kFloat = sizeof(float);
-
-bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
-  return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
-}
 
 // The batch's own numbers: what the host can know of it (the arrays are checked on the device).
 bool batch_ok(const char *name, const RequestBatch *b) {
@@ -66,44 +106,6 @@ bool over_arrays(const RequestBatch *b, const void *out, size_t bytes) {
 
 size_t caches_bytes(const RequestBatch *b, int n_kv_heads, int head_dim) {
   return (size_t)b->slots * b->seq_len * n_kv_heads * head_dim * kFloat;
-}
-
-// The scratch of these calls, which the library stream orders: grown on demand (never during graph capture), kept for the
-// process. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows. A call
-// holds the lock until its kernels are queued, so that another thread's do not come between them.
-std::mutex scratch_mutex;
-void *scratch_memory = nullptr;
-size_t scratch_bytes = 0;
-bool scratch_captured = false;
-
-bool workspace(const char *name, size_t bytes, void **out) {
-  Device &dev = device();
-  if (bytes > scratch_bytes) {
-    if (dev.capturing)
-      return raise("%s needs %zu bytes of workspace during graph capture; run the call once before capturing", name, bytes);
-    if (scratch_memory && !scratch_captured) {
-      (void)hipStreamSynchronize(dev.stream);
-      (void)hipFree(scratch_memory);
-      hbm_release(scratch_bytes);
-    }
-    scratch_memory = nullptr;
-    scratch_bytes = 0;
-    scratch_captured = false;
-    const size_t want = bytes + bytes / 4 + 4096;
-    if (!hbm_claim(want, "the request workspace"))
-      return false;
-    if (hipMalloc(&scratch_memory, want) != hipSuccess) {
-      (void)hipGetLastError();
-      hbm_release(want);
-      scratch_memory = nullptr;
-      return raise("%s: allocating %zu bytes of workspace failed", name, want);
-    }
-    scratch_bytes = want;
-  }
-  if (dev.capturing)
-    scratch_captured = true;
-  *out = scratch_memory;
-  return true;
 }
 
 // One adapter call, F32 or BF16: the segment types differ in their adapters' element only.
@@ -210,7 +212,7 @@ void lora(const char *name, const float *x, int ldx, int m, int k, const int *ad
   }
   std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
-  if (!workspace(name, lora_workspace(job), &scratch))
+  if (!scratch_room(name, lora_workspace(job), &scratch))
     return;
   if (!launch_lora(job, scratch, call.stream()))
     return;
@@ -328,7 +330,7 @@ void llhip_attention_requests(float *out, const float *q, const float *prefix_ke
                            n_kv_heads, head_dim};
   std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
-  if (!workspace(name, attention_requests_workspace(job), &scratch))
+  if (!scratch_room(name, attention_requests_workspace(job), &scratch))
     return;
   if (!launch_attention_requests(job, scratch, call.stream()))
     return;
@@ -408,9 +410,71 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
                       temperature};
   std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
-  if (!workspace(name, verify_workspace(job), &scratch))
+  if (!scratch_room(name, verify_workspace(job), &scratch))
     return;
   if (!launch_verify(job, scratch, call.stream()))
+    return;
+  lock.unlock();
+  call.finish();
+}
+
+void llhip_token_logprobs(float *logprob, float *entropy, int *top_token, float *top_logprob, int top,
+                          const float *logits, size_t ld, const int *tokens, int rows, int vocab, float temperature) {
+  const char *name = "llhip_token_logprobs";
+  if (rows <= 0)
+    return;
+  if (!(temperature > 0.0f) || !std::isfinite(temperature)) {
+    raise("%s: temperature %g must be finite and positive", name, (double)temperature);
+    return;
+  }
+  if (top < 0 || top > LLHIP_MAX_TOP) {
+    raise("%s: %d alternatives, 0 to %d are given", name, top, (int)LLHIP_MAX_TOP);
+    return;
+  }
+  if (vocab <= 0 || ld < (size_t)vocab) {
+    raise("%s: rows of %d logits at a stride of %zu", name, vocab, ld);
+    return;
+  }
+  if (!verify_shape_ok(rows, vocab)) {
+    raise("%s: %d rows of %d tokens, at most 2^20 rows of 2^22 tokens are taken", name, rows, vocab);
+    return;
+  }
+  if (!logits || !tokens != !logprob || (top > 0 && (!top_token || !top_logprob))) {
+    raise("%s: null buffer", name);
+    return;
+  }
+  const size_t n = (size_t)rows * kFloat, most = n * (size_t)top, logits_bytes = ((size_t)(rows - 1) * ld + vocab) * kFloat;
+  const struct {
+    const void *p;
+    size_t bytes;
+  } out[4] = {{logprob, n}, {entropy, n}, {top ? top_token : nullptr, most}, {top ? top_logprob : nullptr, most}};
+  for (int i = 0; i < 4; i++) {
+    bool bad = overlaps(out[i].p, out[i].bytes, logits, logits_bytes) ||
+               overlaps(out[i].p, out[i].bytes, tokens, (size_t)rows * sizeof(int));
+    for (int j = 0; j < i; j++)
+      bad |= overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes);
+    if (bad) {
+      raise("%s: the outputs must not overlap each other or an input", name);
+      return;
+    }
+  }
+  if (!logprob && !entropy && !top)
+    return; // nothing is asked for
+  Call call(name);
+  Ref P = logprob ? call.out(logprob, n, false) : Ref{}, E = entropy ? call.out(entropy, n, false) : Ref{};
+  Ref T = top ? call.out(top_token, most, false) : Ref{}, A = top ? call.out(top_logprob, most, false) : Ref{};
+  Ref L = call.in2d(logits, (size_t)vocab * kFloat, ld * kFloat, (size_t)rows);
+  Ref I = tokens ? call.in(tokens, (size_t)rows * sizeof(int)) : Ref{};
+  if (!call.ready())
+    return;
+  const ScoreJob job{logprob ? call.ptr<float>(P) : nullptr, entropy ? call.ptr<float>(E) : nullptr,
+                     top ? call.ptr<int>(T) : nullptr, top ? call.ptr<float>(A) : nullptr, top,
+                     call.ptr<const float>(L), ld, tokens ? call.ptr<const int>(I) : nullptr, rows, vocab, temperature};
+  std::unique_lock<std::mutex> lock(scratch_mutex);
+  void *scratch = nullptr;
+  if (!scratch_room(name, scores_workspace(job), &scratch))
+    return;
+  if (!launch_scores(job, scratch, call.stream()))
     return;
   lock.unlock();
   call.finish();

@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 #include "llama_hip.h"
 
@@ -26,7 +27,9 @@ struct Device {
   int *error_flags = nullptr; // device: [0] non-finite activation seen by a quantizer, [1] non-finite attention score,
                               // [2] an embedding row id outside the table, [3] a request batch outside its buffers,
                               // [4] two requests of a store in one slot, [5] an adapter id outside its table,
-                              // [6] undecidable logits or [7] a draft outside the vocabulary in a verification
+                              // [6] undecidable logits or [7] a draft outside the vocabulary in a verification,
+                              // [8] a page outside the caches, [9] two requests of an append in one page, [10] undecidable
+                              // logits or [11] a token outside the vocabulary in a scoring
   int *host_flags = nullptr;  // pinned host copy of the 16 flag words, read back with the synchronization
   int cu_count = 0;
   bool capturing = false;
@@ -319,6 +322,58 @@ struct VerifyJob {
 bool verify_shape_ok(int rows, int vocab);
 size_t verify_workspace(const VerifyJob &job); // bytes of scratch the launch takes
 bool launch_verify(const VerifyJob &job, void *workspace, hipStream_t stream);
+
+struct ScoreJob {
+  float *logprob, *entropy; // logprob null: no tokens; entropy may be null
+  int *top_token;
+  float *top_logprob;
+  int top;
+  const float *logits;
+  size_t ld;
+  const int *tokens;
+  int rows, vocab;
+  float temperature;
+};
+size_t scores_workspace(const ScoreJob &job); // bytes of scratch the launch takes
+bool launch_scores(const ScoreJob &job, void *workspace, hipStream_t stream);
+
+// ---- a cache in pages (paged.hip, paged_attention.hip) --------------------------------------------------------------
+// PagedBatch with device addresses, and the strides within a page: place t of KV head g at + t * pos_stride + g *
+// head_base values, pages page_values apart.
+struct PagedDev {
+  const int *start, *length, *pages;
+  int count, rows, max_pages, page_size, num_pages, seq_len;
+  bool bf16;
+  size_t pos_stride, head_base, page_values;
+};
+struct AppendPagedJob {
+  float *q_out;
+  const float *q, *k, *v, *table, *q_norm, *k_norm; // norms null: none
+  size_t q_out_stride, q_stride, kv_stride;
+  float epsilon;
+  PagedDev batch;
+  int n_heads, n_kv_heads, head_dim;
+  void *key, *value;
+};
+bool launch_append_paged(const AppendPagedJob &job, hipStream_t stream);
+struct AttentionPagedJob {
+  float *out;
+  const float *q;
+  size_t q_stride;
+  const void *key, *value;
+  PagedDev batch;
+  int n_heads, n_kv_heads, head_dim;
+};
+size_t attention_paged_workspace(const AttentionPagedJob &job); // bytes of scratch the launch takes
+bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipStream_t stream);
+
+// The scratch of the calls for many requests (abi_requests.cpp): `bytes` of it, false after raise. A call holds the mutex
+// from here until its kernels are queued.
+extern std::mutex scratch_mutex;
+bool scratch_room(const char *name, size_t bytes, void **out);
+inline bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
 
 struct GemmSegmentDev {
   float *c;

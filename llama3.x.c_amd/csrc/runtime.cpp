@@ -175,7 +175,11 @@ bool report_flags(const int *flags) {
                                           "two requests of one call store into the same slot",
                                           "adapter id outside the table",
                                           "logits of a verified row leave no token (a NaN, an infinity or all masked)",
-                                          "drafted token outside the vocabulary"};
+                                          "drafted token outside the vocabulary",
+                                          "a page of a request lies outside the caches",
+                                          "two requests of one call append to the same page",
+                                          "logits of a scored row leave no token (a NaN, an infinity or all masked)",
+                                          "scored token outside the vocabulary"};
   for (size_t i = 0; i < sizeof(kMessages) / sizeof(kMessages[0]); i++)
     if (flags[i]) {
       int zero[16] = {0};

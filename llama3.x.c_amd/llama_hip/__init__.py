@@ -32,7 +32,9 @@ Q8_GEMM_PORTABLE, Q8_GEMM_AVX512, Q8_GEMM_AMX, Q8_GEMM_HIP_MFMA = 0, 1, 2, 3
 # include/llama_hip.h
 LLHIP_FAIL_EXIT, LLHIP_FAIL_RECORD = 0, 1
 # include/llama_hip_requests.h
-LLHIP_MAX_REQUESTS, LLHIP_MAX_LORA_RANK = 1024, 256
+LLHIP_MAX_REQUESTS, LLHIP_MAX_LORA_RANK, LLHIP_MAX_TOP = 1024, 256, 32
+# include/llama_hip_paged.h
+PAGE_F32, PAGE_BF16 = 0, 1
 LOGITS_NONE, LOGITS_LAST, LOGITS_ALL = 0, 1, 2
 
 
@@ -129,6 +131,11 @@ class LoraBf16Segment(ctypes.Structure):  # a, b, a3, b3: BF16 bits
     _fields_ = LoraSegment._fields_
 
 
+class PagedBatch(ctypes.Structure):  # include/llama_hip_paged.h
+    _fields_ = [("start", P), ("length", P), ("pages", P)] + \
+               [(f, I32) for f in ("count", "rows", "max_pages", "page_size", "num_pages", "seq_len", "type")]
+
+
 _SIGNATURES = {
     # many requests on one model (llama_hip_requests.h)
     "llhip_rope_kv_store_requests": (None, [P, P, SZ, P, P, SZ, P, ctypes.POINTER(RequestBatch), I32, I32, I32, P, P]),
@@ -136,6 +143,11 @@ _SIGNATURES = {
     "llhip_lora_f32": (None, [P, I32, I32, I32, P, I32, ctypes.POINTER(LoraSegment), I32]),
     "llhip_lora_bf16": (None, [P, I32, I32, I32, P, I32, ctypes.POINTER(LoraBf16Segment), I32]),
     "llhip_verify_drafts": (None, [P, P, P, SZ, P, SZ, P, P, P, I32, I32, I32, ctypes.c_float]),
+    "llhip_token_logprobs": (None, [P, P, P, P, I32, P, SZ, P, I32, I32, ctypes.c_float]),
+    # a cache in pages (llama_hip_paged.h)
+    "llhip_rope_kv_append_paged": (None, [P, SZ, P, SZ, P, P, SZ, P, P, P, ctypes.c_float, ctypes.POINTER(PagedBatch), I32,
+                                          I32, I32, P, P]),
+    "llhip_attention_paged": (None, [P, P, SZ, P, P, ctypes.POINTER(PagedBatch), I32, I32, I32]),
     # the forward around the matmuls (llama_hip_forward.h)
     "k_rmsnorm": (None, [P, P, P, I32, ctypes.c_float]),
     "k_rmsnorm_rows": (None, [P, P, P, I32, I32, ctypes.c_float]),

@@ -1,0 +1,202 @@
+"""Log probabilities of given tokens, entropies and the likeliest tokens, on the GPU, against float64 (tests/paged_util.py)."""
+import numpy as np
+import pytest
+
+import llama_hip as lh
+from tests import hip_util as hu
+from tests import paged_util as pu
+from tests.requests_util import U
+
+pytestmark = pytest.mark.gpu
+F = np.float32
+
+
+@pytest.fixture
+def L():
+    lib = lh.load()
+    assert lib.llhip_init() == 0, lh.last_error()
+    lh.record_failures()
+    yield lib
+    lib.llhip_synchronize()
+    lib.llhip_clear_error()
+    lib.llhip_set_fail_mode(lh.LLHIP_FAIL_EXIT)
+
+
+def call(L, logits, tokens, temperature=1.0, top=0, entropy=True, ld=None, dev=hu.dev):
+    rows, vocab = logits.shape
+    wide = logits
+    if ld:
+        wide = np.full((rows, ld), np.nan, F)
+        wide[:, :vocab] = logits
+    ld = ld or vocab
+    ins = [dev(wide), None if tokens is None else dev(np.asarray(tokens, np.int32))]
+    outs = [None if tokens is None else dev(np.full(rows, 7.0, F)), dev(np.full(rows, 7.0, F)) if entropy else None,
+            dev(np.full((rows, top), 7, np.int32)) if top else None, dev(np.full((rows, top), 7.0, F)) if top else None]
+    L.llhip_token_logprobs(*[lh.ptr(x) for x in outs], top, lh.ptr(ins[0]), ld, lh.ptr(ins[1]), rows, vocab, temperature)
+    return [None if x is None else x if isinstance(x, np.ndarray) else hu.host(x) for x in outs]
+
+
+def check(L, logits, tokens, temperature=1.0, top=0, **kw):
+    """The bound: with z = (l - max) / T, an exponential is off by (|z| + 4) 2 U of itself (the difference's rounding, the
+    scale's and the exponential's), so the rest of the sum, r = S - 1, by E = U sum over the others of e^z (2 |z| + 8) + 20 U r
+    (16 values a lane, the lanes) and log1p(r) by E / (1 + r) at most; a log probability by that and its own rounding. The
+    entropy log S + sum(-z e^z) / S: its second sum by U sum e^z |z| (2 |z| + 30), both relative to S, and by its own rounding."""
+    got = call(L, logits, tokens, temperature, top, **kw)
+    L.llhip_synchronize()
+    assert not lh.last_error(), lh.last_error()
+    logprob, entropy, tops, top_logprob = pu.scores(logits, tokens, temperature, top)
+    z = logits.astype(np.float64) / float(F(temperature))
+    z = z - z.max(1, keepdims=True)
+    e = np.exp(z)
+    size = np.where(e > 0, -z, 0.0)
+    other = np.where(z < 0, e, 0.0)
+    whole = e.sum(1)
+    off = U * ((other * (2 * size + 8)).sum(1) + 20 * other.sum(1)) / whole
+    if tokens is not None:
+        want = logprob
+        fine = np.isfinite(want)
+        assert np.array_equal(got[0][~fine], want[~fine].astype(F))
+        assert (np.abs(got[0] - want)[fine] <= (off + U * np.abs(want))[fine] + 1e-38).all()
+    if got[1] is not None:
+        second = (e * size).sum(1) / whole
+        bound = off * (1 + second) + U * (e * size * (2 * size + 30)).sum(1) / whole + U * np.abs(entropy) + 1e-38
+        assert (np.abs(got[1] - entropy) <= bound).all(), np.abs(got[1] - entropy) / bound
+    if top:
+        assert np.array_equal(got[2], tops)
+        there = tops >= 0
+        assert (got[3][~there] == -np.inf).all()
+        with np.errstate(invalid="ignore"):
+            wrong = np.abs(got[3] - top_logprob)
+        assert (wrong[there] <= (off[:, None] + U * np.abs(top_logprob))[there] + 1e-38).all()
+    return got
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 63, 64, 65, 300, 1023, 1024, 1025, 5000, 32000, 128256])
+@pytest.mark.parametrize("top", [0, 1, 5, 20, 32])
+@pytest.mark.parametrize("temperature", [1.0, 0.3])
+def test_scores(L, vocab, top, temperature):
+    rng = np.random.default_rng(vocab + top)
+    rows = 5
+    logits = (3.0 * rng.standard_normal((rows, vocab))).astype(F)
+    tokens = rng.integers(0, vocab, rows)
+    tokens[1] = -1
+    tokens[2] = logits[2].argmax()
+    check(L, logits, tokens, temperature, top)
+    check(L, logits, None, temperature, top, ld=vocab + 3)
+    check(L, logits, tokens, temperature, top, entropy=False, ld=vocab + 4)
+
+
+@pytest.mark.parametrize("vocab", [70, 1024, 3000, 40000])
+def test_equal_logits_and_masked_ones(L, vocab):
+    """Rows of one value, of few values (ties go to the lower token), of zeros of both signs, with all but some tokens masked
+    out, and peaked rows."""
+    rng = np.random.default_rng(vocab)
+    logits = np.zeros((9, vocab), F)
+    logits[1] = rng.integers(0, 3, vocab)
+    logits[2] = rng.choice(np.array([0.0, -0.0], F), vocab)
+    logits[3] = -np.inf
+    logits[3, [5, vocab - 1]] = 2.0
+    logits[4] = np.where(rng.random(vocab) < 0.9, -np.inf, rng.standard_normal(vocab))
+    logits[4, 7] = 0.0
+    logits[5] = rng.standard_normal(vocab)
+    logits[5, 3] = 80.0
+    logits[6] = -1e30
+    logits[6, vocab // 2] = 1e30
+    logits[7] = np.linspace(9, -9, vocab)
+    logits[8] = np.linspace(-9, 9, vocab) * F(1e-3)
+    tokens = [vocab - 1, 3, 0, 6, 7, 3, vocab // 2, 0, vocab - 1]
+    for top in (0, 1, 7, 32):
+        got = check(L, logits, tokens, 1.0, top)
+        assert got[0][3] == -np.inf
+    check(L, logits, [5, 0, vocab - 1, 5, 7, 0, 0, 1, 2], 0.01, 32)
+
+
+def test_rows_that_decide_nothing(L):
+    """NaN, +infinity or nothing left: NaN in all places and tokens -1, a failure at the wait, and the rows beside them right."""
+    rng = np.random.default_rng(1)
+    for what in (np.nan, np.inf, None):
+        logits = rng.standard_normal((3, 2000)).astype(F)
+        if what is None:
+            logits[1] = -np.inf
+        else:
+            logits[1, 1500] = what
+        got = call(L, logits, [1, 2, 3], top=4)
+        L.llhip_synchronize()
+        assert "leave no token" in lh.last_error()
+        L.llhip_clear_error()
+        assert np.isnan(got[0][1]) and np.isnan(got[1][1]) and np.isnan(got[3][1]).all() and (got[2][1] == -1).all()
+        rest = [0, 2]
+        want = check(L, logits[rest], [1, 3], top=4)
+        for g, w in zip(got, want):
+            assert np.array_equal(g[rest], w)
+
+
+def test_tokens_outside_the_vocabulary(L):
+    rng = np.random.default_rng(2)
+    logits = rng.standard_normal((4, 100)).astype(F)
+    for bad in (100, -2, 2 ** 31 - 1, -2 ** 31):
+        got = call(L, logits, [5, bad, -1, 99])
+        L.llhip_synchronize()
+        assert "scored token outside the vocabulary" in lh.last_error()
+        L.llhip_clear_error()
+        assert np.isnan(got[0][1]) and got[0][2] == 0.0 and np.isfinite(got[0]).sum() == 3
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 1e-20, 1e-3, 100.0, 3e38])
+def test_temperatures(L, temperature):
+    """Very cold and very hot ones: finite entropies, alternatives in the same order."""
+    rng = np.random.default_rng(3)
+    logits = rng.standard_normal((3, 5000)).astype(F)
+    got = call(L, logits, logits.argmax(1), temperature, top=6)
+    L.llhip_synchronize()
+    assert not lh.last_error()
+    if 1e-30 < temperature:
+        check(L, logits, logits.argmax(1), temperature, top=6)
+    assert np.isfinite(got[1]).all() and (got[0] <= 0.0).all()
+    assert np.array_equal(got[2], np.argsort(-logits, 1, kind="stable")[:, :6])
+
+
+def test_large_vocabularies_and_many_rows(L):
+    rng = np.random.default_rng(4)
+    logits = rng.standard_normal((2, 1 << 22)).astype(F)
+    logits[1] = np.sort(logits[1])
+    check(L, logits, [0, (1 << 22) - 1], top=32)
+    logits = rng.standard_normal((33000, 70)).astype(F)
+    check(L, logits, rng.integers(0, 70, 33000), top=3)
+
+
+def test_host_buffers_and_graphs(L):
+    rng = np.random.default_rng(5)
+    logits = rng.standard_normal((6, 3000)).astype(F)
+    tokens = rng.integers(0, 3000, 6).astype(np.int32)
+    want = check(L, logits, tokens, top=5)
+    got = call(L, logits, tokens, top=5, dev=lambda x: x)
+    assert not lh.last_error()
+    for g, w in zip(got, want):
+        assert np.array_equal(g, w)
+    T = hu.torch()
+    ld, td = hu.dev(logits), hu.dev(tokens)
+    outs = [hu.dev(np.zeros(6, F)), hu.dev(np.zeros(6, F)), hu.dev(np.zeros((6, 5), np.int32)), hu.dev(np.zeros((6, 5), F))]
+    args = [lh.ptr(x) for x in outs] + [5, lh.ptr(ld), 3000, lh.ptr(td), 6, 3000, 0.7]
+    L.llhip_token_logprobs(*args)
+    L.llhip_synchronize()
+    assert L.llhip_graph_begin() == 0
+    L.llhip_token_logprobs(*args)
+    graph = L.llhip_graph_end()
+    assert graph, lh.last_error()
+    for _ in range(3):
+        logits = rng.standard_normal((6, 3000)).astype(F)
+        ld.copy_(T.from_numpy(logits))
+        td.copy_(T.from_numpy(rng.integers(0, 3000, 6).astype(np.int32)))
+        T.cuda.synchronize()
+        L.llhip_token_logprobs(*args)
+        L.llhip_synchronize()
+        eager = [hu.host(x).copy() for x in outs]
+        for x in outs:
+            x.zero_()
+        T.cuda.synchronize()
+        assert L.llhip_graph_launch(graph) == 0
+        L.llhip_synchronize()
+        for g, w in zip(outs, eager):
+            assert np.array_equal(hu.host(g), w)
+    L.llhip_graph_destroy(graph)
