@@ -1,11 +1,19 @@
 // Attention over a cache in pages (gfx950).
 //
+//   attn_paged        block: a slice of a KV head's walks, a walk being a tile of one request's query vectors over its
+//                     positions. One pass over K and V with the softmax's running maximum and sum, products on the matrix
+//                     cores; a walk that several blocks share is joined by the last of them to arrive.
 //   attn_paged_rows   any shape, one row and KV head a block.
 #include <cfloat>
 
 #include "paged_device.h"
 
 #include "lanes.h"
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 namespace llhip {
 namespace {
@@ -160,11 +168,669 @@ template <typename T> __global__ __launch_bounds__(kThreads) void attn_paged_row
   }
 }
 
-} // namespace
+// ---- the matrix-core form ---------------------------------------------------------------------------------------------
 
-size_t attention_paged_workspace(const AttentionPagedJob &) { return 0; }
+constexpr int kWaves = kThreads / kWave;
+constexpr int kStep = 32;              // positions that a wave takes at once
+constexpr int kRound = kWaves * kStep; // positions that a block takes at once in a tile of up to 16 vectors
+constexpr int kTileVectors = 64;       // query vectors of a tile
+constexpr int kMaxBlocksPerCu = 2;
+constexpr int kMaxArrivals = 4096;
+constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far below that its weight is zero, also where a
+                                     // lane has seen nothing else
 
-bool launch_attention_paged(const AttentionPagedJob &job, void *, hipStream_t stream) {
+// How many of a walk's blocks have stored their part, by the block that the walk begins in: zero between launches, as the
+// last to arrive sets it back.
+__device__ unsigned paged_arrivals[kMaxArrivals];
+
+struct FastPaged {
+  AttentionPagedJob job;
+  int kv_mul, blocks; // blocks: of a KV head
+  int tile_rows;      // rows of a full tile
+  float scale2;       // log2(e) / sqrt(hd)
+  // slots of HD + 4 floats, [KV head][block][0: a walk that an earlier block began, 1: one that this block begins][vector]
+  float *partial;
+  int *flags;
+  bool q_vec;   // q in whole 16-byte vectors
+  bool out_vec; // out likewise
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// The thread's number, new to the compiler at each walk: else it keeps what walks derive from it in registers all along.
+__device__ __forceinline__ int own_thread() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+// Nothing moves across: a phase's registers are free before the next one's are taken.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// The walks of a KV head lie one behind the other on a line, each as long as it takes in time, and the line is cut into
+// slices of one length, one for a block: all blocks start together and end together. A walk's begin and end take as long as
+// kBegin positions of a small tile.
+constexpr int kBegin = 256;
+// A slice is at least this long: shorter ones do not pay for a walk's join, and a block inside a walk has some of its
+// positions however they are rounded.
+constexpr int kMinSlice = kBegin + 2 * kRound;
+
+// Waves that walk a tile's positions together, a wave 16 vectors: four, two or one.
+__device__ __forceinline__ int walkers_of(int vectors) { return vectors <= 16 ? 4 : vectors <= 32 ? 2 : 1; }
+// How long a position takes: with fewer waves a tile, longer.
+__device__ __forceinline__ int position_time(int vectors) { return kWaves / walkers_of(vectors); }
+constexpr int kFullPosition = kWaves;
+
+// Where tile t of a request begins on the request's part of the line: t full tiles before it, tile i of length + (i + 1)
+// tile_rows positions.
+__device__ __forceinline__ long long tile_start(const FastPaged &p, int length, long long t) {
+  return t * kBegin + kFullPosition * (t * length + p.tile_rows * (t * (t + 1) / 2));
+}
+__device__ __forceinline__ long long request_time(const FastPaged &p, const PagedRequest &q) {
+  if (q.rows == 0)
+    return 0;
+  const int t = ceil_div(q.rows, p.tile_rows) - 1, rest = q.rows - t * p.tile_rows;
+  return tile_start(p, q.length, t) + kBegin + (long long)position_time(rest * p.kv_mul) * (q.length + q.rows);
+}
+
+struct Plan {
+  long long line[kMaxRequests]; // where request r's walks end
+  long long wave_sum[kWaves];
+};
+
+// x / y of the line's lengths (below 2^50, where the double quotient's whole part is exact), a third of the time that the
+// compiler's division takes.
+__device__ __forceinline__ long long whole(long long x, long long y) { return (long long)((double)x / (double)y); }
+
+// Fills the plan; returns the line's length.
+__device__ long long make_plan(const FastPaged &p, Plan &plan) {
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  constexpr int kPer = kMaxRequests / kThreads; // requests of a thread, at most
+  const PagedDev &b = p.job.batch;
+  const int per = ceil_div(b.count, kThreads), r0 = tid * per;
+  long long sum = 0, time[kPer];
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < kPer; k++) {
+    time[k] = 0;
+    if (k < per && r0 + k < b.count)
+      sum += time[k] = request_time(p, paged_request(b, r0 + k, bad));
+  }
+  if (bad && blockIdx.x == 0)
+    p.flags[3] = 1;
+  long long run = sum; // the threads' up to this one
+  for (int o = 1; o < kWave; o <<= 1) {
+    const long long v = __shfl_up(run, o);
+    if (lane >= o)
+      run += v;
+  }
+  if (lane == kWave - 1)
+    plan.wave_sum[wave] = run;
+  __syncthreads();
+  long long at = run - sum, total = 0;
+  for (int w = 0; w < kWaves; w++) {
+    if (w < wave)
+      at += plan.wave_sum[w];
+    total += plan.wave_sum[w];
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; k++)
+    if (k < per && r0 + k < b.count)
+      plan.line[r0 + k] = at += time[k];
+  __syncthreads();
+  return total;
+}
+
+// A block's part of a walk: query vectors (row row0 + v / kv_mul, head g kv_mul + v % kv_mul for v < vectors) over positions
+// t0 .. t1 - 1 of request r; row row0 + j sees positions up to last0 + j.
+struct Item {
+  int r, g, row0, vectors, last0;
+  int t0, t1;
+  int walkers;  // waves of 16 vectors
+  float *slots; // [vector][HD + 4], or null: the part is the whole, and goes to out
+};
+
+__device__ __forceinline__ float four_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+__device__ __forceinline__ float four_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+
+// x = a + b + c exactly, each of at most eight significant bits (truncated, so that nothing overflows): three BF16 values.
+// Two x give a dword of each part.
+__device__ __forceinline__ void bf16_parts(float x, float y, unsigned (&part)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const unsigned a = __float_as_uint(x), b = __float_as_uint(y);
+    part[i] = __builtin_amdgcn_perm(b, a, 0x07060302); // the upper halves
+    x -= __uint_as_float(a & 0xffff0000u);
+    y -= __uint_as_float(b & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ v4f mfma_bf16(const v4u &a, const v4u &b, v4f c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+
+// Where 16 positions' K or V rows lie (page_size a multiple of 16: in one page), as a buffer: a load past the rows that
+// belong to the walk reads zero, so that nothing of a page's rest, and no page behind the last, is touched.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void *cache, long long offset, int bytes) {
+  const uint64_t base = (uint64_t)(uintptr_t)cache + (uint64_t)offset;
+  return __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)base, (short)0, bytes, 0x00020000);
+}
+
+// The tile's walk: each wave has 16 of its vectors, and takes 32 positions in turn with the other waves that have the same.
+//
+// Lane (lq = lane / 16, lc = lane % 16). S^T = K Q^T and O^T = V^T P^T, so that a lane holds one vector's (lc) scores, weights
+// and sums, and no weight changes lanes: the scores of positions 16 t + 4 lq + e are in the lane that feeds positions 16 t + 4
+// lq + e to the second product, whose order of summation is free.
+//   BF16: 32 dimensions, or 32 positions, an instruction; a lane's V rows (8 positions, 8 dimensions each) are turned by byte
+//   permutes within the lane. Q and P as three exact parts each.
+//   F32: 4 dimensions, or 4 positions, an instruction; FP32 products.
+// Dimension of instruction e's row m: EV dimensions a lane, 16 lanes, further ones EV * 16 behind.
+// MODE: whole heads of HD dimensions, heads of fewer, or either with pages that are no multiple of 16 positions.
+enum { kWhole, kPart, kAny };
+template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p, const Item &it, float *lds) {
+  constexpr bool kBf16 = sizeof(T) == 2, ANY = MODE == kAny;
+  constexpr int E = HD / 16, EV = E < (kBf16 ? 8 : 4) ? E : (kBf16 ? 8 : 4), kVecs = E / EV; // a V row: kVecs loads of EV
+  constexpr int kSteps = kBf16 ? HD / 32 : HD / 16; // a K row: loads of 16 bytes
+  constexpr int kPerLoad = kBf16 ? 8 : 4;           // dimensions of one
+  constexpr int kRow = HD + 4;
+  constexpr unsigned kNowhere = 0x7ffffff0u; // an offset past every buffer
+  const PagedDev &b = p.job.batch;
+  const int tid = own_thread(), lane = tid & (kWave - 1), wave = uniform(tid / kWave), lq = lane >> 4, lc = lane & 15;
+  const int hd = MODE == kWhole ? HD : p.job.head_dim, kv_mul = p.kv_mul;
+  const int v0 = wave / it.walkers * 16;    // the wave's first vector
+  const int mine = min(it.vectors - v0, 16); // its vectors
+  const int first = it.t0 + wave % it.walkers * kStep, stride = it.walkers * kStep;
+  // positions that some of the wave's vectors see
+  const int end = mine > 0 ? min(it.t1, it.last0 + (v0 + mine - 1) / kv_mul + 1) : it.t0;
+  const int all_see = it.last0 + v0 / kv_mul + 1; // positions below are seen by all of them
+  const bool active = lc < mine;
+  const int last = active ? it.last0 + (v0 + lc) / kv_mul : -1; // the lane's vector's last position
+  v4f o[E];
+  float m_run = -FLT_MAX, l_run = 0.0f, odd = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    o[e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  const size_t head = (size_t)it.g * b.head_base;
+  // lane 2 i + t: where positions 16 t .. of the wave's step i (of 32 steps) lie, in bytes
+  long long places = 0;
+  auto look_up = [&](int pos) {
+    const int at = min(pos + lane / 2 * stride + 16 * (lane & 1), max(end - 1, 0));
+    const int number = at / b.page_size, page = page_of(b, it.r, number);
+    if (page < 0)
+      p.flags[8] = 1;
+    places = (long long)(((size_t)max(page, 0) * b.page_values + (size_t)((at - number * b.page_size) & ~15) * b.pos_stride +
+                          head) * sizeof(T));
+  };
+  auto place = [&](int i) {
+    const int lo = __builtin_amdgcn_readlane((int)places, i), hi = __builtin_amdgcn_readlane((int)(places >> 32), i);
+    return (long long)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+  };
+  // any page size: where position t lies, in values
+  auto place_any = [&](int t) {
+    const int at = min(t, max(end - 1, 0)), number = at / b.page_size, page = page_of(b, it.r, number);
+    if (page < 0)
+      p.flags[8] = 1;
+    return (size_t)max(page, 0) * b.page_values + (size_t)(at - number * b.page_size) * b.pos_stride + head;
+  };
+  const unsigned row_bytes = (unsigned)b.pos_stride * (unsigned)sizeof(T);
+  const unsigned k_row = (unsigned)lc * row_bytes, v_row = (unsigned)(4 * lq) * row_bytes;
+  auto k_off = [&](int s) {
+    const int d = (4 * s + lq) * kPerLoad;
+    return d < hd ? k_row + (unsigned)(d * sizeof(T)) : kNowhere;
+  };
+  auto v_off = [&](int e, int u) {
+    const int d = (u * 16 + lc) * EV;
+    return d < hd ? v_row + (unsigned)e * row_bytes + (unsigned)(d * sizeof(T)) : kNowhere;
+  };
+  v4u kr[2][kSteps];
+  unsigned vr[8][kVecs][EV * sizeof(T) / 4]; // positions 16 (j / 4) + 4 lq + j % 4
+  auto load_rows = [&](int pos, int i, auto take) { // both 16-row buffers of the step at pos, the wave's i-th since look_up
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const int rows = min(end - (pos + 16 * t), 16);
+      const int bytes = rows > 0 ? (int)((unsigned)(rows - 1) * row_bytes + (unsigned)(hd * sizeof(T))) : 0;
+      take(t, place(min(2 * i + t, kWave - 1)), bytes);
+    }
+  };
+  auto load_k = [&](int pos, int i) {
+    if constexpr (ANY) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const T *row = (const T *)p.job.key + place_any(pos + 16 * t + lc);
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+          const int d = (4 * s + lq) * kPerLoad;
+          kr[t][s] = *reinterpret_cast<const v4u *>(row + (d < hd ? d : 0)); // there Q is zero
+        }
+      }
+    } else {
+      load_rows(pos, i, [&](int t, long long offset, int bytes) {
+        const auto rsrc = rows_of(p.job.key, offset, bytes);
+#pragma unroll
+        for (int s = 0; s < kSteps; s++)
+          kr[t][s] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rsrc, k_off(s), 0, 0));
+      });
+    }
+  };
+  auto load_v = [&](int pos, int i) {
+    if constexpr (ANY) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int t = pos + 16 * (j / 4) + 4 * lq + j % 4;
+        const T *row = (const T *)p.job.value + place_any(t);
+#pragma unroll
+        for (int u = 0; u < kVecs; u++) {
+          const int d = (u * 16 + lc) * EV;
+          if constexpr (EV * sizeof(T) == 16) {
+            const v4u x = *reinterpret_cast<const v4u *>(row + (d < hd ? d : 0));
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+              vr[j][u][c] = t < end ? x[c] : 0u;
+          } else {
+            const v2u x = *reinterpret_cast<const v2u *>(row + (d < hd ? d : 0));
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+              vr[j][u][c] = t < end ? x[c] : 0u;
+          }
+        }
+      }
+    } else {
+      load_rows(pos, i, [&](int t, long long offset, int bytes) {
+        const auto rsrc = rows_of(p.job.value, offset, bytes);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int u = 0; u < kVecs; u++) {
+            if constexpr (EV * sizeof(T) == 16) {
+              const v4u x = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rsrc, v_off(e, u), 0, 0));
+#pragma unroll
+              for (int c = 0; c < 4; c++)
+                vr[4 * t + e][u][c] = x[c];
+            } else {
+              const v2u x = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(rsrc, v_off(e, u), 0, 0));
+#pragma unroll
+              for (int c = 0; c < 2; c++)
+                vr[4 * t + e][u][c] = x[c];
+            }
+          }
+      });
+    }
+  };
+  if constexpr (!ANY)
+    look_up(first);
+  // the query vectors, scaled, in the order in which K's dimensions come
+  constexpr int kParts = kBf16 ? 3 : 1;
+  v4u qp[kSteps][kParts];
+  {
+    const int v = active ? v0 + lc : 0;
+    const float *src = p.job.q + (size_t)(it.row0 + v / kv_mul) * p.job.q_stride + ((size_t)it.g * kv_mul + v % kv_mul) * hd;
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      const int d = (4 * s + lq) * kPerLoad;
+      const float *at = src + (d < hd ? d : 0);
+      float x[kPerLoad];
+      if (p.q_vec) {
+#pragma unroll
+        for (int c = 0; c < kPerLoad; c += 4) {
+          const float4 four = *reinterpret_cast<const float4 *>(at + c);
+          x[c] = four.x, x[c + 1] = four.y, x[c + 2] = four.z, x[c + 3] = four.w;
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kPerLoad; c++)
+          x[c] = at[c];
+      }
+#pragma unroll
+      for (int c = 0; c < kPerLoad; c++)
+        x[c] = active && d < hd ? x[c] * p.scale2 : 0.0f;
+      if constexpr (kBf16) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          unsigned part[3];
+          bf16_parts(x[2 * c], x[2 * c + 1], part);
+#pragma unroll
+          for (int k = 0; k < 3; k++)
+            qp[s][k][c] = part[k];
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          qp[s][0][c] = __float_as_uint(x[c]);
+      }
+    }
+  }
+  load_k(first, 0);
+  load_v(first, 0);
+  int i = 0; // the step's number since look_up
+  for (int pos = first; pos < end; pos += stride) {
+    v4f sc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      if constexpr (kBf16) {
+#pragma unroll
+        for (int k = 2; k >= 0; k--)
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            sc[t] = mfma_bf16(kr[t][s], qp[s][k], sc[t]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int t = 0; t < 2; t++)
+            sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[t][s][c]), __uint_as_float(qp[s][0][c]), sc[t],
+                                                         0, 0, 0);
+      }
+    }
+    fence();
+    if constexpr (!ANY)
+      if (++i == kWave / 2) { // uniform
+        look_up(pos + stride);
+        i = 0;
+      }
+    load_k(pos + stride, i);
+    fence();
+    // weights
+    float w[8], top = -FLT_MAX;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      w[j] = sc[j / 4][j % 4];
+    if (pos + kStep > all_see || pos + kStep > end || mine < 16) { // a lane without a vector sees nothing
+      const int seen = min(last, end - 1) - pos - 4 * lq;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        w[j] = 16 * (j / 4) + j % 4 <= seen ? w[j] : -FLT_MAX;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      odd = fmaf(w[j], 0.0f, odd);
+      top = fmaxf(top, w[j]);
+    }
+    // the maximum moves only where weights would pass 2^8: rare, and the sums keep their bits
+    if (__any(top > m_run + 8.0f)) {
+      const float m = fmaxf(m_run, four_max(top)), alpha = __builtin_amdgcn_exp2f(m_run - m);
+      l_run *= alpha;
+      m_run = m;
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        o[e] *= alpha;
+    }
+    const float base = fmaxf(m_run, kMasked);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      w[j] = __builtin_amdgcn_exp2f(w[j] - base);
+      l_run += w[j]; // this lane's positions; the four lanes of a vector meet at the end
+    }
+    // A V value that is not finite must reach the vectors that see its position alone, and 0 * infinity would carry it to
+    // those that do not: where some do not, the product takes 0 in its place, and it is added to those that do.
+    if (pos + kStep > all_see && all_see < end) {
+      bool met = false;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int u = 0; u < kVecs; u++)
+#pragma unroll
+          for (unsigned c = 0; c < EV * sizeof(T) / 4; c++) {
+            const unsigned x = vr[j][u][c];
+            if constexpr (kBf16) {
+              const bool lo = (x & 0x7f80u) == 0x7f80u, hi = (x & 0x7f800000u) == 0x7f800000u;
+              met |= lo | hi;
+              vr[j][u][c] = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
+            } else {
+              const bool bad = (x & 0x7f800000u) == 0x7f800000u;
+              met |= bad;
+              vr[j][u][c] = bad ? 0u : x;
+            }
+          }
+      if (__any(met)) {
+        for (int t = pos; t < min(pos + kStep, end); t++) {
+          const T *row = (const T *)p.job.value + place_any(t);
+          int lq4 = 4 * lq; // new to the compiler here: else it keeps what follows from it in registers all along the walk
+          asm volatile("" : "+v"(lq4));
+#pragma unroll
+          for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const int d = (e / EV * 16 + lq4 + r) * EV + e % EV;
+              const float x = value(row + (d < hd ? d : 0));
+              if (d < hd && !isfinite(x) && t <= last)
+                o[e][r] += x;
+            }
+        }
+      }
+    }
+    if constexpr (kBf16) {
+      v4u wp[3];
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        unsigned part[3];
+        bf16_parts(w[2 * c], w[2 * c + 1], part);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          wp[k][c] = part[k];
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        v4u vt;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          vt[c] = __builtin_amdgcn_perm(vr[2 * c + 1][e / EV][e % EV / 2], vr[2 * c][e / EV][e % EV / 2],
+                                        e % 2 ? 0x07060302 : 0x05040100);
+#pragma unroll
+        for (int k = 2; k >= 0; k--)
+          o[e] = mfma_bf16(vt, wp[k], o[e]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][e / EV][e % EV]), w[j], o[e], 0, 0, 0);
+    }
+    fence();
+    load_v(pos + stride, i);
+    fence();
+  }
+  if (odd != 0.0f)
+    p.flags[1] = 1;
+  // vector v's sums: to its slot, or divided by the weights' sum to out
+  auto target = [&](int v) {
+    return it.slots ? it.slots + (size_t)v * kRow
+                    : p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
+  };
+  auto store = [&](float *dst, int d, const float4 &x) { // dimensions d .. d + 3, below hd
+    if (it.slots || p.out_vec) {
+      *reinterpret_cast<float4 *>(dst + d) = x;
+    } else {
+      dst[d] = x.x, dst[d + 1] = x.y, dst[d + 2] = x.z, dst[d + 3] = x.w;
+    }
+  };
+  constexpr int kFours = E / 4; // a lane's r-th row: kFours groups of four dimensions
+  const float l = four_sum(l_run);
+  if (it.walkers > 1) { // the waves' sums meet in LDS: [wave][vector][HD values, maximum, sum]
+    float *dst = lds + (size_t)(wave * 16 + lc) * kRow;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int f = 0; f < kFours; f++) {
+        const int e = 4 * f, d = (e / EV * 16 + 4 * lq + r) * EV + e % EV;
+        *reinterpret_cast<float4 *>(dst + d) = float4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
+      }
+    if (lq == 0)
+      dst[HD] = m_run, dst[HD + 1] = l;
+    __syncthreads();
+    const int hd4 = hd / 4;
+    for (int i = tid; i < it.vectors * hd4; i += kThreads) {
+      const int v = i / hd4, d4 = i % hd4;
+      const float *src = lds + (size_t)(v / 16 * it.walkers * 16 + v % 16) * kRow;
+      float m = -FLT_MAX, whole_l = 0.0f;
+      for (int w = 0; w < it.walkers; w++)
+        m = fmaxf(m, src[(size_t)w * 16 * kRow + HD]);
+      float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int w = 0; w < it.walkers; w++) {
+        const float *at = src + (size_t)w * 16 * kRow;
+        const float scale = __builtin_amdgcn_exp2f(at[HD] - m);
+        const float4 x = *reinterpret_cast<const float4 *>(at + 4 * d4);
+        whole_l = fmaf(scale, at[HD + 1], whole_l);
+        sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
+      }
+      float *to = target(v);
+      if (it.slots) {
+        if (d4 == 0)
+          to[HD] = m, to[HD + 1] = whole_l;
+      } else {
+        sum = float4{sum.x / whole_l, sum.y / whole_l, sum.z / whole_l, sum.w / whole_l};
+      }
+      store(to, 4 * d4, sum);
+    }
+  } else if (active) {
+    float *to = target(v0 + lc);
+    if (it.slots && lq == 0)
+      to[HD] = m_run, to[HD + 1] = l;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int f = 0; f < kFours; f++) {
+        const int e = 4 * f, d = (e / EV * 16 + 4 * lq + r) * EV + e % EV;
+        float4 x = float4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
+        if (!it.slots)
+          x = float4{x.x / l, x.y / l, x.z / l, x.w / l};
+        if (d < hd)
+          store(to, d, x);
+      }
+  }
+}
+
+template <typename T, int HD, int MODE>
+__global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn_paged(FastPaged p) {
+  constexpr int kRow = HD + 4;
+  __shared__ Plan plan;
+  __shared__ __align__(16) float lds[kWaves * 16 * kRow];
+  __shared__ unsigned arrived;
+  const PagedDev &b = p.job.batch;
+  const int tid = threadIdx.x, g = blockIdx.x % p.job.n_kv_heads, block = blockIdx.x / p.job.n_kv_heads;
+  const int hd = p.job.head_dim, kv_mul = p.kv_mul;
+  const long long total = make_plan(p, plan);
+  const long long cut = whole(total + p.blocks - 1, p.blocks), slice = cut > kMinSlice ? cut : kMinSlice;
+  const long long lo = block * slice, hi = lo + slice < total ? lo + slice : total;
+  if (lo >= total)
+    return;
+  int r = 0; // the first request whose walks end behind lo
+  for (int step = kMaxRequests; step > 0; step >>= 1)
+    if (r + step <= b.count && plan.line[r + step - 1] <= lo)
+      r += step;
+  for (long long base = r ? plan.line[r - 1] : 0; r < b.count && base < hi; base = plan.line[r], r++) {
+    bool bad = false;
+    const PagedRequest q = paged_request(b, r, bad);
+    if (q.rows == 0)
+      continue;
+    const int tiles = ceil_div(q.rows, p.tile_rows);
+    int t = 0; // the last tile that begins at or before lo
+    if (base < lo)
+      for (int step = 1 << 20; step > 0; step >>= 1)
+        if (t + step < tiles && base + tile_start(p, q.length, t + step) <= lo)
+          t += step;
+    for (; t < tiles; t++) {
+      const long long w0 = base + tile_start(p, q.length, t);
+      if (w0 >= hi)
+        break;
+      const int row = t * p.tile_rows, rows = min(q.rows - row, p.tile_rows);
+      const int positions = q.length + row + rows;
+      Item it;
+      it.vectors = rows * kv_mul;
+      it.walkers = walkers_of(it.vectors);
+      const int unit = position_time(it.vectors), grain = it.walkers * kStep;
+      const long long end = w0 + kBegin + (long long)unit * positions;
+      // the position that lies at x of the line, in whole rounds
+      auto position_at = [&](long long x) {
+        if (x >= end)
+          return positions;
+        const int at = x <= w0 + kBegin ? 0 : (int)((x - w0 - kBegin) / unit);
+        return min(at / grain * grain, positions);
+      };
+      it.t0 = w0 >= lo ? 0 : position_at(lo);
+      it.t1 = position_at(hi);
+      if (it.t0 >= it.t1)
+        continue; // the rounds leave this block none of it
+      it.r = r, it.g = g;
+      it.row0 = q.first + row, it.last0 = q.length + row;
+      const bool shared = it.t0 > 0 || it.t1 < positions;
+      auto slots = [&](int blk, bool begins) {
+        return p.partial + (((size_t)g * p.blocks + blk) * 2 + begins) * kTileVectors * kRow;
+      };
+      it.slots = shared ? slots(block, w0 >= lo) : nullptr;
+      __syncthreads(); // LDS is free
+      walk<T, HD, MODE>(p, it, lds);
+      if (!shared)
+        continue;
+      // the walk's blocks: first .. last_block, the first of them perhaps without a part
+      const int first = (int)whole(w0, slice), last_block = (int)whole(end - 1, slice);
+      const bool first_has = position_at((first + 1) * slice) > 0;
+      const int from = first_has ? first : first + 1, parts = last_block - from + 1;
+      __syncthreads(); // the block's part is stored
+      if (tid == 0)
+        arrived = __hip_atomic_fetch_add(&paged_arrivals[g * p.blocks + first], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (arrived != (unsigned)(parts - 1))
+        continue;
+      __threadfence(); // the others' parts are seen
+      if (tid == 0)
+        __hip_atomic_store(&paged_arrivals[g * p.blocks + first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int hd4 = hd / 4;
+      for (int i = tid; i < it.vectors * hd4; i += kThreads) {
+        const int v = i / hd4, d4 = i % hd4;
+        float m = -FLT_MAX;
+        for (int k = from; k <= last_block; k++)
+          m = fmaxf(m, slots(k, k == first)[(size_t)v * kRow + HD]);
+        float l = 0.0f;
+        float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int k = from; k <= last_block; k++) { // in the blocks' order, whoever comes last
+          const float *src = slots(k, k == first) + (size_t)v * kRow;
+          const float scale = __builtin_amdgcn_exp2f(src[HD] - m);
+          const float4 x = *reinterpret_cast<const float4 *>(src + 4 * d4);
+          l = fmaf(scale, src[HD + 1], l);
+          sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
+        }
+        float *to = p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + v % kv_mul) * hd + 4 * d4;
+        const float4 x = float4{sum.x / l, sum.y / l, sum.z / l, sum.w / l};
+        if (p.out_vec)
+          *reinterpret_cast<float4 *>(to) = x;
+        else
+          to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+      }
+    }
+  }
+}
+
+int tile_dims(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+// The matrix-core form takes the job: K and V rows in whole 16-byte vectors, offsets within 16 rows of 32 bits, positions
+// within int arithmetic of the steps.
+bool tiled(const AttentionPagedJob &job) {
+  const size_t size = job.batch.bf16 ? 2 : 4;
+  return job.head_dim * size % 16 == 0 && (((uintptr_t)job.key | (uintptr_t)job.value) & 15) == 0 &&
+         job.batch.pos_stride * size * 16 < ((size_t)1 << 30) && job.batch.seq_len < (1 << 30) && job.n_kv_heads <= kMaxArrivals;
+}
+
+int blocks_of(const AttentionPagedJob &job) {
+  const int all = (job.head_dim > 128 ? 1 : kMaxBlocksPerCu) * device().cu_count, cap = kMaxArrivals / job.n_kv_heads;
+  const int n = all / job.n_kv_heads;
+  return n < 1 ? 1 : n < cap ? n : cap;
+}
+
+typedef void (*FastKernel)(FastPaged);
+template <typename T, int HD> FastKernel kernel_of(int mode) {
+  return mode == kWhole ? attn_paged<T, HD, kWhole> : mode == kPart ? attn_paged<T, HD, kPart> : attn_paged<T, HD, kAny>;
+}
+template <typename T> FastKernel kernel_of(int dims, int mode) {
+  return dims == 64 ? kernel_of<T, 64>(mode) : dims == 128 ? kernel_of<T, 128>(mode) : kernel_of<T, 256>(mode);
+}
+
+bool launch_rows(const AttentionPagedJob &job, hipStream_t stream) {
   const PagedAttn p{job, sqrtf((float)job.head_dim), device().error_flags};
   const int most = (1 << 23) / job.n_kv_heads; // a launch holds fewer than 2^32 threads
   for (int row0 = 0; row0 < job.batch.rows; row0 += most) {
@@ -175,6 +841,34 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *, hipStream_t st
       return false;
   }
   return true;
+}
+
+} // namespace
+
+size_t attention_paged_workspace(const AttentionPagedJob &job) {
+  if (!tiled(job))
+    return 0;
+  return (size_t)job.n_kv_heads * blocks_of(job) * 2 * kTileVectors * (tile_dims(job.head_dim) + 4) * sizeof(float);
+}
+
+bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipStream_t stream) {
+  if (!tiled(job))
+    return launch_rows(job, stream);
+  const int dims = tile_dims(job.head_dim);
+  FastPaged p{};
+  p.job = job;
+  p.kv_mul = job.n_heads / job.n_kv_heads;
+  p.blocks = blocks_of(job);
+  p.tile_rows = kTileVectors / p.kv_mul;
+  p.scale2 = (float)(1.4426950408889634 / sqrt((double)job.head_dim));
+  p.partial = (float *)workspace;
+  p.flags = device().error_flags;
+  p.q_vec = job.q_stride % 4 == 0 && ((uintptr_t)job.q & 15) == 0;
+  p.out_vec = ((uintptr_t)job.out & 15) == 0;
+  const int mode = job.batch.page_size % 16 ? kAny : job.head_dim == dims ? kWhole : kPart;
+  const FastKernel kernel = job.batch.bf16 ? kernel_of<uint16_t>(dims, mode) : kernel_of<float>(dims, mode);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(p.blocks * job.n_kv_heads)), dim3(kThreads), 0, stream, p);
+  return launch_ok("attn_paged");
 }
 
 } // namespace llhip

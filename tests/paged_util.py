@@ -81,7 +81,9 @@ def attention(b, q, key, value, heads, kv, hd, layout):
     A factor meets the pages' values whole or as three parts that are exact, so a score sums at most 3 hd products: its error
     is at most (3 hd + 8) U sum|q k| / sqrt(hd) (with the division and the scale to base 2); a weight's twice the largest of
     the row's, relative, with 8 U for the exponential and the rescales; the value sums' (3 positions + 64) U of sum p|v|,
-    every merge and the division included. A value of V below 2^-126 may count as 0."""
+    every merge and the division included. A weight is a float32 relative to one that is at least 1: below 2^-126, the
+    smallest normal number, the exponential (and the lower parts of a weight that is split) may be 0, so that each |v| adds up
+    to 2^-125 of itself: proof enough for values 10^40 apart, where such weights' terms decide a row's sum."""
     mul = heads // kv
     out = np.zeros((b.rows, heads, hd))
     bound = np.zeros_like(out)
@@ -98,7 +100,8 @@ def attention(b, q, key, value, heads, kv, hd, layout):
                 p = np.exp(s - s.max(1, keepdims=True))
                 p /= p.sum(1, keepdims=True)
                 out[i, g * mul:(g + 1) * mul] = p @ v
-                bound[i, g * mul:(g + 1) * mul] = (p @ np.abs(v)) * (2 * off[:, None] + (3 * n + 72) * U) + 2.0 ** -126
+                bound[i, g * mul:(g + 1) * mul] = ((p @ np.abs(v)) * (2 * off[:, None] + (3 * n + 72) * U) +
+                                                   np.abs(v).sum(0) * 2.0 ** -125 + 2.0 ** -126)
     return out.reshape(b.rows, -1), bound.reshape(b.rows, -1)
 
 
