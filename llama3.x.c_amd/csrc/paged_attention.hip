@@ -298,6 +298,19 @@ __device__ __forceinline__ float four_max(float x) {
   return fmaxf(x, __shfl_xor(x, 32));
 }
 
+// A part's sums go past the XCDs' own L2s: stores of agent scope write through, loads of agent scope read what they wrote. (A
+// release and an acquire around plain ones write back and drop a whole L2 a block: 32 requests took 134 us, not %DEC32%.)
+__device__ __forceinline__ void put2(float *p, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long *>(p),
+                     (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float *p) {
+  const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED,
+                                                 __HIP_MEMORY_SCOPE_AGENT);
+  return float2{__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32))};
+}
+
 // x = a + b + c exactly, each of at most eight significant bits (truncated, so that nothing overflows): three BF16 values.
 // Two x give a dword of each part.
 __device__ __forceinline__ void bf16_parts(float x, float y, unsigned (&part)[3]) {
@@ -642,7 +655,10 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
                     : p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
   };
   auto store = [&](float *dst, int d, const float4 &x) { // dimensions d .. d + 3, below hd
-    if (it.slots || p.out_vec) {
+    if (it.slots) {
+      put2(dst + d, x.x, x.y);
+      put2(dst + d + 2, x.z, x.w);
+    } else if (p.out_vec) {
       *reinterpret_cast<float4 *>(dst + d) = x;
     } else {
       dst[d] = x.x, dst[d + 1] = x.y, dst[d + 2] = x.z, dst[d + 3] = x.w;
@@ -680,7 +696,7 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
       float *to = target(v);
       if (it.slots) {
         if (d4 == 0)
-          to[HD] = m, to[HD + 1] = whole_l;
+          put2(to + HD, m, whole_l);
       } else {
         sum = float4{sum.x / whole_l, sum.y / whole_l, sum.z / whole_l, sum.w / whole_l};
       }
@@ -689,7 +705,7 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   } else if (active) {
     float *to = target(v0 + lc);
     if (it.slots && lq == 0)
-      to[HD] = m_run, to[HD + 1] = l;
+      put2(to + HD, m_run, l);
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -770,37 +786,65 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       const int first = (int)whole(w0, slice), last_block = (int)whole(end - 1, slice);
       const bool first_has = position_at((first + 1) * slice) > 0;
       const int from = first_has ? first : first + 1, parts = last_block - from + 1;
-      __syncthreads(); // the block's part is stored
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
+      __syncthreads();                                 // the block's
       if (tid == 0)
-        arrived = __hip_atomic_fetch_add(&paged_arrivals[g * p.blocks + first], 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        arrived = __hip_atomic_fetch_add(&paged_arrivals[g * p.blocks + first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
       if (arrived != (unsigned)(parts - 1))
         continue;
-      __threadfence(); // the others' parts are seen
       if (tid == 0)
         __hip_atomic_store(&paged_arrivals[g * p.blocks + first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int hd4 = hd / 4;
-      for (int i = tid; i < it.vectors * hd4; i += kThreads) {
-        const int v = i / hd4, d4 = i % hd4;
-        float m = -FLT_MAX;
-        for (int k = from; k <= last_block; k++)
-          m = fmaxf(m, slots(k, k == first)[(size_t)v * kRow + HD]);
-        float l = 0.0f;
-        float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int k = from; k <= last_block; k++) { // in the blocks' order, whoever comes last
-          const float *src = slots(k, k == first) + (size_t)v * kRow;
-          const float scale = __builtin_amdgcn_exp2f(src[HD] - m);
-          const float4 x = *reinterpret_cast<const float4 *>(src + 4 * d4);
-          l = fmaf(scale, src[HD + 1], l);
-          sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
+      // the parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
+      // LDS by a wave a vector, then the sums in the parts' order, whoever comes last
+      const int hd4 = hd / 4, some = min(it.vectors, kWaves * 16 * kRow / parts);
+      for (int v0 = 0; v0 < it.vectors; v0 += some) {
+        const int n = min(some, it.vectors - v0);
+        __syncthreads(); // LDS is free
+        for (int v = tid / kWave; v < n; v += kWaves) {
+          float m = -FLT_MAX, l = 0.0f;
+          for (int k = tid % kWave; k < parts; k += kWave)
+            m = fmaxf(m, get2(slots(from + k, from + k == first) + (size_t)(v0 + v) * kRow + HD).x);
+          m = wave_max(m);
+          for (int k = tid % kWave; k < parts; k += kWave) {
+            const float2 end_of = get2(slots(from + k, from + k == first) + (size_t)(v0 + v) * kRow + HD);
+            const float scale = __builtin_amdgcn_exp2f(end_of.x - m);
+            lds[v * parts + k] = scale;
+            l = fmaf(scale, end_of.y, l);
+          }
+          l = wave_sum(l);
+          for (int k = tid % kWave; k < parts; k += kWave)
+            lds[v * parts + k] /= l;
         }
-        float *to = p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + v % kv_mul) * hd + 4 * d4;
-        const float4 x = float4{sum.x / l, sum.y / l, sum.z / l, sum.w / l};
-        if (p.out_vec)
-          *reinterpret_cast<float4 *>(to) = x;
-        else
-          to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+        __syncthreads();
+        for (int i = tid; i < n * hd4; i += kThreads) {
+          const int v = i / hd4, d4 = i % hd4;
+          float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
+          constexpr int kAtOnce = 8;
+          for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
+            float2 x[kAtOnce][2];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+              const int k = from + min(k0 + j, parts - 1);
+              const float *src = slots(k, k == first) + (size_t)(v0 + v) * kRow + 4 * d4;
+              x[j][0] = get2(src), x[j][1] = get2(src + 2);
+            }
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++)
+              if (k0 + j < parts) {
+                const float scale = lds[v * parts + k0 + j];
+                sum = float4{fmaf(scale, x[j][0].x, sum.x), fmaf(scale, x[j][0].y, sum.y), fmaf(scale, x[j][1].x, sum.z),
+                             fmaf(scale, x[j][1].y, sum.w)};
+              }
+          }
+          const int vector = v0 + v;
+          float *to = p.job.out + ((size_t)(it.row0 + vector / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + vector % kv_mul) * hd +
+                      4 * d4;
+          if (p.out_vec)
+            *reinterpret_cast<float4 *>(to) = sum;
+          else
+            to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
+        }
       }
     }
   }
