@@ -211,8 +211,9 @@ __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 // kBegin positions of a small tile.
 constexpr int kBegin = 256;
 // A slice is at least this long: shorter ones do not pay for a walk's join, and a block inside a walk has some of its
-// positions however they are rounded.
-constexpr int kMinSlice = kBegin + 2 * kRound;
+// positions however they are rounded (kRound of a small tile's take as long as a round of any).
+constexpr int kMinSlice = 2 * kRound;
+static_assert(kMinSlice >= kRound, "a slice holds a round");
 
 // Waves that walk a tile's positions together, a wave 16 vectors: four, two or one.
 __device__ __forceinline__ int walkers_of(int vectors) { return vectors <= 16 ? 4 : vectors <= 32 ? 2 : 1; }
@@ -519,6 +520,7 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   load_k(first, 0);
   load_v(first, 0);
   int i = 0; // the step's number since look_up
+  unsigned odd_values = 0;
   for (int pos = first; pos < end; pos += stride) {
     v4f sc[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -578,42 +580,30 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
       l_run += w[j]; // this lane's positions; the four lanes of a vector meet at the end
     }
     // A V value that is not finite must reach the vectors that see its position alone, and 0 * infinity would carry it to
-    // those that do not: where some do not, the product takes 0 in its place, and it is added to those that do.
+    // those that do not: where some do not, the product takes 0 in its place, and it is added to those that do at the end.
     if (pos + kStep > all_see && all_see < end) {
-      bool met = false;
+      // an exponent of ones, plus one, carries into the sign's place
+      unsigned met = 0;
 #pragma unroll
       for (int j = 0; j < 8; j++)
 #pragma unroll
-        for (int u = 0; u < kVecs; u++)
+        for (int u = 0; u < kVecs; u++) {
 #pragma unroll
           for (unsigned c = 0; c < EV * sizeof(T) / 4; c++) {
-            const unsigned x = vr[j][u][c];
+            unsigned &x = vr[j][u][c];
             if constexpr (kBf16) {
-              const bool lo = (x & 0x7f80u) == 0x7f80u, hi = (x & 0x7f800000u) == 0x7f800000u;
-              met |= lo | hi;
-              vr[j][u][c] = (lo ? 0u : x & 0xffffu) | (hi ? 0u : x & 0xffff0000u);
+              const unsigned carry = ((x & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u;
+              met |= carry;
+              x &= ~((carry << 16) - carry);
             } else {
-              const bool bad = (x & 0x7f800000u) == 0x7f800000u;
-              met |= bad;
-              vr[j][u][c] = bad ? 0u : x;
+              const int carry = (int)((x & 0x7f800000u) + 0x00800000u) >> 31;
+              met |= (unsigned)carry;
+              x &= ~(unsigned)carry;
             }
           }
-      if (__any(met)) {
-        for (int t = pos; t < min(pos + kStep, end); t++) {
-          const T *row = (const T *)p.job.value + place_any(t);
-          int lq4 = 4 * lq; // new to the compiler here: else it keeps what follows from it in registers all along the walk
-          asm volatile("" : "+v"(lq4));
-#pragma unroll
-          for (int e = 0; e < E; e++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const int d = (e / EV * 16 + lq4 + r) * EV + e % EV;
-              const float x = value(row + (d < hd ? d : 0));
-              if (d < hd && !isfinite(x) && t <= last)
-                o[e][r] += x;
-            }
+          asm volatile("" : "+v"(met)); // one after the other: registers
         }
-      }
+      odd_values |= met;
     }
     if constexpr (kBf16) {
       v4u wp[3];
@@ -649,6 +639,20 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   }
   if (odd != 0.0f)
     p.flags[1] = 1;
+  if (__any(odd_values != 0)) {
+    for (int pos = first; pos < end; pos += stride) // the steps above
+      for (int t = pos + kStep > all_see ? pos : end; t < min(pos + kStep, end); t++) {
+        const T *row = (const T *)p.job.value + place_any(t);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int d = (e / EV * 16 + 4 * lq + r) * EV + e % EV;
+            const float x = value(row + (d < hd ? d : 0));
+            o[e][r] += d < hd && t <= last && !isfinite(x) ? x : 0.0f;
+          }
+      }
+  }
   // vector v's sums: to its slot, or divided by the weights' sum to out
   auto target = [&](int v) {
     return it.slots ? it.slots + (size_t)v * kRow
@@ -782,10 +786,10 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       walk<T, HD, MODE>(p, it, lds);
       if (!shared)
         continue;
-      // the walk's blocks: first .. last_block, the first of them perhaps without a part
+      // the walk's blocks: from .. last_block
       const int first = (int)whole(w0, slice), last_block = (int)whole(end - 1, slice);
-      const bool first_has = position_at((first + 1) * slice) > 0;
-      const int from = first_has ? first : first + 1, parts = last_block - from + 1;
+      // the first block whose slice ends behind the walk's first round
+      const int from = min(max(first, (int)whole(w0 + kBegin + kRound - 1, slice)), last_block), parts = last_block - from + 1;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
       __syncthreads();                                 // the block's
       if (tid == 0)
