@@ -5,6 +5,7 @@
 //                     cores; a walk that several blocks share is joined by the last of them to arrive.
 //   attn_paged_rows   any shape, one row and KV head a block.
 #include <cfloat>
+#include <type_traits>
 
 #include "paged_device.h"
 
@@ -174,8 +175,10 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kStep = 32;              // positions that a wave takes at once
 constexpr int kRound = kWaves * kStep; // positions that a block takes at once in a tile of up to 16 vectors
 constexpr int kTileVectors = 64;       // query vectors of a tile
+constexpr int kWideVectors = 128;      // of a wide one
 constexpr int kMaxBlocksPerCu = 2;
 constexpr int kMaxArrivals = 4096;
+constexpr unsigned kNowhere = 0x7ffffff0u; // an offset past every buffer: a load reads zero there
 constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far below that its weight is zero, also where a
                                      // lane has seen nothing else
 
@@ -187,8 +190,10 @@ struct FastPaged {
   AttentionPagedJob job;
   int kv_mul, blocks; // blocks: of a KV head
   int tile_rows;      // rows of a full tile
+  int tile_vectors;   // at most, of a tile: kTileVectors or kWideVectors
   float scale2;       // log2(e) / sqrt(hd)
-  // slots of HD + 4 floats, [KV head][block][0: a walk that an earlier block began, 1: one that this block begins][vector]
+  // slots of tile_vectors (HD + 2) floats, [KV head][block][0: a walk that an earlier block began, 1: one that this block
+  // begins]: the vectors' sums, then their maxima and weights' sums
   float *partial;
   int *flags;
   bool q_vec;   // q in whole 16-byte vectors
@@ -287,7 +292,7 @@ struct Item {
   int r, g, row0, vectors, last0;
   int t0, t1;
   int walkers;  // waves of 16 vectors
-  float *slots; // [vector][HD + 4], or null: the part is the whole, and goes to out
+  int slot;     // of the part's sums, or -1: the part is the whole, and goes to out
 };
 
 __device__ __forceinline__ float four_sum(float x) {
@@ -300,14 +305,39 @@ __device__ __forceinline__ float four_max(float x) {
 }
 
 // A part's sums go past the XCDs' own L2s: stores of agent scope write through, loads of agent scope read what they wrote. (A
-// release and an acquire around plain ones write back and drop a whole L2 a block: 32 requests took 134 us, not %DEC32%.)
-__device__ __forceinline__ void put2(float *p, float x, float y) {
-  __hip_atomic_store(reinterpret_cast<unsigned long long *>(p),
-                     (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
-                     __HIP_MEMORY_SCOPE_AGENT);
+// release and an acquire around plain ones write back and drop a whole L2 a block: 32 requests took 134 us, not 65.) Each store
+// takes its place in memory's queues, whatever its size: 16 bytes a lane, side by side, where a lane's own 128 bytes as eights
+// took the prompts from %A% to 236 us.
+//
+// Sums lie row by row, [vector][HD], where the block's threads have them so (kRows), else as lanes have them: [16 vectors][r][e /
+// 4][lane] of four dimensions each.
+constexpr int kAgent = 16; // the cache policy's sc1
+struct Slot {
+  __amdgpu_buffer_rsrc_t rsrc;
+  unsigned ends; // where the maxima and weights' sums begin, in bytes
+};
+template <int HD> __device__ __forceinline__ Slot slot_at(const FastPaged &p, int slot) {
+  const unsigned floats = (unsigned)(p.tile_vectors * (HD + 2));
+  const uint64_t base = (uint64_t)(uintptr_t)p.partial + (uint64_t)uniform(slot) * floats * 4u;
+  return Slot{__builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)base, (short)0, (int)(floats * 4u), 0x00020000),
+              (unsigned)(p.tile_vectors * HD) * 4u};
 }
-__device__ __forceinline__ float2 get2(const float *p) {
-  const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED,
+__device__ __forceinline__ void put4(const Slot &s, unsigned at, const float4 &x) {
+  const v4u bits = {__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(x.z), __float_as_uint(x.w)};
+  __builtin_amdgcn_raw_buffer_store_b128(bits, s.rsrc, at * 16u, 0, kAgent);
+}
+__device__ __forceinline__ float4 get4(const Slot &s, unsigned at) {
+  const v4u x = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(s.rsrc, at * 16u, 0, kAgent));
+  return float4{__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+}
+__device__ __forceinline__ void put_end(const Slot &s, int v, float m, float l) {
+  const v2u bits = {__float_as_uint(m), __float_as_uint(l)};
+  __builtin_amdgcn_raw_buffer_store_b64(bits, s.rsrc, s.ends + 8u * (unsigned)v, 0, kAgent);
+}
+// Of a slot that differs from lane to lane.
+__device__ __forceinline__ float2 load_end(const FastPaged &p, int slot, int v, int dims) {
+  const float *at = p.partial + (size_t)slot * (size_t)(p.tile_vectors * (dims + 2)) + (size_t)(p.tile_vectors * dims) + 2 * v;
+  const unsigned long long x = __hip_atomic_load(reinterpret_cast<const unsigned long long *>(at), __ATOMIC_RELAXED,
                                                  __HIP_MEMORY_SCOPE_AGENT);
   return float2{__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32))};
 }
@@ -351,7 +381,6 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   constexpr int kSteps = kBf16 ? HD / 32 : HD / 16; // a K row: loads of 16 bytes
   constexpr int kPerLoad = kBf16 ? 8 : 4;           // dimensions of one
   constexpr int kRow = HD + 4;
-  constexpr unsigned kNowhere = 0x7ffffff0u; // an offset past every buffer
   const PagedDev &b = p.job.batch;
   const int tid = own_thread(), lane = tid & (kWave - 1), wave = uniform(tid / kWave), lq = lane >> 4, lc = lane & 15;
   const int hd = MODE == kWhole ? HD : p.job.head_dim, kv_mul = p.kv_mul;
@@ -653,23 +682,21 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
           }
       }
   }
-  // vector v's sums: to its slot, or divided by the weights' sum to out
+  // vector v's place in out
   auto target = [&](int v) {
-    return it.slots ? it.slots + (size_t)v * kRow
-                    : p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
+    return p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
   };
-  auto store = [&](float *dst, int d, const float4 &x) { // dimensions d .. d + 3, below hd
-    if (it.slots) {
-      put2(dst + d, x.x, x.y);
-      put2(dst + d + 2, x.z, x.w);
-    } else if (p.out_vec) {
-      *reinterpret_cast<float4 *>(dst + d) = x;
+  auto store = [&](float *dst, const float4 &x) {
+    if (p.out_vec) {
+      *reinterpret_cast<float4 *>(dst) = x;
     } else {
-      dst[d] = x.x, dst[d + 1] = x.y, dst[d + 2] = x.z, dst[d + 3] = x.w;
+      dst[0] = x.x, dst[1] = x.y, dst[2] = x.z, dst[3] = x.w;
     }
   };
+  const bool whole = it.slot < 0;
+  const Slot slot = slot_at<HD>(p, max(it.slot, 0));
   constexpr int kFours = E / 4; // a lane's r-th row: kFours groups of four dimensions
-  const float l = four_sum(l_run);
+  const float l = four_sum(l_run), inverse = 1.0f / l;
   if (it.walkers > 1) { // the waves' sums meet in LDS: [wave][vector][HD values, maximum, sum]
     float *dst = lds + (size_t)(wave * 16 + lc) * kRow;
 #pragma unroll
@@ -697,36 +724,300 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
         whole_l = fmaf(scale, at[HD + 1], whole_l);
         sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
       }
-      float *to = target(v);
-      if (it.slots) {
-        if (d4 == 0)
-          put2(to + HD, m, whole_l);
+      if (whole) {
+        store(target(v) + 4 * d4, float4{sum.x / whole_l, sum.y / whole_l, sum.z / whole_l, sum.w / whole_l});
       } else {
-        sum = float4{sum.x / whole_l, sum.y / whole_l, sum.z / whole_l, sum.w / whole_l};
+        put4(slot, (unsigned)(v * (HD / 4) + d4), sum);
+        if (d4 == 0)
+          put_end(slot, v, m, whole_l);
       }
-      store(to, 4 * d4, sum);
     }
-  } else if (active) {
-    float *to = target(v0 + lc);
-    if (it.slots && lq == 0)
-      put2(to + HD, m_run, l);
+  } else if (mine > 0) {
+    float *to = target(v0 + min(lc, mine - 1));
+    if (!whole && lq == 0 && active)
+      put_end(slot, v0 + lc, m_run, l);
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int f = 0; f < kFours; f++) {
         const int e = 4 * f, d = (e / EV * 16 + 4 * lq + r) * EV + e % EV;
-        float4 x = float4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
-        if (!it.slots)
-          x = float4{x.x / l, x.y / l, x.z / l, x.w / l};
-        if (d < hd)
-          store(to, d, x);
+        const float4 x = float4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
+        if (!whole)
+          put4(slot, (unsigned)((v0 / 16 * 4 + r) * kFours + f) * kWave + lane, x);
+        else if (active && d < hd)
+          store(to + d, float4{x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse});
       }
   }
 }
 
-template <typename T, int HD, int MODE>
+// A tile of more than 64 vectors over BF16 pages: each wave has 32 of them and takes all positions. A step's K and V rows are
+// loaded once for the block, V turned on the way, and staged in LDS as the instructions take them: a K row's 16 bytes and a V
+// operand's serve six instructions each (three parts of two sets of 16 vectors).
+template <int HD> struct WideStage {
+  static constexpr int kKRow = HD + 8; // values: a row's 16 bytes lie four banks behind the row before's
+  uint16_t k[kStep * kKRow];
+  v4u v[HD / 16][kWave]; // [instruction][lane]: eight positions of a dimension
+};
+template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const Item &it, float *lds) {
+  typedef WideStage<HD> Stage;
+  static_assert(2 * sizeof(Stage) <= kWaves * 16 * (HD + 4) * sizeof(float), "two stages in the sums' place");
+  Stage *const stages = reinterpret_cast<Stage *>(lds); // two: a step is staged while the one before is computed
+  constexpr int E = HD / 16, EV = E, kSteps = HD / 32, kRow = HD + 4, NT = 2;
+  constexpr int kKLanes = HD / 8, kKLoads = kStep * kKLanes / kThreads; // lanes of a K row, loads a thread
+  static_assert(kKLoads >= 1 && kThreads / kKLanes % 16 == 0, "a K load's rows in one tile of 16");
+  const PagedDev &b = p.job.batch;
+  const int tid = own_thread(), lane = tid & (kWave - 1), wave = uniform(tid / kWave), lq = lane >> 4, lc = lane & 15;
+  const int hd = MODE == kWhole ? HD : p.job.head_dim, kv_mul = p.kv_mul;
+  const int v0 = wave * 16 * NT, mine = min(it.vectors - v0, 16 * NT);
+  const int all_see = it.last0 + 1;                          // positions below are seen by all of the tile's vectors
+  const int wave_sees = it.last0 + v0 / kv_mul + 1;          // by the wave's
+  const int end = it.t1;
+  int last[NT];
+  v4f o[NT][E];
+  float m_run[NT], l_run[NT], odd = 0.0f;
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    last[n] = 16 * n + lc < mine ? it.last0 + (v0 + 16 * n + lc) / kv_mul : -1;
+    m_run[n] = -FLT_MAX, l_run[n] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      o[n][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const size_t head = (size_t)it.g * b.head_base;
+  long long places = 0; // as in walk, of 32 steps
+  auto look_up = [&](int pos) {
+    const int at = min(pos + 16 * lane, end - 1), number = at / b.page_size, page = page_of(b, it.r, number);
+    if (page < 0)
+      p.flags[8] = 1;
+    places = (long long)(((size_t)max(page, 0) * b.page_values + (size_t)((at - number * b.page_size) & ~15) * b.pos_stride +
+                          head) * sizeof(uint16_t));
+  };
+  const unsigned row_bytes = (unsigned)b.pos_stride * 2u;
+  // 16 rows, tile t of the step at pos, the i-th since look_up
+  auto rows_at = [&](const void *cache, int pos, int i, int t) {
+    const int at = min(2 * i + t, kWave - 1);
+    const int lo = __builtin_amdgcn_readlane((int)places, at), hi = __builtin_amdgcn_readlane((int)(places >> 32), at);
+    const int rows = min(end - (pos + 16 * t), 16);
+    const int bytes = rows > 0 ? (int)((unsigned)(rows - 1) * row_bytes + (unsigned)(hd * 2)) : 0;
+    return rows_of(cache, (long long)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo), bytes);
+  };
+  // a thread's K values: row tid / kKLanes of every 256 / kKLanes, dimensions 8 (tid % kKLanes) ..; its V values: dimensions
+  // EV lc .. of positions j = 2 wave, 2 wave + 1 of its lane group's eight
+  v4u kr[kKLoads];
+  unsigned vr[2][EV / 2];
+  const int k_dim = 8 * (tid % kKLanes), k_row = tid / kKLanes;
+  const unsigned k_at = k_dim < hd ? (unsigned)(k_row % 16) * row_bytes + (unsigned)k_dim * 2u : kNowhere;
+  const unsigned v_at = EV * lc < hd ? (unsigned)(4 * lq + 2 * (wave & 1)) * row_bytes + (unsigned)(EV * lc) * 2u : kNowhere;
+  auto load = [&](int pos, int i) {
+#pragma unroll
+    for (int u = 0; u < kKLoads; u++)
+      kr[u] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(
+                                          rows_at(p.job.key, pos, i, kKLoads > 1 ? u : uniform(k_row / 16)), k_at, 0, 0));
+    const auto rsrc = rows_at(p.job.value, pos, i, wave / 2);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const unsigned at = v_at == kNowhere ? kNowhere : v_at + (unsigned)j * row_bytes;
+      if constexpr (EV == 8) {
+        const v4u x = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          vr[j][c] = x[c];
+      } else {
+        const v2u x = __builtin_bit_cast(v2u, __builtin_amdgcn_raw_buffer_load_b64(rsrc, at, 0, 0));
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+          vr[j][c] = x[c];
+      }
+    }
+  };
+  unsigned odd_values = 0;
+  auto stage = [&](Stage &sh, int pos) {
+#pragma unroll
+    for (int u = 0; u < kKLoads; u++)
+      *reinterpret_cast<v4u *>(&sh.k[(k_row + u * (kThreads / kKLanes)) * Stage::kKRow + k_dim]) = kr[u];
+    if (pos + kStep > all_see) { // as in walk: a value that is not finite is added behind it
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int c = 0; c < EV / 2; c++) {
+          const unsigned carry = ((vr[j][c] & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u;
+          odd_values |= carry;
+          vr[j][c] &= ~((carry << 16) - carry);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      reinterpret_cast<unsigned *>(&sh.v[e][lane])[wave] =
+          __builtin_amdgcn_perm(vr[1][e / 2], vr[0][e / 2], e % 2 ? 0x07060302 : 0x05040100);
+  };
+  int i = 0; // the number since look_up of the step that is loaded next
+  look_up(it.t0);
+  load(it.t0, i++);
+  fence();
+  v4u qp[NT][kSteps][3];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    const bool active = 16 * n + lc < mine;
+    const int v = active ? v0 + 16 * n + lc : 0;
+    const float *src = p.job.q + (size_t)(it.row0 + v / kv_mul) * p.job.q_stride + ((size_t)it.g * kv_mul + v % kv_mul) * hd;
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      const int d = 32 * s + 8 * lq;
+      const float *at = src + (d < hd ? d : 0);
+      float x[8];
+      if (p.q_vec) {
+        const float4 a = reinterpret_cast<const float4 *>(at)[0], c = reinterpret_cast<const float4 *>(at)[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+          x[c] = at[c];
+      }
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        unsigned part[3];
+        const bool there = active && d < hd;
+        bf16_parts(there ? x[2 * c] * p.scale2 : 0.0f, there ? x[2 * c + 1] * p.scale2 : 0.0f, part);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          qp[n][s][k][c] = part[k];
+      }
+    }
+  }
+  stage(stages[0], it.t0);
+  load(it.t0 + kStep, i++);
+  int turn = 0;
+  for (int pos = it.t0; pos < end; pos += kStep, turn ^= 1) {
+    const Stage &sh = stages[turn];
+    __syncthreads(); // the step is staged, the one before it computed
+    v4f sc[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+        sc[n][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < kSteps; s++)
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const v4u a = *reinterpret_cast<const v4u *>(&sh.k[(16 * t + lc) * Stage::kKRow + 32 * s + 8 * lq]);
+#pragma unroll
+        for (int k = 2; k >= 0; k--)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+            sc[n][t] = mfma_bf16(a, qp[n][s][k], sc[n][t]);
+      }
+    stage(stages[turn ^ 1], pos + kStep);
+    if (i == kWave / 2) { // uniform
+      look_up(pos + 2 * kStep);
+      i = 0;
+    }
+    load(pos + 2 * kStep, i++);
+    v4u wp[NT][3];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      float w[8], top = -FLT_MAX;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        w[j] = sc[n][j / 4][j % 4];
+      if (pos + kStep > wave_sees || pos + kStep > end || mine < 16 * NT) { // a lane without a vector sees nothing
+        const int seen = min(last[n], end - 1) - pos - 4 * lq;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          w[j] = 16 * (j / 4) + j % 4 <= seen ? w[j] : -FLT_MAX;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        odd = fmaf(w[j], 0.0f, odd);
+        top = fmaxf(top, w[j]);
+      }
+      if (__any(top > m_run[n] + 8.0f)) { // as in walk
+        const float m = fmaxf(m_run[n], four_max(top)), alpha = __builtin_amdgcn_exp2f(m_run[n] - m);
+        l_run[n] *= alpha;
+        m_run[n] = m;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          o[n][e] *= alpha;
+      }
+      const float base = fmaxf(m_run[n], kMasked);
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        w[j] = __builtin_amdgcn_exp2f(w[j] - base);
+        l_run[n] += w[j];
+      }
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        unsigned part[3];
+        bf16_parts(w[2 * c], w[2 * c + 1], part);
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+          wp[n][k][c] = part[k];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const v4u a = sh.v[e][lane];
+#pragma unroll
+      for (int k = 2; k >= 0; k--)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+          o[n][e] = mfma_bf16(a, wp[n][k], o[n][e]);
+    }
+  }
+  if (odd != 0.0f)
+    p.flags[1] = 1;
+  if (__syncthreads_or(odd_values != 0)) {
+    for (int t = it.t0 + (max(all_see - it.t0, 0) & ~(kStep - 1)); t < end; t++) { // of the steps that some do not see whole
+      const int number = t / b.page_size, page = max(page_of(b, it.r, number), 0);
+      const uint16_t *row = (const uint16_t *)p.job.value + (size_t)page * b.page_values +
+                            (size_t)(t - number * b.page_size) * b.pos_stride + head;
+#pragma unroll
+      for (int e = 0; e < E; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int d = (4 * lq + r) * EV + e;
+          const float x = value(row + (d < hd ? d : 0));
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+            o[n][e][r] += d < hd && t <= last[n] && !isfinite(x) ? x : 0.0f;
+        }
+    }
+  }
+  const bool whole = it.slot < 0;
+  const Slot slot = slot_at<HD>(p, max(it.slot, 0));
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    const float l = four_sum(l_run[n]), inverse = 1.0f / l;
+    const bool active = 16 * n + lc < mine;
+    const int v = active ? v0 + 16 * n + lc : 0;
+    float *to = p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
+    if (16 * n >= mine)
+      continue; // uniform
+    if (!whole && lq == 0 && active)
+      put_end(slot, v, m_run[n], l);
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        const int d = (4 * lq + r) * EV + e;
+        float4 x = float4{o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]};
+        if (!whole) {
+          put4(slot, (unsigned)(((v0 / 16 + n) * 4 + r) * (E / 4) + e / 4) * kWave + lane, x);
+        } else if (active && d < hd) {
+          x = float4{x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse};
+          if (p.out_vec)
+            *reinterpret_cast<float4 *>(to + d) = x;
+          else
+            to[d] = x.x, to[d + 1] = x.y, to[d + 2] = x.z, to[d + 3] = x.w;
+        }
+      }
+  }
+}
+
+template <typename T, int HD, int MODE, bool WIDE>
 __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn_paged(FastPaged p) {
-  constexpr int kRow = HD + 4;
+  constexpr int kRow = HD + 4, E = HD / 16;
+  constexpr int EV = WIDE ? E : E < (sizeof(T) == 2 ? 8 : 4) ? E : (sizeof(T) == 2 ? 8 : 4); // as in the walks
   __shared__ Plan plan;
   __shared__ __align__(16) float lds[kWaves * 16 * kRow];
   __shared__ unsigned arrived;
@@ -778,12 +1069,17 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       it.r = r, it.g = g;
       it.row0 = q.first + row, it.last0 = q.length + row;
       const bool shared = it.t0 > 0 || it.t1 < positions;
-      auto slots = [&](int blk, bool begins) {
-        return p.partial + (((size_t)g * p.blocks + blk) * 2 + begins) * kTileVectors * kRow;
-      };
-      it.slots = shared ? slots(block, w0 >= lo) : nullptr;
+      auto slot_of = [&](int blk, bool begins) { return (g * p.blocks + blk) * 2 + begins; };
+      it.slot = uniform(shared ? slot_of(block, w0 >= lo) : -1);
       __syncthreads(); // LDS is free
-      walk<T, HD, MODE>(p, it, lds);
+      if constexpr (WIDE) {
+        if (it.vectors > kTileVectors)
+          walk_wide<HD, MODE>(p, it, lds);
+        else
+          walk<T, HD, MODE>(p, it, lds);
+      } else {
+        walk<T, HD, MODE>(p, it, lds);
+      }
       if (!shared)
         continue;
       // the walk's blocks: from .. last_block
@@ -799,56 +1095,94 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
         continue;
       if (tid == 0)
         __hip_atomic_store(&paged_arrivals[g * p.blocks + first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      // the parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
-      // LDS by a wave a vector, then the sums in the parts' order, whoever comes last
-      const int hd4 = hd / 4, some = min(it.vectors, kWaves * 16 * kRow / parts);
-      for (int v0 = 0; v0 < it.vectors; v0 += some) {
-        const int n = min(some, it.vectors - v0);
+      // The parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
+      // LDS by a wave a vector, then the sums in the parts' order, whoever comes last. A part's place by its number.
+      auto part = [&](int k) { return slot_at<HD>(p, slot_of(from + k, from + k == first)); };
+      const int hd4 = hd / 4;
+      const bool sets = it.walkers == 1; // sums as lanes have them, in sets of 16 vectors
+      int some = kWaves * 16 * kRow / parts;
+      if (sets && some >= 16)
+        some &= ~15;
+      for (int v0 = 0, n; v0 < it.vectors; v0 += n) {
+        n = min(some, it.vectors - v0);
+        if (sets && some < 16)
+          n = min(n, 16 - v0 % 16); // of one set
         __syncthreads(); // LDS is free
         for (int v = tid / kWave; v < n; v += kWaves) {
           float m = -FLT_MAX, l = 0.0f;
-          for (int k = tid % kWave; k < parts; k += kWave)
-            m = fmaxf(m, get2(slots(from + k, from + k == first) + (size_t)(v0 + v) * kRow + HD).x);
-          m = wave_max(m);
           for (int k = tid % kWave; k < parts; k += kWave) {
-            const float2 end_of = get2(slots(from + k, from + k == first) + (size_t)(v0 + v) * kRow + HD);
-            const float scale = __builtin_amdgcn_exp2f(end_of.x - m);
-            lds[v * parts + k] = scale;
-            l = fmaf(scale, end_of.y, l);
+            const float2 end_of = load_end(p, slot_of(from + k, from + k == first), v0 + v, HD);
+            lds[v * parts + k] = end_of.x;
+            const float top = fmaxf(m, end_of.x);
+            l = l * __builtin_amdgcn_exp2f(m - top) + end_of.y * __builtin_amdgcn_exp2f(end_of.x - top);
+            m = top;
           }
-          l = wave_sum(l);
+          const float top = wave_max(m);
+          l = wave_sum(l * __builtin_amdgcn_exp2f(m - top));
           for (int k = tid % kWave; k < parts; k += kWave)
-            lds[v * parts + k] /= l;
+            lds[v * parts + k] = __builtin_amdgcn_exp2f(lds[v * parts + k] - top) / l;
         }
         __syncthreads();
-        for (int i = tid; i < n * hd4; i += kThreads) {
-          const int v = i / hd4, d4 = i % hd4;
-          float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
-          constexpr int kAtOnce = 8;
-          for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
-            float2 x[kAtOnce][2];
+        const int set0 = v0 & ~15, items = sets ? ceil_div(v0 + n - set0, 16) * 16 * (HD / 4) : n * hd4;
+        // I of the thread's items and K parts at a time: as many loads are in flight
+        auto add_up = [&](auto of_items, auto of_parts) {
+          constexpr int I = decltype(of_items)::value, K = decltype(of_parts)::value;
+          for (int i0 = tid; i0 < items; i0 += I * kThreads) {
+            int v[I], d[I];
+            unsigned at[I];
+            float4 sum[I];
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++) {
-              const int k = from + min(k0 + j, parts - 1);
-              const float *src = slots(k, k == first) + (size_t)(v0 + v) * kRow + 4 * d4;
-              x[j][0] = get2(src), x[j][1] = get2(src + 2);
+            for (int j = 0; j < I; j++) {
+              const int i = i0 + j * kThreads;
+              if (sets) { // [16 vectors][r][e / 4][lane]
+                const int lane = i % kWave, f = i / kWave % (E / 4), r = i / kWave / (E / 4) % 4, e = 4 * f;
+                v[j] = set0 - v0 + i / (16 * (HD / 4)) * 16 + lane % 16;
+                d[j] = (e / EV * 16 + 4 * (lane / 16) + r) * EV + e % EV;
+                at[j] = (unsigned)(set0 * (HD / 4) + i);
+              } else {
+                v[j] = i / hd4, d[j] = i % hd4 * 4;
+                at[j] = (unsigned)((v0 + v[j]) * (HD / 4) + d[j] / 4);
+              }
+              if (i >= items || v[j] < 0 || v[j] >= n || d[j] >= hd)
+                v[j] = 0, d[j] = -1, at[j] = kNowhere / 16; // reads zero
+              sum[j] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            for (int k0 = 0; k0 < parts; k0 += K) {
+              float4 x[K][I];
+#pragma unroll
+              for (int k = 0; k < K; k++) {
+                const Slot slot = part(min(k0 + k, parts - 1));
+#pragma unroll
+                for (int j = 0; j < I; j++)
+                  x[k][j] = get4(slot, k0 + k < parts ? at[j] : kNowhere / 16);
+              }
+#pragma unroll
+              for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int j = 0; j < I; j++) {
+                  const float scale = lds[v[j] * parts + min(k0 + k, parts - 1)];
+                  sum[j] = float4{fmaf(scale, x[k][j].x, sum[j].x), fmaf(scale, x[k][j].y, sum[j].y),
+                                  fmaf(scale, x[k][j].z, sum[j].z), fmaf(scale, x[k][j].w, sum[j].w)};
+                }
             }
 #pragma unroll
-            for (int j = 0; j < kAtOnce; j++)
-              if (k0 + j < parts) {
-                const float scale = lds[v * parts + k0 + j];
-                sum = float4{fmaf(scale, x[j][0].x, sum.x), fmaf(scale, x[j][0].y, sum.y), fmaf(scale, x[j][1].x, sum.z),
-                             fmaf(scale, x[j][1].y, sum.w)};
+            for (int j = 0; j < I; j++)
+              if (d[j] >= 0) {
+                const int vector = v0 + v[j];
+                float *to = p.job.out + ((size_t)(it.row0 + vector / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + vector % kv_mul) * hd + d[j];
+                if (p.out_vec)
+                  *reinterpret_cast<float4 *>(to) = sum[j];
+                else
+                  to[0] = sum[j].x, to[1] = sum[j].y, to[2] = sum[j].z, to[3] = sum[j].w;
               }
           }
-          const int vector = v0 + v;
-          float *to = p.job.out + ((size_t)(it.row0 + vector / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + vector % kv_mul) * hd +
-                      4 * d4;
-          if (p.out_vec)
-            *reinterpret_cast<float4 *>(to) = sum;
-          else
-            to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
-        }
+        };
+        if (items > 2 * kThreads)
+          add_up(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+        else if (parts > 4)
+          add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+        else
+          add_up(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
       }
     }
   }
@@ -871,11 +1205,26 @@ int blocks_of(const AttentionPagedJob &job) {
 }
 
 typedef void (*FastKernel)(FastPaged);
-template <typename T, int HD> FastKernel kernel_of(int mode) {
-  return mode == kWhole ? attn_paged<T, HD, kWhole> : mode == kPart ? attn_paged<T, HD, kPart> : attn_paged<T, HD, kAny>;
+template <typename T, int HD> FastKernel kernel_of(int mode, bool wide) {
+  if constexpr (sizeof(T) == 2 && HD <= 128)
+    if (wide)
+      return mode == kWhole ? attn_paged<T, HD, kWhole, true> : attn_paged<T, HD, kPart, true>;
+  return mode == kWhole  ? attn_paged<T, HD, kWhole, false>
+         : mode == kPart ? attn_paged<T, HD, kPart, false>
+                         : attn_paged<T, HD, kAny, false>;
 }
-template <typename T> FastKernel kernel_of(int dims, int mode) {
-  return dims == 64 ? kernel_of<T, 64>(mode) : dims == 128 ? kernel_of<T, 128>(mode) : kernel_of<T, 256>(mode);
+template <typename T> FastKernel kernel_of(int dims, int mode, bool wide) {
+  return dims == 64 ? kernel_of<T, 64>(mode, wide) : dims == 128 ? kernel_of<T, 128>(mode, wide) : kernel_of<T, 256>(mode, wide);
+}
+
+int mode_of(const AttentionPagedJob &job) {
+  return job.batch.page_size % 16 ? kAny : job.head_dim == tile_dims(job.head_dim) ? kWhole : kPart;
+}
+
+// The kernel with wide tiles, where some request may have more than 64 vectors.
+bool wide_tiles(const AttentionPagedJob &job) {
+  const long long vectors = (long long)job.batch.rows * (job.n_heads / job.n_kv_heads);
+  return job.batch.bf16 && job.head_dim <= 128 && mode_of(job) != kAny && job.batch.rows > job.batch.count && vectors > kTileVectors;
 }
 
 bool launch_rows(const AttentionPagedJob &job, hipStream_t stream) {
@@ -896,7 +1245,8 @@ bool launch_rows(const AttentionPagedJob &job, hipStream_t stream) {
 size_t attention_paged_workspace(const AttentionPagedJob &job) {
   if (!tiled(job))
     return 0;
-  return (size_t)job.n_kv_heads * blocks_of(job) * 2 * kTileVectors * (tile_dims(job.head_dim) + 4) * sizeof(float);
+  return (size_t)job.n_kv_heads * blocks_of(job) * 2 * (wide_tiles(job) ? kWideVectors : kTileVectors) *
+         (tile_dims(job.head_dim) + 2) * sizeof(float);
 }
 
 bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipStream_t stream) {
@@ -907,14 +1257,16 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipSt
   p.job = job;
   p.kv_mul = job.n_heads / job.n_kv_heads;
   p.blocks = blocks_of(job);
-  p.tile_rows = kTileVectors / p.kv_mul;
+  const bool wide = wide_tiles(job);
+  p.tile_vectors = wide ? kWideVectors : kTileVectors;
+  p.tile_rows = p.tile_vectors / p.kv_mul;
   p.scale2 = (float)(1.4426950408889634 / sqrt((double)job.head_dim));
   p.partial = (float *)workspace;
   p.flags = device().error_flags;
   p.q_vec = job.q_stride % 4 == 0 && ((uintptr_t)job.q & 15) == 0;
   p.out_vec = ((uintptr_t)job.out & 15) == 0;
-  const int mode = job.batch.page_size % 16 ? kAny : job.head_dim == dims ? kWhole : kPart;
-  const FastKernel kernel = job.batch.bf16 ? kernel_of<uint16_t>(dims, mode) : kernel_of<float>(dims, mode);
+  const int mode = mode_of(job);
+  const FastKernel kernel = job.batch.bf16 ? kernel_of<uint16_t>(dims, mode, wide) : kernel_of<float>(dims, mode, false);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(p.blocks * job.n_kv_heads)), dim3(kThreads), 0, stream, p);
   return launch_ok("attn_paged");
 }
