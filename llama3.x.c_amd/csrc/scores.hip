@@ -22,6 +22,7 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kChunk = 1024; // tokens of a wave, 16 a lane
 constexpr int kGroup = 64;   // tokens of a maximum: those of 16 lanes' float4
 constexpr int kGroups = kChunk / kGroup;
+constexpr int kPer = 16;       // maxima of a thread of score_rows, at most: rows of more than 4096 groups keep their chunks'
 constexpr int kRankList = 512; // candidates that are ranked each against each
 
 bool launch_ok(const char *what) {
@@ -41,8 +42,9 @@ struct Stat {
 struct Score {
   ScoreJob job;
   Stat *stats;   // [row][chunk]
-  float *maxima; // [row][16 chunks]
+  float *maxima; // [row][maxima of a row], or null
   int chunks;
+  int count; // maxima of a row: its groups', or its chunks'
   float scale2; // log2(e) / T
   int *flags;
   bool vec4;
@@ -80,11 +82,11 @@ __global__ __launch_bounds__(kThreads) void score_stats(Score p, int row0) {
     four[j] = fmaxf(fmaxf(x[4 * j], x[4 * j + 1]), fmaxf(x[4 * j + 2], x[4 * j + 3]));
     four[j] = group_reduce_max(four[j], 16);
   }
-  if (p.maxima) { // group 4 j + lane / 16, by lane 16 (lane / 16) + j
-    const int j = lane % 16;
+  if (p.maxima && p.count != p.chunks) { // group 4 j + lane / 16, by lane 16 (lane / 16) + j
+    const int j = lane % 16, group = chunk * kGroups + 4 * j + lane / 16;
     const float mine = j == 0 ? four[0] : j == 1 ? four[1] : j == 2 ? four[2] : four[3];
-    if (j < 4)
-      p.maxima[((size_t)row * p.chunks + chunk) * kGroups + 4 * j + lane / 16] = mine;
+    if (j < 4 && group < p.count)
+      p.maxima[(size_t)row * p.count + group] = mine;
   }
   float top = fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3]));
   top = fmaxf(top, __shfl_xor(top, 16));
@@ -106,8 +108,11 @@ __global__ __launch_bounds__(kThreads) void score_stats(Score p, int row0) {
     rest = wave_sum(rest);
     weighted = wave_sum(weighted);
   }
-  if (lane == 0)
+  if (lane == 0) {
     p.stats[(size_t)row * p.chunks + chunk] = Stat{bad ? INFINITY : top, ones, rest, weighted};
+    if (p.maxima && p.count == p.chunks)
+      p.maxima[(size_t)row * p.count + chunk] = top;
+  }
 }
 
 __device__ __forceinline__ double wave_add(double v) {
@@ -128,70 +133,106 @@ __device__ __forceinline__ float value_of(uint64_t key) {
   return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 
-// The k largest of n different keys in LDS, in order, to best[0 .. min(n, k) - 1]; by the whole block, which has written
-// the list before a barrier.
-__device__ void largest(const uint64_t *list, int n, int k, uint64_t *best, uint64_t *scratch) {
+__device__ __forceinline__ uint64_t key_max(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// The k largest of n different keys in LDS to take(place among them, key); by the whole block, which has written the list
+// before a barrier.
+template <class Take> __device__ __forceinline__ void largest(const uint64_t *list, int n, int k, uint64_t *scratch, Take take) {
   const int tid = threadIdx.x;
   if (n <= kRankList) { // each key's rank
     for (int i = tid; i < n; i += kThreads) {
       const uint64_t mine = list[i];
       int before = 0;
+#pragma unroll 8
       for (int j = 0; j < n; j++)
         before += list[j] > mine;
       if (before < k)
-        best[before] = mine;
+        take(before, mine);
     }
-    __syncthreads();
     return;
   }
   uint64_t last = ~0ull; // one after the other: many equal logits
   for (int i = 0; i < k; i++) {
     uint64_t mine = 0;
     for (int j = tid; j < n; j += kThreads)
-      mine = list[j] < last && list[j] > mine ? list[j] : mine;
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)mine, o);
-      mine = other > mine ? other : mine;
-    }
+      mine = list[j] < last ? key_max(list[j], mine) : mine;
+    for (int o = 32; o > 0; o >>= 1)
+      mine = key_max(mine, __shfl_xor((unsigned long long)mine, o));
+    __syncthreads(); // scratch is read
     if (tid % kWave == 0)
       scratch[tid / kWave] = mine;
     __syncthreads();
     for (int w = 0; w < kWaves; w++)
-      mine = scratch[w] > mine ? scratch[w] : mine;
+      mine = key_max(mine, scratch[w]);
     last = mine;
     if (tid == 0)
-      best[i] = mine;
-    __syncthreads();
+      take(i, mine);
   }
 }
 
-// What is in LDS: `list` keys of `capacity` groups or 64 top tokens.
-__global__ __launch_bounds__(kThreads) void score_rows(Score p, int capacity) {
+// The k-th largest of the wave's keys, or 1 (below every key) where fewer are not 0.
+__device__ __forceinline__ uint64_t kth_of_wave(uint64_t mine, int k) {
+  int before = 0;
+  const int lo = (int)(uint32_t)mine, hi = (int)(uint32_t)(mine >> 32);
+#pragma unroll
+  for (int j = 0; j < kWave; j++) {
+    const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, j) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane(lo, j);
+    before += other > mine;
+  }
+  const unsigned long long is = __ballot(mine != 0 && before == k - 1);
+  if (!is)
+    return 1;
+  const int at = __builtin_ctzll(is);
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, at) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, at);
+}
+
+// LDS holds `list` keys: those of a thread's maxima of `top` lanes a wave, 16 of each of `top` chunks, 64 of each of `top`
+// groups, whichever are more.
+__global__ __launch_bounds__(kThreads) void score_rows(Score p) {
   extern __shared__ uint64_t list[];
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves][2];
   __shared__ int counts[kWaves];
-  __shared__ uint64_t mine_of[kThreads], best[LLHIP_MAX_TOP], scratch[kWaves];
-  __shared__ uint64_t threshold;
-  __shared__ int found;
+  __shared__ uint64_t thresholds[kWaves], best[LLHIP_MAX_TOP], scratch[kWaves];
+  __shared__ int found[3];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, top = p.job.top;
   const float *logits = p.job.logits + (size_t)row * p.job.ld;
   const Stat *stats = p.stats + (size_t)row * p.chunks;
+  // what can be loaded at once is
   const int token = p.job.tokens ? p.job.tokens[row] : -1;
+  const Stat first = tid < p.chunks ? stats[tid] : Stat{-INFINITY, 0, 0.0f, 0.0f};
+  float maxima[kPer];
+  if (top) {
+    const float *src = p.maxima + (size_t)row * p.count;
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      maxima[j] = tid + j * kThreads < p.count ? src[tid + j * kThreads] : -INFINITY;
+  }
   const bool inside = token >= 0 && token < p.job.vocab;
   const float given = inside ? logits[token] : 0.0f;
-  const Stat first = tid < p.chunks ? stats[tid] : Stat{-INFINITY, 0, 0.0f, 0.0f};
+  if (tid < 3)
+    found[tid] = 0;
   float most = first.top;
   for (int c = tid + kThreads; c < p.chunks; c += kThreads)
     most = fmaxf(most, stats[c].top);
   most = wave_max(most);
   if (lane == 0)
     tops[wave] = most;
+  auto key_at = [&](int j) { return maxima[j] > -INFINITY ? key_of(maxima[j], tid + j * kThreads) : 0; };
+  if (top) { // the top-th of a wave's lanes' largest: a bound that `top` maxima reach
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      mine = key_max(mine, key_at(j));
+    const uint64_t kth = kth_of_wave(mine, top);
+    if (lane == 0)
+      thresholds[wave] = kth;
+  }
   __syncthreads();
   for (int w = 0; w < kWaves; w++)
     most = fmaxf(most, tops[w]);
-  const bool decides = most > -INFINITY && most < INFINITY;
-  if (!decides) { // uniform
+  if (!(most > -INFINITY && most < INFINITY)) { // uniform
     if (tid == 0) {
       p.flags[10] = 1;
       if (p.job.logprob)
@@ -202,6 +243,17 @@ __global__ __launch_bounds__(kThreads) void score_rows(Score p, int capacity) {
     for (int i = tid; i < top; i += kThreads)
       p.job.top_token[(size_t)row * top + i] = -1, p.job.top_logprob[(size_t)row * top + i] = NAN;
     return;
+  }
+  if (top) {
+    uint64_t least = thresholds[0];
+    for (int w = 1; w < kWaves; w++)
+      least = key_max(least, thresholds[w]);
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      const uint64_t key = key_at(j);
+      if (key >= least)
+        list[atomicAdd(&found[0], 1)] = key;
+    }
   }
   // the row's ones, the sum of the others and the weighted sum, in units of the row's maximum
   int ones = 0;
@@ -228,9 +280,14 @@ __global__ __launch_bounds__(kThreads) void score_rows(Score p, int capacity) {
   for (int w = 0; w < kWaves; w++)
     ones += counts[w], rest += sums[w][0], weighted += sums[w][1];
   rest += (double)(ones - 1); // S - 1
-  const double log_sum = log1p(rest), temperature = (double)p.job.temperature;
-  auto logprob = [&](float l) { return (float)(((double)l - (double)most) / temperature - log_sum); };
-  if (tid == 0) {
+  int many = 0, held = 0;
+  if (top) {
+    many = found[0], held = min(many, top);
+    largest(list, many, top, scratch, [&](int at, uint64_t key) { best[at] = key; });
+  }
+  const double log_sum = log1p(rest), inverse = 1.0 / (double)p.job.temperature;
+  auto logprob = [&](float l) { return (float)(((double)l - (double)most) * inverse - log_sum); };
+  if (tid == kThreads - 1) { // of a wave that has least to do
     if (p.job.logprob) {
       p.job.logprob[row] = inside ? logprob(given) : token == -1 ? 0.0f : NAN;
       if (!inside && token != -1)
@@ -241,78 +298,72 @@ __global__ __launch_bounds__(kThreads) void score_rows(Score p, int capacity) {
   }
   if (top == 0)
     return;
-  // the largest group maximum of each thread; the top-th of them is a bound that `top` groups reach
-  const float *maxima = p.maxima + (size_t)row * p.chunks * kGroups;
-  const int groups = (p.job.vocab + kGroup - 1) / kGroup;
-  uint64_t mine = 0;
-  for (int g = tid; g < groups; g += kThreads) {
-    const uint64_t key = maxima[g] > -INFINITY ? key_of(maxima[g], g) : 0;
-    mine = key > mine ? key : mine;
-  }
-  mine_of[tid] = mine;
-  if (tid == 0)
-    found = 0, threshold = 1; // 1: every key there is
-  for (int i = tid; i < top; i += kThreads)
-    best[i] = 0;
-  __syncthreads();
-  int before = 0;
-  for (int j = 0; j < kThreads; j++)
-    before += mine_of[j] > mine;
-  if (mine && before == top - 1)
-    threshold = mine;
-  __syncthreads();
-  const uint64_t least = threshold;
-  for (int g = tid; g < groups; g += kThreads) {
-    const uint64_t key = maxima[g] > -INFINITY ? key_of(maxima[g], g) : 0;
-    if (key >= least) { // of at most `top` threads' groups: `capacity` keys
-      const int at = atomicAdd(&found, 1);
-      if (at < capacity)
-        list[at] = key;
+  __syncthreads(); // best is whole, and the list read
+  if (p.count == p.chunks) { // the chunks' groups, then the largest of those
+    for (int i = wave; i < held; i += kWaves) {
+      const int chunk = place_of(best[i]);
+      float x[kGroups];
+#pragma unroll
+      for (int j = 0; j < kGroups; j++) {
+        const int at = chunk * kChunk + j * kGroup + lane;
+        x[j] = at < p.job.vocab ? logits[at] : -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < kGroups; j++) {
+        const float m = wave_max(x[j]);
+        if (lane == 0 && m > -INFINITY)
+          list[atomicAdd(&found[2], 1)] = key_of(m, chunk * kGroups + j);
+      }
     }
+    __syncthreads();
+    many = found[2];
+    largest(list, many, top, scratch, [&](int at, uint64_t key) { best[at] = key; });
+    held = min(many, top);
+    __syncthreads();
   }
-  __syncthreads();
-  const int many = min(found, capacity);
-  largest(list, many, top, best, scratch);
-  // their tokens that reach the last one's maximum, then the largest of those
-  const int held = min(many, top);
-  const uint64_t weakest = best[held - 1];
-  const float reach = many < top ? -INFINITY : value_of(weakest);
-  int group = 0;
-  __syncthreads(); // every thread has read `found`
-  if (tid == 0)
-    found = 0;
-  __syncthreads();
-  for (int i = wave; i < held; i += kWaves) {
-    group = place_of(best[i]);
-    const int at = group * kGroup + lane;
-    const float x = at < p.job.vocab ? logits[at] : -INFINITY;
-    if (x >= reach && x > -INFINITY)
-      list[atomicAdd(&found, 1)] = key_of(x, at);
+  // the groups' tokens that reach the last one's maximum, then the largest of those
+  const float reach = many < top ? -INFINITY : value_of(best[held - 1]);
+  constexpr int kMost = LLHIP_MAX_TOP / kWaves; // groups of a wave
+  float x[kMost];
+  int place[kMost];
+#pragma unroll
+  for (int i = 0; i < kMost; i++) {
+    const int which = wave + i * kWaves;
+    place[i] = which < held ? place_of(best[which]) * kGroup + lane : p.job.vocab;
+    x[i] = place[i] < p.job.vocab ? logits[place[i]] : -INFINITY;
   }
+#pragma unroll
+  for (int i = 0; i < kMost; i++)
+    if (x[i] >= reach && x[i] > -INFINITY)
+      list[atomicAdd(&found[1], 1)] = key_of(x[i], place[i]);
   __syncthreads();
-  const int tokens = found;
-  __syncthreads(); // best is read
-  largest(list, tokens, top, best, scratch);
-  for (int i = tid; i < top; i += kThreads) {
-    const bool there = i < tokens;
-    p.job.top_token[(size_t)row * top + i] = there ? place_of(best[i]) : -1;
-    p.job.top_logprob[(size_t)row * top + i] = there ? logprob(value_of(best[i])) : -INFINITY;
-  }
+  const int tokens = found[1];
+  largest(list, tokens, top, scratch, [&](int at, uint64_t key) {
+    p.job.top_token[(size_t)row * top + at] = place_of(key);
+    p.job.top_logprob[(size_t)row * top + at] = logprob(value_of(key));
+  });
+  for (int i = tokens + tid; i < top; i += kThreads)
+    p.job.top_token[(size_t)row * top + i] = -1, p.job.top_logprob[(size_t)row * top + i] = -INFINITY;
 }
 
 int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
+int maxima_of(int vocab) {
+  const int groups = (vocab + kGroup - 1) / kGroup;
+  return groups <= kThreads * kPer ? groups : chunks_of(vocab);
+}
+
 } // namespace
 
 size_t scores_workspace(const ScoreJob &job) {
-  const size_t chunks = (size_t)job.rows * chunks_of(job.vocab);
-  return chunks * sizeof(Stat) + (job.top ? chunks * kGroups * sizeof(float) : 0);
+  return (size_t)job.rows * (chunks_of(job.vocab) * sizeof(Stat) + (job.top ? maxima_of(job.vocab) * sizeof(float) : 0));
 }
 
 bool launch_scores(const ScoreJob &job, void *workspace, hipStream_t stream) {
   Score p{};
   p.job = job;
   p.chunks = chunks_of(job.vocab);
+  p.count = maxima_of(job.vocab);
   p.stats = (Stat *)workspace;
   p.maxima = job.top ? (float *)(p.stats + (size_t)job.rows * p.chunks) : nullptr;
   const double scale2 = 1.4426950408889634 / (double)job.temperature;
@@ -327,15 +378,9 @@ bool launch_scores(const ScoreJob &job, void *workspace, hipStream_t stream) {
     if (!launch_ok("score_stats"))
       return false;
   }
-  // a thread's groups of at most `top` threads, or 64 tokens of `top` groups
-  const int groups = p.chunks * kGroups, capacity = job.top * ((groups + kThreads - 1) / kThreads);
-  const int keys = capacity > job.top * kGroup ? capacity : job.top * kGroup;
-  static const hipError_t room = // 4 Mi tokens with 32 alternatives take 64 KB beside the rest
-      hipFuncSetAttribute((const void *)score_rows, hipFuncAttributeMaxDynamicSharedMemorySize, 64 << 10);
-  if (room != hipSuccess)
-    return raise("score_rows: %s", hipGetErrorString(room));
-  hipLaunchKernelGGL(score_rows, dim3((unsigned)job.rows), dim3(kThreads), (size_t)keys * sizeof(uint64_t), stream, p,
-                     capacity);
+  const int per = (p.count + kThreads - 1) / kThreads, keys = job.top * (kGroup > kWaves * per ? kGroup : kWaves * per);
+  static_assert(LLHIP_MAX_TOP * kGroup * sizeof(uint64_t) <= 32 << 10 && kWaves * kPer <= kGroup, "the list's room");
+  hipLaunchKernelGGL(score_rows, dim3((unsigned)job.rows), dim3(kThreads), (size_t)keys * sizeof(uint64_t), stream, p);
   return launch_ok("score_rows");
 }
 
