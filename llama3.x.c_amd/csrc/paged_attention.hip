@@ -503,38 +503,45 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
       });
     }
   };
-  if constexpr (!ANY)
-    look_up(first);
-  // the query vectors, scaled, in the order in which K's dimensions come
+  // the query vectors on their way with the first step's rows, then scaled, in the order in which K's dimensions come
   constexpr int kParts = kBf16 ? 3 : 1;
   v4u qp[kSteps][kParts];
   {
     const int v = active ? v0 + lc : 0;
     const float *src = p.job.q + (size_t)(it.row0 + v / kv_mul) * p.job.q_stride + ((size_t)it.g * kv_mul + v % kv_mul) * hd;
+    float x[kSteps][kPerLoad];
 #pragma unroll
     for (int s = 0; s < kSteps; s++) {
       const int d = (4 * s + lq) * kPerLoad;
       const float *at = src + (d < hd ? d : 0);
-      float x[kPerLoad];
       if (p.q_vec) {
 #pragma unroll
         for (int c = 0; c < kPerLoad; c += 4) {
           const float4 four = *reinterpret_cast<const float4 *>(at + c);
-          x[c] = four.x, x[c + 1] = four.y, x[c + 2] = four.z, x[c + 3] = four.w;
+          x[s][c] = four.x, x[s][c + 1] = four.y, x[s][c + 2] = four.z, x[s][c + 3] = four.w;
         }
       } else {
 #pragma unroll
         for (int c = 0; c < kPerLoad; c++)
-          x[c] = at[c];
+          x[s][c] = at[c];
       }
+    }
+    if constexpr (!ANY)
+      look_up(first);
+    load_k(first, 0);
+    load_v(first, 0);
+    fence();
+#pragma unroll
+    for (int s = 0; s < kSteps; s++) {
+      const bool there = active && (4 * s + lq) * kPerLoad < hd;
 #pragma unroll
       for (int c = 0; c < kPerLoad; c++)
-        x[c] = active && d < hd ? x[c] * p.scale2 : 0.0f;
+        x[s][c] = there ? x[s][c] * p.scale2 : 0.0f;
       if constexpr (kBf16) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           unsigned part[3];
-          bf16_parts(x[2 * c], x[2 * c + 1], part);
+          bf16_parts(x[s][2 * c], x[s][2 * c + 1], part);
 #pragma unroll
           for (int k = 0; k < 3; k++)
             qp[s][k][c] = part[k];
@@ -542,12 +549,10 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
       } else {
 #pragma unroll
         for (int c = 0; c < 4; c++)
-          qp[s][0][c] = __float_as_uint(x[c]);
+          qp[s][0][c] = __float_as_uint(x[s][c]);
       }
     }
   }
-  load_k(first, 0);
-  load_v(first, 0);
   int i = 0; // the step's number since look_up
   unsigned odd_values = 0;
   for (int pos = first; pos < end; pos += stride) {
@@ -1179,6 +1184,8 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
         };
         if (items > 2 * kThreads)
           add_up(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+        else if (parts > 16 && items <= kThreads)
+          add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
         else if (parts > 4)
           add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
         else
@@ -1215,6 +1222,15 @@ template <typename T, int HD> FastKernel kernel_of(int mode, bool wide) {
 }
 template <typename T> FastKernel kernel_of(int dims, int mode, bool wide) {
   return dims == 64 ? kernel_of<T, 64>(mode, wide) : dims == 128 ? kernel_of<T, 128>(mode, wide) : kernel_of<T, 256>(mode, wide);
+}
+
+// Blocks of a KV head that the batch may need, whatever its arrays hold: a small one's are fewer than fill the device.
+int blocks_for(const AttentionPagedJob &job, int tile_rows) {
+  const long long rows = job.batch.rows, count = job.batch.count;
+  const long long tiles = (rows + tile_rows - 1) / tile_rows + (rows < count ? rows : count);
+  const long long line = tiles * (kBegin + kFullPosition * (long long)job.batch.seq_len);
+  const int all = blocks_of(job);
+  return line / kMinSlice < all ? (int)(line / kMinSlice) + 1 : all;
 }
 
 int mode_of(const AttentionPagedJob &job) {
@@ -1256,10 +1272,10 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipSt
   FastPaged p{};
   p.job = job;
   p.kv_mul = job.n_heads / job.n_kv_heads;
-  p.blocks = blocks_of(job);
   const bool wide = wide_tiles(job);
   p.tile_vectors = wide ? kWideVectors : kTileVectors;
   p.tile_rows = p.tile_vectors / p.kv_mul;
+  p.blocks = blocks_for(job, p.tile_rows);
   p.scale2 = (float)(1.4426950408889634 / sqrt((double)job.head_dim));
   p.partial = (float *)workspace;
   p.flags = device().error_flags;
