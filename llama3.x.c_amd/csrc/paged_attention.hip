@@ -306,11 +306,8 @@ __device__ __forceinline__ float four_max(float x) {
 
 // A part's sums go past the XCDs' own L2s: stores of agent scope write through, loads of agent scope read what they wrote. (A
 // release and an acquire around plain ones write back and drop a whole L2 a block: 32 requests took 134 us, not 65.) Each store
-// takes its place in memory's queues, whatever its size: 16 bytes a lane, side by side, where a lane's own 128 bytes as eights
-// took the prompts from %A% to 236 us.
-//
-// Sums lie row by row, [vector][HD], where the block's threads have them so (kRows), else as lanes have them: [16 vectors][r][e /
-// 4][lane] of four dimensions each.
+// takes its place in memory's queues, whatever its size, so the sums go out in whole rows, [vector][HD], 16 bytes a lane: as
+// lanes hold them, 128 bytes each, in stores of 8 bytes the prompts took 236 us, of 16 156.
 constexpr int kAgent = 16; // the cache policy's sc1
 struct Slot {
   __amdgpu_buffer_rsrc_t rsrc;
@@ -373,6 +370,42 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void *cache, lon
 //   permutes within the lane. Q and P as three exact parts each.
 //   F32: 4 dimensions, or 4 positions, an instruction; FP32 products.
 // Dimension of instruction e's row m: EV dimensions a lane, 16 lanes, further ones EV * 16 behind.
+// 16 vectors' sums of a wave, as its lanes hold them, row by row to the part's slot or, multiplied by the inverse of the
+// weights' sums, to out: through the wave's own rows of LDS, so that a store's lanes lie side by side.
+template <int HD, int EV, class Row>
+__device__ __forceinline__ void store_rows(const FastPaged &p, const Slot &slot, bool whole, const v4f (&o)[HD / 16], float inverse,
+                                           float *rows, int lane, int hd, int v0, int count, Row row_of) {
+  constexpr int kRow = HD + 4;
+  const int lq = lane >> 4, lc = lane & 15;
+  const float scale = whole ? inverse : 1.0f;
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int e = 0; e < HD / 16; e += 4) {
+      const int d = (e / EV * 16 + 4 * lq + r) * EV + e % EV;
+      *reinterpret_cast<float4 *>(rows + lc * kRow + d) =
+          float4{o[e][r] * scale, o[e + 1][r] * scale, o[e + 2][r] * scale, o[e + 3][r] * scale};
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // written by one lane, read by another
+  __builtin_amdgcn_wave_barrier();
+  const int hd4 = hd / 4;
+  for (int i = lane; i < count * hd4; i += kWave) {
+    const int v = i / hd4, d = i % hd4 * 4;
+    const float4 x = *reinterpret_cast<const float4 *>(rows + v * kRow + d);
+    if (!whole) {
+      put4(slot, (unsigned)((v0 + v) * (HD / 4) + d / 4), x);
+    } else {
+      float *to = row_of(v0 + v) + d;
+      if (p.out_vec)
+        *reinterpret_cast<float4 *>(to) = x;
+      else
+        to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // read before it is written again
+  __builtin_amdgcn_wave_barrier();
+}
+
 // MODE: whole heads of HD dimensions, heads of fewer, or either with pages that are no multiple of 16 positions.
 enum { kWhole, kPart, kAny };
 template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p, const Item &it, float *lds) {
@@ -737,21 +770,10 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
           put_end(slot, v, m, whole_l);
       }
     }
-  } else if (mine > 0) {
-    float *to = target(v0 + min(lc, mine - 1));
+  } else if (mine > 0) { // uniform
     if (!whole && lq == 0 && active)
       put_end(slot, v0 + lc, m_run, l);
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-      for (int f = 0; f < kFours; f++) {
-        const int e = 4 * f, d = (e / EV * 16 + 4 * lq + r) * EV + e % EV;
-        const float4 x = float4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
-        if (!whole)
-          put4(slot, (unsigned)((v0 / 16 * 4 + r) * kFours + f) * kWave + lane, x);
-        else if (active && d < hd)
-          store(to + d, float4{x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse});
-      }
+    store_rows<HD, EV>(p, slot, whole, o, inverse, lds + (size_t)wave * 16 * kRow, lane, hd, v0, mine, target);
   }
 }
 
@@ -990,39 +1012,25 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
   }
   const bool whole = it.slot < 0;
   const Slot slot = slot_at<HD>(p, max(it.slot, 0));
+  __syncthreads(); // the stages' place is free
+  auto target = [&](int v) {
+    return p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
+  };
 #pragma unroll
   for (int n = 0; n < NT; n++) {
     const float l = four_sum(l_run[n]), inverse = 1.0f / l;
-    const bool active = 16 * n + lc < mine;
-    const int v = active ? v0 + 16 * n + lc : 0;
-    float *to = p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
     if (16 * n >= mine)
       continue; // uniform
-    if (!whole && lq == 0 && active)
-      put_end(slot, v, m_run[n], l);
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const int d = (4 * lq + r) * EV + e;
-        float4 x = float4{o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]};
-        if (!whole) {
-          put4(slot, (unsigned)(((v0 / 16 + n) * 4 + r) * (E / 4) + e / 4) * kWave + lane, x);
-        } else if (active && d < hd) {
-          x = float4{x.x * inverse, x.y * inverse, x.z * inverse, x.w * inverse};
-          if (p.out_vec)
-            *reinterpret_cast<float4 *>(to + d) = x;
-          else
-            to[d] = x.x, to[d + 1] = x.y, to[d + 2] = x.z, to[d + 3] = x.w;
-        }
-      }
+    if (!whole && lq == 0 && 16 * n + lc < mine)
+      put_end(slot, v0 + 16 * n + lc, m_run[n], l);
+    store_rows<HD, EV>(p, slot, whole, o[n], inverse, lds + (size_t)wave * 16 * kRow, lane, hd, v0 + 16 * n,
+                       min(mine - 16 * n, 16), target);
   }
 }
 
 template <typename T, int HD, int MODE, bool WIDE>
 __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn_paged(FastPaged p) {
-  constexpr int kRow = HD + 4, E = HD / 16;
-  constexpr int EV = WIDE ? E : E < (sizeof(T) == 2 ? 8 : 4) ? E : (sizeof(T) == 2 ? 8 : 4); // as in the walks
+  constexpr int kRow = HD + 4;
   __shared__ Plan plan;
   __shared__ __align__(16) float lds[kWaves * 16 * kRow];
   __shared__ unsigned arrived;
@@ -1101,34 +1109,50 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       if (tid == 0)
         __hip_atomic_store(&paged_arrivals[g * p.blocks + first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       // The parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
-      // LDS by a wave a vector, then the sums in the parts' order, whoever comes last. A part's place by its number.
+      // LDS, then the sums in the parts' order, whoever comes last. A part's place by its number.
       auto part = [&](int k) { return slot_at<HD>(p, slot_of(from + k, from + k == first)); };
-      const int hd4 = hd / 4;
-      const bool sets = it.walkers == 1; // sums as lanes have them, in sets of 16 vectors
-      int some = kWaves * 16 * kRow / parts;
-      if (sets && some >= 16)
-        some &= ~15;
-      for (int v0 = 0, n; v0 < it.vectors; v0 += n) {
-        n = min(some, it.vectors - v0);
-        if (sets && some < 16)
-          n = min(n, 16 - v0 % 16); // of one set
+      const int hd4 = hd / 4, some = kWaves * 16 * kRow / parts;
+      for (int v0 = 0; v0 < it.vectors; v0 += some) {
+        const int n = min(some, it.vectors - v0), items = n * hd4;
         __syncthreads(); // LDS is free
-        for (int v = tid / kWave; v < n; v += kWaves) {
-          float m = -FLT_MAX, l = 0.0f;
-          for (int k = tid % kWave; k < parts; k += kWave) {
-            const float2 end_of = load_end(p, slot_of(from + k, from + k == first), v0 + v, HD);
-            lds[v * parts + k] = end_of.x;
-            const float top = fmaxf(m, end_of.x);
-            l = l * __builtin_amdgcn_exp2f(m - top) + end_of.y * __builtin_amdgcn_exp2f(end_of.x - top);
-            m = top;
+        constexpr int kFew = 8;
+        if (parts <= kFew) { // a thread a vector, its loads together
+          for (int v = tid; v < n; v += kThreads) {
+            float2 x[kFew];
+#pragma unroll
+            for (int k = 0; k < kFew; k++)
+              x[k] = load_end(p, slot_of(from + min(k, parts - 1), from + min(k, parts - 1) == first), v0 + v, HD);
+            float m = -FLT_MAX, l = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kFew; k++)
+              m = fmaxf(m, x[k].x);
+#pragma unroll
+            for (int k = 0; k < kFew; k++) {
+              x[k].x = __builtin_amdgcn_exp2f(x[k].x - m);
+              l = k < parts ? fmaf(x[k].x, x[k].y, l) : l;
+            }
+            const float inverse = 1.0f / l;
+#pragma unroll
+            for (int k = 0; k < kFew; k++)
+              if (k < parts)
+                lds[v * parts + k] = x[k].x * inverse;
           }
-          const float top = wave_max(m);
-          l = wave_sum(l * __builtin_amdgcn_exp2f(m - top));
-          for (int k = tid % kWave; k < parts; k += kWave)
-            lds[v * parts + k] = __builtin_amdgcn_exp2f(lds[v * parts + k] - top) / l;
+        } else {
+          for (int v = tid / kWave; v < n; v += kWaves) {
+            float m = -FLT_MAX, l = 0.0f;
+            for (int k = tid % kWave; k < parts; k += kWave) {
+              const float2 end_of = load_end(p, slot_of(from + k, from + k == first), v0 + v, HD);
+              lds[v * parts + k] = end_of.x;
+              const float top = fmaxf(m, end_of.x);
+              l = l * __builtin_amdgcn_exp2f(m - top) + end_of.y * __builtin_amdgcn_exp2f(end_of.x - top);
+              m = top;
+            }
+            const float top = wave_max(m), inverse = 1.0f / wave_sum(l * __builtin_amdgcn_exp2f(m - top));
+            for (int k = tid % kWave; k < parts; k += kWave)
+              lds[v * parts + k] = __builtin_amdgcn_exp2f(lds[v * parts + k] - top) * inverse;
+          }
         }
         __syncthreads();
-        const int set0 = v0 & ~15, items = sets ? ceil_div(v0 + n - set0, 16) * 16 * (HD / 4) : n * hd4;
         // I of the thread's items and K parts at a time: as many loads are in flight
         auto add_up = [&](auto of_items, auto of_parts) {
           constexpr int I = decltype(of_items)::value, K = decltype(of_parts)::value;
@@ -1139,16 +1163,9 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
 #pragma unroll
             for (int j = 0; j < I; j++) {
               const int i = i0 + j * kThreads;
-              if (sets) { // [16 vectors][r][e / 4][lane]
-                const int lane = i % kWave, f = i / kWave % (E / 4), r = i / kWave / (E / 4) % 4, e = 4 * f;
-                v[j] = set0 - v0 + i / (16 * (HD / 4)) * 16 + lane % 16;
-                d[j] = (e / EV * 16 + 4 * (lane / 16) + r) * EV + e % EV;
-                at[j] = (unsigned)(set0 * (HD / 4) + i);
-              } else {
-                v[j] = i / hd4, d[j] = i % hd4 * 4;
-                at[j] = (unsigned)((v0 + v[j]) * (HD / 4) + d[j] / 4);
-              }
-              if (i >= items || v[j] < 0 || v[j] >= n || d[j] >= hd)
+              v[j] = i / hd4, d[j] = i % hd4 * 4;
+              at[j] = (unsigned)((v0 + v[j]) * (HD / 4) + d[j] / 4);
+              if (i >= items)
                 v[j] = 0, d[j] = -1, at[j] = kNowhere / 16; // reads zero
               sum[j] = float4{0.0f, 0.0f, 0.0f, 0.0f};
             }
