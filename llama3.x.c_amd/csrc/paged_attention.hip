@@ -191,6 +191,7 @@ struct FastPaged {
   int kv_mul, blocks; // blocks: of a KV head
   int tile_rows;      // rows of a full tile
   int tile_vectors;   // at most, of a tile: kTileVectors or kWideVectors
+  int full_begin, full_position; // begin_time and position_time of a full tile
   float scale2;       // log2(e) / sqrt(hd)
   // slots of tile_vectors (HD + 2) floats, [KV head][block][0: a walk that an earlier block began, 1: one that this block
   // begins]: the vectors' sums, then their maxima and weights' sums
@@ -213,29 +214,35 @@ __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // The walks of a KV head lie one behind the other on a line, each as long as it takes in time, and the line is cut into
 // slices of one length, one for a block: all blocks start together and end together. A walk's begin and end take as long as
-// kBegin positions of a small tile.
-constexpr int kBegin = 256;
+// begin_time positions of a small tile.
+constexpr int kBegin = 256, kWideBegin = 768;
 // A slice is at least this long: shorter ones do not pay for a walk's join, and a block inside a walk has some of its
-// positions however they are rounded (kRound of a small tile's take as long as a round of any).
+// positions however they are rounded (a round is unit * grain long).
 constexpr int kMinSlice = 2 * kRound;
-static_assert(kMinSlice >= kRound, "a slice holds a round");
 
 // Waves that walk a tile's positions together, a wave 16 vectors: four, two or one.
 __device__ __forceinline__ int walkers_of(int vectors) { return vectors <= 16 ? 4 : vectors <= 32 ? 2 : 1; }
 // How long a position takes: with fewer waves a tile, longer.
-__device__ __forceinline__ int position_time(int vectors) { return kWaves / walkers_of(vectors); }
-constexpr int kFullPosition = kWaves;
+constexpr int kWidePosition = 4;
+__device__ __forceinline__ int position_time(int vectors) {
+  return vectors > kTileVectors ? kWidePosition : kWaves / walkers_of(vectors);
+}
+
+__device__ __forceinline__ int begin_time(int vectors) { return vectors > kTileVectors ? kWideBegin : kBegin; }
+constexpr int kMostTime = kWidePosition > kWaves ? kWidePosition : kWaves;
+static_assert(kMinSlice >= kWidePosition * kStep && kMinSlice >= kRound, "a slice holds a round");
 
 // Where tile t of a request begins on the request's part of the line: t full tiles before it, tile i of length + (i + 1)
 // tile_rows positions.
 __device__ __forceinline__ long long tile_start(const FastPaged &p, int length, long long t) {
-  return t * kBegin + kFullPosition * (t * length + p.tile_rows * (t * (t + 1) / 2));
+  return t * p.full_begin + p.full_position * (t * length + p.tile_rows * (t * (t + 1) / 2));
 }
 __device__ __forceinline__ long long request_time(const FastPaged &p, const PagedRequest &q) {
   if (q.rows == 0)
     return 0;
   const int t = ceil_div(q.rows, p.tile_rows) - 1, rest = q.rows - t * p.tile_rows;
-  return tile_start(p, q.length, t) + kBegin + (long long)position_time(rest * p.kv_mul) * (q.length + q.rows);
+  return tile_start(p, q.length, t) + begin_time(rest * p.kv_mul) +
+         (long long)position_time(rest * p.kv_mul) * (q.length + q.rows);
 }
 
 struct Plan {
@@ -914,6 +921,7 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
   stage(stages[0], it.t0);
   load(it.t0 + kStep, i++);
   int turn = 0;
+  constexpr int kAheadK = 4 < 2 * kSteps ? 4 : 2 * kSteps, kAheadV = 2;
   for (int pos = it.t0; pos < end; pos += kStep, turn ^= 1) {
     const Stage &sh = stages[turn];
     __syncthreads(); // the step is staged, the one before it computed
@@ -923,17 +931,26 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
 #pragma unroll
       for (int t = 0; t < 2; t++)
         sc[n][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    // each operand is read four (two) uses ahead: left to itself the compiler reads one, waits for it and uses it
+    v4u a[2 * kSteps];
+    auto read_k = [&](int i) {
+      a[i] = *reinterpret_cast<const v4u *>(&sh.k[(16 * (i % 2) + lc) * Stage::kKRow + 32 * (i / 2) + 8 * lq]);
+    };
 #pragma unroll
-    for (int s = 0; s < kSteps; s++)
+    for (int i = 0; i < kAheadK; i++)
+      read_k(i);
+    fence();
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        const v4u a = *reinterpret_cast<const v4u *>(&sh.k[(16 * t + lc) * Stage::kKRow + 32 * s + 8 * lq]);
+    for (int i = 0; i < 2 * kSteps; i++) {
+      if (i + kAheadK < 2 * kSteps)
+        read_k(i + kAheadK);
 #pragma unroll
-        for (int k = 2; k >= 0; k--)
+      for (int k = 2; k >= 0; k--)
 #pragma unroll
-          for (int n = 0; n < NT; n++)
-            sc[n][t] = mfma_bf16(a, qp[n][s][k], sc[n][t]);
-      }
+        for (int n = 0; n < NT; n++)
+          sc[n][i % 2] = mfma_bf16(a[i], qp[n][i / 2][k], sc[n][i % 2]);
+      fence();
+    }
     stage(stages[turn ^ 1], pos + kStep);
     if (i == kWave / 2) { // uniform
       look_up(pos + 2 * kStep);
@@ -981,14 +998,21 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
           wp[n][k][c] = part[k];
       }
     }
+    v4u v[E];
+#pragma unroll
+    for (int e = 0; e < kAheadV; e++)
+      v[e] = sh.v[e][lane];
+    fence();
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const v4u a = sh.v[e][lane];
+      if (e + kAheadV < E)
+        v[e + kAheadV] = sh.v[e + kAheadV][lane];
 #pragma unroll
       for (int k = 2; k >= 0; k--)
 #pragma unroll
         for (int n = 0; n < NT; n++)
-          o[n][e] = mfma_bf16(a, wp[n][k], o[n][e]);
+          o[n][e] = mfma_bf16(v[e], wp[n][k], o[n][e]);
+      fence();
     }
   }
   if (odd != 0.0f)
@@ -1066,13 +1090,13 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       Item it;
       it.vectors = rows * kv_mul;
       it.walkers = walkers_of(it.vectors);
-      const int unit = position_time(it.vectors), grain = it.walkers * kStep;
-      const long long end = w0 + kBegin + (long long)unit * positions;
+      const int begin = begin_time(it.vectors), unit = position_time(it.vectors), grain = it.walkers * kStep;
+      const long long end = w0 + begin + (long long)unit * positions;
       // the position that lies at x of the line, in whole rounds
       auto position_at = [&](long long x) {
         if (x >= end)
           return positions;
-        const int at = x <= w0 + kBegin ? 0 : (int)((x - w0 - kBegin) / unit);
+        const int at = x <= w0 + begin ? 0 : (int)((x - w0 - begin) / unit);
         return min(at / grain * grain, positions);
       };
       it.t0 = w0 >= lo ? 0 : position_at(lo);
@@ -1098,7 +1122,7 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       // the walk's blocks: from .. last_block
       const int first = (int)whole(w0, slice), last_block = (int)whole(end - 1, slice);
       // the first block whose slice ends behind the walk's first round
-      const int from = min(max(first, (int)whole(w0 + kBegin + kRound - 1, slice)), last_block), parts = last_block - from + 1;
+      const int from = min(max(first, (int)whole(w0 + begin + unit * grain - 1, slice)), last_block), parts = last_block - from + 1;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
       __syncthreads();                                 // the block's
       if (tid == 0)
@@ -1245,7 +1269,7 @@ template <typename T> FastKernel kernel_of(int dims, int mode, bool wide) {
 int blocks_for(const AttentionPagedJob &job, int tile_rows) {
   const long long rows = job.batch.rows, count = job.batch.count;
   const long long tiles = (rows + tile_rows - 1) / tile_rows + (rows < count ? rows : count);
-  const long long line = tiles * (kBegin + kFullPosition * (long long)job.batch.seq_len);
+  const long long line = tiles * (kWideBegin + kMostTime * (long long)job.batch.seq_len);
   const int all = blocks_of(job);
   return line / kMinSlice < all ? (int)(line / kMinSlice) + 1 : all;
 }
@@ -1292,6 +1316,8 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipSt
   const bool wide = wide_tiles(job);
   p.tile_vectors = wide ? kWideVectors : kTileVectors;
   p.tile_rows = p.tile_vectors / p.kv_mul;
+  p.full_begin = wide ? kWideBegin : kBegin;
+  p.full_position = wide ? kWidePosition : kWaves / (p.tile_rows * p.kv_mul <= 16 ? 4 : p.tile_rows * p.kv_mul <= 32 ? 2 : 1);
   p.blocks = blocks_for(job, p.tile_rows);
   p.scale2 = (float)(1.4426950408889634 / sqrt((double)job.head_dim));
   p.partial = (float *)workspace;
