@@ -184,7 +184,8 @@ constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far be
 
 // How many of a walk's blocks have stored their part, by the block that the walk begins in: zero between launches, as the
 // last to arrive sets it back.
-__device__ unsigned paged_arrivals[kMaxArrivals];
+constexpr int kLine = 32; // each in a cache line of its own: additions to one line wait for each other
+__device__ unsigned paged_arrivals[kMaxArrivals * kLine];
 
 struct FastPaged {
   AttentionPagedJob job;
@@ -1126,12 +1127,12 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
       __syncthreads();                                 // the block's
       if (tid == 0)
-        arrived = __hip_atomic_fetch_add(&paged_arrivals[g * p.blocks + first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        arrived = __hip_atomic_fetch_add(&paged_arrivals[(g * p.blocks + first) * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
       if (arrived != (unsigned)(parts - 1))
         continue;
       if (tid == 0)
-        __hip_atomic_store(&paged_arrivals[g * p.blocks + first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(&paged_arrivals[(g * p.blocks + first) * kLine], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       // The parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
       // LDS, then the sums in the parts' order, whoever comes last. A part's place by its number.
       auto part = [&](int k) { return slot_at<HD>(p, slot_of(from + k, from + k == first)); };

@@ -3,6 +3,7 @@
 //   score_stats   a wave each chunk of 1024 tokens of a row: the chunk's maximum, the sums of exp z and of z exp z relative to
 //                 it, and, where alternatives are asked for, the maximum of each group of 64 tokens. One read. HBM-bound.
 //   score_rows    block (row): the chunks joined; the alternatives from the groups that can hold them.
+//   score_few     both in one launch, for few rows: the last of a row's blocks to arrive joins its chunks.
 //
 // The k likeliest tokens lie in the k groups whose maxima are largest (of equal ones the lower group's): any other group has
 // k groups before it, each with a token at least as large, and lower where it is as large. So the second kernel reads
@@ -24,6 +25,12 @@ constexpr int kGroup = 64;   // tokens of a maximum: those of 16 lanes' float4
 constexpr int kGroups = kChunk / kGroup;
 constexpr int kPer = 16;       // maxima of a thread of score_rows, at most: rows of more than 4096 groups keep their chunks'
 constexpr int kRankList = 512; // candidates that are ranked each against each
+constexpr int kFewRows = 16;   // of score_few, at most: 8 rows with 32 alternatives take 13.1 us there and 13.4 in two launches, 64 with 20 26 and 18
+
+// How many of a row's blocks have stored their chunks: zero between launches, as the last to arrive sets it back. Each in a
+// cache line of its own: additions to one line wait for each other (64 rows: 12 us instead of 19).
+constexpr int kLine = 32;
+__device__ unsigned score_arrivals[kFewRows * kLine];
 
 bool launch_ok(const char *what) {
   const hipError_t e = hipGetLastError();
@@ -50,8 +57,43 @@ struct Score {
   bool vec4;
 };
 
-__global__ __launch_bounds__(kThreads) void score_stats(Score p, int row0) {
-  const int row = row0 + blockIdx.y, lane = threadIdx.x % kWave, chunk = blockIdx.x * kWaves + threadIdx.x / kWave;
+// What one block stores and another of the same launch reads passes the XCDs' own L2s: stores of agent scope write through,
+// loads of agent scope read what they wrote.
+template <bool AGENT> __device__ __forceinline__ void put(float *p, float x) {
+  if constexpr (AGENT)
+    __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else
+    *p = x;
+}
+template <bool AGENT> __device__ __forceinline__ float get(const float *p) {
+  if constexpr (AGENT)
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else
+    return *p;
+}
+struct Halves {
+  unsigned long long lo, hi;
+};
+template <bool AGENT> __device__ __forceinline__ void put(Stat *p, const Stat &x) {
+  if constexpr (AGENT) {
+    const Halves h = __builtin_bit_cast(Halves, x);
+    __hip_atomic_store((unsigned long long *)p, h.lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store((unsigned long long *)p + 1, h.hi, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  } else {
+    *p = x;
+  }
+}
+template <bool AGENT> __device__ __forceinline__ Stat get(const Stat *p) {
+  if constexpr (AGENT)
+    return __builtin_bit_cast(Stat, Halves{__hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                                           __hip_atomic_load((const unsigned long long *)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)});
+  else
+    return *p;
+}
+
+// One chunk of a row, by a wave.
+template <bool AGENT> __device__ __forceinline__ void score_chunk(const Score &p, int row, int chunk) {
+  const int lane = threadIdx.x % kWave;
   const float *src = p.job.logits + (size_t)row * p.job.ld;
   const int i0 = chunk * kChunk, n = min(kChunk, p.job.vocab - i0);
   if (n <= 0)
@@ -86,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void score_stats(Score p, int row0) {
     const int j = lane % 16, group = chunk * kGroups + 4 * j + lane / 16;
     const float mine = j == 0 ? four[0] : j == 1 ? four[1] : j == 2 ? four[2] : four[3];
     if (j < 4 && group < p.count)
-      p.maxima[(size_t)row * p.count + group] = mine;
+      put<AGENT>(&p.maxima[(size_t)row * p.count + group], mine);
   }
   float top = fmaxf(fmaxf(four[0], four[1]), fmaxf(four[2], four[3]));
   top = fmaxf(top, __shfl_xor(top, 16));
@@ -109,10 +151,14 @@ __global__ __launch_bounds__(kThreads) void score_stats(Score p, int row0) {
     weighted = wave_sum(weighted);
   }
   if (lane == 0) {
-    p.stats[(size_t)row * p.chunks + chunk] = Stat{bad ? INFINITY : top, ones, rest, weighted};
+    put<AGENT>(&p.stats[(size_t)row * p.chunks + chunk], Stat{bad ? INFINITY : top, ones, rest, weighted});
     if (p.maxima && p.count == p.chunks)
-      p.maxima[(size_t)row * p.count + chunk] = top;
+      put<AGENT>(&p.maxima[(size_t)row * p.count + chunk], top);
   }
+}
+
+__global__ __launch_bounds__(kThreads) void score_stats(Score p, int row0) {
+  score_chunk<false>(p, row0 + blockIdx.y, blockIdx.x * kWaves + threadIdx.x / kWave);
 }
 
 __device__ __forceinline__ double wave_add(double v) {
@@ -187,27 +233,26 @@ __device__ __forceinline__ uint64_t kth_of_wave(uint64_t mine, int k) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, at) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, at);
 }
 
-// LDS holds `list` keys: those of a thread's maxima of `top` lanes a wave, 16 of each of `top` chunks, 64 of each of `top`
+// A row's chunks joined, by a block. LDS holds `list` keys: those of a thread's maxima of `top` lanes a wave, 16 of each of `top` chunks, 64 of each of `top`
 // groups, whichever are more.
-__global__ __launch_bounds__(kThreads) void score_rows(Score p) {
-  extern __shared__ uint64_t list[];
+template <bool AGENT> __device__ __forceinline__ void score_row(const Score &p, int row, uint64_t *list) {
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves][2];
   __shared__ int counts[kWaves];
   __shared__ uint64_t thresholds[kWaves], best[LLHIP_MAX_TOP], scratch[kWaves];
   __shared__ int found[3];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, top = p.job.top;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave, top = p.job.top;
   const float *logits = p.job.logits + (size_t)row * p.job.ld;
   const Stat *stats = p.stats + (size_t)row * p.chunks;
   // what can be loaded at once is
   const int token = p.job.tokens ? p.job.tokens[row] : -1;
-  const Stat first = tid < p.chunks ? stats[tid] : Stat{-INFINITY, 0, 0.0f, 0.0f};
+  const Stat first = tid < p.chunks ? get<AGENT>(&stats[tid]) : Stat{-INFINITY, 0, 0.0f, 0.0f};
   float maxima[kPer];
   if (top) {
     const float *src = p.maxima + (size_t)row * p.count;
 #pragma unroll
     for (int j = 0; j < kPer; j++)
-      maxima[j] = tid + j * kThreads < p.count ? src[tid + j * kThreads] : -INFINITY;
+      maxima[j] = tid + j * kThreads < p.count ? get<AGENT>(&src[tid + j * kThreads]) : -INFINITY;
   }
   const bool inside = token >= 0 && token < p.job.vocab;
   const float given = inside ? logits[token] : 0.0f;
@@ -215,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void score_rows(Score p) {
     found[tid] = 0;
   float most = first.top;
   for (int c = tid + kThreads; c < p.chunks; c += kThreads)
-    most = fmaxf(most, stats[c].top);
+    most = fmaxf(most, get<AGENT>(&stats[c].top));
   most = wave_max(most);
   if (lane == 0)
     tops[wave] = most;
@@ -268,7 +313,7 @@ __global__ __launch_bounds__(kThreads) void score_rows(Score p) {
   };
   join(first);
   for (int c = tid + kThreads; c < p.chunks; c += kThreads)
-    join(stats[c]);
+    join(get<AGENT>(&stats[c]));
   ones = group_reduce_add(ones, kWave);
   rest = wave_add(rest);
   weighted = wave_add(weighted);
@@ -346,6 +391,28 @@ __global__ __launch_bounds__(kThreads) void score_rows(Score p) {
     p.job.top_token[(size_t)row * top + i] = -1, p.job.top_logprob[(size_t)row * top + i] = -INFINITY;
 }
 
+__global__ __launch_bounds__(kThreads) void score_rows(Score p) {
+  extern __shared__ uint64_t list[];
+  score_row<false>(p, blockIdx.x, list);
+}
+
+__global__ __launch_bounds__(kThreads) void score_few(Score p) {
+  extern __shared__ uint64_t list[];
+  __shared__ unsigned arrived;
+  const int row = blockIdx.y;
+  score_chunk<true>(p, row, blockIdx.x * kWaves + threadIdx.x / kWave);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's stores have arrived
+  __syncthreads();                                 // the block's
+  if (threadIdx.x == 0)
+    arrived = __hip_atomic_fetch_add(&score_arrivals[row * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived != gridDim.x - 1)
+    return;
+  if (threadIdx.x == 0)
+    __hip_atomic_store(&score_arrivals[row * kLine], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  score_row<true>(p, row, list);
+}
+
 int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 int maxima_of(int vocab) {
@@ -370,17 +437,22 @@ bool launch_scores(const ScoreJob &job, void *workspace, hipStream_t stream) {
   p.scale2 = scale2 < 1e38 ? (float)scale2 : 1e38f; // finite: a difference of 0 stays 0
   p.flags = device().error_flags;
   p.vec4 = job.ld % 4 == 0 && ((uintptr_t)job.logits & 15) == 0;
+  const int per = (p.count + kThreads - 1) / kThreads, keys = job.top * (kGroup > kWaves * per ? kGroup : kWaves * per);
+  static_assert(LLHIP_MAX_TOP * kGroup * sizeof(uint64_t) <= 32 << 10 && kWaves * kPer <= kGroup, "the list's room");
+  const size_t list = (size_t)keys * sizeof(uint64_t);
+  const unsigned blocks = (unsigned)((p.chunks + kWaves - 1) / kWaves); // of a row
+  if (job.rows <= kFewRows) {
+    hipLaunchKernelGGL(score_few, dim3(blocks, (unsigned)job.rows), dim3(kThreads), list, stream, p);
+    return launch_ok("score_few");
+  }
   const int most = 32768; // rows of a launch
   for (int row0 = 0; row0 < job.rows; row0 += most) {
-    const dim3 grid((unsigned)((p.chunks + kWaves - 1) / kWaves),
-                    (unsigned)(job.rows - row0 < most ? job.rows - row0 : most));
+    const dim3 grid(blocks, (unsigned)(job.rows - row0 < most ? job.rows - row0 : most));
     hipLaunchKernelGGL(score_stats, grid, dim3(kThreads), 0, stream, p, row0);
     if (!launch_ok("score_stats"))
       return false;
   }
-  const int per = (p.count + kThreads - 1) / kThreads, keys = job.top * (kGroup > kWaves * per ? kGroup : kWaves * per);
-  static_assert(LLHIP_MAX_TOP * kGroup * sizeof(uint64_t) <= 32 << 10 && kWaves * kPer <= kGroup, "the list's room");
-  hipLaunchKernelGGL(score_rows, dim3((unsigned)job.rows), dim3(kThreads), (size_t)keys * sizeof(uint64_t), stream, p);
+  hipLaunchKernelGGL(score_rows, dim3((unsigned)job.rows), dim3(kThreads), list, stream, p);
   return launch_ok("score_rows");
 }
 
