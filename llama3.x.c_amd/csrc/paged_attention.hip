@@ -198,6 +198,7 @@ struct FastPaged {
   // begins]: the vectors' sums, then their maxima and weights' sums
   float *partial;
   int *flags;
+  bool pairs;   // two blocks to a CU, and an even number to a KV head: the first half of them are the CUs' first blocks
   bool q_vec;   // q in whole 16-byte vectors
   bool out_vec; // out likewise
 };
@@ -254,6 +255,27 @@ struct Plan {
 // x / y of the line's lengths (below 2^50, where the double quotient's whole part is exact), a third of the time that the
 // compiler's division takes.
 __device__ __forceinline__ long long whole(long long x, long long y) { return (long long)((double)x / (double)y); }
+
+// The line's slices: as long as it is through all blocks, those of the CUs' first blocks are longer by a kFirstMore-th, those
+// of the second ones shorter, which the CU's arbitration leaves behind (with equal slices the prompts' second blocks took 107 us
+// beside 88; all together 131.5 us, now 126). Without wide tiles memory sets the pace, and equal slices were as good.
+constexpr int kFirstMore = 5;
+struct Slices {
+  long long first, second; // of a block before and from `turn` on
+  int turn;
+  __device__ __forceinline__ long long start(int block) const {
+    return block <= turn ? block * first : turn * first + (block - turn) * second;
+  }
+  __device__ __forceinline__ int block_of(long long x) const { // that x lies in the slice of
+    return x < turn * first ? (int)whole(x, first) : turn + (int)whole(x - turn * first, second);
+  }
+};
+__device__ __forceinline__ Slices make_slices(const FastPaged &p, long long total) {
+  const long long even = whole(total + p.blocks - 1, p.blocks), more = whole(even, kFirstMore);
+  if (!p.pairs || even - more < kMinSlice)
+    return Slices{even > kMinSlice ? even : kMinSlice, even > kMinSlice ? even : kMinSlice, p.blocks};
+  return Slices{even + more, even - more, p.blocks / 2};
+}
 
 // Fills the plan; returns the line's length.
 __device__ long long make_plan(const FastPaged &p, Plan &plan) {
@@ -886,38 +908,45 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
           __builtin_amdgcn_perm(vr[1][e / 2], vr[0][e / 2], e % 2 ? 0x07060302 : 0x05040100);
   };
   int i = 0; // the number since look_up of the step that is loaded next
-  look_up(it.t0);
-  load(it.t0, i++);
-  fence();
   v4u qp[NT][kSteps][3];
+  {
+    float x[NT][kSteps][8]; // on their way with the first step's rows
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    const bool active = 16 * n + lc < mine;
-    const int v = active ? v0 + 16 * n + lc : 0;
-    const float *src = p.job.q + (size_t)(it.row0 + v / kv_mul) * p.job.q_stride + ((size_t)it.g * kv_mul + v % kv_mul) * hd;
+    for (int n = 0; n < NT; n++) {
+      const int v = 16 * n + lc < mine ? v0 + 16 * n + lc : 0;
+      const float *src = p.job.q + (size_t)(it.row0 + v / kv_mul) * p.job.q_stride + ((size_t)it.g * kv_mul + v % kv_mul) * hd;
 #pragma unroll
-    for (int s = 0; s < kSteps; s++) {
-      const int d = 32 * s + 8 * lq;
-      const float *at = src + (d < hd ? d : 0);
-      float x[8];
-      if (p.q_vec) {
-        const float4 a = reinterpret_cast<const float4 *>(at)[0], c = reinterpret_cast<const float4 *>(at)[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
-      } else {
+      for (int s = 0; s < kSteps; s++) {
+        const int d = 32 * s + 8 * lq;
+        const float *at = src + (d < hd ? d : 0);
+        if (p.q_vec) {
+          const float4 a = reinterpret_cast<const float4 *>(at)[0], c = reinterpret_cast<const float4 *>(at)[1];
+          x[n][s][0] = a.x, x[n][s][1] = a.y, x[n][s][2] = a.z, x[n][s][3] = a.w;
+          x[n][s][4] = c.x, x[n][s][5] = c.y, x[n][s][6] = c.z, x[n][s][7] = c.w;
+        } else {
 #pragma unroll
-        for (int c = 0; c < 8; c++)
-          x[c] = at[c];
-      }
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        unsigned part[3];
-        const bool there = active && d < hd;
-        bf16_parts(there ? x[2 * c] * p.scale2 : 0.0f, there ? x[2 * c + 1] * p.scale2 : 0.0f, part);
-#pragma unroll
-        for (int k = 0; k < 3; k++)
-          qp[n][s][k][c] = part[k];
+          for (int c = 0; c < 8; c++)
+            x[n][s][c] = at[c];
+        }
       }
     }
+    look_up(it.t0);
+    load(it.t0, i++);
+    fence();
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int s = 0; s < kSteps; s++) {
+        const bool there = 16 * n + lc < mine && 32 * s + 8 * lq < hd;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          unsigned part[3];
+          bf16_parts(there ? x[n][s][2 * c] * p.scale2 : 0.0f, there ? x[n][s][2 * c + 1] * p.scale2 : 0.0f, part);
+#pragma unroll
+          for (int k = 0; k < 3; k++)
+            qp[n][s][k][c] = part[k];
+        }
+      }
   }
   stage(stages[0], it.t0);
   load(it.t0 + kStep, i++);
@@ -1063,8 +1092,8 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
   const int tid = threadIdx.x, g = blockIdx.x % p.job.n_kv_heads, block = blockIdx.x / p.job.n_kv_heads;
   const int hd = p.job.head_dim, kv_mul = p.kv_mul;
   const long long total = make_plan(p, plan);
-  const long long cut = whole(total + p.blocks - 1, p.blocks), slice = cut > kMinSlice ? cut : kMinSlice;
-  const long long lo = block * slice, hi = lo + slice < total ? lo + slice : total;
+  const Slices slices = make_slices(p, total);
+  const long long lo = slices.start(block), hi = slices.start(block + 1) < total ? slices.start(block + 1) : total;
   if (lo >= total)
     return;
   int r = 0; // the first request whose walks end behind lo
@@ -1121,9 +1150,9 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
       if (!shared)
         continue;
       // the walk's blocks: from .. last_block
-      const int first = (int)whole(w0, slice), last_block = (int)whole(end - 1, slice);
+      const int first = slices.block_of(w0), last_block = slices.block_of(end - 1);
       // the first block whose slice ends behind the walk's first round
-      const int from = min(max(first, (int)whole(w0 + begin + unit * grain - 1, slice)), last_block), parts = last_block - from + 1;
+      const int from = min(max(first, slices.block_of(w0 + begin + unit * grain - 1)), last_block), parts = last_block - from + 1;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
       __syncthreads();                                 // the block's
       if (tid == 0)
@@ -1320,6 +1349,7 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipSt
   p.full_begin = wide ? kWideBegin : kBegin;
   p.full_position = wide ? kWidePosition : kWaves / (p.tile_rows * p.kv_mul <= 16 ? 4 : p.tile_rows * p.kv_mul <= 32 ? 2 : 1);
   p.blocks = blocks_for(job, p.tile_rows);
+  p.pairs = wide && p.blocks % 2 == 0 && p.blocks * job.n_kv_heads == kMaxBlocksPerCu * device().cu_count;
   p.scale2 = (float)(1.4426950408889634 / sqrt((double)job.head_dim));
   p.partial = (float *)workspace;
   p.flags = device().error_flags;
