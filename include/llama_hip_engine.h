@@ -42,6 +42,14 @@ float *engine_forward_batch(Model *model, const int *tokens, int count, int pos0
  * unchanged. */
 int llhip_engine_verify(Model *model, const int *tokens, int count, int pos0, const float *draft_logits, size_t draft_ld,
                         const float *uniform, float temperature, int *next);
+/* A text scored: tokens at pos0 .. pos0 + count - 1 (the prefix [0, pos0) run before), 1 <= count <= engine_max_batch, run
+ * as engine_forward_batch's rows with every row's logits, which stay on the device, and llhip_token_logprobs
+ * (llama_hip_requests.h: temperature, top and the outputs are its arguments, in host or device memory, count rows of
+ * each) of them: logprob[i] is tokens[i + 1]'s behind tokens[0 .. i], the last one 0; entropy (or NULL) and the
+ * alternatives are every row's, the last one's those of the token that would come next. Returns 0, or -1 when the call
+ * failed in record mode. The positions are in the cache afterwards, as engine_forward_batch leaves them. */
+int llhip_engine_logprobs(Model *model, const int *tokens, int count, int pos0, float temperature, int top, float *logprob,
+                          float *entropy, int *top_token, float *top_logprob);
 void engine_free(Model *model);   /* runtime.h:114 */
 int engine_group_size(void);      /* runtime.h:116: the last loaded checkpoint's group size (0 for FP32) */
 /* runtime.h:115 (src/engine.c:191-195) for the last loaded checkpoint: "int8_q8_0", "int8_q8_0_w8a32" (Q8_0 with

@@ -975,6 +975,41 @@ int llhip_engine_verify(Model *model, const int *tokens, int count, int pos0, co
   return accepted;
 }
 
+int llhip_engine_logprobs(Model *model, const int *tokens, int count, int pos0, float temperature, int top, float *logprob,
+                          float *entropy, int *top_token, float *top_logprob) {
+  Engine *e = model ? (Engine *)model->implementation : nullptr;
+  if (!e) {
+    raise("llhip_engine_logprobs: no model loaded");
+    return -1;
+  }
+  llhip_clear_error();
+  const int vocab = e->c.vocab_size;
+  if (!(temperature > 0.0f) || !std::isfinite(temperature)) {
+    raise("llhip_engine_logprobs: temperature %g must be finite and positive", (double)temperature);
+    return -1;
+  }
+  if (top < 0 || top > LLHIP_MAX_TOP) {
+    raise("llhip_engine_logprobs: %d alternatives, 0 to %d are given", top, (int)LLHIP_MAX_TOP);
+    return -1;
+  }
+  if (!logprob || (top > 0 && (!top_token || !top_logprob))) {
+    raise("llhip_engine_logprobs: null buffer");
+    return -1;
+  }
+  if (count > 0 && !verify_shape_ok(count, vocab)) {
+    raise("llhip_engine_logprobs: %d rows of %d tokens, at most 2^20 rows of 2^22 tokens are taken", count, vocab);
+    return -1;
+  }
+  const float *logits = forward_batch_on_device(model, e, tokens, count, pos0);
+  if (!logits)
+    return -1;
+  std::vector<int> next(tokens + 1, tokens + count); // row i's logits say of tokens[i + 1]
+  next.push_back(-1);
+  llhip_token_logprobs(logprob, entropy, top_token, top_logprob, top, logits, (size_t)vocab, next.data(), count, vocab,
+                       temperature);
+  return llhip_last_error()[0] ? -1 : 0;
+}
+
 void engine_kv_stats(Model *model, int position, int verify, KvStats *out) {
   (void)verify;
   Engine *e = model ? (Engine *)model->implementation : nullptr;

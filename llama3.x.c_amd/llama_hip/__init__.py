@@ -174,6 +174,7 @@ _SIGNATURES = {
     "engine_group_size": (I32, []),
     "engine_precision": (ctypes.c_char_p, []),
     "llhip_engine_verify": (I32, [P, P, I32, I32, P, SZ, P, ctypes.c_float, P]),
+    "llhip_engine_logprobs": (I32, [P, P, I32, I32, ctypes.c_float, I32, P, P, P, P]),
     "engine_kv_stats": (None, [P, I32, I32, P]),
     "llhip_hbm_claimed": (SZ, []),
     "k_attention_init": (None, [P, I32, I32, I32, I32]),

@@ -1,8 +1,12 @@
 """Log probabilities of given tokens, entropies and the likeliest tokens, on the GPU, against float64 (tests/paged_util.py)."""
+import ctypes
+import os
+
 import numpy as np
 import pytest
 
 import llama_hip as lh
+from llama_hip import checkpoint as ck
 from tests import hip_util as hu
 from tests import paged_util as pu
 from tests.requests_util import U
@@ -200,3 +204,73 @@ def test_host_buffers_and_graphs(L):
         for g, w in zip(outs, eager):
             assert np.array_equal(hu.host(g), w)
     L.llhip_graph_destroy(graph)
+
+
+ENGINE = dict(dim=128, hidden_dim=192, n_layers=2, n_heads=4, n_kv_heads=2, vocab_size=1100, seq_len=96, head_dim=32)
+
+
+def engine_model(path, kind):
+    gs = 64
+    norms, t = ck.synthetic(ENGINE, gs, 19)
+    if kind == "q8":
+        ck.write_q8_v3(path, ENGINE, gs, norms, t)
+    else:
+        f32 = {n: q.astype(F) * np.repeat(s.reshape(-1), gs).reshape(q.shape).astype(F) for n, (q, s) in t.items()}
+        ck.write_f32_v3(path, ENGINE, norms, f32)
+
+
+@pytest.mark.parametrize("kind", ["q8", "f32", "bf16", "q8_no_gemm"])
+def test_engine_scores_a_text(L, tmp_path, monkeypatch, kind):
+    """llhip_engine_logprobs against float64 on the logits that engine_forward_batch gives for the same rows at the same
+    place: whole texts and one token, behind a prefix, into host and device memory; the model goes on as after
+    engine_forward_batch; refusals leave it usable."""
+    if kind == "bf16":
+        monkeypatch.setenv("LLAMA_PRECISION", "bf16")
+    if kind == "q8_no_gemm":
+        monkeypatch.setenv("LLAMA_PREFILL_GEMM", "off")
+        monkeypatch.setenv("LLAMA_PREFILL_BATCH", "24")
+    L.kernels_kv_layout_select(b"head")
+    path = os.path.join(tmp_path, "tiny.bin")
+    engine_model(path, kind.split("_")[0])
+    vocab = ENGINE["vocab_size"]
+    rng = np.random.default_rng(3)
+    model = lh.Model()
+    at = ctypes.byref(model)
+    try:
+        L.engine_load(at, path.encode())
+        assert model.implementation, lh.last_error()
+        pos = 0
+        for n, top, t in ((20, 5, 1.0), (1, 0, 1.0), (7, 32, 0.5), (24, 1, 1.7)):
+            tokens = rng.integers(0, vocab, n).astype(np.int32)
+            p = L.engine_forward_batch(at, lh.ptr(tokens), n, pos, lh.LOGITS_ALL)
+            assert p, lh.last_error()
+            logits = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), (n, vocab)).copy()
+            want = call(L, logits, np.append(tokens[1:], -1), t, top)
+            L.llhip_synchronize()
+            for dev in (lambda x: x, hu.dev):
+                out = [dev(np.full(n, 7.0, F)), dev(np.full(n, 7.0, F)), dev(np.full((n, top), 7, np.int32)) if top else None,
+                       dev(np.full((n, top), 7.0, F)) if top else None]
+                assert L.llhip_engine_logprobs(at, lh.ptr(tokens), n, pos, t, top, *[lh.ptr(x) for x in out]) == 0, lh.last_error()
+                got = [x if x is None or isinstance(x, np.ndarray) else hu.host(x) for x in out]
+                for g, w in zip(got, want):
+                    assert g is w is None or np.array_equal(g, w)
+            plain = pu.scores(logits, np.append(tokens[1:], -1), t, top)
+            assert np.allclose(got[0], plain[0], atol=1e-5) and (top == 0 or np.array_equal(got[2], plain[2]))
+            pos += n
+        out = np.full(2, 7.0, F)
+        two, ints = np.array([1, 2], np.int32), np.zeros(8, np.int32)
+        for args, words in (((lh.ptr(two), 2, 95, 1.0, 0, lh.ptr(out), None, None, None), "batch input out of range"),
+                            ((lh.ptr(np.array([1, vocab], np.int32)), 2, 0, 1.0, 0, lh.ptr(out), None, None, None), "token="),
+                            ((None, 2, 0, 1.0, 0, lh.ptr(out), None, None, None), "batch input out of range"),
+                            ((lh.ptr(two), 0, 0, 1.0, 0, lh.ptr(out), None, None, None), "batch input out of range"),
+                            ((lh.ptr(two), 2, 0, 0.0, 0, lh.ptr(out), None, None, None), "finite and positive"),
+                            ((lh.ptr(two), 2, 0, 1.0, 33, lh.ptr(out), None, lh.ptr(ints), lh.ptr(ints)), "0 to 32"),
+                            ((lh.ptr(two), 2, 0, 1.0, 1, lh.ptr(out), None, None, None), "null buffer"),
+                            ((lh.ptr(two), 2, 0, 1.0, 0, None, None, None, None), "null buffer")):
+            assert L.llhip_engine_logprobs(at, *args) == -1 and (out == 7.0).all()
+            assert words in lh.last_error(), (words, lh.last_error())
+        assert L.llhip_engine_logprobs(at, lh.ptr(two), 2, 0, 1.0, 0, lh.ptr(out), None, None, None) == 0
+        assert out[1] == 0.0 and out[0] < 0.0
+    finally:
+        L.engine_free(at)
+        L.llhip_clear_error()

@@ -199,3 +199,11 @@ def test_score_refusals(L):
     score_call(L, rows=0, l=None)  # nothing to do
     score_call(L, top=0, p=None, t=None, e=None, tt=None, tp=None)
     assert not lh.last_error()
+
+
+def test_engine_logprobs_without_a_model(L):
+    model, out = lh.Model(), np.full(2, 7.0, F)
+    for m in (None, ctypes.byref(model)):
+        got = L.llhip_engine_logprobs(m, lh.ptr(np.zeros(2, np.int32)), 2, 0, 1.0, 0, lh.ptr(out), None, None, None)
+        assert got == -1 and (out == 7.0).all()
+        refused(L, "no model loaded")
