@@ -179,8 +179,6 @@ constexpr int kWideVectors = 128;      // of a wide one
 constexpr int kMaxBlocksPerCu = 2;
 constexpr int kMaxArrivals = 4096;
 constexpr unsigned kNowhere = 0x7ffffff0u; // an offset past every buffer: a load reads zero there
-constexpr float kMasked = -0x1p126f; // a masked score, -FLT_MAX, lies so far below that its weight is zero, also where a
-                                     // lane has seen nothing else
 
 // How many of a walk's blocks have stored their part, by the block that the walk begins in: zero between launches, as the
 // last to arrive sets it back.
@@ -670,7 +668,7 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
       for (int e = 0; e < E; e++)
         o[e] *= alpha;
     }
-    const float base = fmaxf(m_run, kMasked);
+    const float base = m_run > -FLT_MAX ? m_run : 0.0f; // a masked score, -FLT_MAX, has no weight where a lane has seen no other
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       w[j] = __builtin_amdgcn_exp2f(w[j] - base);
@@ -1013,7 +1011,7 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
         for (int e = 0; e < E; e++)
           o[n][e] *= alpha;
       }
-      const float base = fmaxf(m_run[n], kMasked);
+      const float base = m_run[n] > -FLT_MAX ? m_run[n] : 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         w[j] = __builtin_amdgcn_exp2f(w[j] - base);
@@ -1269,11 +1267,11 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
 int tile_dims(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 // The matrix-core form takes the job: K and V rows in whole 16-byte vectors, offsets within 16 rows of 32 bits, positions
-// within int arithmetic of the steps.
+// within int arithmetic of the steps, and a line below 2^50.
 bool tiled(const AttentionPagedJob &job) {
   const size_t size = job.batch.bf16 ? 2 : 4;
   return job.head_dim * size % 16 == 0 && (((uintptr_t)job.key | (uintptr_t)job.value) & 15) == 0 &&
-         job.batch.pos_stride * size * 16 < ((size_t)1 << 30) && job.batch.seq_len < (1 << 30) && job.n_kv_heads <= kMaxArrivals;
+         job.batch.pos_stride * size * 16 < ((size_t)1 << 30) && job.batch.seq_len < (1 << 30) && job.batch.rows <= (1 << 20) && job.n_kv_heads <= kMaxArrivals;
 }
 
 int blocks_of(const AttentionPagedJob &job) {

@@ -332,6 +332,156 @@ def test_attention_off_alignment(L, bf16, hd, kv, layout, form):
 
 
 @pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows_of", [[1, 1, 1], [6, 70, 1]])
+def test_attention_over_caches_off_alignment(L, bf16, rows_of):
+    """Caches on the alignment of one value."""
+    heads, kv, hd = 8, 2, 64
+    L.kernels_kv_layout_select(b"head")
+    b = pu.Pages(hu.dev, rows_of, [100, 37, 3], page=16, bf16=bf16)
+    rng = np.random.default_rng(4)
+    caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    want, bound = pu.attention(b, q, *caches, heads, kv, hd, "head")
+    T = hu.torch()
+    views = []
+    for c in caches:
+        flat = hu.empty(c.size + 1, T.int16 if bf16 else T.float32)
+        flat[1:].copy_(T.from_numpy((c.view(np.int16) if bf16 else c).reshape(-1)))
+        views.append(flat[1:])
+    qd, out = hu.dev(q), hu.dev(np.zeros_like(q))
+    T.cuda.synchronize()
+    L.llhip_attention_paged(lh.ptr(out), lh.ptr(qd), heads * hd, lh.ptr(views[0]), lh.ptr(views[1]), b.struct, heads, kv, hd)
+    quiet(L)
+    within(hu.host(out), want, bound)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows_of", [[1, 1], [1, 40]])
+def test_attention_of_scores_far_below_zero(L, bf16, rows_of):
+    """Scores of -1e38, the same for all positions: their weights are equal, as for any others."""
+    heads, kv, hd = 8, 2, 8
+    b = pu.Pages(hu.dev, rows_of, [100, 30], page=16, bf16=bf16)
+    rng = np.random.default_rng(5)
+    q = np.full((b.rows, heads * hd), 2.0 ** 60, F)
+    key = np.full(b.shape("head", kv, hd), -(2.0 ** 63), F)  # a dot of -8 * 2^123, a score of -3e37 * sqrt(8)
+    value = b.cache(rng, "head", kv, hd)
+    got = attention_case_equal_scores(L, b, q, pu.to_bf16(key) if bf16 else key, value, heads, kv, hd)
+    for r, rows, length in b.requests():
+        seen = length + rows.stop - rows.start
+        vals = b.gather(value, "head", r, seen)
+        for j, i in enumerate(range(rows.start, rows.stop)):
+            n = length + j + 1
+            mean = np.repeat(vals[:, :n].mean(1), heads // kv, 0)
+            size = np.repeat(np.abs(vals[:, :n]).mean(1), heads // kv, 0)
+            assert (np.abs(got[i].reshape(heads, hd) - mean) <= (3 * n + 72) * ru.U * size).all()
+
+
+def attention_case_equal_scores(L, b, q, key, value, heads, kv, hd):
+    L.kernels_kv_layout_select(b"head")
+    qd, kd, vd, out = hu.dev(q), cache_dev(key), cache_dev(value), hu.dev(np.zeros_like(q))
+    L.llhip_attention_paged(lh.ptr(out), lh.ptr(qd), heads * hd, lh.ptr(kd), lh.ptr(vd), b.struct, heads, kv, hd)
+    quiet(L)
+    return hu.host(out)
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+def test_pages_past_32_bits(L, bf16):
+    """Caches of more than 2^32 bytes and 2^31 values, their last pages in use: appended rows and attention, single rows and a
+    prompt's."""
+    T = hu.torch()
+    L.kernels_kv_layout_select(b"head")
+    heads, kv, hd, page = 8, 2, 128, 64
+    pages = (1 << 31) // (kv * page * hd) + 40
+    dtype = T.int16 if bf16 else T.float32
+    big = [T.empty((pages, kv, page, hd), dtype=dtype, device="cuda") for _ in range(2)]
+    rng = np.random.default_rng(6)
+    b = pu.Pages(lambda x: x, [1, 70, 1], [150, 30, 0], page=page, bf16=bf16)
+    shift = pages - b.pool  # the pool lies at the caches' end
+    keep = [hu.dev(a) for a in (b.start, b.length, np.where(b.table < 0, -1, b.table + shift).astype(np.int32))]
+    b.struct.start, b.struct.length, b.struct.pages = (lh.ptr(a) for a in keep)
+    b.struct.num_pages = pages
+    caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
+    for x, c in zip(big, caches):
+        x[shift:].copy_(T.from_numpy(c.view(np.int16) if bf16 else c))
+    table = rope_table(L, b.seq_len, hd)
+    q, k, v = (rng.standard_normal((b.rows, n * hd), dtype=F) for n in (heads, kv, kv))
+    dev = [hu.dev(x) for x in (q, k, v, table)]
+    rot, out = hu.dev(np.zeros_like(q)), hu.dev(np.zeros_like(q))
+    T.cuda.synchronize()
+    L.llhip_rope_kv_append_paged(lh.ptr(rot), heads * hd, lh.ptr(dev[0]), heads * hd, lh.ptr(dev[1]), lh.ptr(dev[2]), kv * hd,
+                                 lh.ptr(dev[3]), None, None, 0.0, b.struct, heads, kv, hd, lh.ptr(big[0]), lh.ptr(big[1]))
+    L.llhip_attention_paged(lh.ptr(out), lh.ptr(rot), heads * hd, lh.ptr(big[0]), lh.ptr(big[1]), b.struct, heads, kv, hd)
+    quiet(L)
+    for r, rows, length in b.requests():
+        for j, i in enumerate(range(rows.start, rows.stop)):
+            qi, ki = q[i].copy(), k[i].copy()
+            L.k_rope_apply(lh.ptr(qi), lh.ptr(ki), lh.ptr(table[length + j]), heads, kv, hd)
+            for c, x in ((caches[0], ki), (caches[1], v[i])):
+                b.row(c, "head", r, length + j)[:] = (pu.to_bf16(x) if bf16 else x).reshape(kv, hd)
+    for x, c in zip(big, caches):
+        got = hu.host(x[shift:])
+        assert np.array_equal(got.view(np.uint8), c.view(np.uint8))
+    want, bound = pu.attention(b, hu.host(rot), *caches, heads, kv, hd, "head")
+    within(hu.host(out), want, bound)
+
+
+def test_calls_from_two_threads(L):
+    """Attention over pages and scoring from two threads at once, whose kernels share one workspace."""
+    import threading
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(7)
+    heads, kv, hd = 8, 2, 64
+    b = pu.Pages(hu.dev, [1, 3] * 8, rng.integers(0, 2000, 16), page=16)
+    caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    want, bound = pu.attention(b, q, *caches, heads, kv, hd, "head")
+    qd, kd, vd, out = hu.dev(q), hu.dev(caches[0]), hu.dev(caches[1]), hu.dev(np.zeros_like(q))
+    logits, tokens = rng.standard_normal((40, 5000)).astype(F), rng.integers(0, 5000, 40).astype(np.int32)
+    ld, td, lp = hu.dev(logits), hu.dev(tokens), hu.dev(np.zeros(40, F))
+
+    def attend():
+        for _ in range(200):
+            L.llhip_attention_paged(lh.ptr(out), lh.ptr(qd), heads * hd, lh.ptr(kd), lh.ptr(vd), b.struct, heads, kv, hd)
+
+    def score():
+        for _ in range(200):
+            L.llhip_token_logprobs(lh.ptr(lp), None, None, None, 0, lh.ptr(ld), 5000, lh.ptr(td), 40, 5000, 1.0)
+
+    attend(), score()
+    quiet(L)
+    alone = hu.host(lp).copy()
+    team = [threading.Thread(target=f) for f in (attend, score)]
+    for t in team:
+        t.start()
+    for t in team:
+        t.join()
+    quiet(L)
+    within(hu.host(out), want, bound)
+    assert np.array_equal(hu.host(lp), alone)
+
+
+@pytest.mark.parametrize("rows_of,lengths", [([1], [30000]), ([1, 200, 3], [700, 900, 4000])])
+def test_a_call_repeats_itself_bit_for_bit(L, rows_of, lengths):
+    """The parts of a walk are joined in their order, whichever block comes last."""
+    heads, kv, hd = 32, 8, 128
+    L.kernels_kv_layout_select(b"head")
+    for bf16 in (False, True):
+        b = pu.Pages(hu.dev, rows_of, lengths, page=16, bf16=bf16)
+        rng = np.random.default_rng(8)
+        qd = hu.dev(rng.standard_normal((b.rows, heads * hd), dtype=F))
+        caches = [cache_dev(b.cache(rng, "head", kv, hd)) for _ in range(2)]
+        first = None
+        for _ in range(20):
+            out = hu.dev(np.zeros((b.rows, heads * hd), F))
+            L.llhip_attention_paged(lh.ptr(out), lh.ptr(qd), heads * hd, lh.ptr(caches[0]), lh.ptr(caches[1]), b.struct, heads,
+                                    kv, hd)
+            quiet(L)
+            got = hu.host(out)
+            assert first is None or np.array_equal(got, first)
+            first = got
+
+
+@pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("rows_of,lengths", [([1, 1], [33, 200]), ([3, 40], [61, 100])])
 @pytest.mark.parametrize("hd", [64, 128, 72])
 def test_attention_leaves_the_pages_rest_alone(L, bf16, rows_of, lengths, hd):
