@@ -197,6 +197,7 @@ struct FastPaged {
   float *partial;
   int *flags;
   bool pairs;   // two blocks to a CU, and an even number to a KV head: the first half of them are the CUs' first blocks
+  bool fours;   // a page is a multiple of four positions
   bool q_vec;   // q in whole 16-byte vectors
   bool out_vec; // out likewise
 };
@@ -522,10 +523,14 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   };
   auto load_v = [&](int pos, int i) {
     if constexpr (ANY) {
+      size_t four = 0; // where the first of four positions lies
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const int t = pos + 16 * (j / 4) + 4 * lq + j % 4;
-        const T *row = (const T *)p.job.value + place_any(t);
+        if (j % 4 == 0 || !p.fours) // uniform
+          four = place_any(t);
+        // the same page holds the next three; behind the end the first is read again
+        const T *row = (const T *)p.job.value + four + (p.fours && t < end ? (size_t)(j % 4) * b.pos_stride : 0);
 #pragma unroll
         for (int u = 0; u < kVecs; u++) {
           const int d = (u * 16 + lc) * EV;
@@ -1351,6 +1356,7 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipSt
   p.scale2 = (float)(1.4426950408889634 / sqrt((double)job.head_dim));
   p.partial = (float *)workspace;
   p.flags = device().error_flags;
+  p.fours = job.batch.page_size % 4 == 0;
   p.q_vec = job.q_stride % 4 == 0 && ((uintptr_t)job.q & 15) == 0;
   p.out_vec = ((uintptr_t)job.out & 15) == 0;
   const int mode = mode_of(job);
