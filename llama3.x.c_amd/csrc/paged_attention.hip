@@ -3,7 +3,15 @@
 //   attn_paged        block: a slice of a KV head's walks, a walk being a tile of one request's query vectors over its
 //                     positions. One pass over K and V with the softmax's running maximum and sum, products on the matrix
 //                     cores; a walk that several blocks share is joined by the last of them to arrive.
-//   attn_paged_rows   any shape, one row and KV head a block.
+//   attn_paged_rows   any shape, one row and KV head a block: 32 rows of 16 heads over 4 of 100 at 1450 positions on average take
+//                     1.8 ms, where the tiled form takes 32 us for heads of 96.
+//
+// Measured at 32 heads over 8 KV heads of dimension 128, BF16 pages: 32 requests of one row at 2200 positions on average 65 us
+// (290 MB of K and V: 4.5 TB/s), 64 at 5670 262 us (5.7 TB/s), one at 4000 13 us; five prompts' chunks, 1616 rows behind 1146
+// positions on average, 115 to 125 us (310 TFLOP/s, three matrix products each). F32 pages: one row at 35000 positions 70 us
+// (4.1 TB/s), 16 requests of two to seven rows 50 us, the prompts 350 us. Single rows are bound by HBM, behind 5 us of launch, plan
+// and table and before 5 us of join; wide tiles by a step's 1536 cycles of matrix instructions and 950 of vector ones beside
+// the reads from LDS, which overlap little; F32 prompts by the FP32 matrix instructions (103 of 157 TFLOP/s).
 #include <cfloat>
 #include <type_traits>
 
@@ -868,7 +876,36 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
   const int k_dim = 8 * (tid % kKLanes), k_row = tid / kKLanes;
   const unsigned k_at = k_dim < hd ? (unsigned)(k_row % 16) * row_bytes + (unsigned)k_dim * 2u : kNowhere;
   const unsigned v_at = EV * lc < hd ? (unsigned)(4 * lq + 2 * (wave & 1)) * row_bytes + (unsigned)(EV * lc) * 2u : kNowhere;
+  auto place_any = [&](int t) { // as in walk
+    const int at = min(t, end - 1), number = at / b.page_size, page = page_of(b, it.r, number);
+    if (page < 0)
+      p.flags[8] = 1;
+    return (size_t)max(page, 0) * b.page_values + (size_t)(at - number * b.page_size) * b.pos_stride + head;
+  };
   auto load = [&](int pos, int i) {
+    if constexpr (MODE == kAny) {
+      const int k_dims = k_dim < hd ? k_dim : 0, v_dims = EV * lc < hd ? EV * lc : 0; // there Q is zero, or nothing is stored
+#pragma unroll
+      for (int u = 0; u < kKLoads; u++)
+        kr[u] = *reinterpret_cast<const v4u *>((const uint16_t *)p.job.key + place_any(pos + k_row + u * (kThreads / kKLanes)) + k_dims);
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int t = pos + 16 * (wave / 2) + 4 * lq + 2 * (wave & 1) + j;
+        const uint16_t *row = (const uint16_t *)p.job.value + place_any(t) + v_dims;
+        if constexpr (EV == 8) {
+          const v4u x = *reinterpret_cast<const v4u *>(row);
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+            vr[j][c] = t < end ? x[c] : 0u;
+        } else {
+          const v2u x = *reinterpret_cast<const v2u *>(row);
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+            vr[j][c] = t < end ? x[c] : 0u;
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < kKLoads; u++)
       kr[u] = __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(
@@ -933,7 +970,8 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
         }
       }
     }
-    look_up(it.t0);
+    if constexpr (MODE != kAny)
+      look_up(it.t0);
     load(it.t0, i++);
     fence();
 #pragma unroll
@@ -985,7 +1023,7 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
       fence();
     }
     stage(stages[turn ^ 1], pos + kStep);
-    if (i == kWave / 2) { // uniform
+    if (MODE != kAny && i == kWave / 2) { // uniform
       look_up(pos + 2 * kStep);
       i = 0;
     }
@@ -1289,7 +1327,9 @@ typedef void (*FastKernel)(FastPaged);
 template <typename T, int HD> FastKernel kernel_of(int mode, bool wide) {
   if constexpr (sizeof(T) == 2 && HD <= 128)
     if (wide)
-      return mode == kWhole ? attn_paged<T, HD, kWhole, true> : attn_paged<T, HD, kPart, true>;
+      return mode == kWhole  ? attn_paged<T, HD, kWhole, true>
+             : mode == kPart ? attn_paged<T, HD, kPart, true>
+                             : attn_paged<T, HD, kAny, true>;
   return mode == kWhole  ? attn_paged<T, HD, kWhole, false>
          : mode == kPart ? attn_paged<T, HD, kPart, false>
                          : attn_paged<T, HD, kAny, false>;
@@ -1314,7 +1354,7 @@ int mode_of(const AttentionPagedJob &job) {
 // The kernel with wide tiles, where some request may have more than 64 vectors.
 bool wide_tiles(const AttentionPagedJob &job) {
   const long long vectors = (long long)job.batch.rows * (job.n_heads / job.n_kv_heads);
-  return job.batch.bf16 && job.head_dim <= 128 && mode_of(job) != kAny && job.batch.rows > job.batch.count && vectors > kTileVectors;
+  return job.batch.bf16 && job.head_dim <= 128 && job.batch.rows > job.batch.count && vectors > kTileVectors;
 }
 
 bool launch_rows(const AttentionPagedJob &job, hipStream_t stream) {

@@ -484,33 +484,35 @@ def test_a_call_repeats_itself_bit_for_bit(L, rows_of, lengths):
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("rows_of,lengths", [([1, 1], [33, 200]), ([3, 40], [61, 100])])
 @pytest.mark.parametrize("hd", [64, 128, 72])
-def test_attention_leaves_the_pages_rest_alone(L, bf16, rows_of, lengths, hd):
+@pytest.mark.parametrize("page", [64, 20, 27])
+def test_attention_leaves_the_pages_rest_alone(L, bf16, rows_of, lengths, hd, page):
     """NaN and infinities in pages that no request names, and behind the last position of a request's last page."""
     heads, kv = 8, 2
-    b = pu.Pages(hu.dev, rows_of, lengths, page=64, bf16=bf16)
+    b = pu.Pages(hu.dev, rows_of, lengths, page=page, bf16=bf16)
     rng = np.random.default_rng(8)
     caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
     bad = np.array([np.nan, np.inf, -np.inf, 3e38], F)
     for c in caches:
         odd = pu.to_bf16(bad) if bf16 else bad
-        for page in b.free:
-            c[page] = rng.choice(odd, c[page].shape)
+        for free in b.free:
+            c[free] = rng.choice(odd, c[free].shape)
         for r, rows, length in b.requests():
             seen = length + rows.stop - rows.start
-            if seen % 64:
-                c[b.table[r, seen // 64]][:, seen % 64:] = rng.choice(odd, (kv, 64 - seen % 64, hd))
+            if seen % page:
+                c[b.table[r, seen // page]][:, seen % page:] = rng.choice(odd, (kv, page - seen % page, hd))
     attention_case(L, 9, heads, kv, hd, "head", b, caches=caches)
 
 
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("hd", [64, 128, 256, 50])
 @pytest.mark.parametrize("what", [np.inf, -np.inf, np.nan])
-def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(L, bf16, hd, what):
+@pytest.mark.parametrize("page", [16, 12])
+def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(L, bf16, hd, what, page):
     """One V value of a prompt's own rows: the rows before it keep their results, in every dimension; the rows that see it
     have it in its dimension alone, and other requests nothing of it."""
     heads, kv, layout = 8, 2, "head"
     L.kernels_kv_layout_select(layout.encode())
-    b = pu.Pages(hu.dev, [50, 1, 6], [20, 90, 30], page=16, bf16=bf16)
+    b = pu.Pages(hu.dev, [50, 1, 6], [20, 90, 30], page=page, bf16=bf16)
     rng = np.random.default_rng(4)
     key, value = b.cache(rng, layout, kv, hd), b.cache(rng, layout, kv, hd)
     q = rng.standard_normal((b.rows, heads * hd), dtype=F)
