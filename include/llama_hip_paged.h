@@ -66,7 +66,15 @@ void llhip_rope_kv_append_paged(float *q_out, size_t q_out_stride, const float *
  * the request's last position is not used, and a value that is not finite reaches the rows that see its position only. A
  * request with a page outside the caches fails at the next host-visible point; its rows' values are then unspecified. out
  * must not overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most
- * 16 per KV head, head_dim at most 256. */
+ * 16 per KV head, head_dim at most 256.
+ *
+ * Rows of K and V in whole 16-byte vectors (head_dim a multiple of 8 in BF16 pages, of 4 in F32 ones, the caches 16-byte
+ * aligned) take the matrix cores, with at most 2^20 rows and 4096 KV heads; any other shape has each row read what it attends
+ * to by itself, some fifty times slower. Pages of a multiple of 16 positions are the fastest (of 8: 1.15 to 1.4 times longer).
+ * BF16 pages meet the F32 queries and weights as three exact BF16 parts of those, F32 pages in FP32 products, FP32 sums
+ * either way; a weight below 2^-126 of its row's largest counts as 0. A call's parts meet in a workspace and counters that all
+ * calls on a device share: calls ordered on the library's stream are safe, two that may run concurrently on one GPU (graphs
+ * replayed on other streams) race. Run the largest batch once before capturing a step, so that the workspace is there. */
 void llhip_attention_paged(float *out, const float *q, size_t q_stride, const void *key_pages, const void *value_pages,
                            const PagedBatch *batch, int n_heads, int n_kv_heads, int head_dim);
 

@@ -139,7 +139,8 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
  * -infinity. tokens[i] of -1 stands for none (the last row of a prompt): its logprob is 0. tokens NULL with logprob NULL
  * leaves the log probabilities out. A row with a NaN, +infinity or no token left gets NaN in all places and tokens -1, and a
  * token outside the vocabulary NaN; both fail at the next host-visible point. Exponentials are FP32, a row's sums of them
- * FP64 over parts of 16 tokens. The outputs must not overlap each other or an input. At most 2^20 rows and 2^22 tokens. */
+ * FP64 over parts of 1024 tokens. The outputs must not overlap each other or an input. At most 2^20 rows and 2^22 tokens. The
+ * workspace and counters are shared as llhip_attention_paged's (llama_hip_paged.h). */
 enum { LLHIP_MAX_TOP = 32 };
 void llhip_token_logprobs(float *logprob, float *entropy, int *top_token, float *top_logprob, int top,
                           const float *logits, size_t ld, const int *tokens, int rows, int vocab, float temperature);
