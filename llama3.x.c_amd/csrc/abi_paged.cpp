@@ -189,7 +189,7 @@ void llhip_attention_paged(float *out, const float *q, size_t q_stride, const vo
   std::unique_lock<std::mutex> lock(scratch_mutex);
   void *scratch = nullptr;
   const size_t bytes = attention_paged_workspace(job);
-  if (bytes && !scratch_room(name, bytes, &scratch))
+  if (bytes && !scratch_room(name, bytes, &scratch, SCRATCH_PAGES))
     return;
   if (!launch_attention_paged(job, scratch, call.stream()))
     return;

@@ -10,44 +10,45 @@ using namespace llhip;
 
 namespace llhip {
 
-// The scratch of these calls and of those over pages, which the library stream orders: grown on demand (never during
-// graph capture), kept for the
-// process. A graph captured on it replays on it, so a buffer that a capture took is kept when a larger one follows. A call
-// holds the lock until its kernels are queued, so that another thread's do not come between them.
+// The scratch of these calls, and another of the attention over pages (two of its blocks a CU may need 70 MB of it), which the
+// library stream orders: grown on demand (never during graph capture), kept for the process. A graph captured on it replays on
+// it, so a buffer that a capture took is kept when a larger one follows. A call holds the lock until its kernels are queued,
+// so that another thread's do not come between them.
 std::mutex scratch_mutex;
 namespace {
-void *scratch_memory = nullptr;
-size_t scratch_bytes = 0;
-bool scratch_captured = false;
+struct Scratch {
+  void *memory = nullptr;
+  size_t bytes = 0;
+  bool captured = false;
+} scratches[2];
 } // namespace
 
-bool scratch_room(const char *name, size_t bytes, void **out) {
+bool scratch_room(const char *name, size_t bytes, void **out, ScratchOf of) {
   Device &dev = device();
-  if (bytes > scratch_bytes) {
+  Scratch &s = scratches[of];
+  if (bytes > s.bytes) {
     if (dev.capturing)
       return raise("%s needs %zu bytes of workspace during graph capture; run the call once before capturing", name, bytes);
-    if (scratch_memory && !scratch_captured) {
+    if (s.memory && !s.captured) {
       (void)hipStreamSynchronize(dev.stream);
-      (void)hipFree(scratch_memory);
-      hbm_release(scratch_bytes);
+      (void)hipFree(s.memory);
+      hbm_release(s.bytes);
     }
-    scratch_memory = nullptr;
-    scratch_bytes = 0;
-    scratch_captured = false;
+    s = Scratch{};
     const size_t want = bytes + bytes / 4 + 4096;
     if (!hbm_claim(want, "the request workspace"))
       return false;
-    if (hipMalloc(&scratch_memory, want) != hipSuccess) {
+    if (hipMalloc(&s.memory, want) != hipSuccess) {
       (void)hipGetLastError();
       hbm_release(want);
-      scratch_memory = nullptr;
+      s.memory = nullptr;
       return raise("%s: allocating %zu bytes of workspace failed", name, want);
     }
-    scratch_bytes = want;
+    s.bytes = want;
   }
   if (dev.capturing)
-    scratch_captured = true;
-  *out = scratch_memory;
+    s.captured = true;
+  *out = s.memory;
   return true;
 }
 

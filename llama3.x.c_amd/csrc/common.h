@@ -367,10 +367,11 @@ struct AttentionPagedJob {
 size_t attention_paged_workspace(const AttentionPagedJob &job); // bytes of scratch the launch takes
 bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipStream_t stream);
 
-// The scratch of the calls for many requests (abi_requests.cpp): `bytes` of it, false after raise. A call holds the mutex
-// from here until its kernels are queued.
+// The scratch of the calls for many requests, or of the attention over pages (abi_requests.cpp): `bytes` of it, false after
+// raise. A call holds the mutex from here until its kernels are queued.
 extern std::mutex scratch_mutex;
-bool scratch_room(const char *name, size_t bytes, void **out);
+enum ScratchOf { SCRATCH_REQUESTS, SCRATCH_PAGES };
+bool scratch_room(const char *name, size_t bytes, void **out, ScratchOf of = SCRATCH_REQUESTS);
 inline bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
   return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
 }
