@@ -58,11 +58,11 @@ void llhip_rope_kv_append_paged(float *q_out, size_t q_out_stride, const float *
                                 const float *k_norm, float epsilon, const PagedBatch *batch, int n_heads, int n_kv_heads,
                                 int head_dim, void *key_pages, void *value_pages);
 
-/* Causal attention of every request's rows over the positions that its pages hold: row j of request r attends to positions
- * 0 .. length[r] + j (the last rows' are stored before, by llhip_rope_kv_append_paged). Rows of q lie q_stride floats
- * apart, rows of out n_heads * head_dim; scores, softmax and value sums as in k_attention: products of the F32 queries and
- * weights with the pages' values, FP32 sums; a non-finite score fails with "nonfinite value in softmax". The sums are
- * divided by the weights' at the end, so n positions' values must stay below 3e38 / n, as there. What lies in a page behind
+/* Causal attention of every request's rows over the positions that its pages hold: row j of request r attends to positions 0
+ * .. length[r] + j (the last rows' are stored before, by llhip_rope_kv_append_paged). Rows of q lie q_stride floats apart,
+ * rows of out n_heads * head_dim; scores, softmax and value sums as in k_attention: products of the F32 queries and weights
+ * with the pages' values, FP32 sums; a non-finite score fails with "nonfinite value in softmax". The sums are divided by the
+ * weights' at the end, which may reach 2^8 each, so n positions' values must stay below 1e36 / n. What lies in a page behind
  * the request's last position is not used, and a value that is not finite reaches the rows that see its position only. A
  * request with a page outside the caches fails at the next host-visible point; its rows' values are then unspecified. out
  * must not overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most

@@ -222,7 +222,7 @@ __device__ __forceinline__ int own_thread() {
 __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // The walks of a KV head lie one behind the other on a line, each as long as it takes in time, and the line is cut into
-// slices of one length, one for a block: all blocks start together and end together. A walk's begin and end take as long as
+// slices of equal time, one for a block: all blocks start together and end together. A walk's begin and end take as long as
 // begin_time positions of a small tile.
 constexpr int kBegin = 256, kWideBegin = 768;
 // A slice is at least this long: shorter ones do not pay for a walk's join, and a block inside a walk has some of its
@@ -398,15 +398,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void *cache, lon
   return __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)base, (short)0, bytes, 0x00020000);
 }
 
-// The tile's walk: each wave has 16 of its vectors, and takes 32 positions in turn with the other waves that have the same.
-//
-// Lane (lq = lane / 16, lc = lane % 16). S^T = K Q^T and O^T = V^T P^T, so that a lane holds one vector's (lc) scores, weights
-// and sums, and no weight changes lanes: the scores of positions 16 t + 4 lq + e are in the lane that feeds positions 16 t + 4
-// lq + e to the second product, whose order of summation is free.
-//   BF16: 32 dimensions, or 32 positions, an instruction; a lane's V rows (8 positions, 8 dimensions each) are turned by byte
-//   permutes within the lane. Q and P as three exact parts each.
-//   F32: 4 dimensions, or 4 positions, an instruction; FP32 products.
-// Dimension of instruction e's row m: EV dimensions a lane, 16 lanes, further ones EV * 16 behind.
 // 16 vectors' sums of a wave, as its lanes hold them, row by row to the part's slot or, multiplied by the inverse of the
 // weights' sums, to out: through the wave's own rows of LDS, so that a store's lanes lie side by side.
 template <int HD, int EV, class Row>
@@ -443,6 +434,17 @@ __device__ __forceinline__ void store_rows(const FastPaged &p, const Slot &slot,
   __builtin_amdgcn_wave_barrier();
 }
 
+// The tile's walk: each wave has 16 of its vectors, and takes 32 positions in turn with the other waves that have the same.
+//
+// Lane (lq = lane / 16, lc = lane % 16). S^T = K Q^T and O^T = V^T P^T, so that a lane holds one vector's (lc) scores, weights
+// and sums, and no weight changes lanes: the scores of positions 16 t + 4 lq + e are in the lane that feeds positions 16 t + 4
+// lq + e to the second product, whose order of summation is free.
+//   BF16: 32 dimensions, or 32 positions, an instruction; a lane's V rows (8 positions, 8 dimensions each) are turned by byte
+//   permutes within the lane. Q and P as three exact parts each.
+//   F32: 4 dimensions, or 4 positions, an instruction; FP32 products.
+// Dimension of instruction e's row m: EV dimensions a lane, 16 lanes, further ones EV * 16 behind.
+// Pages of a multiple of 16 positions hold 16 rows side by side, named by one entry of the table that a lane has looked up
+// before; of others each K row and each four V rows (each V row, where four may lie in two pages) have a look of their own.
 // MODE: whole heads of HD dimensions, heads of fewer, or either with pages that are no multiple of 16 positions.
 enum { kWhole, kPart, kAny };
 template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p, const Item &it, float *lds) {
