@@ -5,8 +5,9 @@
   attention  llhip_attention_paged: each request's rows attend to the positions that its pages hold.
   logprobs   llhip_token_logprobs: log probabilities of given tokens, the rows' entropies and their likeliest tokens.
 
-run() computes them in elementary torch operations, or, where `own` is set, through the library's entry points. exact()
-is written from the definitions, in float64.
+run() computes them in elementary torch operations, or, where `own` is set, through the library's entry points: those are
+queued on the library's own stream, so what run() returns is read behind llhip_synchronize or a synchronization of the
+device. exact() is written from the definitions, in float64.
 """
 import math
 import os
@@ -192,6 +193,7 @@ def prepare(case, seed):
     st.case = case
     if own:
         st.call = _OWN[case["kind"]](st, case)
+        torch.cuda.synchronize()  # the inputs were made on torch's stream; the library has its own
     return st
 
 
