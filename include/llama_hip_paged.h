@@ -63,10 +63,11 @@ void llhip_rope_kv_append_paged(float *q_out, size_t q_out_stride, const float *
  * rows of out n_heads * head_dim; scores, softmax and value sums as in k_attention: products of the F32 queries and weights
  * with the pages' values, FP32 sums; a non-finite score fails with "nonfinite value in softmax". The sums are divided by the
  * weights' at the end, which may reach 2^8 each, so n positions' values must stay below 1e36 / n. What lies in a page behind
- * the request's last position is not used, and a value that is not finite reaches the rows that see its position only. A
- * request with a page outside the caches fails at the next host-visible point; its rows' values are then unspecified. out
- * must not overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most
- * 16 per KV head, head_dim at most 256.
+ * the request's last position is not used, and a value that is not finite reaches the rows that see its position only, in its
+ * dimension: an infinity gives infinity, whatever its weight, and NaN beside one of the other sign or beside a NaN. A request
+ * with a page outside the caches fails at the next host-visible point; its rows' values are then unspecified. out must not
+ * overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16 per KV
+ * head, head_dim at most 256.
  *
  * Rows of K and V in whole 16-byte vectors (head_dim a multiple of 8 in BF16 pages, of 4 in F32 ones, the caches 16-byte
  * aligned) take the matrix cores, with at most 2^20 rows and 4096 KV heads; any other shape has each row read what it attends

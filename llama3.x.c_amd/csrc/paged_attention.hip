@@ -41,6 +41,11 @@ bool launch_ok(const char *what) {
 __device__ __forceinline__ float value(const float *p) { return *p; }
 __device__ __forceinline__ float value(const uint16_t *p) { return __uint_as_float((uint32_t)*p << 16); }
 
+// x where it is not finite, else 0. A row's sum over values of which some are not finite is the sum of those, whatever their
+// weights: infinity, or NaN beside one of the other sign or a NaN. A product can't tell: weights are above zero, but FP32, or
+// a weight's lower part in BF16, has 0 for many of them, and 0 * infinity is NaN.
+__device__ __forceinline__ float odd_only(float x) { return isfinite(x) ? 0.0f : x; }
+
 struct PagedAttn {
   AttentionPagedJob job;
   float divisor; // sqrtf(head_dim)
@@ -173,7 +178,16 @@ template <typename T> __global__ __launch_bounds__(kThreads) void attn_paged_row
     float total = 0.0f;
     for (int s2 = 0; s2 < shares; s2++)
       total += acc[(size_t)s2 * kv_mul * hd + i];
-    dst[i] = total / run_sum[i / hd];
+    total /= run_sum[i / hd];
+    if (!isfinite(total)) {
+      float odd = 0.0f;
+      for (int t = 0; t < positions; t++) {
+        const int page = max(page_of(b, request, t / b.page_size), 0);
+        odd += odd_only(value(values + (size_t)page * b.page_values + (size_t)(t % b.page_size) * b.pos_stride + i % hd));
+      }
+      total = odd == 0.0f ? total : odd;
+    }
+    dst[i] = total;
   }
 }
 
@@ -398,10 +412,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void *cache, lon
   return __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)base, (short)0, bytes, 0x00020000);
 }
 
+// Not 0 behind a value that is not finite.
+__device__ __forceinline__ float mark_of(const float4 &x, float mark) {
+  return fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, fmaf(x.z, 0.0f, fmaf(x.w, 0.0f, mark))));
+}
+
 // 16 vectors' sums of a wave, as its lanes hold them, row by row to the part's slot or, multiplied by the inverse of the
-// weights' sums, to out: through the wave's own rows of LDS, so that a store's lanes lie side by side.
+// weights' sums, to out: through the wave's own rows of LDS, so that a store's lanes lie side by side. Returns the mark of what
+// it gave to out.
 template <int HD, int EV, class Row>
-__device__ __forceinline__ void store_rows(const FastPaged &p, const Slot &slot, bool whole, const v4f (&o)[HD / 16], float inverse,
+__device__ __forceinline__ float store_rows(const FastPaged &p, const Slot &slot, bool whole, const v4f (&o)[HD / 16], float inverse,
                                            float *rows, int lane, int hd, int v0, int count, Row row_of) {
   constexpr int kRow = HD + 4;
   const int lq = lane >> 4, lc = lane & 15;
@@ -417,12 +437,14 @@ __device__ __forceinline__ void store_rows(const FastPaged &p, const Slot &slot,
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // written by one lane, read by another
   __builtin_amdgcn_wave_barrier();
   const int hd4 = hd / 4;
+  float mark = 0.0f;
   for (int i = lane; i < count * hd4; i += kWave) {
     const int v = i / hd4, d = i % hd4 * 4;
     const float4 x = *reinterpret_cast<const float4 *>(rows + v * kRow + d);
     if (!whole) {
       put4(slot, (unsigned)((v0 + v) * (HD / 4) + d / 4), x);
     } else {
+      mark = mark_of(x, mark);
       float *to = row_of(v0 + v) + d;
       if (p.out_vec)
         *reinterpret_cast<float4 *>(to) = x;
@@ -432,6 +454,7 @@ __device__ __forceinline__ void store_rows(const FastPaged &p, const Slot &slot,
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // read before it is written again
   __builtin_amdgcn_wave_barrier();
+  return mark;
 }
 
 // The tile's walk: each wave has 16 of its vectors, and takes 32 positions in turn with the other waves that have the same.
@@ -446,8 +469,9 @@ __device__ __forceinline__ void store_rows(const FastPaged &p, const Slot &slot,
 // Pages of a multiple of 16 positions hold 16 rows side by side, named by one entry of the table that a lane has looked up
 // before; of others each K row and each four V rows (each V row, where four may lie in two pages) have a look of their own.
 // MODE: whole heads of HD dimensions, heads of fewer, or either with pages that are no multiple of 16 positions.
+// Returns the mark of what it gave to out.
 enum { kWhole, kPart, kAny };
-template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p, const Item &it, float *lds) {
+template <typename T, int HD, int MODE> __device__ float walk(const FastPaged &p, const Item &it, float *lds) {
   constexpr bool kBf16 = sizeof(T) == 2, ANY = MODE == kAny;
   constexpr int E = HD / 16, EV = E < (kBf16 ? 8 : 4) ? E : (kBf16 ? 8 : 4), kVecs = E / EV; // a V row: kVecs loads of EV
   constexpr int kSteps = kBf16 ? HD / 32 : HD / 16; // a K row: loads of 16 bytes
@@ -776,6 +800,7 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   };
   const bool whole = it.slot < 0;
   const Slot slot = slot_at<HD>(p, max(it.slot, 0));
+  float mark = 0.0f;
   constexpr int kFours = E / 4; // a lane's r-th row: kFours groups of four dimensions
   const float l = four_sum(l_run), inverse = 1.0f / l;
   if (it.walkers > 1) { // the waves' sums meet in LDS: [wave][vector][HD values, maximum, sum]
@@ -806,7 +831,9 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
         sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
       }
       if (whole) {
-        store(target(v) + 4 * d4, float4{sum.x / whole_l, sum.y / whole_l, sum.z / whole_l, sum.w / whole_l});
+        const float4 x = float4{sum.x / whole_l, sum.y / whole_l, sum.z / whole_l, sum.w / whole_l};
+        mark = mark_of(x, mark);
+        store(target(v) + 4 * d4, x);
       } else {
         put4(slot, (unsigned)(v * (HD / 4) + d4), sum);
         if (d4 == 0)
@@ -816,8 +843,9 @@ template <typename T, int HD, int MODE> __device__ void walk(const FastPaged &p,
   } else if (mine > 0) { // uniform
     if (!whole && lq == 0 && active)
       put_end(slot, v0 + lc, m_run, l);
-    store_rows<HD, EV>(p, slot, whole, o, inverse, lds + (size_t)wave * 16 * kRow, lane, hd, v0, mine, target);
+    mark = store_rows<HD, EV>(p, slot, whole, o, inverse, lds + (size_t)wave * 16 * kRow, lane, hd, v0, mine, target);
   }
+  return mark;
 }
 
 // A tile of more than 64 vectors over BF16 pages: each wave has 32 of them and takes all positions. A step's K and V rows are
@@ -828,7 +856,7 @@ template <int HD> struct WideStage {
   uint16_t k[kStep * kKRow];
   v4u v[HD / 16][kWave]; // [instruction][lane]: eight positions of a dimension
 };
-template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const Item &it, float *lds) {
+template <int HD, int MODE> __device__ float walk_wide(const FastPaged &p, const Item &it, float *lds) {
   typedef WideStage<HD> Stage;
   static_assert(2 * sizeof(Stage) <= kWaves * 16 * (HD + 4) * sizeof(float), "two stages in the sums' place");
   Stage *const stages = reinterpret_cast<Stage *>(lds); // two: a step is staged while the one before is computed
@@ -1110,6 +1138,7 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
   const bool whole = it.slot < 0;
   const Slot slot = slot_at<HD>(p, max(it.slot, 0));
   __syncthreads(); // the stages' place is free
+  float mark = 0.0f;
   auto target = [&](int v) {
     return p.job.out + ((size_t)(it.row0 + v / kv_mul) * p.job.n_heads + (size_t)it.g * kv_mul + v % kv_mul) * hd;
   };
@@ -1120,25 +1149,52 @@ template <int HD, int MODE> __device__ void walk_wide(const FastPaged &p, const 
       continue; // uniform
     if (!whole && lq == 0 && 16 * n + lc < mine)
       put_end(slot, v0 + 16 * n + lc, m_run[n], l);
-    store_rows<HD, EV>(p, slot, whole, o[n], inverse, lds + (size_t)wave * 16 * kRow, lane, hd, v0 + 16 * n,
-                       min(mine - 16 * n, 16), target);
+    mark += store_rows<HD, EV>(p, slot, whole, o[n], inverse, lds + (size_t)wave * 16 * kRow, lane, hd, v0 + 16 * n,
+                               min(mine - 16 * n, 16), target);
   }
+  return mark;
 }
 
-template <typename T, int HD, int MODE, bool WIDE>
-__global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn_paged(FastPaged p) {
-  constexpr int kRow = HD + 4;
-  __shared__ Plan plan;
-  __shared__ __align__(16) float lds[kWaves * 16 * kRow];
-  __shared__ unsigned arrived;
+// A tile that gave out something not finite: each of its rows gets what its positions' values hold, in the dimensions where
+// one is not finite. Threads (share, dimension), the shares' positions interleaved; LDS free before and behind.
+template <typename T> __device__ __forceinline__ void give_odd(const FastPaged &p, const Item &it, float *lds) {
   const PagedDev &b = p.job.batch;
-  const int tid = threadIdx.x, g = blockIdx.x % p.job.n_kv_heads, block = blockIdx.x / p.job.n_kv_heads;
-  const int hd = p.job.head_dim, kv_mul = p.kv_mul;
-  const long long total = make_plan(p, plan);
-  const Slices slices = make_slices(p, total);
-  const long long lo = slices.start(block), hi = slices.start(block + 1) < total ? slices.start(block + 1) : total;
-  if (lo >= total)
-    return;
+  const int tid = threadIdx.x, hd = p.job.head_dim, shares = kThreads / hd, share = tid / hd, d = tid % hd;
+  auto at = [&](int t) {
+    const int page = max(page_of(b, it.r, t / b.page_size), 0);
+    return odd_only(value((const T *)p.job.value + (size_t)page * b.page_values + (size_t)(t % b.page_size) * b.pos_stride +
+                          (size_t)it.g * b.head_base + d));
+  };
+  float odd = 0.0f;
+  if (share < shares)
+    for (int t = share; t <= it.last0; t += shares)
+      odd += at(t);
+  lds[tid] = odd;
+  __syncthreads();
+  if (share == 0) {
+    for (int s = 1; s < shares; s++)
+      odd += lds[s * hd + d];
+    for (int j = 0; j < it.vectors / p.kv_mul; j++) {
+      odd += j ? at(it.last0 + j) : 0.0f;
+      for (int h = 0; h < p.kv_mul && odd != 0.0f; h++)
+        p.job.out[((size_t)(it.row0 + j) * p.job.n_heads + (size_t)it.g * p.kv_mul + h) * hd + d] = odd;
+    }
+  }
+  __syncthreads();
+}
+
+// A block's part of a walk with what of the line its join needs.
+struct Part {
+  Item it;
+  long long w0, end; // where the walk begins and ends on the line
+  int begin, unit, grain;
+  bool shared, begins; // with other blocks; in this one's slice
+};
+// The parts of the line's lo .. hi - 1, in order.
+template <class Visit>
+__device__ __forceinline__ void each_part(const FastPaged &p, const Plan &plan, int g, long long lo, long long hi, Visit visit) {
+  const PagedDev &b = p.job.batch;
+  const int kv_mul = p.kv_mul;
   int r = 0; // the first request whose walks end behind lo
   for (int step = kMaxRequests; step > 0; step >>= 1)
     if (r + step <= b.count && plan.line[r + step - 1] <= lo)
@@ -1160,7 +1216,8 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
         break;
       const int row = t * p.tile_rows, rows = min(q.rows - row, p.tile_rows);
       const int positions = q.length + row + rows;
-      Item it;
+      Part part;
+      Item &it = part.it;
       it.vectors = rows * kv_mul;
       it.walkers = walkers_of(it.vectors);
       const int begin = begin_time(it.vectors), unit = position_time(it.vectors), grain = it.walkers * kStep;
@@ -1178,134 +1235,182 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
         continue; // the rounds leave this block none of it
       it.r = r, it.g = g;
       it.row0 = q.first + row, it.last0 = q.length + row;
-      const bool shared = it.t0 > 0 || it.t1 < positions;
-      auto slot_of = [&](int blk, bool begins) { return (g * p.blocks + blk) * 2 + begins; };
-      it.slot = uniform(shared ? slot_of(block, w0 >= lo) : -1);
-      __syncthreads(); // LDS is free
-      if constexpr (WIDE) {
-        if (it.vectors > kTileVectors)
-          walk_wide<HD, MODE>(p, it, lds);
-        else
-          walk<T, HD, MODE>(p, it, lds);
-      } else {
-        walk<T, HD, MODE>(p, it, lds);
-      }
-      if (!shared)
-        continue;
-      // the walk's blocks: from .. last_block
-      const int first = slices.block_of(w0), last_block = slices.block_of(end - 1);
-      // the first block whose slice ends behind the walk's first round
-      const int from = min(max(first, slices.block_of(w0 + begin + unit * grain - 1)), last_block), parts = last_block - from + 1;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
-      __syncthreads();                                 // the block's
-      if (tid == 0)
-        arrived = __hip_atomic_fetch_add(&paged_arrivals[(g * p.blocks + first) * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      if (arrived != (unsigned)(parts - 1))
-        continue;
-      if (tid == 0)
-        __hip_atomic_store(&paged_arrivals[(g * p.blocks + first) * kLine], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      // The parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
-      // LDS, then the sums in the parts' order, whoever comes last. A part's place by its number.
-      auto part = [&](int k) { return slot_at<HD>(p, slot_of(from + k, from + k == first)); };
-      const int hd4 = hd / 4, some = kWaves * 16 * kRow / parts;
-      for (int v0 = 0; v0 < it.vectors; v0 += some) {
-        const int n = min(some, it.vectors - v0), items = n * hd4;
-        __syncthreads(); // LDS is free
-        constexpr int kFew = 8;
-        if (parts <= kFew) { // a thread a vector, its loads together
-          for (int v = tid; v < n; v += kThreads) {
-            float2 x[kFew];
-#pragma unroll
-            for (int k = 0; k < kFew; k++)
-              x[k] = load_end(p, slot_of(from + min(k, parts - 1), from + min(k, parts - 1) == first), v0 + v, HD);
-            float m = -FLT_MAX, l = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kFew; k++)
-              m = fmaxf(m, x[k].x);
-#pragma unroll
-            for (int k = 0; k < kFew; k++) {
-              x[k].x = __builtin_amdgcn_exp2f(x[k].x - m);
-              l = k < parts ? fmaf(x[k].x, x[k].y, l) : l;
-            }
-            const float inverse = 1.0f / l;
-#pragma unroll
-            for (int k = 0; k < kFew; k++)
-              if (k < parts)
-                lds[v * parts + k] = x[k].x * inverse;
-          }
-        } else {
-          for (int v = tid / kWave; v < n; v += kWaves) {
-            float m = -FLT_MAX, l = 0.0f;
-            for (int k = tid % kWave; k < parts; k += kWave) {
-              const float2 end_of = load_end(p, slot_of(from + k, from + k == first), v0 + v, HD);
-              lds[v * parts + k] = end_of.x;
-              const float top = fmaxf(m, end_of.x);
-              l = l * __builtin_amdgcn_exp2f(m - top) + end_of.y * __builtin_amdgcn_exp2f(end_of.x - top);
-              m = top;
-            }
-            const float top = wave_max(m), inverse = 1.0f / wave_sum(l * __builtin_amdgcn_exp2f(m - top));
-            for (int k = tid % kWave; k < parts; k += kWave)
-              lds[v * parts + k] = __builtin_amdgcn_exp2f(lds[v * parts + k] - top) * inverse;
-          }
-        }
-        __syncthreads();
-        // I of the thread's items and K parts at a time: as many loads are in flight
-        auto add_up = [&](auto of_items, auto of_parts) {
-          constexpr int I = decltype(of_items)::value, K = decltype(of_parts)::value;
-          for (int i0 = tid; i0 < items; i0 += I * kThreads) {
-            int v[I], d[I];
-            unsigned at[I];
-            float4 sum[I];
-#pragma unroll
-            for (int j = 0; j < I; j++) {
-              const int i = i0 + j * kThreads;
-              v[j] = i / hd4, d[j] = i % hd4 * 4;
-              at[j] = (unsigned)((v0 + v[j]) * (HD / 4) + d[j] / 4);
-              if (i >= items)
-                v[j] = 0, d[j] = -1, at[j] = kNowhere / 16; // reads zero
-              sum[j] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-            for (int k0 = 0; k0 < parts; k0 += K) {
-              float4 x[K][I];
-#pragma unroll
-              for (int k = 0; k < K; k++) {
-                const Slot slot = part(min(k0 + k, parts - 1));
-#pragma unroll
-                for (int j = 0; j < I; j++)
-                  x[k][j] = get4(slot, k0 + k < parts ? at[j] : kNowhere / 16);
-              }
-#pragma unroll
-              for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int j = 0; j < I; j++) {
-                  const float scale = lds[v[j] * parts + min(k0 + k, parts - 1)];
-                  sum[j] = float4{fmaf(scale, x[k][j].x, sum[j].x), fmaf(scale, x[k][j].y, sum[j].y),
-                                  fmaf(scale, x[k][j].z, sum[j].z), fmaf(scale, x[k][j].w, sum[j].w)};
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < I; j++)
-              if (d[j] >= 0) {
-                const int vector = v0 + v[j];
-                float *to = p.job.out + ((size_t)(it.row0 + vector / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + vector % kv_mul) * hd + d[j];
-                if (p.out_vec)
-                  *reinterpret_cast<float4 *>(to) = sum[j];
-                else
-                  to[0] = sum[j].x, to[1] = sum[j].y, to[2] = sum[j].z, to[3] = sum[j].w;
-              }
-          }
-        };
-        if (items > 2 * kThreads)
-          add_up(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
-        else if (parts > 16 && items <= kThreads)
-          add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
-        else if (parts > 4)
-          add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-        else
-          add_up(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
-      }
+      part.w0 = w0, part.end = end, part.begin = begin, part.unit = unit, part.grain = grain;
+      part.shared = it.t0 > 0 || it.t1 < positions;
+      part.begins = w0 >= lo;
+      visit(part);
     }
+  }
+}
+
+template <typename T, int HD, int MODE, bool WIDE>
+__global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn_paged(FastPaged p) {
+  constexpr int kRow = HD + 4;
+  __shared__ Plan plan;
+  __shared__ __align__(16) float lds[kWaves * 16 * kRow];
+  __shared__ unsigned arrived;
+  // which parts' results, as this block gave them out, are not all finite: 1 those of a walk that is its own, 2 those of one
+  // that an earlier block began, 4 those of one that goes on in the next
+  __shared__ unsigned odd;
+  if (threadIdx.x == 0)
+    odd = 0;
+  const int tid = threadIdx.x, g = blockIdx.x % p.job.n_kv_heads, block = blockIdx.x / p.job.n_kv_heads;
+  const int hd = p.job.head_dim, kv_mul = p.kv_mul;
+  const long long total = make_plan(p, plan);
+  const Slices slices = make_slices(p, total);
+  const long long lo = slices.start(block), hi = slices.start(block + 1) < total ? slices.start(block + 1) : total;
+  if (lo >= total)
+    return;
+  each_part(p, plan, g, lo, hi, [&](Part &mine) {
+    Item &it = mine.it;
+    auto slot_of = [&](int blk, bool begins) { return (g * p.blocks + blk) * 2 + begins; };
+    it.slot = uniform(mine.shared ? slot_of(block, mine.begins) : -1);
+    __syncthreads(); // LDS is free
+    float mark;
+    if constexpr (WIDE) {
+      if (it.vectors > kTileVectors)
+        mark = walk_wide<HD, MODE>(p, it, lds);
+      else
+        mark = walk<T, HD, MODE>(p, it, lds);
+    } else {
+      mark = walk<T, HD, MODE>(p, it, lds);
+    }
+    if (!mine.shared) {
+      if (mark != 0.0f)
+        atomicOr(&odd, 1u);
+      return;
+    }
+    const long long w0 = mine.w0, end = mine.end;
+    const int begin = mine.begin, unit = mine.unit, grain = mine.grain;
+    // the walk's blocks: from .. last_block
+    const int first = slices.block_of(w0), last_block = slices.block_of(end - 1);
+    // the first block whose slice ends behind the walk's first round
+    const int from = min(max(first, slices.block_of(w0 + begin + unit * grain - 1)), last_block), parts = last_block - from + 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's sums have arrived
+    __syncthreads();                                 // the block's
+    if (tid == 0)
+      arrived = __hip_atomic_fetch_add(&paged_arrivals[(g * p.blocks + first) * kLine], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != (unsigned)(parts - 1))
+      return;
+    if (tid == 0)
+      __hip_atomic_store(&paged_arrivals[(g * p.blocks + first) * kLine], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The parts of some vectors at a time: each part's share of the vector's sums, exp2(m - the largest) / the whole l, into
+    // LDS, then the sums in the parts' order, whoever comes last. A part's place by its number.
+    auto part = [&](int k) { return slot_at<HD>(p, slot_of(from + k, from + k == first)); };
+    const int hd4 = hd / 4, some = kWaves * 16 * kRow / parts;
+    mark = 0.0f;
+    for (int v0 = 0; v0 < it.vectors; v0 += some) {
+      const int n = min(some, it.vectors - v0), items = n * hd4;
+      __syncthreads(); // LDS is free
+      constexpr int kFew = 8;
+      if (parts <= kFew) { // a thread a vector, its loads together
+        for (int v = tid; v < n; v += kThreads) {
+          float2 x[kFew];
+#pragma unroll
+          for (int k = 0; k < kFew; k++)
+            x[k] = load_end(p, slot_of(from + min(k, parts - 1), from + min(k, parts - 1) == first), v0 + v, HD);
+          float m = -FLT_MAX, l = 0.0f;
+#pragma unroll
+          for (int k = 0; k < kFew; k++)
+            m = fmaxf(m, x[k].x);
+#pragma unroll
+          for (int k = 0; k < kFew; k++) {
+            x[k].x = __builtin_amdgcn_exp2f(x[k].x - m);
+            l = k < parts ? fmaf(x[k].x, x[k].y, l) : l;
+          }
+          const float inverse = 1.0f / l;
+#pragma unroll
+          for (int k = 0; k < kFew; k++)
+            if (k < parts)
+              lds[v * parts + k] = x[k].x * inverse;
+        }
+      } else {
+        for (int v = tid / kWave; v < n; v += kWaves) {
+          float m = -FLT_MAX, l = 0.0f;
+          for (int k = tid % kWave; k < parts; k += kWave) {
+            const float2 end_of = load_end(p, slot_of(from + k, from + k == first), v0 + v, HD);
+            lds[v * parts + k] = end_of.x;
+            const float top = fmaxf(m, end_of.x);
+            l = l * __builtin_amdgcn_exp2f(m - top) + end_of.y * __builtin_amdgcn_exp2f(end_of.x - top);
+            m = top;
+          }
+          const float top = wave_max(m), inverse = 1.0f / wave_sum(l * __builtin_amdgcn_exp2f(m - top));
+          for (int k = tid % kWave; k < parts; k += kWave)
+            lds[v * parts + k] = __builtin_amdgcn_exp2f(lds[v * parts + k] - top) * inverse;
+        }
+      }
+      __syncthreads();
+      // I of the thread's items and K parts at a time: as many loads are in flight
+      auto add_up = [&](auto of_items, auto of_parts) {
+        constexpr int I = decltype(of_items)::value, K = decltype(of_parts)::value;
+        for (int i0 = tid; i0 < items; i0 += I * kThreads) {
+          int v[I], d[I];
+          unsigned at[I];
+          float4 sum[I];
+#pragma unroll
+          for (int j = 0; j < I; j++) {
+            const int i = i0 + j * kThreads;
+            v[j] = i / hd4, d[j] = i % hd4 * 4;
+            at[j] = (unsigned)((v0 + v[j]) * (HD / 4) + d[j] / 4);
+            if (i >= items)
+              v[j] = 0, d[j] = -1, at[j] = kNowhere / 16; // reads zero
+            sum[j] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+          }
+          for (int k0 = 0; k0 < parts; k0 += K) {
+            float4 x[K][I];
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+              const Slot slot = part(min(k0 + k, parts - 1));
+#pragma unroll
+              for (int j = 0; j < I; j++)
+                x[k][j] = get4(slot, k0 + k < parts ? at[j] : kNowhere / 16);
+            }
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+              for (int j = 0; j < I; j++) {
+                const float scale = lds[v[j] * parts + min(k0 + k, parts - 1)];
+                sum[j] = float4{fmaf(scale, x[k][j].x, sum[j].x), fmaf(scale, x[k][j].y, sum[j].y),
+                                fmaf(scale, x[k][j].z, sum[j].z), fmaf(scale, x[k][j].w, sum[j].w)};
+              }
+          }
+#pragma unroll
+          for (int j = 0; j < I; j++)
+            if (d[j] >= 0) {
+              mark = mark_of(sum[j], mark);
+              const int vector = v0 + v[j];
+              float *to = p.job.out + ((size_t)(it.row0 + vector / kv_mul) * p.job.n_heads + (size_t)g * kv_mul + vector % kv_mul) * hd + d[j];
+              if (p.out_vec)
+                *reinterpret_cast<float4 *>(to) = sum[j];
+              else
+                to[0] = sum[j].x, to[1] = sum[j].y, to[2] = sum[j].z, to[3] = sum[j].w;
+            }
+        }
+      };
+      if (items > 2 * kThreads)
+        add_up(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+      else if (parts > 16 && items <= kThreads)
+        add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+      else if (parts > 4)
+        add_up(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+      else
+        add_up(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+    }
+    if (mark != 0.0f)
+      atomicOr(&odd, mine.begins ? 4u : 2u);
+  });
+  // What is not finite is looked for behind all parts, rare as it is: inside the loop its registers cost one F32 row at 35000
+  // positions 73 us instead of 70. The flags are written, by a barrier that does not wait for the rows' stores.
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  if (__builtin_expect(odd != 0, 0)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's rows are stored
+    __syncthreads();                                 // the block's
+    each_part(p, plan, g, lo, hi, [&](Part &mine) {
+      if (odd & (mine.shared ? mine.begins ? 4u : 2u : 1u))
+        give_odd<T>(p, mine.it, lds);
+    });
   }
 }
 

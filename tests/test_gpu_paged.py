@@ -536,6 +536,45 @@ def test_a_value_that_is_not_finite_reaches_the_rows_that_see_it(L, bf16, hd, wh
     within(got[fine], want.reshape(got.shape)[fine], bound.reshape(got.shape)[fine], (hd, what))
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("heads,kv,hd", [(8, 2, 64), (8, 2, 128), (4, 2, 256), (6, 2, 80), (8, 2, 50)])
+@pytest.mark.parametrize("rows_of,lengths", [([1], [70]), ([3, 1], [40, 200]), ([50, 1, 6], [20, 90, 30]), ([1], [9000]),
+                                             ([2, 40], [5000, 3000])])
+@pytest.mark.parametrize("page", [16, 12])
+def test_a_seen_infinity_gives_infinity(L, bf16, heads, kv, hd, rows_of, lengths, page):
+    """V values that are not finite, wherever a row sees them and whatever their weight: infinity gives infinity, both signs or
+    a NaN give NaN, in their dimension alone. One lies at the position of the largest score of some row (a weight of 1, whose
+    lower parts are zero), others where weights are far below the smallest float (scores some hundreds apart), at the first
+    position, in the middle and in the prompts' own rows."""
+    L.kernels_kv_layout_select(b"head")
+    b = pu.Pages(hu.dev, rows_of, lengths, page=page, bf16=bf16)
+    rng = np.random.default_rng(hd + len(rows_of))
+    key, value = b.cache(rng, "head", kv, hd), b.cache(rng, "head", kv, hd)
+    q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+    q[::2] *= F(60.0)
+    clean = value.copy()
+    for r, rows, length in b.requests():
+        seen, n = length + rows.stop - rows.start, rows.stop - rows.start
+        scores = b.gather(key, "head", r, length + 1)[1] @ q[rows.start].reshape(heads, hd)[heads // kv]
+        places = [(0, 0, 1, np.inf), (int(scores.argmax()), 1, 2, np.inf), (int(scores.argmin()), 1, 3, -np.inf),
+                  (length // 2, 0, 4, np.inf), (length // 2 + 1, 0, 4, -np.inf), (length // 3, 1, 5, np.nan),
+                  (length + n // 2, 0, hd - 1, np.inf), (seen - 1, 1, hd - 2, -np.inf)]
+        for t, g, d, x in places:
+            b.row(value, "head", r, t)[g, d] = pu.to_bf16(np.array([x], F))[0] if bf16 else x
+    want, bound = pu.attention(b, q, key, clean, heads, kv, hd, "head")
+    want, bound = want.reshape(b.rows, heads, hd), bound.reshape(b.rows, heads, hd)
+    for r, rows, length in b.requests():
+        vals = b.gather(value, "head", r, length + rows.stop - rows.start)
+        for j, i in enumerate(range(rows.start, rows.stop)):
+            with np.errstate(invalid="ignore"):
+                odd = np.repeat(np.where(np.isfinite(vals), 0.0, vals)[:, :length + j + 1].sum(1), heads // kv, 0)
+            want[i] = np.where(odd == 0.0, want[i], odd)
+    got = attention_case_equal_scores(L, b, q, key, value, heads, kv, hd).reshape(want.shape)
+    odd = ~np.isfinite(want)
+    assert odd.any() and np.array_equal(got[odd], want[odd], equal_nan=True)
+    within(got[~odd], want[~odd], bound[~odd], (heads, kv, hd, page))
+
+
 def test_attention_fails_for_scores_that_are_not_finite(L):
     L.kernels_kv_layout_select(b"head")
     for hd, rows_of, lengths in ((64, [1], [40]), (128, [20], [10]), (40, [1], [13]), (18, [2], [9])):
