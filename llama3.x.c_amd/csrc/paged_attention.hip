@@ -390,6 +390,13 @@ __device__ __forceinline__ float2 load_end(const FastPaged &p, int slot, int v, 
   return float2{__uint_as_float((unsigned)x), __uint_as_float((unsigned)(x >> 32))};
 }
 
+// exp2(x) of what moves sums from one maximum to another, x <= 0: denormal below 2^-126, where the instruction gives 0. The
+// weights in such sums may be 2^8, so that 2^-118 of the largest weight would be lost, and V may hold values 10^40 apart.
+__device__ __forceinline__ float exp2_far(float x) {
+  const float half = __builtin_amdgcn_exp2f(0.5f * x);
+  return half * half;
+}
+
 // x = a + b + c exactly, each of at most eight significant bits (truncated, so that nothing overflows): three BF16 values.
 // Two x give a dword of each part.
 __device__ __forceinline__ void bf16_parts(float x, float y, unsigned (&part)[3]) {
@@ -700,7 +707,7 @@ template <typename T, int HD, int MODE> __device__ float walk(const FastPaged &p
     }
     // the maximum moves only where weights would pass 2^8: rare, and the sums keep their bits
     if (__any(top > m_run + 8.0f)) {
-      const float m = fmaxf(m_run, four_max(top)), alpha = __builtin_amdgcn_exp2f(m_run - m);
+      const float m = fmaxf(m_run, four_max(top)), alpha = exp2_far(m_run - m);
       l_run *= alpha;
       m_run = m;
 #pragma unroll
@@ -825,7 +832,7 @@ template <typename T, int HD, int MODE> __device__ float walk(const FastPaged &p
       float4 sum = float4{0.0f, 0.0f, 0.0f, 0.0f};
       for (int w = 0; w < it.walkers; w++) {
         const float *at = src + (size_t)w * 16 * kRow;
-        const float scale = __builtin_amdgcn_exp2f(at[HD] - m);
+        const float scale = exp2_far(at[HD] - m);
         const float4 x = *reinterpret_cast<const float4 *>(at + 4 * d4);
         whole_l = fmaf(scale, at[HD + 1], whole_l);
         sum = float4{fmaf(scale, x.x, sum.x), fmaf(scale, x.y, sum.y), fmaf(scale, x.z, sum.z), fmaf(scale, x.w, sum.w)};
@@ -1077,7 +1084,7 @@ template <int HD, int MODE> __device__ float walk_wide(const FastPaged &p, const
         top = fmaxf(top, w[j]);
       }
       if (__any(top > m_run[n] + 8.0f)) { // as in walk
-        const float m = fmaxf(m_run[n], four_max(top)), alpha = __builtin_amdgcn_exp2f(m_run[n] - m);
+        const float m = fmaxf(m_run[n], four_max(top)), alpha = exp2_far(m_run[n] - m);
         l_run[n] *= alpha;
         m_run[n] = m;
 #pragma unroll
@@ -1316,7 +1323,7 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
             m = fmaxf(m, x[k].x);
 #pragma unroll
           for (int k = 0; k < kFew; k++) {
-            x[k].x = __builtin_amdgcn_exp2f(x[k].x - m);
+            x[k].x = exp2_far(x[k].x - m);
             l = k < parts ? fmaf(x[k].x, x[k].y, l) : l;
           }
           const float inverse = 1.0f / l;
@@ -1337,7 +1344,7 @@ __global__ __launch_bounds__(kThreads, HD > 128 ? 1 : kMaxBlocksPerCu) void attn
           }
           const float top = wave_max(m), inverse = 1.0f / wave_sum(l * __builtin_amdgcn_exp2f(m - top));
           for (int k = tid % kWave; k < parts; k += kWave)
-            lds[v * parts + k] = __builtin_amdgcn_exp2f(lds[v * parts + k] - top) * inverse;
+            lds[v * parts + k] = exp2_far(lds[v * parts + k] - top) * inverse;
         }
       }
       __syncthreads();

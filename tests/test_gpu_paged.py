@@ -575,6 +575,32 @@ def test_a_seen_infinity_gives_infinity(L, bf16, heads, kv, hd, rows_of, lengths
     within(got[~odd], want[~odd], bound[~odd], (heads, kv, hd, page))
 
 
+STAIRS = [([1], [400], (3, 131, 259)), ([6], [400], (3, 131, 259)), ([60], [400], (3, 131, 259)),
+          ([1], [9000], (3, 131, 8900)), ([40], [5000], (3, 131, 4900))]
+# beside long requests, which make the parts of 8 KV heads' walks longer
+LONG_STAIRS = [([1] * 11, [400] + [4000] * 10, (3, 131, 259)), ([60] + [1] * 12, [400] + [6000] * 12, (3, 35, 67))]
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("heads,kv,hd,rows_of,lengths,places",
+                         [(*shape, *c) for shape in [(8, 2, 64), (8, 2, 128), (4, 2, 256), (6, 2, 50)] for c in STAIRS] +
+                         [(16, 8, 64, *c) for c in STAIRS + LONG_STAIRS])
+def test_weights_near_the_smallest_float(L, bf16, heads, kv, hd, rows_of, lengths, places):
+    """Scores, in powers of two, of 0, 7.9 and 126.5, in steps of one wave that follow each other and in two parts of a walk:
+    the second's weight is 2^-118.6 of the largest, and with a V of 1e30 there it is all that the row has."""
+    L.kernels_kv_layout_select(b"head")
+    b = pu.Pages(hu.dev, rows_of, lengths, page=16, bf16=bf16)
+    key, value = (np.zeros(b.shape("head", kv, hd), F) for _ in range(2))
+    q = np.zeros((b.rows, heads, hd), F)
+    q[:, :, 0] = np.sqrt(hd) * np.log(2.0)
+    key[..., 0] = -100.0
+    for t, score in zip(places, (0.0, 7.90625, 126.5)):
+        b.row(key, "head", 0, t)[:, 0] = score
+    b.row(value, "head", 0, places[1])[:] = 1e30
+    caches = [pu.to_bf16(x) if bf16 else x for x in (key, value)]
+    attention_case(L, 1, heads, kv, hd, "head", b, caches=caches, q=q.reshape(b.rows, -1))
+
+
 def test_attention_fails_for_scores_that_are_not_finite(L):
     L.kernels_kv_layout_select(b"head")
     for hd, rows_of, lengths in ((64, [1], [40]), (128, [20], [10]), (40, [1], [13]), (18, [2], [9])):
