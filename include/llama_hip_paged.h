@@ -66,7 +66,7 @@ void llhip_rope_kv_append_paged(float *q_out, size_t q_out_stride, const float *
  * the request's last position is not used, and a value that is not finite reaches the rows that see its position only, in its
  * dimension: an infinity gives infinity, whatever its weight, and NaN beside one of the other sign or beside a NaN. A request
  * with a page outside the caches fails at the next host-visible point; its rows' values are then unspecified. out must not
- * overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, at most 16 per KV
+ * overlap q, a cache or the batch's arrays. The shapes are k_attention's: n_heads a multiple of n_kv_heads, 1 to 16 per KV
  * head, head_dim at most 256.
  *
  * Rows of K and V in whole 16-byte vectors (head_dim a multiple of 8 in BF16 pages, of 4 in F32 ones, the caches 16-byte

@@ -155,9 +155,9 @@ void llhip_attention_paged(float *out, const float *q, size_t q_stride, const vo
     return;
   if (!batch_ok(name, batch))
     return;
-  if (!attention_shape_ok(n_heads, n_kv_heads, head_dim)) {
-    raise("%s: %d heads over %d KV heads of dimension %d are not supported (n_heads a multiple of n_kv_heads, at most "
-          "16 per KV head, head_dim <= 256)", name, n_heads, n_kv_heads, head_dim);
+  if (n_heads <= 0 || !attention_shape_ok(n_heads, n_kv_heads, head_dim)) {
+    raise("%s: %d heads over %d KV heads of dimension %d are not supported (n_heads positive and a multiple of n_kv_heads, "
+          "at most 16 per KV head, head_dim <= 256)", name, n_heads, n_kv_heads, head_dim);
     return;
   }
   const size_t dq = (size_t)n_heads * head_dim, rows = (size_t)batch->rows;

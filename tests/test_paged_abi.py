@@ -109,6 +109,14 @@ def test_attention_refusals(L):
         assert not lh.last_error()
 
 
+def test_attention_of_no_heads_is_refused(L):
+    """No head, or fewer: the tiles' rows would be a quotient by the heads of a KV head."""
+    b, rows, cache = make(), np.zeros((3, 32), F), np.zeros((2, 6, 2, 16, 8), F)
+    for heads in (0, -2, -2 ** 31):
+        L.llhip_attention_paged(lh.ptr(rows), lh.ptr(rows.copy()), 32, lh.ptr(cache[0]), lh.ptr(cache[1]), b.struct, heads, 2, 8)
+        refused(L, f"{heads} heads over 2 KV heads")
+
+
 def append_call(L, batch, heads=4, kv=2, hd=8, rows=3, o_stride=None, q_stride=None, kv_stride=None, **over):
     a = {"o": np.zeros((rows, heads * hd), F), "q": np.zeros((rows, heads * hd), F), "k": np.zeros((rows, kv * hd), F),
          "v": np.zeros((rows, kv * hd), F), "t": np.zeros((64, 2 * hd), F), "qn": np.zeros(hd, F), "kn": np.zeros(hd, F),
