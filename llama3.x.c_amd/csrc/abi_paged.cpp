@@ -30,7 +30,7 @@ bool batch_ok(const char *name, const PagedBatch *b) {
 size_t table_ints(const PagedBatch *b) { return (size_t)b->count * b->max_pages; }
 
 size_t cache_bytes(const PagedBatch *b, int n_kv_heads, int head_dim) {
-  return (size_t)b->num_pages * b->page_size * n_kv_heads * head_dim * value_bytes(b);
+  return product(product((size_t)b->num_pages * b->page_size, (size_t)n_kv_heads * head_dim), value_bytes(b));
 }
 
 // Whether a call that writes these bytes would write over the batch's arrays, which its other blocks still read.
@@ -110,9 +110,13 @@ void llhip_rope_kv_append_paged(float *q_out, size_t q_out_stride, const float *
     raise("%s: q_out is q at another stride (%zu and %zu)", name, q_out_stride, q_stride);
     return;
   }
-  const size_t q_bytes = ((rows - 1) * q_stride + dq) * kFloat, out_bytes = ((rows - 1) * q_out_stride + dq) * kFloat;
-  const size_t kv_bytes = ((rows - 1) * kv_stride + dkv) * kFloat, norm_bytes = (size_t)head_dim * kFloat;
+  const size_t q_bytes = rows_bytes(rows, q_stride, dq), out_bytes = rows_bytes(rows, q_out_stride, dq);
+  const size_t kv_bytes = rows_bytes(rows, kv_stride, dkv), norm_bytes = (size_t)head_dim * kFloat;
   const size_t cache = cache_bytes(batch, n_kv_heads, head_dim);
+  if (q_bytes >= kNoRoom || out_bytes >= kNoRoom || kv_bytes >= kNoRoom || cache >= kNoRoom) {
+    raise("%s: the rows or the caches take more than 2^56 bytes", name);
+    return;
+  }
   const size_t table_bytes = (size_t)batch->seq_len * 2 * head_dim * kFloat;
   bool bad = overlaps(key_pages, cache, value_pages, cache) ||
              (q_out != q && rows_meet(q_out, dq, q_out_stride, q, dq, q_stride, rows)) ||
@@ -169,8 +173,12 @@ void llhip_attention_paged(float *out, const float *q, size_t q_stride, const vo
     raise("%s: null buffer", name);
     return;
   }
-  const size_t q_bytes = ((rows - 1) * q_stride + dq) * kFloat, out_bytes = rows * dq * kFloat;
+  const size_t q_bytes = rows_bytes(rows, q_stride, dq), out_bytes = rows_bytes(rows, dq, dq);
   const size_t cache = cache_bytes(batch, n_kv_heads, head_dim);
+  if (q_bytes >= kNoRoom || cache >= kNoRoom) {
+    raise("%s: the rows or the caches take more than 2^56 bytes", name);
+    return;
+  }
   if (overlaps(out, out_bytes, q, q_bytes) || overlaps(out, out_bytes, key_pages, cache) ||
       overlaps(out, out_bytes, value_pages, cache) || over_arrays(batch, out, out_bytes)) {
     raise("%s: out must not overlap q, a cache or the batch's arrays", name);

@@ -444,7 +444,11 @@ void llhip_token_logprobs(float *logprob, float *entropy, int *top_token, float 
     raise("%s: null buffer", name);
     return;
   }
-  const size_t n = (size_t)rows * kFloat, most = n * (size_t)top, logits_bytes = ((size_t)(rows - 1) * ld + vocab) * kFloat;
+  const size_t n = (size_t)rows * kFloat, most = n * (size_t)top, logits_bytes = rows_bytes((size_t)rows, ld, (size_t)vocab);
+  if (logits_bytes >= kNoRoom) {
+    raise("%s: the logits take more than 2^56 bytes", name);
+    return;
+  }
   const struct {
     const void *p;
     size_t bytes;

@@ -372,6 +372,16 @@ bool launch_attention_paged(const AttentionPagedJob &job, void *workspace, hipSt
 extern std::mutex scratch_mutex;
 enum ScratchOf { SCRATCH_REQUESTS, SCRATCH_PAGES };
 bool scratch_room(const char *name, size_t bytes, void **out, ScratchOf of = SCRATCH_REQUESTS);
+// The product of sizes that a caller gives, or kNoRoom: more than any memory holds, where addresses might wrap.
+constexpr size_t kNoRoom = (size_t)1 << 56;
+inline size_t product(size_t a, size_t b) {
+  size_t c;
+  return __builtin_mul_overflow(a, b, &c) || c > kNoRoom ? kNoRoom : c;
+}
+// The bytes from the first of `rows` rows of `row` floats, `stride` floats apart, to the last one's end, or kNoRoom.
+inline size_t rows_bytes(size_t rows, size_t stride, size_t row) {
+  return product(product(rows - 1, stride) + product(row, 1), sizeof(float));
+}
 inline bool overlaps(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
   return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
 }

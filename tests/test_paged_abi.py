@@ -209,6 +209,24 @@ def test_score_refusals(L):
     assert not lh.last_error()
 
 
+def test_sizes_that_no_memory_holds(L):
+    """Products of sizes past 64 bits, some of them 0 modulo 2^64: refused before an address is formed of them."""
+    for stride in (1 << 61, 1 << 62, (1 << 62) + 32, (1 << 63) - 1, (1 << 64) - 1, 1 << 56):
+        attention_call(L, make().struct, q_stride=stride)
+        refused(L, "more than 2^56 bytes")
+        for name in ("o_stride", "q_stride", "kv_stride"):
+            append_call(L, make().struct, **{name: stride})
+            refused(L, "more than 2^56 bytes")
+        score_call(L, ld=stride)
+        refused(L, "more than 2^56 bytes")
+    for pages, page in ((2 ** 31 - 1, 2 ** 31 - 1), (2 ** 30, 2 ** 30), (2 ** 27, 2 ** 30)):
+        for call, kv in ((attention_call, 2), (append_call, 2), (attention_call, 4)):
+            b = make()
+            b.struct.num_pages, b.struct.page_size = pages, page
+            call(L, b.struct, kv=kv)
+            refused(L, "more than 2^56 bytes")
+
+
 def test_engine_logprobs_without_a_model(L):
     model, out = lh.Model(), np.full(2, 7.0, F)
     for m in (None, ctypes.byref(model)):
