@@ -160,6 +160,129 @@ def test_temperatures(L, temperature):
     assert np.array_equal(got[2], np.argsort(-logits, 1, kind="stable")[:, :6])
 
 
+@pytest.mark.parametrize("rows", [5, 8, 9, 16, 17, 64])
+@pytest.mark.parametrize("vocab,top", [(1, 1), (65, 32), (1025, 5), (5000, 20), (32000, 0), (128256, 20), (128256, 32)])
+@pytest.mark.parametrize("temperature", [1.0, 0.3])
+def test_scores_of_few_and_many_rows(L, rows, vocab, top, temperature):
+    """Both forms, one launch and two, over one chunk and many."""
+    rng = np.random.default_rng(vocab + top + rows)
+    logits = (3.0 * rng.standard_normal((rows, vocab))).astype(F)
+    tokens = rng.integers(0, vocab, rows)
+    tokens[1] = -1
+    tokens[2] = logits[2].argmax()
+    check(L, logits, tokens, temperature, top)
+    check(L, logits, None, temperature, top, ld=vocab + 3)
+    check(L, logits, tokens, temperature, top, entropy=False, ld=vocab + 4)
+
+
+@pytest.mark.parametrize("rows", [5, 16, 17])
+def test_vocabularies_past_the_groups_maxima(L, rows):
+    """More than 262144 tokens: chunks' maxima in the groups' place; random rows, sorted ones, few values, masked ones."""
+    rng = np.random.default_rng(rows)
+    vocab = 300001
+    logits = rng.standard_normal((rows, vocab)).astype(F)
+    logits[1] = np.sort(logits[1])
+    logits[2] = rng.integers(0, 3, vocab)
+    logits[3] = np.where(rng.random(vocab) < 0.9999, -np.inf, logits[3])
+    logits[3, 7] = 0.0
+    logits[4] = np.sort(logits[4])[::-1]
+    for top in (1, 32):
+        check(L, logits, rng.integers(0, vocab, rows), 0.8, top)
+
+
+@pytest.mark.parametrize("rows", [9, 17, 40])
+@pytest.mark.parametrize("vocab", [70, 1024, 3000, 40000, 128256])
+def test_equal_logits_and_masked_ones_of_many_rows(L, rows, vocab):
+    """As test_equal_logits_and_masked_ones, each kind of row again and again; 32 alternatives of rows of one value, where more
+    than 512 candidates meet."""
+    rng = np.random.default_rng(vocab + rows)
+    logits, tokens = np.zeros((rows, vocab), F), np.zeros(rows, np.int64)
+    for i in range(rows):
+        x, kind = logits[i], i % 8
+        tokens[i] = rng.integers(0, vocab)
+        if kind == 1:
+            x[:] = rng.integers(0, 3, vocab)
+        elif kind == 2:
+            x[:] = rng.choice(np.array([0.0, -0.0], F), vocab)
+        elif kind == 3:
+            x[:] = -np.inf
+            x[[5, vocab - 1]] = 2.0
+        elif kind == 4:
+            x[:] = np.where(rng.random(vocab) < 0.9, -np.inf, rng.standard_normal(vocab))
+            x[7] = 0.0
+        elif kind == 5:
+            x[:] = rng.standard_normal(vocab)
+            x[3] = 80.0
+        elif kind == 6:
+            x[:] = -1e30
+            x[vocab // 2] = 1e30
+        elif kind == 7:
+            x[:] = np.linspace(9, -9, vocab)
+    for top in (0, 1, 7, 32):
+        check(L, logits, tokens, 1.0, top)
+
+
+@pytest.mark.parametrize("vocab", [2000, 128256, 270000])
+def test_rows_that_decide_nothing_among_many(L, vocab):
+    """As test_rows_that_decide_nothing, in two launches; the other rows' results are those of the rows without them."""
+    rng = np.random.default_rng(vocab)
+    rows = 20
+    for what in (np.nan, np.inf, None):
+        logits = rng.standard_normal((rows, vocab)).astype(F)
+        tokens = rng.integers(0, vocab, rows)
+        bad = [0, 7, 19]
+        for i in bad:
+            if what is None:
+                logits[i] = -np.inf
+            else:
+                logits[i, rng.integers(0, vocab)] = what
+        got = call(L, logits, tokens, top=20)
+        L.llhip_synchronize()
+        assert "leave no token" in lh.last_error()
+        L.llhip_clear_error()
+        for i in bad:
+            assert np.isnan(got[0][i]) and np.isnan(got[1][i]) and np.isnan(got[3][i]).all() and (got[2][i] == -1).all()
+        rest = [i for i in range(rows) if i not in bad]
+        want = check(L, logits[rest], tokens[rest], top=20)
+        for g, w in zip(got, want):
+            assert np.array_equal(g[rest], w)
+
+
+def test_tokens_outside_the_vocabulary_among_many(L):
+    rng = np.random.default_rng(2)
+    rows, vocab = 33, 5000
+    logits = rng.standard_normal((rows, vocab)).astype(F)
+    good = rng.integers(0, vocab, rows)
+    want = check(L, logits, good, top=3)
+    for bad in (vocab, -2, 2 ** 31 - 1, -2 ** 31):
+        tokens = good.copy()
+        tokens[20] = bad
+        got = call(L, logits, tokens, top=3)
+        L.llhip_synchronize()
+        assert "scored token outside the vocabulary" in lh.last_error()
+        L.llhip_clear_error()
+        assert np.isnan(got[0][20])
+        assert np.array_equal(np.delete(got[0], 20), np.delete(want[0], 20))
+        for g, w in zip(got[1:], want[1:]):
+            assert np.array_equal(g, w)
+
+
+@pytest.mark.parametrize("vocab", [700, 5000, 128256, 300001])
+def test_a_row_scores_the_same_beside_any_others(L, vocab):
+    """Bit for bit, in one launch and in two."""
+    rng = np.random.default_rng(vocab)
+    logits = (2.0 * rng.standard_normal((17, vocab))).astype(F)
+    logits[3] = rng.integers(0, 3, vocab)
+    tokens = rng.integers(0, vocab, 17)
+    many = call(L, logits, tokens, 0.7, 32)
+    for rows in ([3], [0, 3, 5, 16, 9], list(range(8)), list(range(9))):
+        few = call(L, logits[rows], tokens[rows], 0.7, 32)
+        for m, f in zip(many, few):
+            assert np.array_equal(m[rows], f)
+    L.llhip_synchronize()
+    assert not lh.last_error()
+
+
 def test_large_vocabularies_and_many_rows(L):
     rng = np.random.default_rng(4)
     logits = rng.standard_normal((2, 1 << 22)).astype(F)
