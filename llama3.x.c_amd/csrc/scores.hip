@@ -25,7 +25,10 @@ constexpr int kGroup = 64;   // tokens of a maximum: those of 16 lanes' float4
 constexpr int kGroups = kChunk / kGroup;
 constexpr int kPer = 16;       // maxima of a thread of score_rows, at most: rows of more than 4096 groups keep their chunks'
 constexpr int kRankList = 512; // candidates that are ranked each against each
-constexpr int kFewRows = 16;   // of score_few, at most: 8 rows with 32 alternatives take 13.1 us there and 13.4 in two launches, 64 with 20 26 and 18
+// Rows of score_few, at most: where the two forms meet over 128256 tokens. In us, one launch and two: 8 rows 6.0 and 8.1 without
+// alternatives, 11.8 and 12.4 with 20; 16 rows 6.8 and 8.0, 13.0 and 13.2; 24 rows 7.6 and 8.5, 15.2 and 14.2; 64 rows 12.3 and
+// 11.5, 26 and 18. (Over 32000 tokens they meet at 64 rows, 0.3 to 0.5 apart up to there.)
+constexpr int kFewRows = 16;
 
 // How many of a row's blocks have stored their chunks: zero between launches, as the last to arrive sets it back. Each in a
 // cache line of its own: additions to one line wait for each other (64 rows: 12 us instead of 19).
