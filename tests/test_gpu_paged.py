@@ -1,6 +1,11 @@
 """A cache in pages, on the GPU: appended rows against the single calls bit for bit (and, behind norms, against float64),
 attention against its plain float64 form (tests/paged_util.py, the bounds derived there), index checks, host buffers, captured
 calls, and the two operators together as a server uses them."""
+import os
+import subprocess
+import sys
+import threading
+
 import numpy as np
 import pytest
 
@@ -783,6 +788,141 @@ def test_a_captured_step_follows_the_arrays(L, rows_of):
         plain, bound = pu.attention(b, hu.host(rot), cache_host(caches[0]), cache_host(caches[1]), heads, kv, hd, "head")
         within(hu.host(out), plain, bound, lengths)
     L.llhip_graph_destroy(graph)
+
+
+GROWING = r'''
+import sys
+sys.path[:0] = [sys.argv[1], sys.argv[1] + "/llama3.x.c_amd"]
+import numpy as np
+import llama_hip as lh
+from tests import hip_util as hu, paged_util as pu
+L = lh.load()
+assert L.llhip_init() == 0
+lh.record_failures()
+L.kernels_kv_layout_select(b"head")
+T = hu.torch()
+rng = np.random.default_rng(1)
+
+def make(rows_of, lengths, heads, kv, hd):
+    b = pu.Pages(hu.dev, rows_of, lengths, page=16, bf16=True)
+    caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
+    q = rng.standard_normal((b.rows, heads * hd), dtype=np.float32)
+    want, bound = pu.attention(b, q, *caches, heads, kv, hd, "head")
+    dev = [hu.dev(q)] + [hu.dev(c.view(np.int16)) for c in caches]
+    return dict(b=b, dev=dev, out=hu.dev(np.zeros_like(q)), want=want, bound=bound, shape=(heads, kv, hd))
+
+def call(m):
+    q, k, v = (lh.ptr(x) for x in m["dev"])
+    heads, kv, hd = m["shape"]
+    L.llhip_attention_paged(lh.ptr(m["out"]), q, heads * hd, k, v, m["b"].struct, heads, kv, hd)
+
+def right(m):
+    got = hu.host(m["out"]).astype(np.float64)
+    assert not lh.last_error(), lh.last_error()
+    assert (np.abs(got - m["want"]) <= m["bound"]).all()
+    m["out"].zero_()
+    T.cuda.synchronize()
+
+small, large = make([1, 1, 1], [3000, 2500, 40], 8, 2, 64), make([1, 40, 6], [900, 2900, 310], 8, 2, 128)
+start = L.llhip_hbm_claimed()
+call(small)
+right(small)
+one = L.llhip_hbm_claimed() - start
+assert one > 0
+assert L.llhip_graph_begin() == 0, lh.last_error()
+call(small)
+assert not lh.last_error(), lh.last_error()
+graph = L.llhip_graph_end()
+assert graph, lh.last_error()
+# a capture that would need more is refused, and nothing of it is kept
+assert L.llhip_graph_begin() == 0, lh.last_error()
+call(large)
+message = lh.last_error()
+L.llhip_clear_error()
+empty = L.llhip_graph_end()
+if empty:
+    L.llhip_graph_destroy(empty)
+L.llhip_clear_error()
+assert "workspace during graph capture" in message, message
+assert L.llhip_hbm_claimed() - start == one
+for turn in range(3):
+    assert L.llhip_graph_launch(graph) == 0
+    right(small)
+    call(large)
+    right(large)
+    assert L.llhip_hbm_claimed() - start > 2.25 * one, (one, L.llhip_hbm_claimed())  # another buffer, beside the captured one
+    other = T.full((64 << 20,), float("nan"), device="cuda")
+    T.cuda.synchronize()
+    assert L.llhip_graph_launch(graph) == 0
+    call(large)
+    right(small)
+    right(large)
+    assert T.isnan(other).all()
+L.llhip_graph_destroy(graph)
+print("workspace ok", flush=True)
+'''
+
+
+def test_a_captured_call_keeps_its_workspace():
+    """In a process of its own, whose workspace no other test has grown: a graph captured on the first workspace replays right
+    behind eager calls that take a larger one, which comes beside it; a capture that would need more than there is is refused."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", GROWING, root], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "workspace ok" in r.stdout, (r.stdout[-2000:], r.stderr[-4000:])
+
+
+def test_calls_from_threads_that_share_a_workspace(L):
+    """Two batches' attention over pages at once, which share the pages' workspace and counters, beside scoring and attention
+    behind a shared prefix, which share the requests'."""
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(17)
+    heads, kv, hd = 8, 2, 64
+    jobs = []
+    for rows_of, lengths, bf16 in (([1, 3] * 8, rng.integers(0, 2000, 16), False), ([2, 70, 1], [4000, 300, 2500], True)):
+        b = pu.Pages(hu.dev, rows_of, lengths, page=16, bf16=bf16)
+        caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
+        q = rng.standard_normal((b.rows, heads * hd), dtype=F)
+        want, bound = pu.attention(b, q, *caches, heads, kv, hd, "head")
+        dev, out = [hu.dev(q)] + [cache_dev(c) for c in caches], hu.dev(np.zeros_like(q))
+
+        def attend(b=b, dev=dev, out=out):
+            L.llhip_attention_paged(lh.ptr(out), lh.ptr(dev[0]), heads * hd, lh.ptr(dev[1]), lh.ptr(dev[2]), b.struct, heads, kv,
+                                    hd)
+
+        jobs.append((attend, lambda out=out, want=want, bound=bound: within(hu.host(out), want, bound)))
+    logits, tokens = rng.standard_normal((40, 5000)).astype(F), rng.integers(0, 5000, 40).astype(np.int32)
+    ld, td, lp = hu.dev(logits), hu.dev(tokens), hu.dev(np.zeros(40, F))
+    scored = pu.scores(logits, tokens, 1.0, 0)[0]
+
+    def score():
+        L.llhip_token_logprobs(lh.ptr(lp), None, None, None, 0, lh.ptr(ld), 5000, lh.ptr(td), 40, 5000, 1.0)
+
+    # z of at most 10: the sum is off by (2 * 10 + 28) U of itself, a log probability of at most 16 by U of its own, together
+    # below 4e-6
+    jobs.append((score, lambda: within(hu.host(lp), scored, np.full(40, 1e-5))))
+    r = ru.Batch(hu.dev, [1] * 20, rng.integers(0, 100, 20), prefix=300, prefix_seq_len=300, seq_len=128)
+    a = [rng.standard_normal(n, dtype=F) for n in ((r.rows, heads * hd), (kv, 300, hd), (kv, 300, hd), (r.slots, kv, 128, hd),
+                                                   (r.slots, kv, 128, hd))]
+    behind, behind_bound = ru.attention(r, *a, heads, kv, hd, "head")
+    rdev, rout = [hu.dev(x) for x in a], hu.dev(np.zeros_like(a[0]))
+    jobs.append((lambda: L.llhip_attention_requests(lh.ptr(rout), *[lh.ptr(x) for x in rdev], r.struct, heads, kv, hd),
+                 lambda: within(hu.host(rout), behind, behind_bound)))
+    for run, _ in jobs:
+        run()
+    quiet(L)
+
+    def many(run):
+        for _ in range(150):
+            run()
+
+    team = [threading.Thread(target=many, args=(run,)) for run, _ in jobs]
+    for t in team:
+        t.start()
+    for t in team:
+        t.join()
+    quiet(L)
+    for _, check in jobs:
+        check()
 
 
 @pytest.mark.parametrize("bf16", [False, True])
