@@ -172,15 +172,16 @@ template <typename T> __global__ __launch_bounds__(kThreads) void attn_paged_row
       if (h < kv_mul)
         acc[((size_t)share * kv_mul + h) * hd + d] = o[h];
   }
-  __syncthreads();
+  const bool failed = __syncthreads_or(bad);
   float *dst = job.out + ((size_t)row * job.n_heads + (size_t)g * kv_mul) * hd;
   for (int i = tid; i < kv_mul * hd; i += kThreads) {
     float total = 0.0f;
     for (int s2 = 0; s2 < shares; s2++)
       total += acc[(size_t)s2 * kv_mul * hd + i];
     total /= run_sum[i / hd];
-    if (!isfinite(total)) {
+    if (!isfinite(total) && !failed) {
       float odd = 0.0f;
+#pragma unroll 8
       for (int t = 0; t < positions; t++) {
         const int page = max(page_of(b, request, t / b.page_size), 0);
         odd += odd_only(value(values + (size_t)page * b.page_values + (size_t)(t % b.page_size) * b.pos_stride + i % hd));
@@ -1174,8 +1175,15 @@ template <typename T> __device__ __forceinline__ void give_odd(const FastPaged &
   };
   float odd = 0.0f;
   if (share < shares)
-    for (int t = share; t <= it.last0; t += shares)
-      odd += at(t);
+    for (int t = share; t <= it.last0; t += 8 * shares) { // eight on their way at once; the last one again does no harm
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        x[i] = at(min(t + i * shares, it.last0));
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        odd += x[i];
+    }
   lds[tid] = odd;
   __syncthreads();
   if (share == 0) {
