@@ -122,6 +122,34 @@ def test_appended_rows_equal_the_single_calls_bit_for_bit(L, layout, bf16, heads
     assert np.array_equal(cache_host(vd).view(np.uint8), caches[1].view(np.uint8))
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (5, 5, 6), (3, 1, 130)])
+def test_appended_values_of_every_kind_round_as_bf16_does(L, heads, kv, hd):
+    """Ties both ways, denormals, the largest floats (which round to infinity), zeros of both signs, infinities and NaN."""
+    L.kernels_kv_layout_select(b"head")
+    rng = np.random.default_rng(hd)
+    b = pu.Pages(hu.dev, [3, 40], [5, 0], bf16=True)
+    bits = rng.integers(0, 1 << 32, (b.rows, kv * hd), dtype=np.uint64).astype(np.uint32)  # any float at all
+    kinds = np.array([0x3F808000, 0x3F818000, 0x3F817FFF, 0x3F818001, 1, 0x8000, 0x18000, 0x807FFFFF, 0x007F8000, 0x7F7FFFFF,
+                      0x7F7F7FFF, 0xFF7FFFFF, 0, 0x80000000, 0x7F800000, 0xFF800000, 0x7FC00000, 0xFF800001], np.uint32)
+    bits[:, :len(kinds)] = kinds[:kv * hd]
+    bits[::2, :len(kinds)] = kinds[::-1][:kv * hd]
+    v = bits.view(F)
+    table = rope_table(L, b.seq_len, hd)
+    q, k = (rng.standard_normal((b.rows, n * hd), dtype=F) for n in (heads, kv))
+    caches = [b.cache(rng, "head", kv, hd) for _ in range(2)]
+    kd, vd, out = cache_dev(caches[0]), cache_dev(caches[1]), hu.dev(np.zeros_like(q))
+    ins = [hu.dev(x) for x in (q, k, v, table)]
+    L.llhip_rope_kv_append_paged(lh.ptr(out), heads * hd, lh.ptr(ins[0]), heads * hd, lh.ptr(ins[1]), lh.ptr(ins[2]), kv * hd,
+                                 lh.ptr(ins[3]), None, None, 0.0, b.struct, heads, kv, hd, lh.ptr(kd), lh.ptr(vd))
+    quiet(L)
+    got = cache_host(vd)
+    for r, rows, length in b.requests():
+        for j, i in enumerate(range(rows.start, rows.stop)):
+            mine, want = b.row(got, "head", r, length + j).reshape(-1), pu.to_bf16(v[i])
+            nan = np.isnan(v[i])
+            assert np.isnan(pu.values(mine)[nan]).all() and np.array_equal(mine[~nan], want[~nan])
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (3, 1, 128), (5, 5, 6), (8, 2, 80), (2, 1, 256), (3, 1, 130)])
 @pytest.mark.parametrize("which", ["both", "q", "k"])
@@ -379,6 +407,21 @@ def test_attention_of_scores_far_below_zero(L, bf16, rows_of):
             mean = np.repeat(vals[:, :n].mean(1), heads // kv, 0)
             size = np.repeat(np.abs(vals[:, :n]).mean(1), heads // kv, 0)
             assert (np.abs(got[i].reshape(heads, hd) - mean) <= (3 * n + 72) * ru.U * size).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows_of", [[1, 1], [7], [1, 40]])
+@pytest.mark.parametrize("hd", [64, 128, 50])
+def test_attention_over_denormal_keys(L, bf16, rows_of, hd):
+    """Keys below 2^-126 under queries of 2^124: scores as any others."""
+    heads, kv = 8, 2
+    b = pu.Pages(hu.dev, rows_of, [100, 30][:len(rows_of)], page=16, bf16=bf16)
+    rng = np.random.default_rng(6)
+    key = (rng.integers(-15, 16, b.shape("head", kv, hd)) * 2.0 ** -132).astype(F)
+    assert (np.abs(key) < 2.0 ** -126).all()
+    q = (rng.standard_normal((b.rows, heads * hd)) * 2.0 ** 124).astype(F)
+    caches = [pu.to_bf16(key) if bf16 else key, b.cache(rng, "head", kv, hd)]
+    attention_case(L, 3, heads, kv, hd, "head", b, caches=caches, q=q)
 
 
 def attention_case_equal_scores(L, b, q, key, value, heads, kv, hd):
