@@ -46,8 +46,11 @@ int llhip_engine_verify(Model *model, const int *tokens, int count, int pos0, co
  * as engine_forward_batch's rows with every row's logits, which stay on the device, and llhip_token_logprobs
  * (llama_hip_requests.h: temperature, top and the outputs are its arguments, in host or device memory, count rows of
  * each) of them: logprob[i] is tokens[i + 1]'s behind tokens[0 .. i], the last one 0; entropy (or NULL) and the
- * alternatives are every row's, the last one's those of the token that would come next. Returns 0, or -1 when the call
- * failed in record mode. The positions are in the cache afterwards, as engine_forward_batch leaves them. */
+ * alternatives are every row's, the last one's those of the token that would come next. A text longer than engine_max_batch
+ * takes several calls: a call's last row does not know the token behind it, so the next call begins with that row again (at
+ * the same position, where it stores the same token's keys and values), or else that token's log probability is lost. Returns
+ * 0, or -1 when the call failed in record mode. The positions are in the cache afterwards, as engine_forward_batch leaves
+ * them. */
 int llhip_engine_logprobs(Model *model, const int *tokens, int count, int pos0, float temperature, int top, float *logprob,
                           float *entropy, int *top_token, float *top_logprob);
 void engine_free(Model *model);   /* runtime.h:114 */

@@ -140,7 +140,8 @@ void llhip_verify_drafts(int *accepted, int *next, const float *logits, size_t l
  * leaves the log probabilities out. A row with a NaN, +infinity or no token left gets NaN in all places and tokens -1, and a
  * token outside the vocabulary NaN; both fail at the next host-visible point. Exponentials are FP32, a row's sums of them
  * FP64 over parts of 1024 tokens. The outputs must not overlap each other or an input. At most 2^20 rows and 2^22 tokens. The
- * workspace and counters are shared as llhip_attention_paged's (llama_hip_paged.h). */
+ * workspace is the one of the calls above, the counters (of up to 16 rows) are these calls' own: two that may run concurrently on
+ * one GPU race, and a counter that they leave off zero makes later calls' rows wrong, too (as in llama_hip_paged.h). */
 enum { LLHIP_MAX_TOP = 32 };
 void llhip_token_logprobs(float *logprob, float *entropy, int *top_token, float *top_logprob, int top,
                           const float *logits, size_t ld, const int *tokens, int rows, int vocab, float temperature);
