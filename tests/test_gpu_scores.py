@@ -397,3 +397,37 @@ def test_engine_scores_a_text(L, tmp_path, monkeypatch, kind):
     finally:
         L.engine_free(at)
         L.llhip_clear_error()
+
+
+def test_engine_scores_a_long_text_in_several_calls(L, tmp_path, monkeypatch):
+    """Each call begins with the last token of the call before: bit for bit the text in one call, where rows run one at a time."""
+    monkeypatch.setenv("LLAMA_PREFILL_GEMM", "off")
+    monkeypatch.setenv("LLAMA_PREFILL_BATCH", "24")
+    L.kernels_kv_layout_select(b"head")
+    path = os.path.join(tmp_path, "tiny.bin")
+    engine_model(path, "q8")
+    tokens = np.random.default_rng(4).integers(0, ENGINE["vocab_size"], 24).astype(np.int32)
+    model = lh.Model()
+    at = ctypes.byref(model)
+
+    def score(a, b, top=3):
+        n = b - a
+        out = [np.zeros(n, F), np.zeros(n, F), np.zeros((n, top), np.int32), np.zeros((n, top), F)]
+        mine = np.ascontiguousarray(tokens[a:b])
+        assert L.llhip_engine_logprobs(at, lh.ptr(mine), n, a, 0.8, top, *[lh.ptr(x) for x in out]) == 0, lh.last_error()
+        return out
+
+    try:
+        L.engine_load(at, path.encode())
+        assert model.implementation, lh.last_error()
+        whole = score(0, 24)
+        for cuts in ((0, 9, 24), (0, 1, 2, 16, 24)):
+            parts = []
+            for i, (a, b) in enumerate(zip(cuts, cuts[1:])):
+                got = score(a - 1 if i else a, b)
+                parts.append([x if b == 24 else x[:-1] for x in got])
+            for w, *p in zip(whole, *parts):
+                assert np.array_equal(np.concatenate(p), w), cuts
+    finally:
+        L.engine_free(at)
+        L.llhip_clear_error()
