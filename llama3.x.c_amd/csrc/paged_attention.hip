@@ -429,8 +429,8 @@ __device__ __forceinline__ float mark_of(const float4 &x, float mark) {
 // weights' sums, to out: through the wave's own rows of LDS, so that a store's lanes lie side by side. Returns the mark of what
 // it gave to out.
 template <int HD, int EV, class Row>
-__device__ __forceinline__ float store_rows(const FastPaged &p, const Slot &slot, bool whole, const v4f (&o)[HD / 16], float inverse,
-                                           float *rows, int lane, int hd, int v0, int count, Row row_of) {
+__device__ __forceinline__ float store_rows(const FastPaged &p, const Slot &slot, bool whole, const v4f (&o)[HD / 16],
+                                            float inverse, float *rows, int lane, int hd, int v0, int count, Row row_of) {
   constexpr int kRow = HD + 4;
   const int lq = lane >> 4, lc = lane & 15;
   const float scale = whole ? inverse : 1.0f;
