@@ -343,6 +343,25 @@ def test_attention_split_over_a_long_cache(L, bf16, heads, kv, hd, length):
     attention_case(L, length, heads, kv, hd, "rows", b)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows_of", [[1], [6], [12], [40], [1, 30, 2]])
+@pytest.mark.parametrize("heads,kv,hd,length,page", [(256, 128, 8, 19000, 16), (256, 128, 8, 19000, 48), (600, 600, 8, 6000, 64),
+                                                     (600, 600, 8, 2000, 20)])
+def test_attention_of_many_kv_heads(L, bf16, rows_of, heads, kv, hd, length, page):
+    """So many KV heads that one or four blocks take all positions of one: thousands of positions a wave, past those whose pages
+    it looks up at once."""
+    b = pu.Pages(hu.dev, rows_of, [length, 40, 700][:len(rows_of)], page=page, bf16=bf16)
+    attention_case(L, length, heads, kv, hd, "head", b)
+
+
+@pytest.mark.parametrize("kv,hd", [(4096, 8), (4097, 8)])
+@pytest.mark.parametrize("bf16", [False, True])
+def test_attention_of_the_most_kv_heads(L, bf16, kv, hd):
+    """On both sides of the matrix-core form's limit."""
+    b = pu.Pages(hu.dev, [1, 5], [70, 3], page=16, bf16=bf16)
+    attention_case(L, kv, kv, kv, hd, "rows", b)
+
+
 @pytest.mark.parametrize("count", [64, 255, 257, 1024])
 def test_attention_many_requests(L, count):
     rng = np.random.default_rng(count)
