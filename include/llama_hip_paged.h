@@ -77,9 +77,9 @@ void llhip_rope_kv_append_paged(float *q_out, size_t q_out_stride, const float *
  * calls on a device share: calls ordered on the library's stream are safe, from any thread. Two that may run concurrently on one
  * GPU (graphs replayed on other streams) race, and the damage lasts: a counter that they leave off zero makes later calls' rows
  * wrong, too, until the process ends. The workspace is as large as any lengths may need: 22 MB of HBM for head_dim up to 64, 43
- * up to 256, twice that for BF16 pages of head_dim up to 128 where rows outnumber requests (and one may have more than 64 query
- * vectors of a KV head), also for a call of one short row; it stays. Run the largest batch once before capturing a step, so that
- * the workspace is there. */
+ * up to 256 (of up to 512 KV heads), twice that for BF16 pages of head_dim up to 128 where rows outnumber requests (and one may
+ * have more than 64 query vectors of a KV head), also for a call of one short row; it stays. Run the largest batch once before
+ * capturing a step, so that the workspace is there. */
 void llhip_attention_paged(float *out, const float *q, size_t q_stride, const void *key_pages, const void *value_pages,
                            const PagedBatch *batch, int n_heads, int n_kv_heads, int head_dim);
 
